@@ -34,6 +34,8 @@
 #include "kernels/optim_api.h"
 #include "kernels/stft_api.h"
 #include "kernels/topk_api.h"
+#include "ops/checkpoint.h"
+#include "ops/heads.h"
 #include "ops/linear.h"
 #include "optim/adamw_plan.h"
 #include "optim/bucket_hook.h"
@@ -869,4 +871,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                            batch, in, out);
   });
   m.def("_linear_native", &linear_native, py::arg("input"), py::arg("weight"), py::arg("bias") = py::none());
+
+  // ---- operators of a decoder block ---------------------------------------------------------------------
+  m.def("_pack8", &pack8, py::call_guard<py::gil_scoped_release>());
+  m.def("_unpack8", [](const at::Tensor& codes, const at::Tensor& scales, const std::vector<int64_t>& shape, at::ScalarType type) {
+    py::gil_scoped_release free;
+    return unpack8(codes, scales, shape, type);
+  });
+  m.def("_norm_rotate", &norm_rotate, py::call_guard<py::gil_scoped_release>());
+  m.def("_norm_rotate_packed", &norm_rotate_packed, py::call_guard<py::gil_scoped_release>());
 }

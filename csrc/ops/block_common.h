@@ -1,0 +1,51 @@
+// What the operators of a decoder block share: their checks, types and error reports.
+#pragma once
+
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <string>
+
+#include "common/errors.h"
+#include "kernels/pack8_api.h"
+#include "ops/ordinary.h"
+
+namespace mccl {
+
+#define BLOCK_CK(expr)                                                       \
+  do {                                                                       \
+    cudaError_t _e = (expr);                                                 \
+    if (_e != cudaSuccess) {                                                 \
+      cudaGetLastError();                                                    \
+      throw DeviceError(std::string(#expr) + ": " + cudaGetErrorString(_e)); \
+    }                                                                        \
+  } while (0)
+
+inline kern::Elem elem_of(const at::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return kern::Elem::kF32;
+    case at::kHalf: return kern::Elem::kF16;
+    case at::kBFloat16: return kern::Elem::kBF16;
+    default: throw TensorError(std::string(what) + ": float32, float16 or bfloat16 expected, got " + c10::toString(t.scalar_type()));
+  }
+}
+// A tensor that the kernels may read: dense memory of a B200, no wrapper and no tangent that they would lose.
+inline void check_block_tensor(const at::Tensor& t, const char* what) {
+  MCCL_CHECK_T(TensorError, t.defined() && t.is_cuda() && t.layout() == at::kStrided, what << ": a dense CUDA tensor expected");
+  MCCL_CHECK_T(TensorError, ordinary(t), what << ": tensor subclasses, transforms and forward-mode tangents are not supported");
+  const auto* p = at::cuda::getDeviceProperties(t.get_device());
+  MCCL_CHECK_T(DeviceError, p->major == 10 && p->minor == 0, what << ": built for compute capability 10.0, got " << p->major << "." << p->minor);
+}
+// `t` as rows along its last dimension: a view where its layout allows it, else a copy.
+inline at::Tensor rows_of(const at::Tensor& t) {
+  const int64_t cols = t.dim() ? t.size(-1) : 1;
+  int64_t rows = 1;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) rows *= t.size(d);
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({rows, cols});
+  if (r.numel() > 0 && (r.stride(1) != 1 && cols != 1)) r = r.contiguous();
+  return r;
+}
+inline int64_t row_stride(const at::Tensor& r) { return r.size(0) <= 1 ? r.size(1) : r.stride(0); }
+
+}  // namespace mccl

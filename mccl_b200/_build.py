@@ -43,6 +43,8 @@ CPP_SOURCES = [
     "cpu/reduce.cpp",
     "transforms/stft.cpp",
     "ops/linear.cpp",
+    "ops/checkpoint.cpp",
+    "ops/heads.cpp",
     "p2p/nccl_p2p.cpp",
 ]
 CUDA_SOURCES = [
@@ -57,6 +59,8 @@ CUDA_SOURCES = [
     "kernels/stft.cu",
     "kernels/adamw.cu",
     "kernels/gemm_f32.cu",
+    "kernels/pack8.cu",
+    "kernels/heads.cu",
     "kernels/noalloc.cu",
 ]
 
