@@ -35,6 +35,7 @@
 #include "kernels/stft_api.h"
 #include "kernels/topk_api.h"
 #include "ops/checkpoint.h"
+#include "ops/gated.h"
 #include "ops/heads.h"
 #include "ops/linear.h"
 #include "optim/adamw_plan.h"
@@ -878,6 +879,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     py::gil_scoped_release free;
     return unpack8(codes, scales, shape, type);
   });
+  m.def("_gated_feed_forward", &gated_feed_forward, py::call_guard<py::gil_scoped_release>());
+  m.def("_gated_with_limit", &gated_with_limit);
   m.def("_norm_rotate", &norm_rotate, py::call_guard<py::gil_scoped_release>());
   m.def("_norm_rotate_packed", &norm_rotate_packed, py::call_guard<py::gil_scoped_release>());
 }

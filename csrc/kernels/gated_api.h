@@ -1,0 +1,62 @@
+// Launchers of the gated feed-forward block's products (plain C++ header).
+//
+//     g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
+//
+// of `tokens` rows, `width` numbers in and out, `hidden` between.  Six products; what stands between them is inside of them.
+#pragma once
+
+#include <cuda_runtime_api.h>
+
+#include <cstdint>
+
+namespace mccl {
+namespace kern {
+
+enum class GatedProduct {
+  kUp,          // a0 = x, b0 = Wg, b1 = Wu: h to out0, g and u to `kept`
+  kDown,        // a0 = h, b0 = Wd: y to out0
+  kGate,        // a0 = dy, b0 = Wd: with dh = dy Wd: h to out0, dg to out1, du to out2, from `kept`
+  kInput,       // a0 = dg, a1 = du, b0 = Wg, b1 = Wu: dx to out0
+  kWeightUp,    // a0 = dg, a1 = du, b0 = x: dWg to out0, dWu to out1
+  kWeightDown,  // a0 = dy, b0 = h: dWd to out0
+};
+enum class GatedActivation { kSilu, kGeluTanh };
+// How g and u wait for the backward pass: not at all, as floats of three bytes, as codes of 8 bits.
+enum class GatedKeep { kNone, kWide, kEight };
+
+struct GatedShape {
+  int64_t tokens, width, hidden;
+  bool bf16;  // else fp16
+  GatedActivation activation;
+  GatedKeep keep;
+};
+// Elements from row to row of h, dg and du: `hidden` padded to whole groups; what is beyond `hidden` is zero.
+inline int64_t gated_pitch(int64_t hidden) { return (hidden + 63) / 64 * 64; }
+int64_t gated_kept_bytes(const GatedShape& s);
+
+// Rows of 16-bit numbers, 16-byte aligned and so many elements apart.
+struct GatedOperand {
+  const void* data;
+  int64_t ld;
+};
+struct GatedArgs {
+  GatedProduct product;
+  GatedShape shape;
+  GatedOperand a0, a1, b0, b1;
+  void *out0, *out1, *out2;
+  int64_t ldo;          // of the outputs
+  void* kept;
+  float* partial;       // gated_partial_bytes
+  uint32_t* failed;     // set to 1 where a wait runs out, whose tiles then are NaN; or null
+  int64_t wait_limit;   // cycles of a quarter of a wait; negative: about a second in all
+};
+int64_t gated_partial_bytes(GatedProduct p, const GatedShape& s);
+cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s);
+
+// The same in fp32, between products of their own (kernels/gate_f32.cu): h of n numbers g and u; with dh, their gradients too.
+cudaError_t launch_gate_f32(const float* g, const float* u, float* h, int64_t n, GatedActivation act, cudaStream_t s);
+cudaError_t launch_gate_f32_backward(const float* g, const float* u, const float* dh, float* dg, float* du, int64_t n, GatedActivation act,
+                                     cudaStream_t s);
+
+}  // namespace kern
+}  // namespace mccl

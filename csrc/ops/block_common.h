@@ -7,20 +7,11 @@
 
 #include <string>
 
-#include "common/errors.h"
 #include "kernels/pack8_api.h"
 #include "ops/ordinary.h"
+#include "ops/wait_status.h"
 
 namespace mccl {
-
-#define BLOCK_CK(expr)                                                       \
-  do {                                                                       \
-    cudaError_t _e = (expr);                                                 \
-    if (_e != cudaSuccess) {                                                 \
-      cudaGetLastError();                                                    \
-      throw DeviceError(std::string(#expr) + ": " + cudaGetErrorString(_e)); \
-    }                                                                        \
-  } while (0)
 
 inline kern::Elem elem_of(const at::Tensor& t, const char* what) {
   switch (t.scalar_type()) {

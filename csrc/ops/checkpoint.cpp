@@ -13,7 +13,7 @@ std::tuple<at::Tensor, at::Tensor> pack8(const at::Tensor& x) {
   at::Tensor codes = at::empty({rows, pitch}, x.options().dtype(at::kChar));
   at::Tensor scales = at::empty({rows, kern::pack8_groups(cols)}, x.options().dtype(at::kFloat));
   const kern::Packed8Rows p{codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows, cols, pitch};
-  BLOCK_CK(kern::launch_pack8(r.const_data_ptr(), type, row_stride(r), p, at::cuda::getCurrentCUDAStream()));
+  OPS_CK(kern::launch_pack8(r.const_data_ptr(), type, row_stride(r), p, at::cuda::getCurrentCUDAStream()));
   return {codes, scales};
 }
 
@@ -36,7 +36,7 @@ at::Tensor unpack8(const at::Tensor& codes, const at::Tensor& scales, at::IntArr
   at::Tensor x = at::empty(shape, codes.options().dtype(type));
   const kern::Packed8Rows p{const_cast<int8_t*>(codes.const_data_ptr<int8_t>()), const_cast<float*>(scales.const_data_ptr<float>()), rows, cols,
                             kern::pack8_pitch(cols)};
-  BLOCK_CK(kern::launch_unpack8(p, x.data_ptr(), elem_of(x, "unpack8"), cols, at::cuda::getCurrentCUDAStream()));
+  OPS_CK(kern::launch_unpack8(p, x.data_ptr(), elem_of(x, "unpack8"), cols, at::cuda::getCurrentCUDAStream()));
   return x;
 }
 

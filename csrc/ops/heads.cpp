@@ -82,7 +82,7 @@ std::tuple<at::Tensor, at::Tensor> forward_of(const kern::HeadsShape& s, const a
   at::Tensor qo = out_like(q), ko = out_like(k);
   a.q_out = qo.data_ptr();
   a.k_out = ko.data_ptr();
-  BLOCK_CK(kern::launch_heads_forward(a, at::cuda::getCurrentCUDAStream()));
+  OPS_CK(kern::launch_heads_forward(a, at::cuda::getCurrentCUDAStream()));
   return {qo, ko};
 }
 
@@ -134,7 +134,7 @@ variable_list backward_of(AutogradContext* ctx, const at::Tensor& q, const at::T
     a.dq_weight = need_qw ? qw.data_ptr() : nullptr;
     a.dk_weight = need_kw ? kw.data_ptr() : nullptr;
   }
-  BLOCK_CK(kern::launch_heads_backward(a, at::cuda::getCurrentCUDAStream()));
+  OPS_CK(kern::launch_heads_backward(a, at::cuda::getCurrentCUDAStream()));
   return {qw, kw};
 }
 

@@ -6,46 +6,15 @@
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "common/errors.h"
 #include "kernels/gemm_api.h"
 #include "ops/ordinary.h"
+#include "ops/wait_status.h"
 
 namespace mccl {
 
 namespace {
-
-#define LINEAR_CK(expr)                                                      \
-  do {                                                                       \
-    cudaError_t _e = (expr);                                                 \
-    if (_e != cudaSuccess) {                                                 \
-      cudaGetLastError();                                                    \
-      throw DeviceError(std::string(#expr) + ": " + cudaGetErrorString(_e)); \
-    }                                                                        \
-  } while (0)
-
-// Words of mapped host memory, one per device, in which a kernel notes that one of its bounded waits ran out.
-constexpr int kDevices = 64;
-uint32_t* wait_status(const at::Tensor& t) {
-  static uint32_t* words = [] {
-    void* p = nullptr;
-    auto mode = cudaStreamCaptureModeRelaxed;  // the first call may be under capture
-    LINEAR_CK(cudaThreadExchangeStreamCaptureMode(&mode));
-    const cudaError_t e = cudaHostAlloc(&p, kDevices * sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable);
-    LINEAR_CK(cudaThreadExchangeStreamCaptureMode(&mode));
-    LINEAR_CK(e);
-    std::fill_n(static_cast<uint32_t*>(p), kDevices, 0u);
-    return static_cast<uint32_t*>(p);
-  }();
-  return words + t.get_device() % kDevices;
-}
-// Reports what a kernel has noted on the device, once.  What it gave up is NaN.
-void check_waits(const at::Tensor& t) {
-  uint32_t* word = wait_status(t);
-  if (*static_cast<volatile uint32_t*>(word) != 0 && __atomic_exchange_n(word, 0u, __ATOMIC_RELAXED) != 0)
-    throw DeviceError("a wait inside an earlier matrix product kernel ran out; what it should have written is NaN");
-}
 
 bool rows_ok(const at::Tensor& t) {
   return t.scalar_type() == at::kFloat && t.dim() == 2 && t.numel() > 0 && t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1));
@@ -99,7 +68,7 @@ at::Tensor forward_product(const at::Tensor& x, const at::Tensor& w, const at::T
   char* image = s.take(plan.b_image);
   auto* partial = reinterpret_cast<float*>(s.take(plan.partial));
   const kern::SplitJob job{matrix(x), image, plan.cols, nullptr};
-  LINEAR_CK(kern::launch_split_f32(&job, 1, nullptr, tickets, plan.tickets, stream));
+  OPS_CK(kern::launch_split_f32(&job, 1, nullptr, tickets, plan.tickets, stream));
   const kern::MatrixF32 wm = matrix(w);
   kern::GemmArgs g{};
   g.product = kern::Product::kForward;
@@ -114,7 +83,7 @@ at::Tensor forward_product(const at::Tensor& x, const at::Tensor& w, const at::T
   g.tickets = tickets;
   g.failed = wait_status(x);
   g.wait_limit = wait_limit;
-  LINEAR_CK(kern::launch_gemm_f32(g, stream));
+  OPS_CK(kern::launch_gemm_f32(g, stream));
   return y;
 }
 
@@ -148,7 +117,7 @@ Gradients backward_products(const at::Tensor& grad, const at::Tensor& x, const a
   if (need_bias) r.bias = at::empty({out}, x.options());
   const kern::SplitJob jobs[2] = {{matrix(grad), own_x ? gx : nullptr, px.cols, own_w ? gw : nullptr},
                                   {matrix(x), nullptr, 0, xw}};
-  LINEAR_CK(kern::launch_split_f32(jobs, own_w ? 2 : 1, need_bias ? r.bias.data_ptr<float>() : nullptr, tickets,
+  OPS_CK(kern::launch_split_f32(jobs, own_w ? 2 : 1, need_bias ? r.bias.data_ptr<float>() : nullptr, tickets,
                                    px.tickets + pw.tickets, stream));
   if (own_x) {
     r.x = at::empty({batch, in}, x.options());
@@ -165,7 +134,7 @@ Gradients backward_products(const at::Tensor& grad, const at::Tensor& x, const a
     g.tickets = tickets;
     g.failed = wait_status(x);
     g.wait_limit = wait_limit;
-    LINEAR_CK(kern::launch_gemm_f32(g, stream));
+    OPS_CK(kern::launch_gemm_f32(g, stream));
   }
   if (own_w) {
     r.w = at::empty({out, in}, x.options());
@@ -180,7 +149,7 @@ Gradients backward_products(const at::Tensor& grad, const at::Tensor& x, const a
     g.tickets = tickets + px.tickets;
     g.failed = wait_status(x);
     g.wait_limit = wait_limit;
-    LINEAR_CK(kern::launch_gemm_f32(g, stream));
+    OPS_CK(kern::launch_gemm_f32(g, stream));
   }
   return r;
 }
@@ -235,6 +204,13 @@ std::vector<at::Tensor> linear_with_limit(const at::Tensor& x, const at::Tensor&
               "not a gradient for the kernels");
   const Gradients g = backward_products(*grad, x, w, true, true, false, wait_limit);
   return {g.x, g.w};
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_gradients(const at::Tensor& grad, const at::Tensor& x, const at::Tensor& w, bool need_x, bool need_w) {
+  const at::Tensor g = rows_ok(grad) ? grad : grad.contiguous();
+  if (!rows_ok(g) || !rows_ok(x) || !rows_ok(w)) return {need_x ? g.mm(w) : at::Tensor(), need_w ? g.t().mm(x) : at::Tensor()};
+  const Gradients r = backward_products(g, x, w, need_x, need_w, false);
+  return {r.x, r.w};
 }
 
 at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias) {

@@ -45,6 +45,7 @@ CPP_SOURCES = [
     "ops/linear.cpp",
     "ops/checkpoint.cpp",
     "ops/heads.cpp",
+    "ops/gated.cpp",
     "p2p/nccl_p2p.cpp",
 ]
 CUDA_SOURCES = [
@@ -61,6 +62,8 @@ CUDA_SOURCES = [
     "kernels/gemm_f32.cu",
     "kernels/pack8.cu",
     "kernels/heads.cu",
+    "kernels/gated.cu",
+    "kernels/gate_f32.cu",
     "kernels/noalloc.cu",
 ]
 

@@ -1,0 +1,102 @@
+"""Gated feed-forward block, ``(act(x w_gate^T) * (x w_up^T)) w_down^T``, with its gradients (``csrc/kernels/gated.cu``).
+
+Both projections, the activation and the product are one kernel on the tensor cores, the projection back a second one; the
+backward pass takes four.  ``float16`` and ``bfloat16``: sums in fp32; ``h``, the result of activation and product, and the
+gradients of its two factors are rounded to 16 bits once, as operands of the next product (in ``float16`` what is beyond its
+range becomes infinite there).  ``float32``: the products of ``mccl_b200.ops.linear``, with one pass between them.
+
+What the backward pass needs of the two projections is kept with 16 significant bits (three bytes a number); with
+``checkpoint="int8"`` it is kept, and the input too, as 8-bit codes with a scale for each group of 64 (see
+``mccl_b200.ops.checkpoint``), and the gradients are those of the kept values.  The backward pass is not differentiable itself.
+CPU tensors take the same formulas in torch.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from .checkpoint import pack8, unpack8
+
+ACTIVATIONS = ("silu", "gelu_tanh")
+
+
+def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
+                       activation: str = "silu", checkpoint: Optional[str] = None) -> torch.Tensor:
+    """``x`` [..., width], ``w_gate`` and ``w_up`` [hidden, width], ``w_down`` [width, hidden], all of one type.
+
+    ``activation``: ``"silu"`` or ``"gelu_tanh"``.  ``checkpoint``: ``None`` or ``"int8"``.  Under autocast all four are cast
+    to its type first.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation is one of {ACTIVATIONS}, got {activation!r}")
+    if checkpoint not in (None, "int8"):
+        raise ValueError(f"checkpoint is None or 'int8', got {checkpoint!r}")
+    if x.is_cuda:
+        from .. import require_native
+        if torch.is_autocast_enabled("cuda"):
+            to = torch.get_autocast_dtype("cuda")
+            x, w_gate, w_up, w_down = x.to(to), w_gate.to(to), w_up.to(to), w_down.to(to)
+            with torch.autocast("cuda", enabled=False):
+                return require_native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+        return require_native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+    return _Plain.apply(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+
+
+def _act(name, g):
+    """The activation and its slope."""
+    c = 2 * math.sqrt(2 / math.pi)
+    s = torch.sigmoid(g if name == "silu" else c * (g + 0.044715 * g ** 3))
+    return g * s, s + g * s * (1 - s) * (1 if name == "silu" else c * (1 + 3 * 0.044715 * g * g))
+
+
+class _Plain(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation, eight):
+        g, u = F.linear(x, w_gate), F.linear(x, w_up)
+        kept = [pack8(t) for t in (x, g, u)] if eight else [x, g, u]
+        ctx.kept_as = [p[2:] for p in kept] if eight else None
+        ctx.activation = activation
+        ctx.save_for_backward(w_gate, w_up, w_down, *([t for p in kept for t in p[:2]] if eight else kept))
+        return F.linear(_act(activation, g)[0] * u, w_down)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        w_gate, w_up, w_down, *kept = ctx.saved_tensors
+        if ctx.kept_as is not None:
+            from .checkpoint import Packed8
+            kept = [unpack8(Packed8(kept[2 * i], kept[2 * i + 1], *ctx.kept_as[i])) for i in range(3)]
+        x, g, u = (t.flatten(0, -2) if t.dim() > 1 else t[None] for t in kept)
+        rows = dy.reshape(-1, dy.shape[-1])
+        a, slope = _act(ctx.activation, g)
+        dh = rows @ w_down
+        dg, du = dh * u * slope, dh * a
+        dx = (dg @ w_gate + du @ w_up).view(dy.shape)
+        return dx, dg.t() @ x, du.t() @ x, rows.t() @ (a * u), None, None
+
+
+class GatedFeedForward(nn.Module):
+    """:func:`gated_feed_forward` with its weights, initialised like ``torch.nn.Linear``'s, without biases."""
+
+    def __init__(self, width: int, hidden: int, *, activation: str = "silu", checkpoint: Optional[str] = None, device=None, dtype=None):
+        super().__init__()
+        if activation not in ACTIVATIONS or checkpoint not in (None, "int8"):
+            raise ValueError(f"activation is one of {ACTIVATIONS} and checkpoint None or 'int8'")
+        self.activation, self.checkpoint = activation, checkpoint
+        like = dict(device=device, dtype=dtype)
+        self.w_gate = nn.Parameter(torch.empty(hidden, width, **like))
+        self.w_up = nn.Parameter(torch.empty(hidden, width, **like))
+        self.w_down = nn.Parameter(torch.empty(width, hidden, **like))
+        for w in (self.w_gate, self.w_up, self.w_down):
+            nn.init.kaiming_uniform_(w, a=math.sqrt(5))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return gated_feed_forward(x, self.w_gate, self.w_up, self.w_down, activation=self.activation, checkpoint=self.checkpoint)
+
+    def extra_repr(self) -> str:
+        hidden, width = self.w_gate.shape
+        return f"width={width}, hidden={hidden}, activation={self.activation!r}, checkpoint={self.checkpoint!r}"
