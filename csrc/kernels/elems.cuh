@@ -6,6 +6,30 @@
 namespace mccl {
 namespace kern {
 
+// Two numbers of 16 bits next to each other: one instruction, where two conversions and their joining are four.
+template <typename T> __device__ __forceinline__ uint32_t store_pair(float a, float b);
+template <> __device__ __forceinline__ uint32_t store_pair<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t store_pair<__half>(float a, float b) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+// V numbers as they lie in memory.
+template <typename T, int V, typename Raw>
+__device__ __forceinline__ Raw pack_run(const float* v) {
+  Raw raw;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) reinterpret_cast<uint32_t*>(&raw)[i / 2] = store_pair<T>(v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) reinterpret_cast<T*>(&raw)[i] = Traits<T>::store(v[i]);
+  }
+  return raw;
+}
+
 // V numbers of a row: in chunks of 16 (or all 8) bytes where `vec` says that they are aligned to that, one by one and only the
 // first n otherwise.
 template <int kBytes> struct Chunk { using type = uint4; };
@@ -36,11 +60,8 @@ __device__ __forceinline__ void store_run(T* p, int n, bool vec, const float (&v
     if (vec && n >= V) {
 #pragma unroll
       for (int c = 0; c < V / kPer; ++c) {
-        typename Chunk<kBytes>::type raw;
-        T* x = reinterpret_cast<T*>(&raw);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] = Traits<T>::store(v[c * kPer + i]);
-        *reinterpret_cast<typename Chunk<kBytes>::type*>(p + c * kPer) = raw;
+        using Raw = typename Chunk<kBytes>::type;
+        *reinterpret_cast<Raw*>(p + c * kPer) = pack_run<T, kPer, Raw>(&v[c * kPer]);
       }
       return;
     }
@@ -63,21 +84,21 @@ __device__ __forceinline__ Scale8 scale8(float most) {
   if (most < kTiny8) return {0.f, 0.f};
   return {__fdiv_rn(most, 127.f), __fdiv_rn(127.f, most)};
 }
-// Four codes, the first in the lowest byte.  `inverse` 0 (nothing to keep, or a NaN group): zeros, whatever x is.
+// Four codes, the first in the lowest byte: 1.5 2^23 and a number of at most 127 is a float whose lowest byte is that number,
+// rounded to the nearest integer, halves to even.  (A conversion of each to an integer has a quarter of the additions' rate.)
+// `inverse` 0 (nothing to keep, or a NaN group): zeros, whatever x is.
 __device__ __forceinline__ uint32_t codes8(float x0, float x1, float x2, float x3, float inverse) {
-  const int a = __float2int_rn(x0 * inverse), b = __float2int_rn(x1 * inverse), c = __float2int_rn(x2 * inverse),
-            d = __float2int_rn(x3 * inverse);
-  const uint32_t w = (a & 0xFF) | (b & 0xFF) << 8 | (c & 0xFF) << 16 | static_cast<uint32_t>(d) << 24;
+  constexpr float kMagic = 12582912.f;
+  const uint32_t a = __float_as_uint(__fadd_rn(__fmul_rn(x0, inverse), kMagic)), b = __float_as_uint(__fadd_rn(__fmul_rn(x1, inverse), kMagic)),
+                 c = __float_as_uint(__fadd_rn(__fmul_rn(x2, inverse), kMagic)), d = __float_as_uint(__fadd_rn(__fmul_rn(x3, inverse), kMagic));
+  const uint32_t w = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
   return inverse == 0.f ? 0u : w;
 }
 __device__ __forceinline__ float value8(uint32_t word, int i, float scale) {
   return static_cast<float>(static_cast<int8_t>(word >> (8 * i))) * scale;
 }
-// The largest magnitude, a NaN where there is one (fmaxf drops it).
-__device__ __forceinline__ float most8(float a, float x) {
-  const float b = fabsf(x);
-  return b != b ? b : (a != a ? a : fmaxf(a, b));
-}
+// The largest magnitude, as bits: those of a NaN are above those of all numbers.
+__device__ __forceinline__ uint32_t most8(uint32_t most, float x) { return max(most, __float_as_uint(x) & 0x7FFFFFFFu); }
 
 }  // namespace kern
 }  // namespace mccl

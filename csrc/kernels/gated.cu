@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kernels/elems.cuh"
 #include "kernels/gated_api.h"
@@ -26,11 +27,9 @@ constexpr int kPairs = 74;               // of SMs: a pair computes one tile
 constexpr int kTile = 256;               // rows and columns of a tile; each CTA of the pair has 128 of the rows
 constexpr int kHalf = 128;
 constexpr int kDepth = 64;               // k per stage
-constexpr int kStages = 6;
 constexpr int kOperand = kHalf * kDepth * 2, kStage = 2 * kOperand;   // bytes a CTA has of a stage
-constexpr int kSmem = kStages * kStage + 1024;
 constexpr int kColumns = 512;            // of tensor memory: two accumulators
-// warp 0 loads, warp 1 issues products, warp 2 has the tensor memory, warps 4 .. 11 take the accumulators out
+// warp 0 loads, warp 1 issues products, warp 2 has the tensor memory, the warps from 4 on take the accumulators out
 constexpr int kLoader = 0, kIssuer = 1, kOwner = 2, kFirstOut = 4, kOutWarps = 8, kThreads = 32 * (kFirstOut + kOutWarps);
 
 // ---- PTX ----------------------------------------------------------------------------------------------------
@@ -41,13 +40,15 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// (What it orders is tensor memory, for which there are fences of its own: a release at cluster scope would wait for all of the
+// warp's stores, a microsecond or two a tile.)
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
       : "r"(bar), "r"(parity)
       : "memory");
@@ -81,6 +82,13 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, in
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t from, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(from) : "memory");
+}
+__device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// All of this thread's groups have left shared memory; are done.
+__device__ __forceinline__ void stores_left() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // Shared-memory matrix descriptors, 128-byte swizzle.  k innermost: rows of 128 bytes (64 k), 1024 bytes per eight rows.  Own
 // index innermost: rows of 128 bytes (64 of the index, one k), 1024 bytes per eight k, 8192 from 64 of the index to the next.
 template <bool kInner>
@@ -111,29 +119,36 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// 32 consecutive columns of the calling thread's lane
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
-      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(addr));
+// kN consecutive columns of the calling thread's lane, which are there behind the wait: its operands keep whatever uses them from
+// moving before it.
+template <int kN>
+__device__ __forceinline__ void tmem_load(uint32_t addr, float* v) {
+  static_assert(kN == 16 || kN % 32 == 0, "runs of 16 or 32 columns");
+  if constexpr (kN == 16) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+                   "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(addr));
+  } else {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < kN; i += 32, v += 32)
+      asm volatile(
+          "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+          "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+          : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+            "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]),
+            "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]),
+            "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+          : "r"(addr + i));
+  }
 }
-// ... which are there behind this: the operands keep whatever uses them from moving before it.
-__device__ __forceinline__ void tmem_wait32(float* v) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
-                 "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]),
-                 "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27])
-               :
-               : "memory");
-  asm volatile("" : "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
+template <int kN>
+__device__ __forceinline__ void tmem_wait(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < kN; i += 16, v += 16)
+    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                     "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
 __device__ __forceinline__ bool elect() {
   uint32_t one;
@@ -142,19 +157,37 @@ __device__ __forceinline__ bool elect() {
 }
 
 // ---- what a launch is told ----------------------------------------------------------------------------------
+// act(z) = z s(z), s = 1 / (1 + 2^(z (c0 + c1 z^2))): silu has c0 = -log2(e) and c1 = 0, gelu 2 sqrt(2/pi) times as much and
+// 0.044715 of that.  Exponential and quotient are within 2^-21 of theirs, which 16 bits do not show.
+struct Curve {
+  float c0, c1;
+  __device__ __forceinline__ float square(float z) const { return fminf(z * z, 1e30f); }  // no infinity for c1 = 0 to meet
+  __device__ __forceinline__ float gate(float z) const {
+    float e, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * fmaf(c1, square(z), c0)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+    return s;
+  }
+  // act' = s + z s (1 - s) (c0 + 3 c1 z^2) / -log2(e)
+  __device__ __forceinline__ float slope(float z, float s) const {
+    return fmaf(z * (s - s * s), fmaf(-0.6931471805599453f * 3.f * c1, square(z), -0.6931471805599453f * c0), s);
+  }
+};
+
 enum Out { kStore, kActivate, kDerive };  // what follows the product
 
 struct Finish {
   void *out0, *out1, *out2;
   int64_t ldo;
-  bool wide;              // rows of out0 (kStore) may be written 16 bytes at a time
-  bool bf16, silu;
+  bool wide;              // there are maps of the outputs: their rows are aligned to 16 bytes
+  bool bf16;
+  Curve curve;
   char* kept;
   int64_t rows, cols;     // of one result: tokens x hidden for kActivate and kDerive
   int64_t pitch;          // of h, dg, du
 };
 struct Work {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[2], b[2], out[3];
   Finish f;
   int rows_segment;       // kStore: tiles of rows of the first of two results (dWg, then dWu); all of them where there is one
   int tiles_i, tiles_j;   // tiles_i: of all results
@@ -206,16 +239,6 @@ __device__ __forceinline__ void store16(void* row, int64_t col, const float* v, 
       make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16), pack2(v[4], v[5], bf16), pack2(v[6], v[7], bf16));
 }
 
-// s and the slope of act at z.  The exponential and the quotient are within 2^-21 of theirs, which 16 bits do not show.
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-constexpr float kGelu = 1.5957691216057308f, kCubic = 0.044715f;  // 2 sqrt(2 / pi)
-__device__ __forceinline__ float gate_of(float z, bool silu) { return logistic(silu ? z : kGelu * (z + kCubic * z * z * z)); }
-__device__ __forceinline__ float slope_of(float z, float s, bool silu) {
-  const float t = s * (1.f - s);
-  // (where the curve is flat the cubic's slope may be infinite)
-  return t > 0.f ? s + z * t * (silu ? 1.f : kGelu * (1.f + 3.f * kCubic * z * z)) : s;
-}
-
 // Floats of three bytes: the upper 24 bits, rounded to nearest; infinities and NaN cut off.
 __device__ __forceinline__ uint32_t three_bytes(float x) {
   const uint32_t b = __float_as_uint(x);
@@ -250,10 +273,10 @@ __device__ __forceinline__ void keep_wide(const Wide& k, int which, int64_t at, 
   uint32_t b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) b[i] = three_bytes(v[i]);
-  k.upper[which][at] = make_uint4(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632), __byte_perm(b[4], b[5], 0x7632),
-                                  __byte_perm(b[6], b[7], 0x7632));
-  k.lower[which][at] = make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0051), __byte_perm(b[2], b[3], 0x0051), 0x5410),
-                                  __byte_perm(__byte_perm(b[4], b[5], 0x0051), __byte_perm(b[6], b[7], 0x0051), 0x5410));
+  __stcs(k.upper[which] + at, make_uint4(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632), __byte_perm(b[4], b[5], 0x7632),
+                                         __byte_perm(b[6], b[7], 0x7632)));
+  __stcs(k.lower[which] + at, make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0051), __byte_perm(b[2], b[3], 0x0051), 0x5410),
+                                  __byte_perm(__byte_perm(b[4], b[5], 0x0051), __byte_perm(b[6], b[7], 0x0051), 0x5410)));
 }
 __device__ __forceinline__ void take_wide(const uint4& up, const uint2& low, float* v) {
   const uint32_t u[4] = {up.x, up.y, up.z, up.w}, l[2] = {low.x, low.y};
@@ -264,37 +287,54 @@ __device__ __forceinline__ void take_wide(const uint4& up, const uint2& low, flo
   }
 }
 
-// Columns col .. col + kN of a row of a result.
-template <int kN>
-__device__ __forceinline__ void finish_store(const Finish& f, void* out, int64_t rows, int64_t row, int64_t col, const float* v) {
-  if (row >= rows || col >= f.cols) return;
-  uint16_t* to = static_cast<uint16_t*>(out) + row * f.ldo;
-  if (f.wide && col + kN <= f.cols) {
+// Where 8 numbers of a thread's row go, `i` columns from where it is: straight to memory, which costs a request for each row (the
+// joining kernel, results that are not aligned), or to the warp's boxes of 32 rows and 64 columns in shared memory, 128-byte swizzle,
+// which then leave as a whole.  (Straight to memory kGate took 99 us of 8192 x 1024 x 2816, bound by its requests.)
+constexpr int kTurn = 64, kBoxBytes = 32 * kTurn * 2;
+struct Direct {
+  uint16_t* out[3];
+  bool on, bf16, wide;
+  int64_t left;  // numbers of the row from here on
+  __device__ __forceinline__ void put(int which, int i, const float* v) const {
+    if (!on) return;
+    if (wide && i + 8 <= left) {
+      store16(out[which], i, v, bf16);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kN; i += 8) store16(to, col + i, v + i, f.bf16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kN; i += 2) {
-      const uint32_t p = pack2(v[i], v[i + 1], f.bf16);
-      if (col + i < f.cols) to[col + i] = static_cast<uint16_t>(p);
-      if (col + i + 1 < f.cols) to[col + i + 1] = static_cast<uint16_t>(p >> 16);
+      for (int e = 0; e < 8; e += 2) {
+        const uint32_t p = pack2(v[e], v[e + 1], bf16);
+        if (i + e < left) out[which][i + e] = static_cast<uint16_t>(p);
+        if (i + e + 1 < left) out[which][i + e + 1] = static_cast<uint16_t>(p >> 16);
+      }
     }
   }
-}
+};
+struct Staged {
+  uint32_t row;       // of the first box
+  int swizzle;
+  bool bf16;
+  __device__ __forceinline__ Staged(uint32_t boxes, int lane, bool half) : row(boxes + lane * 128), swizzle(lane & 7), bf16(half) {}
+  __device__ __forceinline__ void put(int which, int i, const float* v) const {
+    const uint32_t to = row + which * kBoxBytes + ((i / 8) ^ swizzle) * 16;
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pack2(v[0], v[1], bf16)), "r"(pack2(v[2], v[3], bf16)),
+                 "r"(pack2(v[4], v[5], bf16)), "r"(pack2(v[6], v[7], bf16))
+                 : "memory");
+  }
+};
 // kN columns of g and u to h and to what is kept.
-template <GatedKeep kKeep, int kN>
-__device__ __forceinline__ void finish_activate(const Finish& f, int64_t row, int64_t col, const float* g, const float* u) {
-  if (row >= f.rows || col >= f.pitch) return;
-  if constexpr (kKeep == GatedKeep::kEight) {
-    static_assert(kN == kGroup8, "a thread has a whole group");
+template <GatedKeep kKeep, int kN, typename Sink>
+__device__ __forceinline__ void finish_activate(const Finish& f, int64_t row, int64_t col, const float* g, const float* u, const Sink& sink, int i0) {
+  const bool there = row < f.rows;
+  if (kKeep == GatedKeep::kEight && there) {
+    static_assert(kKeep != GatedKeep::kEight || kN == kGroup8, "a thread has a whole group");
     const Eight k(f.kept, f.rows, f.pitch);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       const float* v = which ? u : g;
-      float most = 0.f;
+      uint32_t most = 0u;
 #pragma unroll
       for (int i = 0; i < kN; ++i) most = most8(most, v[i]);
-      const Scale8 s = scale8(most);
+      const Scale8 s = scale8(__uint_as_float(most));
       k.scales[which][col / kGroup8 * f.rows + row] = s.scale;
 #pragma unroll
       for (int i = 0; i < kN; i += 16)
@@ -303,10 +343,9 @@ __device__ __forceinline__ void finish_activate(const Finish& f, int64_t row, in
                        codes8(v[i + 8], v[i + 9], v[i + 10], v[i + 11], s.inverse), codes8(v[i + 12], v[i + 13], v[i + 14], v[i + 15], s.inverse));
     }
   }
-  uint16_t* to = static_cast<uint16_t*>(f.out0) + row * f.pitch;
 #pragma unroll
   for (int i = 0; i < kN; i += 8) {
-    if constexpr (kKeep == GatedKeep::kWide) {
+    if (kKeep == GatedKeep::kWide && there) {
       const Wide k(f.kept, f.rows, f.pitch);
       const int64_t at = (col + i) / 8 * f.rows + row;
       keep_wide(k, 0, at, g + i);
@@ -314,111 +353,152 @@ __device__ __forceinline__ void finish_activate(const Finish& f, int64_t row, in
     }
     float h[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = g[i + e] * gate_of(g[i + e], f.silu) * u[i + e];
-    store16(to, col + i, h, f.bf16);
+    for (int e = 0; e < 8; ++e) h[e] = g[i + e] * f.curve.gate(g[i + e]) * u[i + e];
+    sink.put(0, i0 + i, h);
   }
 }
-// kN columns (a multiple of 16) of dh to h, dg and du.
-template <GatedKeep kKeep, int kN>
-__device__ __forceinline__ void finish_derive(const Finish& f, int64_t row, int64_t col, const float* dh) {
-  if (row >= f.rows || col >= f.pitch) return;
-  const int64_t to = row * f.pitch;
+// 16 columns of g and u as they were kept.
+template <GatedKeep kKeep>
+struct Kept {
+  uint4 upper[2][2];
+  uint2 lower[2][2];
+  __device__ __forceinline__ void load(const Finish& f, int64_t row, int64_t col) {
+    const Wide k(f.kept, f.rows, f.pitch);
+    const int64_t at = col / 8 * f.rows + row;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        upper[which][b] = __ldcs(k.upper[which] + at + b * f.rows);
+        lower[which][b] = __ldcs(k.lower[which] + at + b * f.rows);
+      }
+  }
+  __device__ __forceinline__ void value(int b, float* g, float* u) const {  // 8 of them
+    take_wide(upper[0][b], lower[0][b], g);
+    take_wide(upper[1][b], lower[1][b], u);
+  }
+};
+template <>
+struct Kept<GatedKeep::kEight> {
+  uint4 codes[2];
   float scale[2];
-  if constexpr (kKeep == GatedKeep::kEight) {
+  __device__ __forceinline__ void load(const Finish& f, int64_t row, int64_t col) {
     const Eight k(f.kept, f.rows, f.pitch);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) scale[which] = k.scales[which][col / kGroup8 * f.rows + row];
+    for (int which = 0; which < 2; ++which) {
+      codes[which] = __ldcs(k.codes[which] + col / 16 * f.rows + row);
+      scale[which] = __ldg(k.scales[which] + col / kGroup8 * f.rows + row);
+    }
   }
+  __device__ __forceinline__ void value(int b, float* g, float* u) const {
+    const uint32_t p[2] = {b ? codes[0].z : codes[0].x, b ? codes[0].w : codes[0].y}, q[2] = {b ? codes[1].z : codes[1].x, b ? codes[1].w : codes[1].y};
 #pragma unroll
-  for (int i = 0; i < kN; i += 16) {
-    float z[2][16];
-    if constexpr (kKeep == GatedKeep::kEight) {
-      const Eight k(f.kept, f.rows, f.pitch);
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const uint4 c = __ldcs(k.codes[which] + (col + i) / 16 * f.rows + row);
-        const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) z[which][e] = value8(words[e / 4], e % 4, scale[which]);
-      }
-    } else {
-      const Wide k(f.kept, f.rows, f.pitch);
-#pragma unroll
-      for (int which = 0; which < 2; ++which)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int64_t at = ((col + i) / 8 + b) * f.rows + row;
-          take_wide(__ldcs(k.upper[which] + at), __ldcs(k.lower[which] + at), &z[which][8 * b]);
-        }
+    for (int e = 0; e < 8; ++e) {
+      g[e] = value8(p[e / 4], e % 4, scale[0]);
+      u[e] = value8(q[e / 4], e % 4, scale[1]);
     }
+  }
+};
+// 16 columns of dh to h, dg and du.
+template <GatedKeep kKeep, typename Sink>
+__device__ __forceinline__ void finish_derive(const Finish& f, const float* dh, const Kept<kKeep>& kept, const Sink& sink, int i0) {
 #pragma unroll
-    for (int b = 0; b < 16; b += 8) {
-      float h[8], dg[8], du[8];
+  for (int b = 0; b < 2; ++b) {
+    float g[8], u[8], h[8], dg[8], du[8];
+    kept.value(b, g, u);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float g = z[0][b + e], u = z[1][b + e], d = dh[i + b + e];
-        const float s = gate_of(g, f.silu), a = g * s;
-        h[e] = a * u;
-        du[e] = d * a;
-        dg[e] = d * u * slope_of(g, s, f.silu);
-      }
-      store16(static_cast<uint16_t*>(f.out0) + to, col + i + b, h, f.bf16);
-      store16(static_cast<uint16_t*>(f.out1) + to, col + i + b, dg, f.bf16);
-      store16(static_cast<uint16_t*>(f.out2) + to, col + i + b, du, f.bf16);
+    for (int e = 0; e < 8; ++e) {
+      const float d = dh[8 * b + e], s = f.curve.gate(g[e]), a = g[e] * s;
+      h[e] = a * u[e];
+      du[e] = d * a;
+      dg[e] = d * u[e] * f.curve.slope(g[e], s);
     }
+    sink.put(0, i0 + 8 * b, h);
+    sink.put(1, i0 + 8 * b, dg);
+    sink.put(2, i0 + 8 * b, du);
   }
 }
 
 // ---- product ------------------------------------------------------------------------------------------------
-// The columns that a thread takes at a time: of h for kActivate (two accumulator columns each), of c else.
+// The columns that a thread takes out of the accumulator at a time (of h for kActivate: of c two each; an 8-bit group is one
+// thread's).  64 columns leave together.
 template <Out kOut, GatedKeep kKeep>
-constexpr int kTake = kOut == kActivate && kKeep == GatedKeep::kEight ? 64 : 32;
+constexpr int kTake = kOut == kActivate && kKeep == GatedKeep::kEight ? 64 : 16;
+template <Out kOut>
+constexpr int kBoxes = kOut == kDerive ? 3 : 1;
+template <Out kOut>
+constexpr int kStages = kOut == kDerive ? 4 : 6;
+template <Out kOut>
+constexpr int kSmem = kStages<kOut> * kStage + kOutWarps * kBoxes<kOut> * kBoxBytes + 1024;  // of 227 KB
 
-template <Out kOut, GatedKeep kKeep, typename Fetch>
-__device__ __forceinline__ void finish_tile(const Work& w, int ti, int tj, int row_in_tile, int first, int last, const Fetch& fetch) {
+// What a thread needs from memory for its first columns of a tile is asked for while the products still run, for the next ones while
+// it is busy with these.
+struct Nothing {
+  __device__ __forceinline__ void load(const Finish&, int64_t, int64_t) {}
+};
+template <Out kOut, GatedKeep kKeep>
+using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, Nothing>;
+
+// A thread's row and columns of a tile: `row` of the result that the tile is of, its columns from `col` on.
+struct Spot {
+  int64_t row, col;
+  int which;      // kStore: which of two results
+};
+template <Out kOut>
+__device__ __forceinline__ Spot spot_of(const Work& w, int ti, int tj, int row_in_tile) {
+  const int second = kOut == kStore && ti >= w.rows_segment;
+  return {static_cast<int64_t>(second ? ti - w.rows_segment : ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * (kOut == kActivate ? kHalf : kTile), second};
+}
+// kCols columns from `c` of the tile on, into a sink.
+template <Out kOut, GatedKeep kKeep, int kCols, typename Fetch, typename Sink>
+__device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int c, int last, Ahead<kOut, kKeep>& ahead, const Fetch& fetch, const Sink& sink) {
   constexpr int kN = kTake<kOut, kKeep>;
-  const Finish& f = w.f;
 #pragma unroll 1
-  for (int c = first; c < last; c += kN) {
+  for (int i = 0; i < kCols; i += kN) {
     if constexpr (kOut == kActivate) {
       float g[kN], u[kN];
-      fetch(c, g);
-      fetch(kHalf + c, u);
-      finish_activate<kKeep, kN>(f, static_cast<int64_t>(ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * kHalf + c, g, u);
+      fetch(c + i, g);
+      fetch(kHalf + c + i, u);
+      finish_activate<kKeep, kN>(f, at.row, at.col + c + i, g, u, sink, i);
     } else {
       float v[kN];
-      fetch(c, v);
       if constexpr (kOut == kDerive) {
-        finish_derive<kKeep, kN>(f, static_cast<int64_t>(ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * kTile + c, v);
+        const Kept<kKeep> now = ahead;
+        if (c + i + kN < last) ahead.load(f, min(at.row, f.rows - 1), at.col + c + i + kN);
+        fetch(c + i, v);
+        finish_derive<kKeep>(f, v, now, sink, i);
       } else {
-        const bool second = ti >= w.rows_segment;
-        finish_store<kN>(f, second ? f.out1 : f.out0, f.rows, static_cast<int64_t>(second ? ti - w.rows_segment : ti) * kTile + row_in_tile,
-                         static_cast<int64_t>(tj) * kTile + c, v);
+        fetch(c + i, v);
+#pragma unroll
+        for (int e = 0; e < kN; e += 8) sink.put(0, i + e, v + e);
       }
     }
   }
 }
+template <Out kOut>
+__device__ __forceinline__ int64_t columns_of(const Finish& f) { return kOut == kStore ? f.cols : f.pitch; }
 
 // A pair of CTAs per tile of 256 x 256, tiles in turn: each CTA loads half of either operand's rows and has half of the
 // accumulator's; the first one issues the products of both.  Two accumulators, so that a tile is taken out while the next one
 // is multiplied.
 template <bool kAInner, bool kBInner, Out kOut, GatedKeep kKeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work w) {
+  constexpr int kDepths = kStages<kOut>, kOuts = kBoxes<kOut>;
   extern __shared__ char raw[];
-  __shared__ alignas(8) uint64_t bars[2 * kStages + 5];
+  __shared__ alignas(8) uint64_t bars[2 * kDepths + 5];
   __shared__ uint32_t tmem_base;
   const uint32_t smem0 = (smem_addr(raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t bar0 = smem_addr(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
-  auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
-  auto acc_full = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
-  auto acc_free = [&](int b) { return bar0 + 8u * (2 * kStages + 2 + b); };
-  const uint32_t drained = bar0 + 8u * (2 * kStages + 4);
+  auto empty = [&](int s) { return bar0 + 8u * (kDepths + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * kDepths + b); };
+  auto acc_free = [&](int b) { return bar0 + 8u * (2 * kDepths + 2 + b); };
+  const uint32_t drained = bar0 + 8u * (2 * kDepths + 4);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kDepths; ++s) {
       bar_init(full(s), 1);
       bar_init(empty(s), 1);
     }
@@ -467,13 +547,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
             load_box(to + kOperand, b, j0, k0, bar);
             load_box(to + kOperand + kOperand / 2, b, j0 + 64, k0, bar);
           }
-          if (++s == kStages) s = 0, ++turn;
+          if (++s == kDepths) s = 0, ++turn;
         }
       }
       // the products' last arrivals, before the barriers are another's
-      for (int left = 0; ok && left < kStages; ++left) {
+      for (int left = 0; ok && left < kDepths; ++left) {
         ok = bar_wait(empty(s), (turn & 1) ^ 1, w.limit);
-        if (++s == kStages) s = 0, ++turn;
+        if (++s == kDepths) s = 0, ++turn;
       }
     }
     __syncwarp();
@@ -498,61 +578,83 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
 #pragma unroll
           for (int k = 0; k < kDepth / 16; ++k) mma(acc, a + k * kStep<kAInner>, b + k * kStep<kBInner>, idesc, c > t.c0 || k > 0);
           mma_commit(empty(s));
-          if (++s == kStages) s = 0, ++turn;
+          if (++s == kDepths) s = 0, ++turn;
         }
         if (ok) mma_commit(acc_full(buffer));
       }
     }
     __syncwarp();
   } else if (warp >= kFirstOut) {
-    // lanes 32 q .. 32 q + 31 of tensor memory are open to the warps with warp % 4 == q; two of them share the columns
-    const int q = warp & 3, half = (warp - kFirstOut) >> 2;
+    // lanes 32 q .. 32 q + 31 of tensor memory are open to the warps with warp % 4 == q, which share the columns
+    constexpr int kN = kTake<kOut, kKeep>, kShares = kOutWarps / 4, kShare = (kOut == kActivate ? kHalf : kTile) / kShares;
+    const int q = warp & 3, share = (warp - kFirstOut) >> 2;
     const int row = rank * kHalf + 32 * q + lane;
-    constexpr int kShare = (kOut == kActivate ? kHalf : kTile) / 2;
+    const uint32_t boxes = smem0 + kDepths * kStage + (warp - kFirstOut) * (kOuts * kBoxBytes);
+    const int64_t columns = columns_of<kOut>(w.f);
     int done = 0;
     for (int item = pair; item < w.items; item += pairs, ++done) {
       const Item t(w, item);
       const int buffer = done & 1;
+      const Spot at = spot_of<kOut>(w, t.ti, t.tj, row);
+      Ahead<kOut, kKeep> ahead;
+      if (t.part < 0 && at.col + share * kShare < columns) ahead.load(w.f, min(at.row, w.f.rows - 1), at.col + share * kShare);
       if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_full(buffer), (done >> 1) & 1, w.limit));
       fence_after();
       const uint32_t from = tmem + buffer * kTile + (static_cast<uint32_t>(32 * q) << 16);
       auto fetch = [&](int c, float* v) {
-        constexpr int kN = kTake<kOut, kKeep>;
         if (ok) {
-#pragma unroll
-          for (int i = 0; i < kN; i += 32) tmem_load32(from + c + i, v + i);
-#pragma unroll
-          for (int i = 0; i < kN; i += 32) tmem_wait32(v + i);
+          tmem_load<kN>(from + c, v);
+          tmem_wait<kN>(v);
         } else {
 #pragma unroll
           for (int i = 0; i < kN; ++i) v[i] = NAN;  // no number that looks like a result
         }
       };
       if (t.part < 0) {
-        finish_tile<kOut, kKeep>(w, t.ti, t.tj, row, half * kShare, half * kShare + kShare, fetch);
+        const int64_t left = columns - at.col;
+        const int first = share * kShare, last = static_cast<int>(min(static_cast<int64_t>(first + kShare), left));
+        if (w.f.wide) {
+          const int y = static_cast<int>(at.row) - lane;
+#pragma unroll 1
+          for (int c = first; c < last; c += kTurn) {
+            if (lane == 0) stores_left();
+            __syncwarp();
+            finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged(boxes, lane, w.f.bf16));
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (y < w.f.rows)
+#pragma unroll
+                for (int b = 0; b < kOuts; ++b)
+                  store_box(&w.out[kOut == kDerive ? b : at.which], boxes + b * kBoxBytes, static_cast<int>(at.col) + c, y);
+              stores_commit();
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int c = first; c < last; c += kTurn) {
+            const Direct sink{{static_cast<uint16_t*>(at.which ? w.f.out1 : w.f.out0) + at.row * w.f.ldo + at.col + c, nullptr, nullptr}, at.row < w.f.rows,
+                              w.f.bf16, false, left - c};
+            finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, sink);
+          }
+        }
       } else {
-        const bool second = t.ti >= w.rows_segment;
-        const bool there = static_cast<int64_t>(second ? t.ti - w.rows_segment : t.ti) * kTile + row < w.f.rows;
         float* to = w.partial + static_cast<int64_t>(t.part) * (kTile * kTile) + row;
 #pragma unroll 1
-        for (int c = half * kHalf; c < half * kHalf + kHalf; c += 32) {
-          float v[kTake<kOut, kKeep>];
-          if (ok) {
-            tmem_load32(from + c, v);
-            tmem_wait32(v);
-          } else {
+        for (int c = share * (kTile / kShares); c < (share + 1) * (kTile / kShares); c += kN) {
+          float v[kN];
+          fetch(c, v);
+          if (at.row < w.f.rows)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = NAN;
-          }
-          if (there)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) __stcg(to + static_cast<int64_t>(c + i) * kTile, v[i]);
+            for (int i = 0; i < kN; ++i) __stcg(to + static_cast<int64_t>(c + i) * kTile, v[i]);
         }
       }
       fence_before();
       __syncwarp();
       if (lane == 0 && ok) bar_arrive_cluster(in_leader(acc_free(buffer)));
     }
+    if (lane == 0) stores_done();
+    __syncwarp();
   }
   fence_before();
   const bool failed = __syncthreads_or(!ok);
@@ -574,28 +676,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
   if (warp == kOwner) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kColumns));
 }
 
-// Adds up the parts of the tiles whose reduction was shared, in order, and finishes them.  A block has 32 (64) columns of half a
+// Adds up the parts of the tiles whose reduction was shared, in order, and finishes them.  A block has 16 (64) columns of half a
 // tile; a part is read in runs of 128 numbers.
 template <Out kOut, GatedKeep kKeep>
 __global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant__ Work w) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kN = kTake<kOut, kKeep>;
-  const int tile = blockIdx.x, first = blockIdx.z * kN, row = blockIdx.y * kHalf + threadIdx.x;
+  const int tile = blockIdx.x, c = blockIdx.z * kN, row = blockIdx.y * kHalf + threadIdx.x;
   int ti, tj;
   tile_place(w, w.whole + tile, ti, tj);
-  if (static_cast<int64_t>(ti >= w.rows_segment ? ti - w.rows_segment : ti) * kTile + row >= w.f.rows) return;
+  const Finish& f = w.f;
+  const Spot at = spot_of<kOut>(w, ti, tj, row);
+  const int64_t left = columns_of<kOut>(f) - at.col - c;
+  if (at.row >= f.rows || left <= 0) return;
   const float* from = w.partial + static_cast<int64_t>(tile) * w.splits * (kTile * kTile) + row;
   auto fetch = [&](int c, float* v) {
 #pragma unroll
     for (int i = 0; i < kN; ++i) v[i] = 0.f;
-    for (int p = 0; p < w.splits; ++p) {
-      const float* x = from + static_cast<int64_t>(p) * (kTile * kTile) + static_cast<int64_t>(c) * kTile;
+    constexpr int kParts = kN == 64 ? 1 : 4;  // in flight
+    for (int p = 0; p < w.splits; p += kParts) {
+      float x[kParts][kN];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) v[i] += __ldcg(x + i * kTile);
+      for (int j = 0; j < kParts; ++j)
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+          x[j][i] = p + j < w.splits ? __ldcg(from + static_cast<int64_t>(p + j) * (kTile * kTile) + static_cast<int64_t>(c + i) * kTile) : 0.f;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j)
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] += x[j][i];
     }
   };
-  finish_tile<kOut, kKeep>(w, ti, tj, row, first, first + kN, fetch);
+  Ahead<kOut, kKeep> ahead;
+  ahead.load(f, at.row, at.col + c);
+  const int64_t to = at.row * (kOut == kStore ? f.ldo : f.pitch) + at.col + c;
+  const Direct sink{{static_cast<uint16_t*>(at.which ? f.out1 : f.out0) + to, static_cast<uint16_t*>(f.out1) + to, static_cast<uint16_t*>(f.out2) + to},
+                    true, f.bf16, f.wide, left};
+  finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, sink);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
@@ -665,11 +783,13 @@ EncodeTiled encode_tiled() {
   }();
   return fn;
 }
-// A matrix of `outer` rows of `inner` numbers; boxes of 64 of a row, and of 128 rows (k innermost) or 64 (own index innermost).
-bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t outer, bool k_inner, bool bf16) {
+// A matrix of `outer` rows of `inner` numbers, read in boxes of 64 of a row and of 128 rows (k innermost) or 64 (own index innermost),
+// or written in boxes of 64 of a row and of 32 rows.
+enum class Box { kInnerK, kOwn, kResult };
+bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t outer, Box kind, bool bf16) {
   if (m.data == nullptr || reinterpret_cast<uintptr_t>(m.data) % 16 != 0 || m.ld % 8 != 0 || m.ld < inner || inner > 0x7FFFFFFF || outer > 0x7FFFFFFF) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)}, strides[1] = {static_cast<cuuint64_t>(m.ld) * 2};
-  const cuuint32_t box[2] = {64, k_inner ? 128u : 64u}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {64, kind == Box::kResult ? 32u : kind == Box::kInnerK ? 128u : 64u}, one[2] = {1, 1};
   return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(m.data), dims, strides, box, one,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -684,7 +804,7 @@ cudaError_t run(const Work& w, int64_t tail, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = 1ull << (device & 63);
   if (!(smem_set.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<kOut>);
     if (e != cudaSuccess) return e;
     smem_set.fetch_or(bit, std::memory_order_release);
   }
@@ -694,15 +814,14 @@ cudaError_t run(const Work& w, int64_t tail, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min(w.items, kPairs)));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = kSmem<kOut>;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   note_launch();
   e = cudaLaunchKernelEx(&cfg, kernel, w);
   if (e != cudaSuccess || tail == 0) return e;
-  constexpr int kN = kTake<kOut, kKeep>;
-  cfg.gridDim = dim3(static_cast<unsigned>(tail), w.f.rows > kHalf ? 2 : 1, (kOut == kActivate ? kHalf : kTile) / kN);
+  cfg.gridDim = dim3(static_cast<unsigned>(tail), w.f.rows > kHalf ? 2 : 1, (kOut == kActivate ? kHalf : kTile) / kTake<kOut, kKeep>);
   cfg.blockDim = dim3(kHalf);
   cfg.dynamicSmemBytes = 0;
   note_launch();
@@ -736,16 +855,25 @@ cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s) {
   const bool b_inner = g.product == GatedProduct::kUp || g.product == GatedProduct::kDown;
   const GatedOperand a[2] = {g.a0, z.results * z.parts > 1 ? g.a1 : g.a0}, b[2] = {g.b0, z.gate || z.parts > 1 ? g.b1 : g.b0};
   for (int i = 0; i < 2; ++i)
-    if (!make_map(&w.a[i], a[i], a_inner ? z.depth : z.rows, a_inner ? z.rows : z.depth, a_inner, h.bf16) ||
-        !make_map(&w.b[i], b[i], b_inner ? z.depth : z.cols, b_inner ? z.cols : z.depth, b_inner, h.bf16))
+    if (!make_map(&w.a[i], a[i], a_inner ? z.depth : z.rows, a_inner ? z.rows : z.depth, a_inner ? Box::kInnerK : Box::kOwn, h.bf16) ||
+        !make_map(&w.b[i], b[i], b_inner ? z.depth : z.cols, b_inner ? z.cols : z.depth, b_inner ? Box::kInnerK : Box::kOwn, h.bf16))
       return cudaErrorInvalidValue;
   w.f.out0 = g.out0;
   w.f.out1 = g.out1;
   w.f.out2 = g.out2;
   w.f.ldo = g.ldo;
-  w.f.wide = g.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out0) | reinterpret_cast<uintptr_t>(g.out1)) % 16 == 0;
+  // h, dg and du have rows of whole groups; the others are a caller's
+  const bool between = g.product == GatedProduct::kUp || g.product == GatedProduct::kGate;
+  const int64_t ldo = between ? gated_pitch(h.hidden) : g.ldo;
+  w.f.wide = ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out0) | reinterpret_cast<uintptr_t>(g.out1) | reinterpret_cast<uintptr_t>(g.out2)) % 16 == 0;
+  if (between && !w.f.wide) return cudaErrorInvalidValue;
+  void* const outs[3] = {g.out0, g.out1, g.out2};
+  for (int i = 0; i < 3; ++i)
+    if (w.f.wide && outs[i] != nullptr && !make_map(&w.out[i], {outs[i], ldo}, between ? ldo : z.cols, z.rows, Box::kResult, h.bf16)) return cudaErrorInvalidValue;
   w.f.bf16 = h.bf16;
-  w.f.silu = h.activation == GatedActivation::kSilu;
+  const double log2e = 1.4426950408889634, gelu = 1.5957691216057308;  // 2 sqrt(2 / pi)
+  w.f.curve = h.activation == GatedActivation::kSilu ? Curve{static_cast<float>(-log2e), 0.f}
+                                                     : Curve{static_cast<float>(-log2e * gelu), static_cast<float>(-log2e * gelu * 0.044715)};
   w.f.kept = static_cast<char*>(g.kept);
   w.f.rows = z.rows;
   w.f.cols = z.cols;

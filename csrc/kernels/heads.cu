@@ -9,6 +9,7 @@
 // rotation moves nothing between lanes and the norm is the only sum over a team.  A team takes several heads of its token, for
 // which the angles stay in registers.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels/elems.cuh"
 #include "kernels/heads_api.h"
@@ -67,39 +68,39 @@ struct Lane {
   }
 };
 
-// First and second members of a lane's pairs.
+// A lane's pairs as they lie in memory: two runs of V numbers.  A run of four or eight is there whole or not at all (run_of).
+template <typename T, int V>
+using RunOf = std::conditional_t<V == 1, T, std::conditional_t<V * sizeof(T) == 8, uint2, uint4>>;
+
 template <typename T, int V, bool kNear>
-__device__ __forceinline__ void load_pairs(const T* row, const Lane<V, kNear>& l, bool on, float (&a)[V], float (&b)[V]) {
-  float x[V], y[V];
-  load_run<T, V>(row + l.at, on ? l.n : 0, true, x);
-  load_run<T, V>(row + l.at2, on ? l.n2 : 0, true, y);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (kNear) {
-      a[i] = 2 * i < V ? x[2 * i < V ? 2 * i : 0] : y[2 * i >= V ? 2 * i - V : 0];
-      b[i] = 2 * i + 1 < V ? x[2 * i + 1 < V ? 2 * i + 1 : 0] : y[2 * i + 1 >= V ? 2 * i + 1 - V : 0];
-    } else {
-      a[i] = x[i];
-      b[i] = y[i];
-    }
+struct Pairs {
+  using Raw = RunOf<T, V>;
+  Raw run[2];
+  __device__ __forceinline__ void load(const T* row, const Lane<V, kNear>& l, bool on) {
+    run[0] = on && l.n > 0 ? *reinterpret_cast<const Raw*>(row + l.at) : Raw{};
+    run[1] = on && l.n2 > 0 ? *reinterpret_cast<const Raw*>(row + l.at2) : Raw{};
   }
-}
-template <typename T, int V, bool kNear>
-__device__ __forceinline__ void store_pairs(T* row, const Lane<V, kNear>& l, bool on, const float (&a)[V], const float (&b)[V]) {
-  float x[V], y[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (kNear) {
-      x[i] = i % 2 ? b[i / 2] : a[i / 2];
-      y[i] = (V + i) % 2 ? b[(V + i) / 2] : a[(V + i) / 2];
-    } else {
-      x[i] = a[i];
-      y[i] = b[i];
-    }
+  __device__ __forceinline__ void store(T* row, const Lane<V, kNear>& l, bool on) const {
+    if (on && l.n > 0) *reinterpret_cast<Raw*>(row + l.at) = run[0];
+    if (on && l.n2 > 0) *reinterpret_cast<Raw*>(row + l.at2) = run[1];
   }
-  store_run<T, V>(row + l.at, on ? l.n : 0, true, x);
-  store_run<T, V>(row + l.at2, on ? l.n2 : 0, true, y);
-}
+  // the members of pair i
+  __device__ __forceinline__ float a(int i) const { return kNear ? get(2 * i) : get(i); }
+  __device__ __forceinline__ float b(int i) const { return kNear ? get(2 * i + 1) : get(V + i); }
+  __device__ __forceinline__ void set(const float (&a)[V], const float (&b)[V]) {
+    float v[2 * V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[kNear ? 2 * i : i] = a[i];
+      v[kNear ? 2 * i + 1 : V + i] = b[i];
+    }
+    run[0] = pack_run<T, V, Raw>(v);
+    run[1] = pack_run<T, V, Raw>(v + V);
+  }
+
+ private:
+  __device__ __forceinline__ float get(int i) const { return Traits<T>::load(reinterpret_cast<const T*>(&run[i / V])[i % V]); }
+};
 
 template <typename T, int V, bool kNear>
 __device__ __forceinline__ void load_weight(const void* w, bool f32, const Lane<V, kNear>& l, float (&a)[V], float (&b)[V]) {
@@ -173,9 +174,10 @@ __device__ __forceinline__ const T* token_rows(const HeadRows& r, const Token& k
   return static_cast<const T*>(r.data) + k.b * r.batch + k.t * r.token;
 }
 
-// kRows rows of each team are in flight before the first is used.
+// kRows rows of each team are in flight before the first is used: the first of a token before its angles are asked for, the next
+// ones while the results leave.
 template <typename T, int V, int K, bool kNear, int kRows>
-__global__ void __launch_bounds__(kThreads) heads_forward_kernel(const HeadsShape s, const Plan w) {
+__global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 3 : 1) heads_forward_kernel(const HeadsShape s, const Plan w) {
   const Walk walk(w);
   const Side& d = w.side[walk.side];
   const int lane = walk.lane;
@@ -186,6 +188,17 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const HeadsShap
   const float inv = 1.f / static_cast<float>(s.dim);
   for (int64_t base = walk.base; base < d.units; base += walk.step) {
     const Token token(d, s, base + walk.mine);
+    const T* from = token_rows<T>(d.x, token);
+    Pairs<T, V, kNear> x[kRows][K];
+    auto load = [&](int h0) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int h = h0 + j * d.parts + token.first;
+#pragma unroll
+        for (int k = 0; k < K; ++k) x[j][k].load(from + h * d.x.head, Lane<V, kNear>(s, lane, k * w.team), token.there && h < d.heads);
+      }
+    };
+    load(0);
     const int64_t position = position_of(s, token.b, token.t);
     float c[K][V], sn[K][V];
 #pragma unroll
@@ -193,17 +206,9 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const HeadsShap
       const Lane<V, kNear> l(s, lane, k * w.team);
       load_angles<V>(s, position, l.pair, l.rotated, c[k], sn[k]);
     }
-    const T* from = token_rows<T>(d.x, token);
     T* to = reinterpret_cast<T*>(d.out) + token.at * d.out_token;
     for (int h0 = 0; h0 < d.heads; h0 += kRows * d.parts) {
-      float x[kRows][K][2][V];
-#pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int h = h0 + j * d.parts + token.first;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          load_pairs<T, V, kNear>(from + h * d.x.head, Lane<V, kNear>(s, lane, k * w.team), token.there && h < d.heads, x[j][k][0], x[j][k][1]);
-      }
+      if (h0 > 0) load(h0);
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
         const int h = h0 + j * d.parts + token.first;
@@ -211,19 +216,28 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const HeadsShap
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int i = 0; i < V; ++i) sum += x[j][k][0][i] * x[j][k][0][i] + x[j][k][1][i] * x[j][k][1][i];
+          for (int i = 0; i < V; ++i) sum += x[j][k].a(i) * x[j][k].a(i) + x[j][k].b(i) * x[j][k].b(i);
         const float r = rsqrtf(team_sum(sum, w.team) * inv + s.eps);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const Lane<V, kNear> l(s, lane, k * w.team);
-          float ya[V], yb[V];
+          float na[V], nb[V];
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float na = x[j][k][0][i] * r * weight[k][0][i], nb = x[j][k][1][i] * r * weight[k][1][i];
-            ya[i] = l.rotated ? na * c[k][i] - nb * sn[k][i] : na;
-            yb[i] = l.rotated ? nb * c[k][i] + na * sn[k][i] : nb;
+            na[i] = x[j][k].a(i) * r * weight[k][0][i];
+            nb[i] = x[j][k].b(i) * r * weight[k][1][i];
           }
-          store_pairs<T, V, kNear>(to + static_cast<int64_t>(h) * s.dim, l, token.there && h < d.heads, ya, yb);
+          if (l.rotated) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float a = na[i];
+              na[i] = a * c[k][i] - nb[i] * sn[k][i];
+              nb[i] = nb[i] * c[k][i] + a * sn[k][i];
+            }
+          }
+          Pairs<T, V, kNear> y;
+          y.set(na, nb);
+          y.store(to + static_cast<int64_t>(h) * s.dim, l, token.there && h < d.heads);
         }
       }
     }
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(kThreads) heads_forward_kernel(const HeadsShap
 // The gradients of the weights: each lane adds up its columns over all of its rows, the block's teams are joined in shared
 // memory, and heads_weights_kernel adds the blocks, all in a fixed order.
 template <typename T, int V, int K, bool kNear, int kRows>
-__global__ void __launch_bounds__(kThreads) heads_backward_kernel(const HeadsShape s, const Plan w, float* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 2 : 1) heads_backward_kernel(const HeadsShape s, const Plan w, float* __restrict__ partial) {
   const Walk walk(w);
   const Side& d = w.side[walk.side];
   const int lane = walk.lane;
@@ -246,9 +260,9 @@ __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const HeadsSha
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const Lane<V, kNear> l(s, lane, k * w.team);
-          float a[V], b[V];
-          load_pairs<T, V, kNear>(from + h * d.x.head, l, true, a, b);
-          store_pairs<T, V, kNear>(to + static_cast<int64_t>(h) * s.dim, l, true, a, b);
+          Pairs<T, V, kNear> x;
+          x.load(from + h * d.x.head, l, true);
+          x.store(to + static_cast<int64_t>(h) * s.dim, l, true);
         }
     }
     return;
@@ -263,6 +277,22 @@ __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const HeadsSha
   const float inv = 1.f / static_cast<float>(s.dim);
   for (int64_t base = walk.base; base < d.units; base += walk.step) {
     const Token token(d, s, base + walk.mine);
+    const T *from = token_rows<T>(d.x, token), *gfrom = token_rows<T>(d.dy, token);
+    Pairs<T, V, kNear> x[kRows][K], g[kRows][K];
+    auto load = [&](int h0) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int h = h0 + j * d.parts + token.first;
+        const bool on = token.there && h < d.heads;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const Lane<V, kNear> l(s, lane, k * w.team);
+          x[j][k].load(from + h * d.x.head, l, on);
+          g[j][k].load(gfrom + h * d.dy.head, l, on);
+        }
+      }
+    };
+    load(0);
     const int64_t position = position_of(s, token.b, token.t);
     float c[K][V], sn[K][V];
 #pragma unroll
@@ -270,37 +300,35 @@ __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const HeadsSha
       const Lane<V, kNear> l(s, lane, k * w.team);
       load_angles<V>(s, position, l.pair, l.rotated, c[k], sn[k]);
     }
-    const T *from = token_rows<T>(d.x, token), *gfrom = token_rows<T>(d.dy, token);
     T* to = reinterpret_cast<T*>(d.out) + token.at * d.out_token;
     for (int h0 = 0; h0 < d.heads; h0 += kRows * d.parts) {
-      float x[kRows][K][2][V], g[kRows][K][2][V];
+      if (h0 > 0) load(h0);
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
         const int h = h0 + j * d.parts + token.first;
         const bool on = token.there && h < d.heads;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const Lane<V, kNear> l(s, lane, k * w.team);
-          load_pairs<T, V, kNear>(from + h * d.x.head, l, on, x[j][k][0], x[j][k][1]);
-          load_pairs<T, V, kNear>(gfrom + h * d.dy.head, l, on, g[j][k][0], g[j][k][1]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int h = h0 + j * d.parts + token.first;
-        const bool on = token.there && h < d.heads;
-        float sum = 0.f, dot = 0.f;
+        float sum = 0.f, dot = 0.f, na[K][V], nb[K][V];  // the gradient rotated back
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const Lane<V, kNear> l(s, lane, k * w.team);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float xa = x[j][k][0][i], xb = x[j][k][1][i], ga = g[j][k][0][i], gb = g[j][k][1][i];
-            const float na = l.rotated ? ga * c[k][i] + gb * sn[k][i] : ga, nb = l.rotated ? gb * c[k][i] - ga * sn[k][i] : gb;
-            g[j][k][0][i] = na;
-            g[j][k][1][i] = nb;
+            na[k][i] = g[j][k].a(i);
+            nb[k][i] = g[j][k].b(i);
+          }
+          if (l.rotated) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float a = na[k][i];
+              na[k][i] = a * c[k][i] + nb[k][i] * sn[k][i];
+              nb[k][i] = nb[k][i] * c[k][i] - a * sn[k][i];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float xa = x[j][k].a(i), xb = x[j][k].b(i);
             sum += xa * xa + xb * xb;
-            dot += na * weight[k][0][i] * xa + nb * weight[k][1][i] * xb;
+            dot += na[k][i] * weight[k][0][i] * xa + nb[k][i] * weight[k][1][i] * xb;
           }
         }
         const float r = rsqrtf(team_sum(sum, w.team) * inv + s.eps);
@@ -311,15 +339,17 @@ __global__ void __launch_bounds__(kThreads) heads_backward_kernel(const HeadsSha
           float ya[V], yb[V];
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float ua = x[j][k][0][i] * r, ub = x[j][k][1][i] * r, na = g[j][k][0][i], nb = g[j][k][1][i];
-            ya[i] = r * (na * weight[k][0][i] - ua * (r * mean));
-            yb[i] = r * (nb * weight[k][1][i] - ub * (r * mean));
+            const float ua = x[j][k].a(i) * r, ub = x[j][k].b(i) * r;
+            ya[i] = r * (na[k][i] * weight[k][0][i] - ua * (r * mean));
+            yb[i] = r * (nb[k][i] * weight[k][1][i] - ub * (r * mean));
             if (on) {  // an idle team has rotated a row of zeros by a token's angles, which may be NaN
-              grad[k][0][i] += na * ua;
-              grad[k][1][i] += nb * ub;
+              grad[k][0][i] += na[k][i] * ua;
+              grad[k][1][i] += nb[k][i] * ub;
             }
           }
-          store_pairs<T, V, kNear>(to + static_cast<int64_t>(h) * s.dim, l, on, ya, yb);
+          Pairs<T, V, kNear> y;
+          y.set(ya, yb);
+          y.store(to + static_cast<int64_t>(h) * s.dim, l, on);
         }
       }
     }
@@ -391,18 +421,18 @@ bool fits(const HeadRows& r, const HeadsShape& s, int heads, size_t bytes) {
          (s.tokens <= 1 || r.token * e % bytes == 0) && (heads <= 1 || r.head * e % bytes == 0);
 }
 int pairs_of(const HeadsShape& s) { return s.rotary / 2 + (s.dim - s.rotary + 1) / 2; }
-// Pairs a lane: 8 or 4 where runs of so many divide both the rotated pairs and the others and every row is aligned to them (16 or,
-// 4 of 16 bits, 8 bytes), else one.
+// Pairs a lane: 8, of fp32 4, where runs of so many divide both the rotated pairs and the others and every row is aligned to them
+// (16 bytes); 4 of 16-bit types (8 bytes); else one.
 int run_of(const HeadsShape& s, const Plan& w) {
-  for (const int v : {8, 4}) {
-    const size_t e = size_of(s.type), bytes = std::min<size_t>(16, v * e);
-    bool ok = s.rotary / 2 % v == 0 && (s.dim - s.rotary) % (2 * v) == 0 && pairs_of(s) <= 32 * v && reinterpret_cast<uintptr_t>(s.table) % 16 == 0;
+  const size_t e = size_of(s.type);
+  for (int run = e == 2 ? 8 : 4; run >= 4; run /= 2) {
+    const size_t bytes = run * e;
+    bool ok = s.rotary / 2 % run == 0 && (s.dim - s.rotary) % (2 * run) == 0 && reinterpret_cast<uintptr_t>(s.table) % 16 == 0;
     for (int i = 0; ok && i < w.sides; ++i) {
       const Side& d = w.side[i];
-      ok = fits(d.x, s, d.heads, bytes) && fits(d.dy, s, d.heads, bytes) && reinterpret_cast<uintptr_t>(d.out) % bytes == 0 &&
-           d.out_token * e % bytes == 0;
+      ok = fits(d.x, s, d.heads, bytes) && fits(d.dy, s, d.heads, bytes) && reinterpret_cast<uintptr_t>(d.out) % bytes == 0 && d.out_token * e % bytes == 0;
     }
-    if (ok) return v;
+    if (ok) return run;
   }
   return 1;
 }
@@ -433,7 +463,7 @@ constexpr int kForwardBlocks = 16, kBackwardBlocks = 6;  // an SM, at most
 template <typename T, int V, int K>
 cudaError_t forward_run(const HeadsShape& h, Plan& w, cudaStream_t s) {
   cut(w, h, V, K, kForwardBlocks);
-  constexpr int kRows = V == 8 ? 2 : 1;
+  constexpr int kRows = V == 8 ? 2 : V == 4 && K == 1 ? 4 : 1;
   note_launch();
   if (h.interleaved) heads_forward_kernel<T, V, K, true, kRows><<<w.blocks, kThreads, 0, s>>>(h, w);
   else heads_forward_kernel<T, V, K, false, kRows><<<w.blocks, kThreads, 0, s>>>(h, w);
@@ -441,27 +471,28 @@ cudaError_t forward_run(const HeadsShape& h, Plan& w, cudaStream_t s) {
 }
 template <typename T>
 cudaError_t forward_type(const HeadsShape& h, Plan& w, cudaStream_t s) {
-  switch (run_of(h, w)) {
-    case 8: return forward_run<T, 8, 1>(h, w, s);
-    case 4: return forward_run<T, 4, 1>(h, w, s);
-    default: return pairs_of(h) <= 64 ? forward_run<T, 1, 2>(h, w, s) : forward_run<T, 1, 8>(h, w, s);
-  }
+  const int run = run_of(h, w);
+  if constexpr (sizeof(T) == 2)
+    if (run == 8) return forward_run<T, 8, 1>(h, w, s);
+  if (run == 4) return pairs_of(h) <= 128 ? forward_run<T, 4, 1>(h, w, s) : forward_run<T, 4, 2>(h, w, s);
+  return pairs_of(h) <= 64 ? forward_run<T, 1, 2>(h, w, s) : forward_run<T, 1, 8>(h, w, s);
 }
 template <typename T, int V, int K>
 cudaError_t backward_run(const HeadsShape& h, Plan& w, float* partial, cudaStream_t s) {
   cut(w, h, V, K, kBackwardBlocks);
+  constexpr int kRows = V == 4 && K == 1 ? 2 : 1;
   note_launch();
-  if (h.interleaved) heads_backward_kernel<T, V, K, true, 1><<<w.blocks, kThreads, 0, s>>>(h, w, partial);
-  else heads_backward_kernel<T, V, K, false, 1><<<w.blocks, kThreads, 0, s>>>(h, w, partial);
+  if (h.interleaved) heads_backward_kernel<T, V, K, true, kRows><<<w.blocks, kThreads, 0, s>>>(h, w, partial);
+  else heads_backward_kernel<T, V, K, false, kRows><<<w.blocks, kThreads, 0, s>>>(h, w, partial);
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t backward_type(const HeadsShape& h, Plan& w, float* partial, cudaStream_t s) {
-  switch (run_of(h, w)) {
-    case 8: return backward_run<T, 8, 1>(h, w, partial, s);
-    case 4: return backward_run<T, 4, 1>(h, w, partial, s);
-    default: return pairs_of(h) <= 64 ? backward_run<T, 1, 2>(h, w, partial, s) : backward_run<T, 1, 8>(h, w, partial, s);
-  }
+  const int run = run_of(h, w);
+  if constexpr (sizeof(T) == 2)
+    if (run == 8) return backward_run<T, 8, 1>(h, w, partial, s);
+  if (run == 4) return pairs_of(h) <= 128 ? backward_run<T, 4, 1>(h, w, partial, s) : backward_run<T, 4, 2>(h, w, partial, s);
+  return pairs_of(h) <= 64 ? backward_run<T, 1, 2>(h, w, partial, s) : backward_run<T, 1, 8>(h, w, partial, s);
 }
 
 bool shape_ok(const HeadsShape& s) {

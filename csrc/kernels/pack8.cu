@@ -12,110 +12,144 @@ namespace mccl {
 namespace kern {
 namespace {
 
-constexpr int kThreads = 256, kLanes = 8;       // threads of a block, and of a group: eight numbers each
+constexpr int kThreads = 256, kLanes = 4;       // threads of a block, and of a group: two runs of eight numbers each, 32 apart
 constexpr int kUnits = kThreads / kLanes;       // groups a block has in hand at a time
+constexpr int kDeep = 2;                        // groups of a thread in flight
+constexpr int kTurn = kUnits * kDeep;           // groups of a block's turn
 
-// Where group `at` of the whole lies.
+// Where a group lies.  Rows that are whole groups, one behind the other, are one row.
+struct Steps {
+  int64_t all, groups;    // of the whole, of a row
+};
 struct Place {
   int64_t row;
-  int group;
+  int64_t col;
+  __device__ __forceinline__ Place(const Steps& t, int64_t unit, bool linear) {
+    if (linear) {
+      row = 0;
+      col = unit * kGroup8;
+    } else {
+      row = t.all <= 0xFFFFFFFFll ? static_cast<uint32_t>(unit) / static_cast<uint32_t>(t.groups) : unit / t.groups;
+      col = (unit - row * t.groups) * kGroup8;
+    }
+  }
 };
-__device__ __forceinline__ Place place_of(int64_t at, int64_t groups, bool few) {
-  const int64_t row = few ? static_cast<int64_t>(static_cast<uint32_t>(at) / static_cast<uint32_t>(groups)) : at / groups;
-  return {row, static_cast<int>(at - row * groups)};
+__device__ __forceinline__ int present(int64_t cols, int64_t col, bool there) {
+  return there ? static_cast<int>(min(max(cols - col, static_cast<int64_t>(0)), static_cast<int64_t>(8))) : 0;
 }
 
-// Bound by memory: one pass, 2 (4) bytes read and 1 + 1/16 written for each number.  Eight lanes share a group, so a warp
-// reads 512 (1024) bytes in a run; kDeep groups are in flight for each of them before the first is looked at.
-template <typename T, int kDeep>
-__global__ void __launch_bounds__(kThreads) pack8_kernel(const T* __restrict__ x, int64_t ld, bool vec, const Packed8Rows p) {
-  const int64_t groups = (p.cols + kGroup8 - 1) / kGroup8, all = p.rows * groups;
-  const bool few = all <= 0xFFFFFFFFll;
+// Bound by memory: one pass, 2 (4) bytes read and 1 + 1/16 written for each number.  Four lanes share a group, so that few
+// instructions are spent on what a group needs once; kDeep groups of each are in flight before the first is looked at.
+template <typename T, bool kLinear>
+__global__ void __launch_bounds__(kThreads, 4) pack8_kernel(const T* __restrict__ x, int64_t ld, bool vec, const Packed8Rows p, const Steps t) {
   const int sub = threadIdx.x % kLanes;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kUnits * kDeep); base < all;
-       base += static_cast<int64_t>(gridDim.x) * (kUnits * kDeep)) {
-    const int64_t first = base + threadIdx.x / kLanes;
-    float v[kDeep][8];
-    Place at[kDeep];
-    int n[kDeep];
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTurn; base < t.all; base += static_cast<int64_t>(gridDim.x) * kTurn) {
+    const int64_t unit = base + threadIdx.x / kLanes;
+    float v[kDeep][2][8];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      const int64_t u = first + d * kUnits;
-      at[d] = place_of(u < all ? u : 0, groups, few);
-      const int64_t left = p.cols - at[d].group * static_cast<int64_t>(kGroup8) - sub * 8;
-      n[d] = u < all ? static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(8))) : 0;
-      load_run<T, 8>(x + at[d].row * ld + at[d].group * static_cast<int64_t>(kGroup8) + sub * 8, n[d], vec, v[d]);
+      const int64_t u = unit + d * kUnits;
+      const Place at(t, u < t.all ? u : 0, kLinear);
+      const int64_t col = at.col + sub * 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const T* from = x + at.row * ld + col + 32 * h;
+        load_run<T, 8>(from, kLinear ? (u < t.all ? 8 : 0) : present(p.cols, col + 32 * h, u < t.all), kLinear || vec, v[d][h]);
+      }
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      float most = 0.f;
+      uint32_t bits = 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) most = most8(most, v[d][i]);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int m = kLanes / 2; m > 0; m /= 2) most = most8(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
-      const Scale8 s = scale8(most);
-      if (first + d * kUnits >= all) continue;
-      const int64_t col = at[d].group * static_cast<int64_t>(kGroup8) + sub * 8;
-      if (col < p.pitch)
-        *reinterpret_cast<uint2*>(p.codes + at[d].row * p.pitch + col) =
-            make_uint2(codes8(v[d][0], v[d][1], v[d][2], v[d][3], s.inverse), codes8(v[d][4], v[d][5], v[d][6], v[d][7], s.inverse));
-      if (sub == 0) p.scales[at[d].row * groups + at[d].group] = s.scale;
+        for (int i = 0; i < 8; ++i) bits = most8(bits, v[d][h][i]);
+#pragma unroll
+      for (int m = kLanes / 2; m > 0; m /= 2) bits = max(bits, __shfl_xor_sync(0xFFFFFFFFu, bits, m));
+      // scale8, its two quotients in two lanes
+      const float most = __uint_as_float(bits);
+      const bool finite = most < INFINITY, kept = finite && most >= kTiny8;
+      const float quotient = __fdiv_rn(sub == 0 ? most : 127.f, sub == 0 ? 127.f : most);
+      const float shared = __shfl_sync(0xFFFFFFFFu, quotient, 1, kLanes), inverse = kept ? shared : 0.f;
+      const int64_t u = unit + d * kUnits;
+      if (u >= t.all) continue;
+      const Place at(t, u, kLinear);
+      const int64_t col = at.col + sub * 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (kLinear || col + 32 * h < p.pitch)
+          *reinterpret_cast<uint2*>(p.codes + at.row * p.pitch + col + 32 * h) =
+              make_uint2(codes8(v[d][h][0], v[d][h][1], v[d][h][2], v[d][h][3], inverse), codes8(v[d][h][4], v[d][h][5], v[d][h][6], v[d][h][7], inverse));
+      if (sub == 0) p.scales[u] = kept ? quotient : finite ? 0.f : NAN;
     }
   }
 }
 
-template <typename T, int kDeep>
-__global__ void __launch_bounds__(kThreads) unpack8_kernel(const Packed8Rows p, T* __restrict__ x, int64_t ld, bool vec) {
-  const int64_t groups = (p.cols + kGroup8 - 1) / kGroup8, all = p.rows * groups;
-  const bool few = all <= 0xFFFFFFFFll;
+template <typename T, bool kLinear>
+__global__ void __launch_bounds__(kThreads, 4) unpack8_kernel(const Packed8Rows p, T* __restrict__ x, int64_t ld, bool vec, const Steps t) {
   const int sub = threadIdx.x % kLanes;
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * (kUnits * kDeep) + threadIdx.x / kLanes; first < all;
-       first += static_cast<int64_t>(gridDim.x) * (kUnits * kDeep)) {
-    uint2 word[kDeep];
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kTurn + threadIdx.x / kLanes; unit < t.all; unit += static_cast<int64_t>(gridDim.x) * kTurn) {
+    uint2 word[kDeep][2];
     float scale[kDeep];
-    T* to[kDeep];
-    int n[kDeep];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      const int64_t u = first + d * kUnits;
-      const Place at = place_of(u < all ? u : 0, groups, few);
-      const int64_t col = at.group * static_cast<int64_t>(kGroup8) + sub * 8, left = p.cols - col;
-      n[d] = u < all ? static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(8))) : 0;
-      word[d] = n[d] > 0 ? __ldcs(reinterpret_cast<const uint2*>(p.codes + at.row * p.pitch + col)) : make_uint2(0u, 0u);
-      scale[d] = n[d] > 0 ? p.scales[at.row * groups + at.group] : 0.f;
-      to[d] = x + at.row * ld + col;
+      const int64_t u = unit + d * kUnits;
+      const bool there = u < t.all;
+      const Place at(t, there ? u : 0, kLinear);
+      const int64_t col = at.col + sub * 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        word[d][h] = there && (kLinear || col + 32 * h < p.cols) ? __ldcs(reinterpret_cast<const uint2*>(p.codes + at.row * p.pitch + col + 32 * h))
+                                                                 : make_uint2(0u, 0u);
+      scale[d] = there ? p.scales[u] : 0.f;
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      float v[8];
+      const int64_t u = unit + d * kUnits;
+      const Place at(t, u < t.all ? u : 0, kLinear);
+      const int64_t col = at.col + sub * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = value8(i < 4 ? word[d].x : word[d].y, i & 3, scale[d]);
-      store_run<T, 8>(to[d], n[d], vec, v);
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = value8(i < 4 ? word[d][h].x : word[d][h].y, i & 3, scale[d]);
+        store_run<T, 8>(x + at.row * ld + col + 32 * h, kLinear ? (u < t.all ? 8 : 0) : present(p.cols, col + 32 * h, u < t.all), kLinear || vec, v);
+      }
     }
   }
 }
 
 constexpr int kSms = 148;
-int blocks_for(const Packed8Rows& p, int deep) {
-  const int64_t all = p.rows * pack8_groups(p.cols), per = static_cast<int64_t>(kUnits) * deep;
-  return static_cast<int>(std::min<int64_t>((all + per - 1) / per, 8 * kSms));
-}
-bool wide(const void* p, int64_t ld, size_t size) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * static_cast<int64_t>(size) % 16 == 0;
+struct Shape {
+  int blocks;
+  bool vec, linear;
+  Steps t;
+};
+// One row (`linear`) where rows are whole groups that follow each other, aligned: no division, no ends inside of a group.
+Shape shape_of(const Packed8Rows& p, const void* x, int64_t ld, size_t size) {
+  Shape s{};
+  s.vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * static_cast<int64_t>(size) % 16 == 0;
+  s.linear = s.vec && p.cols % kGroup8 == 0 && p.pitch == p.cols && (ld == p.cols || p.rows == 1);
+  s.t.groups = pack8_groups(p.cols);
+  s.t.all = p.rows * s.t.groups;
+  s.blocks = static_cast<int>(std::min<int64_t>((s.t.all + kTurn - 1) / kTurn, 32 * kSms));
+  return s;
 }
 
 template <typename T>
 cudaError_t pack(const void* x, int64_t ld, const Packed8Rows& p, cudaStream_t s) {
-  constexpr int kDeep = 4;
+  const Shape h = shape_of(p, x, ld, sizeof(T));
   note_launch();
-  pack8_kernel<T, kDeep><<<blocks_for(p, kDeep), kThreads, 0, s>>>(static_cast<const T*>(x), ld, wide(x, ld, sizeof(T)), p);
+  if (h.linear) pack8_kernel<T, true><<<h.blocks, kThreads, 0, s>>>(static_cast<const T*>(x), ld, h.vec, p, h.t);
+  else pack8_kernel<T, false><<<h.blocks, kThreads, 0, s>>>(static_cast<const T*>(x), ld, h.vec, p, h.t);
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t unpack(const Packed8Rows& p, void* x, int64_t ld, cudaStream_t s) {
-  constexpr int kDeep = 4;
+  const Shape h = shape_of(p, x, ld, sizeof(T));
   note_launch();
-  unpack8_kernel<T, kDeep><<<blocks_for(p, kDeep), kThreads, 0, s>>>(p, static_cast<T*>(x), ld, wide(x, ld, sizeof(T)));
+  if (h.linear) unpack8_kernel<T, true><<<h.blocks, kThreads, 0, s>>>(p, static_cast<T*>(x), ld, h.vec, h.t);
+  else unpack8_kernel<T, false><<<h.blocks, kThreads, 0, s>>>(p, static_cast<T*>(x), ld, h.vec, h.t);
   return cudaGetLastError();
 }
 
