@@ -53,6 +53,20 @@ struct GatedArgs {
 int64_t gated_partial_bytes(GatedProduct p, const GatedShape& s);
 cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s);
 
+// A whole forward pass of few rows, two launches that read the weights at the rate of memory (kernels/gated_few.cu).  Rows of any
+// alignment.  `h`: scratch of 2 x tokens x gated_pitch(hidden) 16-bit numbers.
+constexpr int64_t kFewTokens = 32;
+// Whether it is faster than the tiles: from 17 tokens on only where the block is narrow (32 tokens of 1024 x 2816 18.3 and 28 us, of
+// 2048 x 5632 40 and 37).
+inline bool gated_is_few(const GatedShape& s) { return s.tokens <= 16 || (s.tokens <= kFewTokens && s.width * s.hidden <= (8 << 20)); }
+struct GatedFew {
+  GatedShape shape;
+  GatedOperand x, w_gate, w_up, w_down;
+  void* h;
+  void* y;   // rows of `width`
+};
+cudaError_t launch_gated_few(const GatedFew& g, cudaStream_t s);
+
 // The same in fp32, between products of their own (kernels/gate_f32.cu): h of n numbers g and u; with dh, their gradients too.
 cudaError_t launch_gate_f32(const float* g, const float* u, float* h, int64_t n, GatedActivation act, cudaStream_t s);
 cudaError_t launch_gate_f32_backward(const float* g, const float* u, const float* dh, float* dg, float* du, int64_t n, GatedActivation act,

@@ -1,0 +1,213 @@
+// Gated feed-forward block for few rows, such as one token of each of a few sequences (sm_100a).
+//
+// Bound by the weights' way from memory, 6 bytes of them for width x hidden numbers.  A block has 8 rows of each of the two
+// projections (of the projection back 8), its warps share the reduction; a lane reads 8 numbers of a weight row and 8 of a token's
+// and these are what it gives to the matrix instructions: which of the 32 numbers of a step is called k = 0 does not matter as long as
+// both operands agree, so nothing is rearranged.  The products are a few instructions a kilobyte; with multiplications and additions
+// instead 16 tokens of 1024 x 2816 took 78 us (the tokens' numbers came from the cache for every row), and the tiles of 256 rows of
+// gated.cu take 28 for any number of tokens up to 64.  h is the sum of two 16-bit numbers here, as good as in 32 bits.
+// us (B200, weights of six blocks in turn), 1, 8, 16, 32 tokens: 1024 x 2816 8.3, 9.4, 13.4, 18.3; 2048 x 5632 18.2 (69 MB: 3.8 TB/s),
+// 20.6, 31.6, 40.0.  A run of a block's rows ahead of the products, 4 or 16 warps a block, more of the row in flight: all slower.
+#include <type_traits>
+
+#include "kernels/elems.cuh"
+#include "kernels/gated_api.h"
+#include "kernels/launch_count.h"
+
+namespace mccl {
+namespace kern {
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32, kRows = 8, kStep = 32;  // k of a step of one warp
+
+struct Few {
+  const void* x[2];    // tokens; h as its upper and lower part
+  const void* w[2];
+  void* out[2];
+  int64_t ldx, ldw[2], ldo;
+  int64_t rows, depth; // of the weights
+  int tokens;
+  float c0, c1;        // the curve, see gated.cu
+};
+
+__device__ __forceinline__ float gate(float z, float c0, float c1) {
+  return 1.f / (1.f + exp2f(z * fmaf(c1, fminf(z * z, 1e30f), c0)));
+}
+template <typename T>
+__device__ __forceinline__ void multiply(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 numbers of a row from column `at` of `depth`; zeros beyond it.  Aligned rows are whole runs of 8, and no branch stands between
+// one load and the next.
+template <bool kVec, typename T>
+__device__ __forceinline__ uint4 eight(const T* row, int64_t at, int64_t depth, bool there) {
+  if constexpr (kVec) {
+    const bool in = there && at < depth;
+    const uint4 v = *reinterpret_cast<const uint4*>(row + (in ? at : 0));
+    return make_uint4(in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u);
+  }
+  uint32_t v[4] = {0u, 0u, 0u, 0u};
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(row + at);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (there && at + i < depth) v[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// kGroups groups of 8 tokens (the last ones may be none).  kUp: gate and up and what follows them, else one product of h.
+template <typename T, int kGroups, bool kUp, bool kVec>
+__global__ void __launch_bounds__(kThreads, kGroups == 2 ? 3 : 2) few_kernel(const Few w) {
+  constexpr int kX = kUp ? 1 : 2, kW = kUp ? 2 : 1, kAhead = !kUp && kGroups == 1 ? 8 : 4;
+  constexpr int kHeld = kUp ? 4 : 2;  // accumulators of a lane and group that mean something
+  __shared__ float part[kWarps][kGroups][kHeld][32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows;
+  const bool there = first + g < w.rows;
+  const T* weight[kW];
+#pragma unroll
+  for (int i = 0; i < kW; ++i) weight[i] = static_cast<const T*>(w.w[i]) + (there ? first + g : 0) * w.ldw[i];
+  const int64_t begin = warp * kStep + t * 8, step = kWarps * kStep;
+  uint4 run[kAhead][kW];
+  auto load = [&](int64_t at) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int i = 0; i < kW; ++i) run[a][i] = eight<kVec>(weight[i], at + a * step, w.depth, there);
+  };
+  // The second launch is let in behind the first one's wait: whatever wrote the weights is done by then, and their first runs are
+  // asked for before h is there.
+  if constexpr (!kUp) load(begin);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (kUp) load(begin);
+  float sum[kGroups][4];
+#pragma unroll
+  for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[n][i] = 0.f;
+  const T* token[kGroups][kX];  // of tokens that there are not, the first one's
+#pragma unroll
+  for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+    for (int p = 0; p < kX; ++p) token[n][p] = static_cast<const T*>(w.x[p]) + (8 * n + g < w.tokens ? 8 * n + g : 0) * w.ldx;
+  for (int64_t at = begin; at < w.depth + t * 8; at += kAhead * step) {  // alike in a warp's lanes
+    if (at != begin) load(at);
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) {
+      uint4 b[kAhead][kX];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int p = 0; p < kX; ++p) b[a][p] = eight<kVec>(token[n][p], at + a * step, w.depth, true);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int p = 0; p < kX; ++p) {
+          const uint4 a0 = run[a][0], a1 = kUp ? run[a][kW - 1] : make_uint4(0u, 0u, 0u, 0u), y = b[a][p];
+          multiply<T>(sum[n], a0.x, a1.x, a0.y, a1.y, y.x, y.y);
+          multiply<T>(sum[n], a0.z, a1.z, a0.w, a1.w, y.z, y.w);
+        }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) part[warp][n][i][lane] = sum[n][i];
+  __syncthreads();
+  // a lane has rows g (and of the second projection g again), tokens 2 t and 2 t + 1 of a group
+  for (int item = threadIdx.x; item < kGroups * 64; item += kThreads) {
+    const int at = item % 32, i = item / 32 % 2, n = item / 64;
+    const int m = 8 * n + 2 * (at % 4) + i;
+    const int64_t row = first + at / 4;
+    float v[kUp ? 2 : 1];
+#pragma unroll
+    for (int k = 0; k < (kUp ? 2 : 1); ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int p = 0; p < kWarps; ++p) v[k] += part[p][n][2 * k + i][at];
+    }
+    if (m >= w.tokens || row >= w.rows) continue;
+    if constexpr (kUp) {
+      const float h = v[0] * gate(v[0], w.c0, w.c1) * v[1];
+      const T upper = Traits<T>::store(h);
+      const float rest = h - Traits<T>::load(upper);
+      static_cast<T*>(w.out[0])[m * w.ldo + row] = upper;
+      static_cast<T*>(w.out[1])[m * w.ldo + row] = Traits<T>::store(fabsf(rest) < INFINITY ? rest : 0.f);  // (infinity less itself)
+    } else {
+      static_cast<T*>(w.out[0])[m * w.ldo + row] = Traits<T>::store(v[0]);
+    }
+  }
+}
+
+template <typename T, bool kUp, bool kVec>
+cudaError_t run(const Few& w, cudaStream_t s) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((w.rows + kRows - 1) / kRows));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  note_launch();
+  if (w.tokens <= 8) return cudaLaunchKernelEx(&cfg, few_kernel<T, 1, kUp, kVec>, w);
+  if (w.tokens <= 16) return cudaLaunchKernelEx(&cfg, few_kernel<T, 2, kUp, kVec>, w);
+  return cudaLaunchKernelEx(&cfg, few_kernel<T, 4, kUp, kVec>, w);
+}
+bool aligned(const GatedOperand& m, int64_t rows) { return reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && (rows <= 1 || m.ld % 8 == 0); }
+
+template <typename T>
+cudaError_t both(const GatedFew& g, cudaStream_t s) {
+  const GatedShape& h = g.shape;
+  const double log2e = 1.4426950408889634, gelu = 1.5957691216057308;  // 2 sqrt(2 / pi)
+  const int64_t pitch = gated_pitch(h.hidden);
+  T* const parts[2] = {static_cast<T*>(g.h), static_cast<T*>(g.h) + h.tokens * pitch};
+  Few w{};
+  w.c0 = static_cast<float>(h.activation == GatedActivation::kSilu ? -log2e : -log2e * gelu);
+  w.c1 = h.activation == GatedActivation::kSilu ? 0.f : static_cast<float>(-log2e * gelu * 0.044715);
+  w.tokens = static_cast<int>(h.tokens);
+  w.x[0] = g.x.data;
+  w.ldx = g.x.ld;
+  w.w[0] = g.w_gate.data;
+  w.w[1] = g.w_up.data;
+  w.ldw[0] = g.w_gate.ld;
+  w.ldw[1] = g.w_up.ld;
+  w.out[0] = parts[0];
+  w.out[1] = parts[1];
+  w.ldo = pitch;
+  w.rows = h.hidden;
+  w.depth = h.width;
+  const bool whole = h.width % 8 == 0 && aligned(g.x, h.tokens) && aligned(g.w_gate, h.hidden) && aligned(g.w_up, h.hidden);
+  const cudaError_t e = whole ? run<T, true, true>(w, s) : run<T, true, false>(w, s);
+  if (e != cudaSuccess) return e;
+  w.x[0] = parts[0];
+  w.x[1] = parts[1];
+  w.ldx = pitch;
+  w.w[0] = g.w_down.data;
+  w.ldw[0] = g.w_down.ld;
+  w.out[0] = g.y;
+  w.ldo = h.width;
+  w.rows = h.width;
+  w.depth = h.hidden;
+  return h.hidden % 8 == 0 && aligned(g.w_down, h.width) ? run<T, false, true>(w, s) : run<T, false, false>(w, s);
+}
+
+}  // namespace
+
+cudaError_t launch_gated_few(const GatedFew& g, cudaStream_t s) {
+  const GatedShape& h = g.shape;
+  if (h.tokens <= 0 || h.tokens > kFewTokens || h.width <= 0 || h.hidden <= 0 || reinterpret_cast<uintptr_t>(g.h) % 16 != 0) return cudaErrorInvalidValue;
+  if (h.width > 0x7FFFFFFFll || h.hidden > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  return h.bf16 ? both<__nv_bfloat16>(g, s) : both<__half>(g, s);
+}
+
+}  // namespace kern
+}  // namespace mccl

@@ -21,6 +21,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kSms = 148;
+constexpr int kForwardResident = 2, kBackwardResident = 2;  // blocks an SM, for their registers
+constexpr int kCopies = 4;                                   // rows of values in flight
 
 // Queries, keys and (backward, one gradient for all three) values are sides with blocks of their own: a thread then has one
 // weight and one gradient of it in registers (with both it took 223 of them backward, one block an SM).
@@ -30,8 +32,8 @@ struct Side {
   int64_t out_token;      // elements from one token's rows to the next
   const void* weight;
   int heads;
-  int parts;              // teams that share a token's heads
-  int64_t units;          // tokens x parts
+  int parts;              // teams that share a token's heads: 2^parts
+  int64_t units;          // tokens x 2^parts
   int first, blocks;      // of the grid
 };
 struct Plan {
@@ -102,9 +104,22 @@ struct Pairs {
   __device__ __forceinline__ float get(int i) const { return Traits<T>::load(reinterpret_cast<const T*>(&run[i / V])[i % V]); }
 };
 
+// The lane's weights, element by element unless they are fp32 in aligned runs.
 template <typename T, int V, bool kNear>
 __device__ __forceinline__ void load_weight(const void* w, bool f32, const Lane<V, kNear>& l, float (&a)[V], float (&b)[V]) {
-  // (read once by each thread: element by element, whatever their alignment)
+  if constexpr (V > 1) {
+    if (f32 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+      float v[2 * V];
+      load_run<float, V>(static_cast<const float*>(w) + l.at, l.n, l.n > 0, *reinterpret_cast<float(*)[V]>(v));
+      load_run<float, V>(static_cast<const float*>(w) + l.at2, l.n2, l.n2 > 0, *reinterpret_cast<float(*)[V]>(v + V));
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        a[i] = v[kNear ? 2 * i : i];
+        b[i] = v[kNear ? 2 * i + 1 : V + i];
+      }
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int ia = kNear ? l.at + 2 * i : l.at + i, ib = kNear ? ia + 1 : l.at2 + i;
@@ -114,16 +129,17 @@ __device__ __forceinline__ void load_weight(const void* w, bool f32, const Lane<
   }
 }
 
+// Cosines and sines of a lane's pairs, which are rotated.
 template <int V>
-__device__ __forceinline__ void load_angles(const HeadsShape& s, int64_t position, int pair, bool rotated, float (&c)[V], float (&n)[V]) {
+__device__ __forceinline__ void load_angles(const HeadsShape& s, int64_t position, int pair, float (&c)[V], float (&n)[V]) {
   const bool inside = position >= 0 && position < s.table_rows;
   const float* row = s.table + (inside ? position : 0) * s.rotary + pair;
-  load_run<float, V>(row, rotated && inside ? V : 0, true, c);
-  load_run<float, V>(row + s.rotary / 2, rotated && inside ? V : 0, true, n);
+  if (inside) {
+    load_run<float, V>(row, V, true, c);
+    load_run<float, V>(row + s.rotary / 2, V, true, n);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (!rotated) c[i] = 1.f, n[i] = 0.f;
-    else if (!inside) c[i] = n[i] = NAN;
+    for (int i = 0; i < V; ++i) c[i] = n[i] = NAN;
   }
 }
 
@@ -158,14 +174,11 @@ struct Token {
   __device__ __forceinline__ Token(const Side& d, const HeadsShape& s, int64_t unit) {
     there = unit < d.units;
     if (!there) unit = 0;
-    if (d.units <= 0xFFFFFFFFll) {
-      at = static_cast<uint32_t>(unit) / static_cast<uint32_t>(d.parts);
-      b = static_cast<uint32_t>(at) / static_cast<uint32_t>(s.tokens);  // no more tokens than units
-    } else {
-      at = unit / d.parts;
-      b = at / s.tokens;
-    }
-    first = static_cast<int>(unit - at * d.parts);
+    at = unit >> d.parts;
+    first = static_cast<int>(unit) & ((1 << d.parts) - 1);
+    if (s.batches == 1) b = 0;
+    else if (d.units <= 0xFFFFFFFFll) b = static_cast<uint32_t>(at) / static_cast<uint32_t>(s.tokens);  // no more tokens than units
+    else b = at / s.tokens;
     t = at - b * s.tokens;
   }
 };
@@ -175,16 +188,12 @@ __device__ __forceinline__ const T* token_rows(const HeadRows& r, const Token& k
 }
 
 // kRows rows of each team are in flight before the first is used: the first of a token before its angles are asked for, the next
-// ones while the results leave.
+// ones while the results leave.  Weights and angles become one factor for each member of a pair in each result.
 template <typename T, int V, int K, bool kNear, int kRows>
-__global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 3 : 1) heads_forward_kernel(const HeadsShape s, const Plan w) {
+__global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? kForwardResident : 1) heads_forward_kernel(const HeadsShape s, const Plan w) {
   const Walk walk(w);
   const Side& d = w.side[walk.side];
-  const int lane = walk.lane;
-  float weight[K][2][V];
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    load_weight<T>(d.weight, s.weights_f32, Lane<V, kNear>(s, lane, k * w.team), weight[k][0], weight[k][1]);
+  const int lane = walk.lane, step = 1 << d.parts;
   const float inv = 1.f / static_cast<float>(s.dim);
   for (int64_t base = walk.base; base < d.units; base += walk.step) {
     const Token token(d, s, base + walk.mine);
@@ -193,25 +202,36 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 3 : 1) heads_forwa
     auto load = [&](int h0) {
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        const int h = h0 + j * d.parts + token.first;
+        const int h = h0 + j * step + token.first;
 #pragma unroll
         for (int k = 0; k < K; ++k) x[j][k].load(from + h * d.x.head, Lane<V, kNear>(s, lane, k * w.team), token.there && h < d.heads);
       }
     };
     load(0);
     const int64_t position = position_of(s, token.b, token.t);
-    float c[K][V], sn[K][V];
+    float fa[K][2][V], fb[K][2][V];  // of a in a' and b', of b in b' and a'
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const Lane<V, kNear> l(s, lane, k * w.team);
-      load_angles<V>(s, position, l.pair, l.rotated, c[k], sn[k]);
+      load_weight<T>(d.weight, s.weights_f32, l, fa[k][0], fb[k][0]);
+      if (l.rotated) {
+        float c[V], n[V];
+        load_angles<V>(s, position, l.pair, c, n);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          fa[k][1][i] = fa[k][0][i] * n[i];
+          fb[k][1][i] = -fb[k][0][i] * n[i];
+          fa[k][0][i] *= c[i];
+          fb[k][0][i] *= c[i];
+        }
+      }
     }
     T* to = reinterpret_cast<T*>(d.out) + token.at * d.out_token;
-    for (int h0 = 0; h0 < d.heads; h0 += kRows * d.parts) {
+    for (int h0 = 0; h0 < d.heads; h0 += kRows * step) {
       if (h0 > 0) load(h0);
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        const int h = h0 + j * d.parts + token.first;
+        const int h = h0 + j * step + token.first;
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -224,15 +244,12 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 3 : 1) heads_forwa
           float na[V], nb[V];
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            na[i] = x[j][k].a(i) * r * weight[k][0][i];
-            nb[i] = x[j][k].b(i) * r * weight[k][1][i];
-          }
-          if (l.rotated) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float a = na[i];
-              na[i] = a * c[k][i] - nb[i] * sn[k][i];
-              nb[i] = nb[i] * c[k][i] + a * sn[k][i];
+            const float a = x[j][k].a(i) * r, b = x[j][k].b(i) * r;
+            na[i] = a * fa[k][0][i];
+            nb[i] = b * fb[k][0][i];
+            if (l.rotated) {
+              na[i] += b * fb[k][1][i];
+              nb[i] += a * fa[k][1][i];
             }
           }
           Pairs<T, V, kNear> y;
@@ -247,33 +264,36 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 3 : 1) heads_forwa
 // The gradients of the weights: each lane adds up its columns over all of its rows, the block's teams are joined in shared
 // memory, and heads_weights_kernel adds the blocks, all in a fixed order.
 template <typename T, int V, int K, bool kNear, int kRows>
-__global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 2 : 1) heads_backward_kernel(const HeadsShape s, const Plan w, float* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? kBackwardResident : 1) heads_backward_kernel(const HeadsShape s, const Plan w, float* __restrict__ partial) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // heads_weights_kernel, which waits for all of this
   const Walk walk(w);
   const Side& d = w.side[walk.side];
-  const int lane = walk.lane;
+  const int lane = walk.lane, step = 1 << d.parts;
   if (walk.side == 2) {  // values: their gradient goes to its place
     for (int64_t base = walk.base; base < d.units; base += walk.step) {
       const Token token(d, s, base + walk.mine);
       const T* from = token_rows<T>(d.x, token);
       T* to = reinterpret_cast<T*>(d.out) + token.at * d.out_token;
-      for (int h = token.first; h < d.heads && token.there; h += d.parts)
+      for (int h0 = token.first; h0 < d.heads && token.there; h0 += kCopies * step) {
+        Pairs<T, V, kNear> x[kCopies][K];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const Lane<V, kNear> l(s, lane, k * w.team);
-          Pairs<T, V, kNear> x;
-          x.load(from + h * d.x.head, l, true);
-          x.store(to + static_cast<int64_t>(h) * s.dim, l, true);
-        }
+        for (int j = 0; j < kCopies; ++j)
+#pragma unroll
+          for (int k = 0; k < K; ++k) x[j][k].load(from + (h0 + j * step) * d.x.head, Lane<V, kNear>(s, lane, k * w.team), h0 + j * step < d.heads);
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j)
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            x[j][k].store(to + static_cast<int64_t>(h0 + j * step) * s.dim, Lane<V, kNear>(s, lane, k * w.team), h0 + j * step < d.heads);
+      }
     }
     return;
   }
-  float weight[K][2][V], grad[K][2][V];
+  float grad[K][2][V];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    load_weight<T>(d.weight, s.weights_f32, Lane<V, kNear>(s, lane, k * w.team), weight[k][0], weight[k][1]);
+  for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) grad[k][0][i] = grad[k][1][i] = 0.f;
-  }
   const float inv = 1.f / static_cast<float>(s.dim);
   for (int64_t base = walk.base; base < d.units; base += walk.step) {
     const Token token(d, s, base + walk.mine);
@@ -282,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 2 : 1) heads_backw
     auto load = [&](int h0) {
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        const int h = h0 + j * d.parts + token.first;
+        const int h = h0 + j * step + token.first;
         const bool on = token.there && h < d.heads;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -294,18 +314,19 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 2 : 1) heads_backw
     };
     load(0);
     const int64_t position = position_of(s, token.b, token.t);
-    float c[K][V], sn[K][V];
+    float weight[K][2][V], c[K][V], sn[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const Lane<V, kNear> l(s, lane, k * w.team);
-      load_angles<V>(s, position, l.pair, l.rotated, c[k], sn[k]);
+      load_weight<T>(d.weight, s.weights_f32, l, weight[k][0], weight[k][1]);
+      if (l.rotated) load_angles<V>(s, position, l.pair, c[k], sn[k]);
     }
     T* to = reinterpret_cast<T*>(d.out) + token.at * d.out_token;
-    for (int h0 = 0; h0 < d.heads; h0 += kRows * d.parts) {
+    for (int h0 = 0; h0 < d.heads; h0 += kRows * step) {
       if (h0 > 0) load(h0);
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        const int h = h0 + j * d.parts + token.first;
+        const int h = h0 + j * step + token.first;
         const bool on = token.there && h < d.heads;
         float sum = 0.f, dot = 0.f, na[K][V], nb[K][V];  // the gradient rotated back
 #pragma unroll
@@ -313,26 +334,15 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 2 : 1) heads_backw
           const Lane<V, kNear> l(s, lane, k * w.team);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            na[k][i] = g[j][k].a(i);
-            nb[k][i] = g[j][k].b(i);
-          }
-          if (l.rotated) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float a = na[k][i];
-              na[k][i] = a * c[k][i] + nb[k][i] * sn[k][i];
-              nb[k][i] = nb[k][i] * c[k][i] - a * sn[k][i];
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float xa = x[j][k].a(i), xb = x[j][k].b(i);
+            const float ga = g[j][k].a(i), gb = g[j][k].b(i), xa = x[j][k].a(i), xb = x[j][k].b(i);
+            na[k][i] = l.rotated ? ga * c[k][i] + gb * sn[k][i] : ga;
+            nb[k][i] = l.rotated ? gb * c[k][i] - ga * sn[k][i] : gb;
             sum += xa * xa + xb * xb;
-            dot += na[k][i] * weight[k][0][i] * xa + nb[k][i] * weight[k][1][i] * xb;
+            dot += (na[k][i] * weight[k][0][i]) * xa + (nb[k][i] * weight[k][1][i]) * xb;
           }
         }
         const float r = rsqrtf(team_sum(sum, w.team) * inv + s.eps);
-        const float mean = team_sum(dot, w.team) * inv;
+        const float fall = r * r * (team_sum(dot, w.team) * inv);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const Lane<V, kNear> l(s, lane, k * w.team);
@@ -340,12 +350,11 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? 2 : 1) heads_backw
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             const float ua = x[j][k].a(i) * r, ub = x[j][k].b(i) * r;
-            ya[i] = r * (na[k][i] * weight[k][0][i] - ua * (r * mean));
-            yb[i] = r * (nb[k][i] * weight[k][1][i] - ub * (r * mean));
-            if (on) {  // an idle team has rotated a row of zeros by a token's angles, which may be NaN
-              grad[k][0][i] += na[k][i] * ua;
-              grad[k][1][i] += nb[k][i] * ub;
-            }
+            ya[i] = (na[k][i] * weight[k][0][i]) * r - ua * fall;
+            yb[i] = (nb[k][i] * weight[k][1][i]) * r - ub * fall;
+            // (an idle team has rotated a row of zeros by a token's angles, which may be NaN)
+            grad[k][0][i] += on ? na[k][i] * ua : 0.f;
+            grad[k][1][i] += on ? nb[k][i] * ub : 0.f;
           }
           Pairs<T, V, kNear> y;
           y.set(ya, yb);
@@ -437,8 +446,10 @@ int run_of(const HeadsShape& s, const Plan& w) {
   return 1;
 }
 
-// A token's heads are shared by as many teams as a warp has, so that a warp reads its rows in one run; by more where the tokens
-// do not fill the device.
+constexpr int kFull = 512;  // threads of an SM that a launch should at least have
+// A team takes as many of a token's heads as leave the device full of teams: what a token costs by itself, its place and its
+// angles, is then spent once for many rows.  (As many teams to a token as a warp has, two rows each: 19 and 38 instructions a number
+// forward and backward, where the arithmetic is 6 and 12.)
 void cut(Plan& w, const HeadsShape& s, int run, int runs, int blocks_per_sm) {
   const int lanes = (pairs_of(s) + run - 1) / run;
   w.team = 1;
@@ -449,21 +460,31 @@ void cut(Plan& w, const HeadsShape& s, int run, int runs, int blocks_per_sm) {
   w.blocks = 0;
   for (int i = 0; i < w.sides; ++i) {
     Side& d = w.side[i];
-    d.parts = std::min(32 / w.team, d.heads);
-    while (d.parts < d.heads && tokens * d.parts < 2 * kSms * teams) d.parts = std::min(2 * d.parts, d.heads);
-    d.units = tokens * d.parts;
+    d.parts = 0;
+    while ((1 << d.parts) < d.heads && (tokens << d.parts) * w.team < static_cast<int64_t>(kFull) * kSms * d.heads / heads) ++d.parts;
+    d.units = tokens << d.parts;
     const int64_t most = std::max<int64_t>(1, static_cast<int64_t>(blocks_per_sm) * kSms * d.heads / heads);
     d.blocks = static_cast<int>(std::min((d.units + teams - 1) / teams, most));
     d.first = w.blocks;
     w.blocks += d.blocks;
   }
 }
-constexpr int kForwardBlocks = 16, kBackwardBlocks = 6;  // an SM, at most
+// One batch where the next one's tokens follow: no division in the kernels.
+void flatten(HeadsShape& s, Plan& w) {
+  if (s.batches <= 1) return;
+  for (int i = 0; i < w.sides; ++i)
+    for (const HeadRows* r : {&w.side[i].x, &w.side[i].dy})
+      if (r->data != nullptr && r->batch != s.tokens * r->token) return;
+  if (s.positions == nullptr || s.pos_batch != s.tokens * s.pos_token) return;
+  s.tokens *= s.batches;
+  s.batches = 1;
+}
+constexpr int kForwardBlocks = 16, kBackwardBlocks = 12;  // an SM, at most
 
 template <typename T, int V, int K>
 cudaError_t forward_run(const HeadsShape& h, Plan& w, cudaStream_t s) {
   cut(w, h, V, K, kForwardBlocks);
-  constexpr int kRows = V == 8 ? 2 : V == 4 && K == 1 ? 4 : 1;
+  constexpr int kRows = V == 1 || K > 1 ? 1 : 4;
   note_launch();
   if (h.interleaved) heads_forward_kernel<T, V, K, true, kRows><<<w.blocks, kThreads, 0, s>>>(h, w);
   else heads_forward_kernel<T, V, K, false, kRows><<<w.blocks, kThreads, 0, s>>>(h, w);
@@ -480,7 +501,7 @@ cudaError_t forward_type(const HeadsShape& h, Plan& w, cudaStream_t s) {
 template <typename T, int V, int K>
 cudaError_t backward_run(const HeadsShape& h, Plan& w, float* partial, cudaStream_t s) {
   cut(w, h, V, K, kBackwardBlocks);
-  constexpr int kRows = V == 4 && K == 1 ? 2 : 1;
+  constexpr int kRows = V == 1 || K > 1 ? 1 : 2;
   note_launch();
   if (h.interleaved) heads_backward_kernel<T, V, K, true, kRows><<<w.blocks, kThreads, 0, s>>>(h, w, partial);
   else heads_backward_kernel<T, V, K, false, kRows><<<w.blocks, kThreads, 0, s>>>(h, w, partial);
@@ -502,13 +523,14 @@ bool shape_ok(const HeadsShape& s) {
 }  // namespace
 
 cudaError_t launch_heads_forward(const HeadsForward& a, cudaStream_t s) {
-  const HeadsShape& h = a.shape;
+  HeadsShape h = a.shape;
   if (!shape_ok(h)) return cudaErrorInvalidValue;
   if (h.batches * h.tokens == 0) return cudaSuccess;
   Plan w{};
   w.sides = 2;
   w.side[0] = {a.q, {}, static_cast<char*>(a.q_out), static_cast<int64_t>(h.heads) * h.dim, h.q_weight, h.heads};
   w.side[1] = {a.k, {}, static_cast<char*>(a.k_out), static_cast<int64_t>(h.kv_heads) * h.dim, h.k_weight, h.kv_heads};
+  flatten(h, w);
   switch (h.type) {
     case Elem::kF32: return forward_type<float>(h, w, s);
     case Elem::kF16: return forward_type<__half>(h, w, s);
@@ -519,7 +541,7 @@ cudaError_t launch_heads_forward(const HeadsForward& a, cudaStream_t s) {
 int heads_partials() { return kBackwardBlocks * kSms + 2; }
 
 cudaError_t launch_heads_backward(const HeadsBackward& a, cudaStream_t s) {
-  const HeadsShape& h = a.shape;
+  HeadsShape h = a.shape;
   if (!shape_ok(h)) return cudaErrorInvalidValue;
   if (h.batches * h.tokens == 0) return cudaSuccess;
   Plan w{};
@@ -527,6 +549,7 @@ cudaError_t launch_heads_backward(const HeadsBackward& a, cudaStream_t s) {
   w.side[0] = {a.q, a.dq, static_cast<char*>(a.dq_out), a.dq_token, h.q_weight, h.heads};
   w.side[1] = {a.k, a.dk, static_cast<char*>(a.dk_out), a.dk_token, h.k_weight, h.kv_heads};
   if (a.dv_out != nullptr) w.side[2] = {a.dv, {}, static_cast<char*>(a.dv_out), a.dv_token, nullptr, h.kv_heads};
+  flatten(h, w);
   cudaError_t e;
   switch (h.type) {
     case Elem::kF32: e = backward_type<float>(h, w, a.partial, s); break;
@@ -534,10 +557,18 @@ cudaError_t launch_heads_backward(const HeadsBackward& a, cudaStream_t s) {
     default: e = backward_type<__nv_bfloat16>(h, w, a.partial, s);
   }
   if (e != cudaSuccess || a.partial == nullptr) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((h.dim + 31) / 32, 2);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   note_launch();
-  heads_weights_kernel<<<dim3((h.dim + 31) / 32, 2), kThreads, 0, s>>>(a.partial, w.side[0].blocks, w.side[1].blocks, h.dim, a.dq_weight, a.dk_weight,
-                                                                       h.weights_f32, h.type);
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, heads_weights_kernel, static_cast<const float*>(a.partial), w.side[0].blocks, w.side[1].blocks, h.dim, a.dq_weight,
+                            a.dk_weight, h.weights_f32, h.type);
 }
 
 }  // namespace kern

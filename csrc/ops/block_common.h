@@ -5,6 +5,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <atomic>
 #include <string>
 
 #include "kernels/pack8_api.h"
@@ -21,12 +22,21 @@ inline kern::Elem elem_of(const at::Tensor& t, const char* what) {
     default: throw TensorError(std::string(what) + ": float32, float16 or bfloat16 expected, got " + c10::toString(t.scalar_type()));
   }
 }
+// Whether a device is a B200, asked once.
+inline bool device_fits(int device) {
+  static std::atomic<uint64_t> fits{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (fits.load(std::memory_order_relaxed) & bit) return true;
+  const auto* p = at::cuda::getDeviceProperties(static_cast<c10::DeviceIndex>(device));
+  if (p->major != 10 || p->minor != 0) return false;
+  if (device < 64) fits.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 // A tensor that the kernels may read: dense memory of a B200, no wrapper and no tangent that they would lose.
 inline void check_block_tensor(const at::Tensor& t, const char* what) {
   MCCL_CHECK_T(TensorError, t.defined() && t.is_cuda() && t.layout() == at::kStrided, what << ": a dense CUDA tensor expected");
   MCCL_CHECK_T(TensorError, ordinary(t), what << ": tensor subclasses, transforms and forward-mode tangents are not supported");
-  const auto* p = at::cuda::getDeviceProperties(t.get_device());
-  MCCL_CHECK_T(DeviceError, p->major == 10 && p->minor == 0, what << ": built for compute capability 10.0, got " << p->major << "." << p->minor);
+  MCCL_CHECK_T(DeviceError, device_fits(t.get_device()), what << ": built for compute capability 10.0");
 }
 // `t` as rows along its last dimension: a view where its layout allows it, else a copy.
 inline at::Tensor rows_of(const at::Tensor& t) {

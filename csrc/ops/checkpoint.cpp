@@ -8,7 +8,8 @@ std::tuple<at::Tensor, at::Tensor> pack8(const at::Tensor& x) {
   check_block_tensor(x, "pack8");
   const kern::Elem type = elem_of(x, "pack8");
   c10::cuda::CUDAGuard guard(x.device());
-  const at::Tensor r = rows_of(x.detach());
+  at::AutoDispatchBelowADInplaceOrView no_graph;
+  const at::Tensor r = rows_of(x);
   const int64_t rows = r.size(0), cols = r.size(1), pitch = kern::pack8_pitch(cols);
   at::Tensor codes = at::empty({rows, pitch}, x.options().dtype(at::kChar));
   at::Tensor scales = at::empty({rows, kern::pack8_groups(cols)}, x.options().dtype(at::kFloat));

@@ -69,6 +69,8 @@ void launch(kern::GatedArgs& a, const at::Tensor& partial, const at::Tensor& lik
   OPS_CK(kern::launch_gated(a, at::cuda::getCurrentCUDAStream()));
 }
 
+at::Tensor few_rows(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+
 // y of 16-bit rows; g and u to `kept` where there is one.
 at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, kern::GatedActivation act,
                      kern::GatedKeep keep, at::Tensor* kept, int64_t wait_limit = -1) {
@@ -78,6 +80,14 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
   const kern::GatedShape s = shape_of(x, wg.size(0), act, keep);
   if (keep != kern::GatedKeep::kNone) *kept = at::empty({kern::gated_kept_bytes(s)}, x.options().dtype(at::kByte));
   if (x.size(0) == 0) return y;
+  if (keep == kern::GatedKeep::kNone && kern::gated_is_few(s) && wait_limit < 0) {
+    const at::Tensor rows[4] = {few_rows(x), few_rows(wg), few_rows(wu), few_rows(wd)};
+    const at::Tensor h = at::empty({2, s.tokens, kern::gated_pitch(s.hidden)}, x.options());
+    kern::GatedOperand m[4];
+    for (int i = 0; i < 4; ++i) m[i] = {rows[i].const_data_ptr(), row_stride(rows[i])};
+    OPS_CK(kern::launch_gated_few({s, m[0], m[1], m[2], m[3], h.data_ptr(), y.data_ptr()}, at::cuda::getCurrentCUDAStream()));
+    return y;
+  }
   const Operand ox = operand(x), og = operand(wg), ou = operand(wu), od = operand(wd);
   const at::Tensor h = at::empty({s.tokens, kern::gated_pitch(s.hidden)}, x.options());
   const at::Tensor partial = partial_for({GatedProduct::kUp, GatedProduct::kDown}, s, x.options());

@@ -63,6 +63,7 @@ CUDA_SOURCES = [
     "kernels/pack8.cu",
     "kernels/heads.cu",
     "kernels/gated.cu",
+    "kernels/gated_few.cu",
     "kernels/gate_f32.cu",
     "kernels/noalloc.cu",
 ]

@@ -19,7 +19,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .checkpoint import pack8, unpack8
+from .. import require_native
+from .checkpoint import Packed8, pack8, unpack8
 
 ACTIVATIONS = ("silu", "gelu_tanh")
 
@@ -36,7 +37,6 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if checkpoint not in (None, "int8"):
         raise ValueError(f"checkpoint is None or 'int8', got {checkpoint!r}")
     if x.is_cuda:
-        from .. import require_native
         if torch.is_autocast_enabled("cuda"):
             to = torch.get_autocast_dtype("cuda")
             x, w_gate, w_up, w_down = x.to(to), w_gate.to(to), w_up.to(to), w_down.to(to)
@@ -68,7 +68,6 @@ class _Plain(torch.autograd.Function):
     def backward(ctx, dy):
         w_gate, w_up, w_down, *kept = ctx.saved_tensors
         if ctx.kept_as is not None:
-            from .checkpoint import Packed8
             kept = [unpack8(Packed8(kept[2 * i], kept[2 * i + 1], *ctx.kept_as[i])) for i in range(3)]
         x, g, u = (t.flatten(0, -2) if t.dim() > 1 else t[None] for t in kept)
         rows = dy.reshape(-1, dy.shape[-1])

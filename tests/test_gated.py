@@ -156,6 +156,39 @@ def test_matches_64_bits(tokens, width, hidden, dtype, activation, eight):
         _check({"y": gated_feed_forward(*args, activation=activation)}, {"y": want["y"]})
 
 
+# single tokens and a few: their own kernels, at whole and ragged rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,activation", [(torch.bfloat16, "silu"), (torch.float16, "gelu_tanh")])
+@pytest.mark.parametrize("width,hidden", [(1024, 2816), (1000, 2731), (8, 24), (5, 3), (256, 264), (3000, 520), (136, 9000)])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 7, 8, 9, 16, 17, 25, 32, 33])
+def test_few_tokens_match_64_bits(tokens, width, hidden, dtype, activation):
+    x, wg, wu, wd, _ = _inputs(tokens, width, hidden, dtype, seed=tokens)
+    want = _want(x, wg, wu, wd, None, activation, False, Rounding(dtype))
+    _check({"y": gated_feed_forward(x, wg, wu, wd, activation=activation)}, want)
+
+    def odd(t):
+        big = torch.zeros(t.shape[0], t.shape[1] + 5, dtype=dtype, device="cuda")[:, 3:3 + t.shape[1]]
+        return big.copy_(t)
+
+    _check({"y": gated_feed_forward(odd(x), odd(wg), wu.t().contiguous().t(), odd(wd), activation=activation)}, want)
+    same = gated_feed_forward(x[:1].expand(tokens, width), wg, wu, wd, activation=activation)
+    _check({"y": same[-1:]}, {"y": tuple(t[:1] for t in want["y"])})
+
+
+# what is launched before the kernels has written the weights they read
+@pytest.mark.gpu
+def test_few_tokens_see_new_weights():
+    x, wg, wu, wd, _ = _inputs(4, 2048, 5632, torch.bfloat16)
+    want = gated_feed_forward(x, wg, wu, wd)
+    new = [torch.empty_like(t) for t in (wg, wu, wd)]
+    for _ in range(20):
+        for t in new:
+            t.zero_()
+        for t, w in zip(new, (wg, wu, wd)):
+            t.copy_(w)
+        assert torch.equal(gated_feed_forward(x, *new), want)
+
+
 # a device full of whole tiles and more, in bands of rows; long reductions that several pairs share
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens,width,hidden", [(5000, 520, 1100), (20000, 256, 136)])
