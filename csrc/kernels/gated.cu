@@ -882,10 +882,14 @@ cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s) {
   const bool a_inner = g.product != GatedProduct::kWeightUp && g.product != GatedProduct::kWeightDown;
   const bool b_inner = g.product == GatedProduct::kUp || g.product == GatedProduct::kDown;
   const GatedOperand a[2] = {g.a0, z.results * z.parts > 1 ? g.a1 : g.a0}, b[2] = {g.b0, z.gate || z.parts > 1 ? g.b1 : g.b0};
-  for (int i = 0; i < 2; ++i)
-    if (!make_map(&w.a[i], a[i], a_inner ? z.depth : z.rows, a_inner ? z.rows : z.depth, a_inner ? Box::kInnerK : Box::kOwn, h.bf16) ||
-        !make_map(&w.b[i], b[i], b_inner ? z.depth : z.cols, b_inner ? z.cols : z.depth, b_inner ? Box::kInnerK : Box::kOwn, h.bf16))
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && a[1].data == a[0].data && a[1].ld == a[0].ld) w.a[1] = w.a[0];
+    else if (!make_map(&w.a[i], a[i], a_inner ? z.depth : z.rows, a_inner ? z.rows : z.depth, a_inner ? Box::kInnerK : Box::kOwn, h.bf16))
       return cudaErrorInvalidValue;
+    if (i == 1 && b[1].data == b[0].data && b[1].ld == b[0].ld) w.b[1] = w.b[0];
+    else if (!make_map(&w.b[i], b[i], b_inner ? z.depth : z.cols, b_inner ? z.cols : z.depth, b_inner ? Box::kInnerK : Box::kOwn, h.bf16))
+      return cudaErrorInvalidValue;
+  }
   w.f.out0 = g.out0;
   w.f.out1 = g.out1;
   w.f.out2 = g.out2;

@@ -6,7 +6,8 @@
 
 Flags follow reference examples/ddp_dummy_train.py:45-70 (``--backend``, ``--baseline``,
 ``--steps``, ``--batch-size`` per rank, ``--bucket-mb``, ``--stress-model``, ``--fp16``,
-``--save-stats``, ``--warmup``) plus ``--model`` (heavy | mlp | resnet50 | gpt2-medium | gpt2-tiny),
+``--save-stats``, ``--warmup``) plus ``--model`` (heavy | mlp | resnet50 | gpt2-medium | gpt2-tiny |
+gated-medium | gated-tiny, the decoders of gated blocks; ``--checkpoint int8`` keeps their activations in 8 bits),
 ``--compression`` (none | fp16 | topk) and ``--fused-optim``.  AdamW lr 1e-4 wd 0.01 by
 default; after the run the first weights are broadcast from rank 0 and compared on every
 rank (replicas must be identical).
@@ -29,7 +30,7 @@ def parse():
     ap = argparse.ArgumentParser()
     ap.add_argument("--backend", default="mccl", choices=["mccl", "nccl", "gloo"])
     ap.add_argument("--baseline", action="store_true", help="single process, no DDP")
-    ap.add_argument("--model", default="heavy", choices=["heavy", "mlp", "resnet50", "gpt2-medium", "gpt2-tiny"])
+    ap.add_argument("--model", default="heavy", choices=["heavy", "mlp", "resnet50", "gpt2-medium", "gpt2-tiny", "gated-medium", "gated-tiny"])
     ap.add_argument("--steps", type=int, default=500)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--batch-size", type=int, default=128, help="per rank")
@@ -39,6 +40,7 @@ def parse():
     ap.add_argument("--stress-model", action="store_true", help="double the hidden size")
     ap.add_argument("--fp16", action="store_true", help="bf16 autocast for forward/backward")
     ap.add_argument("--compression", default=None, choices=[None, "none", "fp16", "topk"])
+    ap.add_argument("--checkpoint", default=None, choices=["int8"], help="activations of the gated models in 8 bits")
     ap.add_argument("--topk-ratio", type=float, default=0.01)
     ap.add_argument("--fused-optim", action="store_true", help="use the fused AdamW kernel")
     ap.add_argument("--lr", type=float, default=1e-4)
@@ -58,6 +60,10 @@ def build(args, device):
         return models.ResNet50().to(device), "image"
     if args.model == "gpt2-medium":
         return models.gpt2_medium().to(device), "tokens"
+    if args.model == "gated-medium":
+        return models.gated_medium(checkpoint=args.checkpoint).to(device), "tokens"
+    if args.model == "gated-tiny":
+        return models.gated_tiny(checkpoint=args.checkpoint).to(device), "tokens-tiny"
     return models.gpt2_tiny().to(device), "tokens-tiny"
 
 
