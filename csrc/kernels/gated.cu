@@ -288,25 +288,15 @@ __device__ __forceinline__ void take_wide(const uint4& up, const uint2& low, flo
 }
 
 // Where 8 numbers of a thread's row go, `i` columns from where it is: straight to memory, which costs a request for each row (the
-// joining kernel, results that are not aligned), or to the warp's boxes of 32 rows and 64 columns in shared memory, 128-byte swizzle,
+// joining kernel), or to the warp's boxes of 32 rows and 64 columns in shared memory, 128-byte swizzle,
 // which then leave as a whole.  (Straight to memory kGate took 99 us of 8192 x 1024 x 2816, bound by its requests.)
 constexpr int kTurn = 64, kBoxBytes = 32 * kTurn * 2;
 struct Direct {
   uint16_t* out[3];
-  bool on, bf16, wide;
-  int64_t left;  // numbers of the row from here on
+  bool bf16;
+  int64_t left;  // numbers of the row from here on, a multiple of 8
   __device__ __forceinline__ void put(int which, int i, const float* v) const {
-    if (!on) return;
-    if (wide && i + 8 <= left) {
-      store16(out[which], i, v, bf16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const uint32_t p = pack2(v[e], v[e + 1], bf16);
-        if (i + e < left) out[which][i + e] = static_cast<uint16_t>(p);
-        if (i + e + 1 < left) out[which][i + e + 1] = static_cast<uint16_t>(p >> 16);
-      }
-    }
+    if (i < left) store16(out[which], i, v, bf16);
   }
 };
 struct Staged {
@@ -616,29 +606,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
       if (t.part < 0) {
         const int64_t left = columns - at.col;
         const int first = share * kShare, last = static_cast<int>(min(static_cast<int64_t>(first + kShare), left));
-        if (w.f.wide) {
-          const int y = static_cast<int>(at.row) - lane;
+        const int64_t y = at.row - lane;  // the warp's first row
 #pragma unroll 1
-          for (int c = first; c < last; c += kTurn) {
-            if (lane == 0) stores_left();
-            __syncwarp();
-            finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged(boxes, lane, w.f.bf16));
+        for (int c = first; c < last; c += kTurn) {
+          if (lane == 0) stores_left();
+          __syncwarp();
+          finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged(boxes, lane, w.f.bf16));
+          if (kOut != kStore || w.f.wide) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
               if (y < w.f.rows)
 #pragma unroll
                 for (int b = 0; b < kOuts; ++b)
-                  store_box(&w.out[kOut == kDerive ? b : at.which], boxes + b * kBoxBytes, static_cast<int>(at.col) + c, y);
+                  store_box(&w.out[kOut == kDerive ? b : at.which], boxes + b * kBoxBytes, static_cast<int>(at.col) + c, static_cast<int>(y));
               stores_commit();
             }
-          }
-        } else {
-#pragma unroll 1
-          for (int c = first; c < last; c += kTurn) {
-            const Direct sink{{static_cast<uint16_t*>(at.which ? w.f.out1 : w.f.out0) + at.row * w.f.ldo + at.col + c, nullptr, nullptr}, at.row < w.f.rows,
-                              w.f.bf16, false, left - c};
-            finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, sink);
+          } else {  // rows that are not aligned: two numbers a lane, row by row
+            __syncwarp();
+            const int n = static_cast<int>(min(static_cast<int64_t>(32), w.f.rows - y));
+            uint16_t* to = static_cast<uint16_t*>(at.which ? w.f.out1 : w.f.out0) + y * w.f.ldo + at.col + c + 2 * lane;
+            const int here = last - c - 2 * lane;
+#pragma unroll 4
+            for (int r = 0; r < n; ++r, to += w.f.ldo) {
+              uint32_t v;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(boxes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
+              if (here > 0) to[0] = static_cast<uint16_t>(v);
+              if (here > 1) to[1] = static_cast<uint16_t>(v >> 16);
+            }
+            __syncwarp();
           }
         }
       } else {
@@ -728,18 +724,62 @@ __global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant
     for (int i = 0; i < 4; ++i) sums[(warp + 4 * (i0 + i)) * 32 + lane] = sum[i];
   }
   __syncthreads();
-  if (at.row >= f.rows) return;
   auto fetch = [&](int col, float* v) {
     const float* s = reinterpret_cast<const float*>(sums) + (col >= kHalf && kOut == kActivate ? kN : 0) * kHalf + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kN; ++i) v[i] = s[i * kHalf];
   };
+  if constexpr (kOut == kStore) {
+    if (!f.wide) {  // rows that are not aligned: handed over once more, two of them a warp and turn
+      float v[kN];
+      fetch(c, v);
+      __syncthreads();
+      uint32_t* rows = reinterpret_cast<uint32_t*>(sums);  // [128][9]
+#pragma unroll
+      for (int i = 0; i < kN; i += 2) rows[threadIdx.x * 9 + i / 2] = pack2(v[i], v[i + 1], f.bf16);
+      __syncthreads();
+      const int64_t y = at.row - threadIdx.x;
+      uint16_t* to = static_cast<uint16_t*>(at.which ? f.out1 : f.out0) + at.col + c;
+      for (int i = threadIdx.x; i < kHalf * kN; i += kHalf) {
+        const int r = i / kN, e = i % kN;
+        if (y + r < f.rows && e < left) to[(y + r) * f.ldo + e] = static_cast<uint16_t>(rows[r * 9 + e / 2] >> (16 * (e % 2)));
+      }
+      return;
+    }
+  }
+  if (at.row >= f.rows) return;
   Ahead<kOut, kKeep> ahead;
   ahead.load(f, at.row, at.col + c);
   const int64_t to = at.row * (kOut == kStore ? f.ldo : f.pitch) + at.col + c;
   const Direct sink{{static_cast<uint16_t*>(at.which ? f.out1 : f.out0) + to, static_cast<uint16_t*>(f.out1) + to, static_cast<uint16_t*>(f.out2) + to},
-                    true, f.bf16, f.wide, left};
+                    f.bf16, left};
   finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, sink);
+}
+
+// ---- rows that are not aligned --------------------------------------------------------------------------------
+struct Copies {
+  GatedCopy job[kGatedCopies];
+  int64_t first[kGatedCopies + 1];  // blocks
+};
+constexpr int kCopyRows = 8, kCopyCols = 512;  // of a block; a warp has a row, two neighbours a lane and turn
+__global__ void __launch_bounds__(256) gated_copies_kernel(const Copies w) {
+  int j = 0;
+  while (static_cast<int64_t>(blockIdx.x) >= w.first[j + 1]) ++j;
+  const GatedCopy& c = w.job[j];
+  const int64_t across = (c.cols + kCopyCols - 1) / kCopyCols, block = blockIdx.x - w.first[j];
+  const int64_t row = block / across * kCopyRows + threadIdx.x / 32, col = block % across * kCopyCols + threadIdx.x % 32 * 2;
+  if (row >= c.rows) return;
+  const uint16_t* from = static_cast<const uint16_t*>(c.from) + row * c.row_stride;
+  uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(c.to) + row * c.ld);
+  uint32_t v[kCopyCols / 64];
+#pragma unroll
+  for (int i = 0; i < kCopyCols / 64; ++i) {
+    const int64_t at = col + 64 * i;
+    v[i] = (at < c.cols ? from[at * c.col_stride] : 0u) | (at + 1 < c.cols ? static_cast<uint32_t>(from[(at + 1) * c.col_stride]) << 16 : 0u);
+  }
+#pragma unroll
+  for (int i = 0; i < kCopyCols / 64; ++i)
+    if (col + 64 * i < c.cols) to[(col + 64 * i) / 2] = v[i];
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
@@ -865,6 +905,22 @@ int64_t gated_kept_bytes(const GatedShape& s) {
 int64_t gated_partial_bytes(GatedProduct p, const GatedShape& s) {
   const Plan l = plan_of(p, s);
   return l.tail * l.splits * kTile * kTile * 4;
+}
+
+cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, cudaStream_t s) {
+  if (n < 1 || n > kGatedCopies) return cudaErrorInvalidValue;
+  Copies w{};
+  for (int j = 0; j < kGatedCopies; ++j) {
+    const bool there = j < n && jobs[j].rows > 0 && jobs[j].cols > 0;
+    if (there) w.job[j] = jobs[j];
+    w.first[j + 1] = w.first[j] + (there ? ceil_div(jobs[j].rows, kCopyRows) * ceil_div(jobs[j].cols, kCopyCols) : 0);
+  }
+  const int64_t blocks = w.first[kGatedCopies];
+  if (blocks == 0) return cudaSuccess;
+  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  note_launch();
+  gated_copies_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(w);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s) {

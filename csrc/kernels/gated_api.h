@@ -53,6 +53,18 @@ struct GatedArgs {
 int64_t gated_partial_bytes(GatedProduct p, const GatedShape& s);
 cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s);
 
+// Matrices of 16-bit numbers whose rows are not 16-byte aligned (or whose numbers do not lie side by side) copied to ones that are,
+// up to five in one launch.
+struct GatedCopy {
+  const void* from;
+  int64_t row_stride, col_stride, rows, cols;  // elements
+  void* to;                                    // 16-byte aligned
+  int64_t ld;                                  // gated_row(cols)
+};
+inline int64_t gated_row(int64_t cols) { return (cols + 7) / 8 * 8; }
+constexpr int kGatedCopies = 5;
+cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, cudaStream_t s);
+
 // A whole forward pass of few rows, two launches that read the weights at the rate of memory (kernels/gated_few.cu).  Rows of any
 // alignment.  `h`: scratch of 2 x tokens x gated_pitch(hidden) 16-bit numbers.
 constexpr int64_t kFewTokens = 32;

@@ -55,6 +55,15 @@ __device__ __forceinline__ uint4 eight(const T* row, int64_t at, int64_t depth, 
   }
   uint32_t v[4] = {0u, 0u, 0u, 0u};
   const uint16_t* p = reinterpret_cast<const uint16_t*>(row + at);
+  if (there && at + 8 <= depth) {  // in pairs, from the first that is aligned on
+    if ((reinterpret_cast<uintptr_t>(p) & 2) == 0) {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+      return make_uint4(q[0], q[1], q[2], q[3]);
+    }
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(p + 1);
+    const uint32_t a = q[0], b = q[1], c = q[2];
+    return make_uint4(p[0] | a << 16, __funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), c >> 16 | static_cast<uint32_t>(p[7]) << 16);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (there && at + i < depth) v[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));

@@ -42,19 +42,42 @@ kern::GatedShape shape_of(const at::Tensor& rows, int64_t hidden, kern::GatedAct
   return {rows.size(0), rows.size(1), hidden, rows.scalar_type() == at::kBFloat16, act, keep};
 }
 
-// A matrix as the products read it: rows of 16-byte multiples.  One that is not laid out so is copied.
-struct Operand {
-  at::Tensor held;
-  kern::GatedOperand m;
+// Matrices as the products read them: rows of 16-byte multiples.  Those that are not laid out so are copied, all in one launch.
+class Operands {
+ public:
+  // Which of them it is.
+  int add(const at::Tensor& t) {
+    const int64_t rows = t.size(0), cols = t.size(1), ld = rows <= 1 ? kern::gated_row(cols) : t.stride(0);
+    if ((cols <= 1 || t.stride(1) == 1) && ld % 8 == 0 && ld >= cols && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0) {
+      m_[n_] = {t.const_data_ptr(), ld};
+    } else {
+      m_[n_] = {nullptr, kern::gated_row(cols)};
+      copies_[copied_] = {t.const_data_ptr(), t.stride(0), t.stride(1), rows, cols, nullptr, kern::gated_row(cols)};
+      of_[copied_++] = n_;
+      bytes_ += (rows * kern::gated_row(cols) * 2 + 255) / 256 * 256;
+    }
+    return n_++;
+  }
+  void copy(const at::Tensor& like) {
+    if (copied_ == 0) return;
+    held_ = at::empty({bytes_}, like.options().dtype(at::kByte));
+    char* at = static_cast<char*>(held_.data_ptr());
+    for (int i = 0; i < copied_; ++i) {
+      copies_[i].to = at;
+      m_[of_[i]].data = at;
+      at += (copies_[i].rows * copies_[i].ld * 2 + 255) / 256 * 256;
+    }
+    OPS_CK(kern::launch_gated_copies(copies_, copied_, at::cuda::getCurrentCUDAStream()));
+  }
+  const kern::GatedOperand& operator[](int i) const { return m_[i]; }
+
+ private:
+  int n_ = 0, copied_ = 0, of_[kern::kGatedCopies] = {};
+  int64_t bytes_ = 0;
+  kern::GatedOperand m_[kern::kGatedCopies] = {};
+  kern::GatedCopy copies_[kern::kGatedCopies] = {};
+  at::Tensor held_;
 };
-Operand operand(const at::Tensor& t) {
-  const int64_t rows = t.size(0), cols = t.size(1), ld = rows <= 1 ? (cols + 7) / 8 * 8 : t.stride(0);
-  if ((cols <= 1 || t.stride(1) == 1) && ld % 8 == 0 && ld >= cols && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0)
-    return {t, {t.const_data_ptr(), ld}};
-  at::Tensor copy = at::empty({rows, (cols + 7) / 8 * 8}, t.options());
-  copy.narrow(1, 0, cols).copy_(t);
-  return {copy, {copy.const_data_ptr(), copy.size(1)}};
-}
 
 // Partial sums of the products of one pass, which follow each other on a stream.
 at::Tensor partial_for(std::initializer_list<GatedProduct> ps, const kern::GatedShape& s, const at::TensorOptions& like) {
@@ -88,15 +111,17 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
     OPS_CK(kern::launch_gated_few({s, m[0], m[1], m[2], m[3], h.data_ptr(), y.data_ptr()}, at::cuda::getCurrentCUDAStream()));
     return y;
   }
-  const Operand ox = operand(x), og = operand(wg), ou = operand(wu), od = operand(wd);
+  Operands m;
+  const int ox = m.add(x), og = m.add(wg), ou = m.add(wu), od = m.add(wd);
+  m.copy(x);
   const at::Tensor h = at::empty({s.tokens, kern::gated_pitch(s.hidden)}, x.options());
   const at::Tensor partial = partial_for({GatedProduct::kUp, GatedProduct::kDown}, s, x.options());
   kern::GatedArgs a{};
   a.product = GatedProduct::kUp;
   a.shape = s;
-  a.a0 = ox.m;
-  a.b0 = og.m;
-  a.b1 = ou.m;
+  a.a0 = m[ox];
+  a.b0 = m[og];
+  a.b1 = m[ou];
   a.out0 = h.data_ptr();
   a.kept = kept ? kept->data_ptr() : nullptr;
   launch(a, partial, x, wait_limit);
@@ -104,7 +129,7 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
   a.product = GatedProduct::kDown;
   a.shape = s;
   a.a0 = {h.const_data_ptr(), h.size(1)};
-  a.b0 = od.m;
+  a.b0 = m[od];
   a.out0 = y.data_ptr();
   a.ldo = s.width;
   launch(a, partial, x, wait_limit);
@@ -118,7 +143,7 @@ struct Gradients {
   at::Tensor x, gate, up, down;
 };
 
-Gradients backward16(const at::Tensor& dy, const Operand& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, const at::Tensor& kept,
+Gradients backward16(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, const at::Tensor& kept,
                      kern::GatedActivation act, kern::GatedKeep keep, const Needs& need) {
   check_waits(dy);
   c10::cuda::CUDAGuard guard(dy.device());
@@ -137,29 +162,33 @@ Gradients backward16(const at::Tensor& dy, const Operand& x, const at::Tensor& w
     return r;
   }
   const int64_t pitch = kern::gated_pitch(s.hidden);
-  const Operand ody = operand(dy), od = operand(wd);
-  const at::Tensor h = at::empty({s.tokens, pitch}, like), dg = at::empty({s.tokens, pitch}, like), du = at::empty({s.tokens, pitch}, like);
+  Operands m;
+  const int ody = m.add(dy), od = m.add(wd);
+  const int og = need.x ? m.add(wg) : 0, ou = need.x ? m.add(wu) : 0, ox = need.gate || need.up ? m.add(x) : 0;
+  m.copy(dy);
+  const at::Tensor between = at::empty({3, s.tokens, pitch}, like);
+  const int64_t each = s.tokens * pitch * 2;
+  char *const h = static_cast<char*>(between.data_ptr()), *const dg = h + each, *const du = dg + each;
   const at::Tensor partial = partial_for({GatedProduct::kGate, GatedProduct::kInput, GatedProduct::kWeightUp, GatedProduct::kWeightDown}, s, like);
-  const kern::GatedOperand mh{h.const_data_ptr(), pitch}, mg{dg.const_data_ptr(), pitch}, mu{du.const_data_ptr(), pitch};
+  const kern::GatedOperand mh{h, pitch}, mg{dg, pitch}, mu{du, pitch};
   kern::GatedArgs a{};
   a.product = GatedProduct::kGate;
   a.shape = s;
-  a.a0 = ody.m;
-  a.b0 = od.m;
-  a.out0 = h.data_ptr();
-  a.out1 = dg.data_ptr();
-  a.out2 = du.data_ptr();
+  a.a0 = m[ody];
+  a.b0 = m[od];
+  a.out0 = h;
+  a.out1 = dg;
+  a.out2 = du;
   a.kept = kept.data_ptr();
   launch(a, partial, dy);
   if (need.x) {
-    const Operand og = operand(wg), ou = operand(wu);
     a = {};
     a.product = GatedProduct::kInput;
     a.shape = s;
     a.a0 = mg;
     a.a1 = mu;
-    a.b0 = og.m;
-    a.b1 = ou.m;
+    a.b0 = m[og];
+    a.b1 = m[ou];
     a.out0 = r.x.data_ptr();
     a.ldo = s.width;
     launch(a, partial, dy);
@@ -170,7 +199,7 @@ Gradients backward16(const at::Tensor& dy, const Operand& x, const at::Tensor& w
     a.shape = s;
     a.a0 = mg;
     a.a1 = mu;
-    a.b0 = x.m;
+    a.b0 = m[ox];
     a.out0 = r.gate.data_ptr();
     a.out1 = r.up.data_ptr();
     a.ldo = s.width;
@@ -180,7 +209,7 @@ Gradients backward16(const at::Tensor& dy, const Operand& x, const at::Tensor& w
     a = {};
     a.product = GatedProduct::kWeightDown;
     a.shape = s;
-    a.a0 = ody.m;
+    a.a0 = m[ody];
     a.b0 = mh;
     a.out0 = r.down.data_ptr();
     a.ldo = s.hidden;
@@ -290,8 +319,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
       }
       r = backward32(dy, x, wg, wu, wd, g, u, act, need);
     } else {
-      Operand x{};
-      if (need_up && rows > 0) x = operand(eight ? unpacked(saved[3], saved[4], rows, width, wg.options()) : saved[3]);
+      const at::Tensor x = !need_up || rows == 0 ? at::Tensor() : eight ? unpacked(saved[3], saved[4], rows, width, wg.options()) : saved[3];
       r = backward16(dy, x, wg, wu, wd, saved.back(), act, eight ? kern::GatedKeep::kEight : kern::GatedKeep::kWide, need);
     }
     return {r.x, need.gate ? r.gate : at::Tensor(), need.up ? r.up : at::Tensor(), r.down, {}, {}};
