@@ -15,61 +15,79 @@ constexpr float kGelu = 1.5957691216057308f, kCubic = 0.044715f;  // 2 sqrt(2 / 
 
 __device__ __forceinline__ float gate_of(float z, bool silu) { return 1.f / (1.f + expf(-(silu ? z : kGelu * (z + kCubic * z * z * z)))); }
 
-__global__ void __launch_bounds__(kThreads) gate_forward_kernel(const float* __restrict__ g, const float* __restrict__ u, float* __restrict__ h,
-                                                                int64_t n, bool vec, bool silu) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * kThreads;
-  auto one = [&](float z, float y) { return z * gate_of(z, silu) * y; };
-  const int64_t runs = vec ? n / 4 : 0;
-  for (int64_t i = at; i < runs; i += step) {
-    const float4 a = reinterpret_cast<const float4*>(g)[i], b = reinterpret_cast<const float4*>(u)[i];
-    reinterpret_cast<float4*>(h)[i] = make_float4(one(a.x, b.x), one(a.y, b.y), one(a.z, b.z), one(a.w, b.w));
+// Rows of g and of u, `ld` numbers apart, `cols` of each; h and dh have theirs one behind the other.
+struct Rows {
+  const float *g, *u;
+  int64_t ld, rows, cols;
+  bool vec, silu;
+};
+__global__ void __launch_bounds__(kThreads) gate_forward_kernel(const Rows w, float* __restrict__ h) {
+  auto one = [&](float z, float y) { return z * gate_of(z, w.silu) * y; };
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 4;
+  if (col >= w.cols) return;
+  for (int64_t row = blockIdx.y; row < w.rows; row += gridDim.y) {
+    const float *g = w.g + row * w.ld + col, *u = w.u + row * w.ld + col;
+    float* to = h + row * w.cols + col;
+    if (w.vec) {
+      const float4 a = *reinterpret_cast<const float4*>(g), b = *reinterpret_cast<const float4*>(u);
+      *reinterpret_cast<float4*>(to) = make_float4(one(a.x, b.x), one(a.y, b.y), one(a.z, b.z), one(a.w, b.w));
+    } else {
+      for (int i = 0; i < 4 && col + i < w.cols; ++i) to[i] = one(g[i], u[i]);
+    }
   }
-  for (int64_t i = 4 * runs + at; i < n; i += step) h[i] = one(g[i], u[i]);
 }
 
-__global__ void __launch_bounds__(kThreads) gate_backward_kernel(const float* __restrict__ g, const float* __restrict__ u, const float* __restrict__ dh,
-                                                                 float* __restrict__ dg, float* __restrict__ du, int64_t n, bool vec, bool silu) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * kThreads;
+__global__ void __launch_bounds__(kThreads) gate_backward_kernel(const Rows w, const float* __restrict__ dh, float* __restrict__ dgu) {
   auto one = [&](float z, float y, float d, float& a, float& b) {
-    const float s = gate_of(z, silu), t = s * (1.f - s);
+    const float s = gate_of(z, w.silu), t = s * (1.f - s);
     b = d * (z * s);
     // (where the curve is flat the cubic's slope may be infinite)
-    a = d * y * (t > 0.f ? s + z * t * (silu ? 1.f : kGelu * (1.f + 3.f * kCubic * z * z)) : s);
+    a = d * y * (t > 0.f ? s + z * t * (w.silu ? 1.f : kGelu * (1.f + 3.f * kCubic * z * z)) : s);
   };
-  const int64_t runs = vec ? n / 4 : 0;
-  for (int64_t i = at; i < runs; i += step) {
-    const float4 z = reinterpret_cast<const float4*>(g)[i], y = reinterpret_cast<const float4*>(u)[i], d = reinterpret_cast<const float4*>(dh)[i];
-    float4 a, b;
-    one(z.x, y.x, d.x, a.x, b.x);
-    one(z.y, y.y, d.y, a.y, b.y);
-    one(z.z, y.z, d.z, a.z, b.z);
-    one(z.w, y.w, d.w, a.w, b.w);
-    reinterpret_cast<float4*>(dg)[i] = a;
-    reinterpret_cast<float4*>(du)[i] = b;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 4;
+  if (col >= w.cols) return;
+  for (int64_t row = blockIdx.y; row < w.rows; row += gridDim.y) {
+    const float *g = w.g + row * w.ld + col, *u = w.u + row * w.ld + col, *d = dh + row * w.cols + col;
+    float *dg = dgu + row * 2 * w.cols + col, *du = dg + w.cols;
+    if (w.vec) {
+      const float4 z = *reinterpret_cast<const float4*>(g), y = *reinterpret_cast<const float4*>(u), x = *reinterpret_cast<const float4*>(d);
+      float4 a, b;
+      one(z.x, y.x, x.x, a.x, b.x);
+      one(z.y, y.y, x.y, a.y, b.y);
+      one(z.z, y.z, x.z, a.z, b.z);
+      one(z.w, y.w, x.w, a.w, b.w);
+      *reinterpret_cast<float4*>(dg) = a;
+      *reinterpret_cast<float4*>(du) = b;
+    } else {
+      for (int i = 0; i < 4 && col + i < w.cols; ++i) one(g[i], u[i], d[i], dg[i], du[i]);
+    }
   }
-  for (int64_t i = 4 * runs + at; i < n; i += step) one(g[i], u[i], dh[i], dg[i], du[i]);
 }
 
-int blocks_for(int64_t n) { return static_cast<int>(std::min<int64_t>((n + 4 * kThreads - 1) / (4 * kThreads), 8 * kSms)); }
-bool wide(std::initializer_list<const void*> ps) {
-  uintptr_t all = 0;
-  for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
-  return all % 16 == 0;
+dim3 grid_for(const Rows& w) {
+  const int64_t across = (w.cols + 4 * kThreads - 1) / (4 * kThreads);
+  return dim3(static_cast<unsigned>(across), static_cast<unsigned>(std::min<int64_t>(w.rows, std::max<int64_t>(1, 16 * kSms / across))));
+}
+Rows rows_of(const float* g, const float* u, int64_t ld, int64_t rows, int64_t cols, GatedActivation act, std::initializer_list<const void*> others) {
+  uintptr_t all = reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(u);
+  for (const void* p : others) all |= reinterpret_cast<uintptr_t>(p);
+  return {g, u, ld, rows, cols, all % 16 == 0 && cols % 4 == 0 && ld % 4 == 0, act == GatedActivation::kSilu};
 }
 
 }  // namespace
 
-cudaError_t launch_gate_f32(const float* g, const float* u, float* h, int64_t n, GatedActivation act, cudaStream_t s) {
-  if (n <= 0) return cudaSuccess;
+cudaError_t launch_gate_f32(const float* g, const float* u, int64_t ld, float* h, int64_t rows, int64_t cols, GatedActivation act, cudaStream_t s) {
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  const Rows w = rows_of(g, u, ld, rows, cols, act, {h});
   note_launch();
-  gate_forward_kernel<<<blocks_for(n), kThreads, 0, s>>>(g, u, h, n, wide({g, u, h}), act == GatedActivation::kSilu);
+  gate_forward_kernel<<<grid_for(w), kThreads, 0, s>>>(w, h);
   return cudaGetLastError();
 }
-cudaError_t launch_gate_f32_backward(const float* g, const float* u, const float* dh, float* dg, float* du, int64_t n, GatedActivation act,
-                                     cudaStream_t s) {
-  if (n <= 0) return cudaSuccess;
+cudaError_t launch_gate_f32_backward(const float* gu, const float* dh, float* dgu, int64_t rows, int64_t cols, GatedActivation act, cudaStream_t s) {
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  const Rows w = rows_of(gu, gu + cols, 2 * cols, rows, cols, act, {dh, dgu});
   note_launch();
-  gate_backward_kernel<<<blocks_for(n), kThreads, 0, s>>>(g, u, dh, dg, du, n, wide({g, u, dh, dg, du}), act == GatedActivation::kSilu);
+  gate_backward_kernel<<<grid_for(w), kThreads, 0, s>>>(w, dh, dgu);
   return cudaGetLastError();
 }
 

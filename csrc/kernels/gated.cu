@@ -91,14 +91,12 @@ __device__ __forceinline__ void stores_left() { asm volatile("cp.async.bulk.wait
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // Shared-memory matrix descriptors, 128-byte swizzle.  k innermost: rows of 128 bytes (64 k), 1024 bytes per eight rows.  Own
 // index innermost: rows of 128 bytes (64 of the index, one k), 1024 bytes per eight k, 8192 from 64 of the index to the next.
-template <bool kInner>
-__device__ __forceinline__ uint64_t make_desc(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kInner ? 1 : 8192 >> 4) << 16) |
+__device__ __forceinline__ uint64_t make_desc(uint32_t addr, bool inner) {
+  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(inner ? 1 : 8192 >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // from 16 k to the next, in descriptor units
-template <bool kInner>
-constexpr uint32_t kStep = (kInner ? 32 : 2048) >> 4;
+__device__ __forceinline__ uint32_t step_of(bool inner) { return (inner ? 32 : 2048) >> 4; }
 __device__ __forceinline__ uint32_t make_idesc(bool bf16, bool a_inner, bool b_inner) {
   const uint32_t type = bf16 ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | (a_inner ? 0u : 1u << 15) | (b_inner ? 0u : 1u << 16) |
@@ -177,23 +175,34 @@ struct Curve {
 enum Out { kStore, kActivate, kDerive };  // what follows the product
 
 struct Finish {
-  void *out0, *out1, *out2;
-  int64_t ldo;
-  bool wide;              // there are maps of the outputs: their rows are aligned to 16 bytes
   bool bf16;
   Curve curve;
   char* kept;
-  int64_t rows, cols;     // of one result: tokens x hidden for kActivate and kDerive
-  int64_t pitch;          // of h, dg, du
+  int64_t rows, pitch;    // of what is kept, and of h, dg and du
 };
-struct Work {
+// One product: tiles, and how they become items of work.
+struct Job {
   CUtensorMap a[2], b[2], out[3];
+  void* to[3];
+  int64_t rows, cols, ldo;  // of one result; cols: of h, dg and du their pitch
+  bool a_inner, b_inner;    // k innermost
+  bool wide;                // there are maps of the results: their rows are aligned to 16 bytes
+  int rows_segment;         // tiles of rows of the first of two results (dWg, then dWu); all of them where there is one
+  int tiles_i, tiles_j;     // tiles_i: of all results
+  int stages, segment;      // of the reduction; stages of its first part (dg Wg, then du Wu)
+  int first;                // item
+  int whole;                // items that are whole tiles; behind them tiles whose reduction `splits` pairs share, with partial sums from `part` on
+  int splits, per_split, part;
+  int join;                 // the first such tile among those of all jobs
+};
+constexpr int kMostJobs = 3;
+template <Out kOut>
+constexpr int kJobs = kOut == kStore ? kMostJobs : 1;
+template <int kN>
+struct Work {
+  Job job[kN];
   Finish f;
-  int rows_segment;       // kStore: tiles of rows of the first of two results (dWg, then dWu); all of them where there is one
-  int tiles_i, tiles_j;   // tiles_i: of all results
-  int stages, segment;    // of the reduction; stages of its first part (dg Wg, then du Wu)
-  int whole;              // items that are whole tiles; behind them tiles whose reduction `splits` pairs share
-  int items, splits, per_split;
+  int jobs, items;
   float* partial;
   uint32_t* failed;
   long long limit;
@@ -201,29 +210,40 @@ struct Work {
 
 // A tile's place, so that the pairs at work at a time read few rows of each operand: kBand tiles of rows, column by column.
 constexpr int kBand = 8;
-__device__ __forceinline__ void tile_place(const Work& w, int tile, int& ti, int& tj) {
-  const int band = tile / (kBand * w.tiles_j), in_band = tile - band * kBand * w.tiles_j;
-  const int high = min(kBand, w.tiles_i - band * kBand);
+__device__ __forceinline__ void tile_place(const Job& j, int tile, int& ti, int& tj) {
+  const int band = tile / (kBand * j.tiles_j), in_band = tile - band * kBand * j.tiles_j;
+  const int high = min(kBand, j.tiles_i - band * kBand);
   tj = in_band / high;
   ti = band * kBand + in_band - tj * high;
 }
 struct Item {
-  int ti, tj, c0, c1, part;  // part: which partial sum, or -1
-  __device__ __forceinline__ Item(const Work& w, int item) {
-    if (item < w.whole) {
-      tile_place(w, item, ti, tj);
+  int job, ti, tj, c0, c1, part;  // part: which partial sum, or -1
+  template <int kN>
+  __device__ __forceinline__ Item(const Work<kN>& w, int item) {
+    job = 0;
+    while (job + 1 < w.jobs && item >= w.job[job + 1].first) ++job;
+    const Job& j = w.job[job];
+    item -= j.first;
+    if (item < j.whole) {
+      tile_place(j, item, ti, tj);
       c0 = 0;
-      c1 = w.stages;
+      c1 = j.stages;
       part = -1;
     } else {
-      part = item - w.whole;
-      const int t = part / w.splits;
-      tile_place(w, w.whole + t, ti, tj);
-      c0 = (part - t * w.splits) * w.per_split;
-      c1 = min(w.stages, c0 + w.per_split);
+      part = item - j.whole;
+      const int t = part / j.splits;
+      tile_place(j, j.whole + t, ti, tj);
+      c0 = (part - t * j.splits) * j.per_split;
+      c1 = min(j.stages, c0 + j.per_split);
+      part += j.part;
     }
   }
 };
+// A pair's items.  Several jobs come the longest items first: the pair that had the longest of the first round gets the shortest of the
+// others.
+__device__ __forceinline__ int item_of(int round, int pair, int pairs, int jobs) {
+  return round * pairs + (round > 0 && jobs > 1 ? pairs - 1 - pair : pair);
+}
 
 // ---- after the product --------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
@@ -438,9 +458,9 @@ struct Spot {
   int which;      // kStore: which of two results
 };
 template <Out kOut>
-__device__ __forceinline__ Spot spot_of(const Work& w, int ti, int tj, int row_in_tile) {
-  const int second = kOut == kStore && ti >= w.rows_segment;
-  return {static_cast<int64_t>(second ? ti - w.rows_segment : ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * (kOut == kActivate ? kHalf : kTile), second};
+__device__ __forceinline__ Spot spot_of(const Job& j, int ti, int tj, int row_in_tile) {
+  const int second = kOut == kStore && ti >= j.rows_segment;
+  return {static_cast<int64_t>(second ? ti - j.rows_segment : ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * (kOut == kActivate ? kHalf : kTile), second};
 }
 // kCols columns from `c` of the tile on, into a sink.
 template <Out kOut, GatedKeep kKeep, int kCols, typename Fetch, typename Sink>
@@ -468,14 +488,11 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
     }
   }
 }
-template <Out kOut>
-__device__ __forceinline__ int64_t columns_of(const Finish& f) { return kOut == kStore ? f.cols : f.pitch; }
-
 // A pair of CTAs per tile of 256 x 256, tiles in turn: each CTA loads half of either operand's rows and has half of the
 // accumulator's; the first one issues the products of both.  Two accumulators, so that a tile is taken out while the next one
 // is multiplied.
-template <bool kAInner, bool kBInner, Out kOut, GatedKeep kKeep>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work w) {
+template <Out kOut, GatedKeep kKeep>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   constexpr int kDepths = kStages<kOut>, kOuts = kBoxes<kOut>;
   extern __shared__ char raw[];
   __shared__ alignas(8) uint64_t bars[2 * kDepths + 5];
@@ -517,25 +534,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
   if (warp == kLoader) {
     if (elect()) {
       int s = 0, turn = 0;
-      for (int item = pair; ok && item < w.items; item += pairs) {
+      for (int round = 0, item = pair; ok && item < w.items; item = item_of(++round, pair, pairs, w.jobs)) {
         const Item t(w, item);
-        const int i_second = t.ti >= w.rows_segment, i0 = (i_second ? t.ti - w.rows_segment : t.ti) * kTile + rank * kHalf;
+        const Job& j = w.job[t.job];
+        const int i_second = t.ti >= j.rows_segment, i0 = (i_second ? t.ti - j.rows_segment : t.ti) * kTile + rank * kHalf;
         // g and u side by side: one CTA has the rows of Wg, the other those of Wu
         const int j0 = kOut == kActivate ? t.tj * kHalf : t.tj * kTile + rank * kHalf;
+        const bool a_inner = j.a_inner, b_inner = j.b_inner;
         for (int c = t.c0; ok && c < t.c1; ++c) {
           ok = bar_wait(empty(s), (turn & 1) ^ 1, w.limit);
           if (!ok) break;
-          const int k_second = c >= w.segment, k0 = (k_second ? c - w.segment : c) * kDepth;
-          const CUtensorMap* a = &w.a[i_second | k_second];
-          const CUtensorMap* b = &w.b[kOut == kActivate ? rank : k_second];
+          const int k_second = c >= j.segment, k0 = (k_second ? c - j.segment : c) * kDepth;
+          const CUtensorMap* a = &j.a[i_second | k_second];
+          const CUtensorMap* b = &j.b[kOut == kActivate ? rank : k_second];
           const uint32_t to = smem0 + s * kStage, bar = in_leader(full(s));
           if (rank == 0) bar_expect(full(s), 2 * kStage);
-          if (kAInner) load_box(to, a, k0, i0, bar);
+          if (a_inner) load_box(to, a, k0, i0, bar);
           else {
             load_box(to, a, i0, k0, bar);
             load_box(to + kOperand / 2, a, i0 + 64, k0, bar);
           }
-          if (kBInner) load_box(to + kOperand, b, k0, j0, bar);
+          if (b_inner) load_box(to + kOperand, b, k0, j0, bar);
           else {
             load_box(to + kOperand, b, j0, k0, bar);
             load_box(to + kOperand + kOperand / 2, b, j0 + 64, k0, bar);
@@ -554,11 +573,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
     if (rank == 0 && elect()) {
       issued = true;
       ok = w.limit > 0;  // a limit of zero, of tests: no product is issued, and all others wait in vain
-      const uint32_t idesc = make_idesc(w.f.bf16, kAInner, kBInner);
-      const uint64_t a0 = make_desc<kAInner>(smem0), b0 = make_desc<kBInner>(smem0 + kOperand);
       int s = 0, turn = 0, done = 0;
-      for (int item = pair; ok && item < w.items; item += pairs, ++done) {
+      for (int round = 0, item = pair; ok && item < w.items; item = item_of(++round, pair, pairs, w.jobs), ++done) {
         const Item t(w, item);
+        const bool a_inner = w.job[t.job].a_inner, b_inner = w.job[t.job].b_inner;
+        const uint32_t idesc = make_idesc(w.f.bf16, a_inner, b_inner), step_a = step_of(a_inner), step_b = step_of(b_inner);
+        const uint64_t a0 = make_desc(smem0, a_inner), b0 = make_desc(smem0 + kOperand, b_inner);
         const int buffer = done & 1;
         ok = bar_wait(acc_free(buffer), ((done >> 1) & 1) ^ 1, w.limit);
         fence_after();
@@ -569,7 +589,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           fence_after();
           const uint64_t a = a0 + s * (kStage >> 4), b = b0 + s * (kStage >> 4);
 #pragma unroll
-          for (int k = 0; k < kDepth / 16; ++k) mma(acc, a + k * kStep<kAInner>, b + k * kStep<kBInner>, idesc, c > t.c0 || k > 0);
+          for (int k = 0; k < kDepth / 16; ++k) mma(acc, a + k * step_a, b + k * step_b, idesc, c > t.c0 || k > 0);
           mma_commit(empty(s));
           if (++s == kDepths) s = 0, ++turn;
         }
@@ -583,14 +603,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
     const int q = warp & 3, share = (warp - kFirstOut) >> 2;
     const int row = rank * kHalf + 32 * q + lane;
     const uint32_t boxes = smem0 + kDepths * kStage + (warp - kFirstOut) * (kOuts * kBoxBytes);
-    const int64_t columns = columns_of<kOut>(w.f);
     int done = 0;
-    for (int item = pair; item < w.items; item += pairs, ++done) {
+    for (int round = 0, item = pair; item < w.items; item = item_of(++round, pair, pairs, w.jobs), ++done) {
       const Item t(w, item);
+      const Job& j = w.job[t.job];
       const int buffer = done & 1;
-      const Spot at = spot_of<kOut>(w, t.ti, t.tj, row);
+      const Spot at = spot_of<kOut>(j, t.ti, t.tj, row);
       Ahead<kOut, kKeep> ahead;
-      if (t.part < 0 && at.col + share * kShare < columns) ahead.load(w.f, min(at.row, w.f.rows - 1), at.col + share * kShare);
+      if (t.part < 0 && at.col + share * kShare < j.cols) ahead.load(w.f, min(at.row, w.f.rows - 1), at.col + share * kShare);
       if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_full(buffer), (done >> 1) & 1, w.limit));
       fence_after();
       const uint32_t from = tmem + buffer * kTile + (static_cast<uint32_t>(32 * q) << 16);
@@ -604,7 +624,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
         }
       };
       if (t.part < 0) {
-        const int64_t left = columns - at.col;
+        const int64_t left = j.cols - at.col;
         const int first = share * kShare, last = static_cast<int>(min(static_cast<int64_t>(first + kShare), left));
         const int64_t y = at.row - lane;  // the warp's first row
 #pragma unroll 1
@@ -612,23 +632,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           if (lane == 0) stores_left();
           __syncwarp();
           finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged(boxes, lane, w.f.bf16));
-          if (kOut != kStore || w.f.wide) {
+          if (kOut != kStore || j.wide) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-              if (y < w.f.rows)
+              if (y < j.rows)
 #pragma unroll
                 for (int b = 0; b < kOuts; ++b)
-                  store_box(&w.out[kOut == kDerive ? b : at.which], boxes + b * kBoxBytes, static_cast<int>(at.col) + c, static_cast<int>(y));
+                  store_box(&j.out[kOut == kDerive ? b : at.which], boxes + b * kBoxBytes, static_cast<int>(at.col) + c, static_cast<int>(y));
               stores_commit();
             }
           } else {  // rows that are not aligned: two numbers a lane, row by row
             __syncwarp();
-            const int n = static_cast<int>(min(static_cast<int64_t>(32), w.f.rows - y));
-            uint16_t* to = static_cast<uint16_t*>(at.which ? w.f.out1 : w.f.out0) + y * w.f.ldo + at.col + c + 2 * lane;
+            const int n = static_cast<int>(min(static_cast<int64_t>(32), j.rows - y));
+            uint16_t* to = static_cast<uint16_t*>(j.to[at.which]) + y * j.ldo + at.col + c + 2 * lane;
             const int here = last - c - 2 * lane;
 #pragma unroll 4
-            for (int r = 0; r < n; ++r, to += w.f.ldo) {
+            for (int r = 0; r < n; ++r, to += j.ldo) {
               uint32_t v;
               asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(boxes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
               if (here > 0) to[0] = static_cast<uint16_t>(v);
@@ -643,7 +663,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
         for (int c = share * (kTile / kShares); c < (share + 1) * (kTile / kShares); c += kN) {
           float v[kN];
           fetch(c, v);
-          if (at.row < w.f.rows)
+          if (at.row < j.rows)
 #pragma unroll
             for (int i = 0; i < kN; ++i) __stcg(to + static_cast<int64_t>(c + i) * kTile, v[i]);
         }
@@ -679,19 +699,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
 // tile: its warps add up a column each, four rows a lane, and hand them over in shared memory to the thread that has the row.
 // (Each thread its own row's numbers: 14.5 us for 18 MB of parts, a quarter of it in flight.)
 template <Out kOut, GatedKeep kKeep>
-__global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant__ Work w) {
+__global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kN = kTake<kOut, kKeep>, kAll = kN * (kOut == kActivate ? 2 : 1), kEach = kAll / 4, kParts = 4;
   extern __shared__ float4 sums[];  // [kAll][32]
-  const int tile = blockIdx.x, c = blockIdx.z * kN, row = blockIdx.y * kHalf + threadIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int job = 0;
+  while (job + 1 < w.jobs && static_cast<int>(blockIdx.x) >= w.job[job + 1].join) ++job;
+  const Job& j = w.job[job];
+  const int tile = static_cast<int>(blockIdx.x) - j.join, c = blockIdx.z * kN, row = blockIdx.y * kHalf + threadIdx.x, lane = threadIdx.x % 32,
+            warp = threadIdx.x / 32;
   int ti, tj;
-  tile_place(w, w.whole + tile, ti, tj);
+  tile_place(j, j.whole + tile, ti, tj);
   const Finish& f = w.f;
-  const Spot at = spot_of<kOut>(w, ti, tj, row);
-  const int64_t left = columns_of<kOut>(f) - at.col - c;
-  if (left <= 0) return;
-  const float* from = w.partial + static_cast<int64_t>(tile) * w.splits * (kTile * kTile) + blockIdx.y * kHalf + 4 * lane;
+  const Spot at = spot_of<kOut>(j, ti, tj, row);
+  const int64_t left = j.cols - at.col - c;
+  if (left <= 0 || at.row - threadIdx.x >= j.rows) return;
+  const float* from = w.partial + (j.part + static_cast<int64_t>(tile) * j.splits) * (kTile * kTile) + blockIdx.y * kHalf + 4 * lane;
 #pragma unroll 1
   for (int i0 = 0; i0 < kEach; i0 += 4) {
     float4 sum[4];
@@ -702,22 +726,22 @@ __global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant
       column[i] = from + (col < kN ? c + col : kHalf + c + col - kN) * kTile;
       sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    for (int p = 0; p < w.splits; p += kParts) {
+    for (int p = 0; p < j.splits; p += kParts) {
       float4 x[4][kParts];
 #pragma unroll
-      for (int j = 0; j < kParts; ++j)
+      for (int q = 0; q < kParts; ++q)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          x[i][j] = __ldcg(reinterpret_cast<const float4*>(column[i] + static_cast<int64_t>(min(p + j, w.splits - 1)) * (kTile * kTile)));
+          x[i][q] = __ldcg(reinterpret_cast<const float4*>(column[i] + static_cast<int64_t>(min(p + q, j.splits - 1)) * (kTile * kTile)));
 #pragma unroll
-      for (int j = 0; j < kParts; ++j)
+      for (int q = 0; q < kParts; ++q)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (p + j < w.splits) {
-            sum[i].x += x[i][j].x;
-            sum[i].y += x[i][j].y;
-            sum[i].z += x[i][j].z;
-            sum[i].w += x[i][j].w;
+          if (p + q < j.splits) {
+            sum[i].x += x[i][q].x;
+            sum[i].y += x[i][q].y;
+            sum[i].z += x[i][q].z;
+            sum[i].w += x[i][q].w;
           }
     }
 #pragma unroll
@@ -730,7 +754,7 @@ __global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant
     for (int i = 0; i < kN; ++i) v[i] = s[i * kHalf];
   };
   if constexpr (kOut == kStore) {
-    if (!f.wide) {  // rows that are not aligned: handed over once more, two of them a warp and turn
+    if (!j.wide) {  // rows that are not aligned: handed over once more, two of them a warp and turn
       float v[kN];
       fetch(c, v);
       __syncthreads();
@@ -739,20 +763,19 @@ __global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant
       for (int i = 0; i < kN; i += 2) rows[threadIdx.x * 9 + i / 2] = pack2(v[i], v[i + 1], f.bf16);
       __syncthreads();
       const int64_t y = at.row - threadIdx.x;
-      uint16_t* to = static_cast<uint16_t*>(at.which ? f.out1 : f.out0) + at.col + c;
+      uint16_t* to = static_cast<uint16_t*>(j.to[at.which]) + at.col + c;
       for (int i = threadIdx.x; i < kHalf * kN; i += kHalf) {
         const int r = i / kN, e = i % kN;
-        if (y + r < f.rows && e < left) to[(y + r) * f.ldo + e] = static_cast<uint16_t>(rows[r * 9 + e / 2] >> (16 * (e % 2)));
+        if (y + r < j.rows && e < left) to[(y + r) * j.ldo + e] = static_cast<uint16_t>(rows[r * 9 + e / 2] >> (16 * (e % 2)));
       }
       return;
     }
   }
-  if (at.row >= f.rows) return;
+  if (at.row >= j.rows) return;
   Ahead<kOut, kKeep> ahead;
   ahead.load(f, at.row, at.col + c);
-  const int64_t to = at.row * (kOut == kStore ? f.ldo : f.pitch) + at.col + c;
-  const Direct sink{{static_cast<uint16_t*>(at.which ? f.out1 : f.out0) + to, static_cast<uint16_t*>(f.out1) + to, static_cast<uint16_t*>(f.out2) + to},
-                    f.bf16, left};
+  const int64_t to = at.row * j.ldo + at.col + c;
+  const Direct sink{{static_cast<uint16_t*>(j.to[at.which]) + to, static_cast<uint16_t*>(j.to[1]) + to, static_cast<uint16_t*>(j.to[2]) + to}, f.bf16, left};
   finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, sink);
 }
 
@@ -802,10 +825,16 @@ Sizes sizes_of(GatedProduct p, const GatedShape& s) {
 }
 struct Plan {
   int64_t tiles_i, tiles_j, stages, segment;
-  int64_t whole, tail, splits, per_split;
+  int64_t whole, tail, splits, per_split;   // tail: tiles that are shared along the reduction
+  int64_t longest() const { return whole > 0 ? stages : per_split; }
 };
-// Whole tiles as long as they fill the device; the rest, less than one tile a pair, is shared along the reduction where
-// that saves more than the partial sums and their launch cost.
+constexpr double kStageUs = 0.37;
+// Whether sharing tiles along the reduction saves more than it costs: a partial sum is written and read at 4 TB/s, behind 4 us for
+// the launch that adds them up.
+bool split_pays(const Plan& l, int64_t tiles, int64_t splits, int64_t per, int64_t rows) {
+  const double saved = kStageUs * static_cast<double>(l.stages - per);
+  return saved > 4.0 + 8.0 * static_cast<double>(tiles * splits * kTile * std::min<int64_t>(kTile, rows)) / 4e6;
+}
 Plan plan_of(GatedProduct p, const GatedShape& s) {
   const Sizes z = sizes_of(p, s);
   Plan l{};
@@ -813,29 +842,70 @@ Plan plan_of(GatedProduct p, const GatedShape& s) {
   l.tiles_j = ceil_div(z.cols, z.gate ? kHalf : kTile);
   l.segment = ceil_div(z.depth, kDepth);
   l.stages = l.segment * z.parts;
-  const int64_t tiles = l.tiles_i * l.tiles_j;
-  l.tail = tiles % kPairs;
-  l.whole = tiles - l.tail;
+  l.whole = l.tiles_i * l.tiles_j;
   l.splits = 1;
   l.per_split = l.stages;
-  if (l.tail > 0) {
-    const int64_t most = std::min<int64_t>({kPairs / l.tail, l.stages / 4, 16});
-    if (most >= 2) {
-      const int64_t per = ceil_div(l.stages, most), splits = ceil_div(l.stages, per);
-      // microseconds: a stage takes 0.37; a partial sum is written and read at 4 TB/s, behind 4 for the launch
-      const double saved = 0.37 * static_cast<double>(l.stages - per);
-      const double cost = 4.0 + 8.0 * static_cast<double>(l.tail * splits * kTile * std::min<int64_t>(kTile, z.rows)) / 4e6;
-      if (saved > cost) {
-        l.splits = splits;
-        l.per_split = per;
-      }
+  return l;
+}
+void share(Plan& l, int64_t tiles, int64_t most, int64_t rows) {
+  most = std::min<int64_t>({most, l.stages / 4, 16});
+  if (most < 2) return;
+  const int64_t per = ceil_div(l.stages, most), splits = ceil_div(l.stages, per);
+  if (!split_pays(l, tiles, splits, per, rows)) return;
+  l.whole -= tiles;
+  l.tail = tiles;
+  l.splits = splits;
+  l.per_split = per;
+}
+// One product: whole tiles as long as they fill the device; the rest, less than one tile a pair, is shared along the reduction where that
+// pays.
+void plan_one(GatedProduct p, const GatedShape& s, Plan& l) {
+  l = plan_of(p, s);
+  const int64_t tail = l.whole % kPairs;
+  if (tail > 0) share(l, tail, kPairs / tail, sizes_of(p, s).rows);
+}
+// Stages that a product by itself takes, with 8 us for sums that are joined and 4 for a launch.
+double stages_alone(const Plan& l) {
+  const int64_t rounds = ceil_div(l.whole, kPairs);
+  return static_cast<double>(rounds * l.stages + (l.tail > 0 ? l.per_split : 0)) + (l.tail > 0 ? 12.0 : 4.0) / kStageUs;
+}
+// Several products side by side: whole tiles, but for a product whose tiles are so few and long that the device would wait for them.
+// Whether that is faster than one after the other, of which each leaves part of the device idle in its last round: 8192 tokens of 1024 x
+// 2816 168 us and 183, 1024 33 and 48, 64 of 640 x 2112 16 and 26; 16384 of 2048 x 5632, fourteen rounds, 1302 and 1246, for what
+// different operands in the second-level cache cost (a twentieth, taken into account).
+bool plan_together(const GatedProduct* p, const GatedShape& s, int n, Plan* l, int* order) {
+  int64_t total = 0;
+  double alone = 0;
+  for (int i = 0; i < n; ++i) {
+    Plan one{};
+    plan_one(p[i], s, one);
+    alone += stages_alone(one);
+    l[i] = plan_of(p[i], s);
+    total += l[i].whole * l[i].stages;
+    order[i] = i;
+  }
+  const int64_t fair = std::max<int64_t>(ceil_div(total, kPairs), 8);
+  bool joins = false;
+  for (int i = 0; i < n; ++i) {
+    if (2 * l[i].stages > 3 * fair) share(l[i], l[i].whole, ceil_div(l[i].stages, fair), sizes_of(p[i], s).rows);
+    joins = joins || l[i].tail > 0;
+  }
+  std::sort(order, order + n, [&](int a, int b) { return l[a].longest() != l[b].longest() ? l[a].longest() > l[b].longest() : a < b; });
+  int64_t tiles = 0;
+  for (int i = 0; i < n; ++i) tiles += l[i].whole;
+  if (tiles > 40 * kPairs) return false;  // little idle in so many rounds, and long to add up
+  // what the pair with the most to do has: item_of's order
+  int64_t load[kPairs] = {}, most = 0, item = 0;
+  for (int i = 0; i < n; ++i) {
+    const Plan& q = l[order[i]];
+    for (int64_t t = 0; t < q.whole + q.tail * q.splits; ++t, ++item) {
+      const int64_t round = item / kPairs, at = item % kPairs;
+      int64_t& mine = load[round > 0 ? kPairs - 1 - at : at];
+      mine += q.longest();
+      most = std::max(most, mine);
     }
   }
-  if (l.splits == 1) {
-    l.whole = tiles;
-    l.tail = 0;
-  }
-  return l;
+  return 1.05 * static_cast<double>(most) + (joins ? 12.0 : 4.0) / kStageUs < alone;
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -861,9 +931,17 @@ bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t ou
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool kAInner, bool kBInner, Out kOut, GatedKeep kKeep>
-cudaError_t run(const Work& w, int64_t tail, cudaStream_t s) {
-  const auto kernel = gated_kernel<kAInner, kBInner, kOut, kKeep>;
+template <Out kOut, GatedKeep kKeep>
+cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_t s) {
+  Work<kJobs<kOut>> w;
+  for (int i = 0; i < kJobs<kOut>; ++i) w.job[i] = all.job[i];
+  w.f = all.f;
+  w.jobs = all.jobs;
+  w.items = all.items;
+  w.partial = all.partial;
+  w.failed = all.failed;
+  w.limit = all.limit;
+  const auto kernel = gated_kernel<kOut, kKeep>;
   static std::atomic<uint64_t> smem_set{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -889,11 +967,42 @@ cudaError_t run(const Work& w, int64_t tail, cudaStream_t s) {
   note_launch();
   e = cudaLaunchKernelEx(&cfg, kernel, w);
   if (e != cudaSuccess || tail == 0) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(tail), w.f.rows > kHalf ? 2 : 1, (kOut == kActivate ? kHalf : kTile) / kTake<kOut, kKeep>);
+  cfg.gridDim = dim3(static_cast<unsigned>(tail), high ? 2 : 1, (kOut == kActivate ? kHalf : kTile) / kTake<kOut, kKeep>);
   cfg.blockDim = dim3(kHalf);
   cfg.dynamicSmemBytes = kJoinSmem<kOut, kKeep>;
   note_launch();
   return cudaLaunchKernelEx(&cfg, gated_join_kernel<kOut, kKeep>, w);
+}
+
+// A product's maps and shape.
+bool make_job(Job& j, const GatedArgs& g, const GatedShape& h) {
+  const Sizes z = sizes_of(g.product, h);
+  j.a_inner = g.product != GatedProduct::kWeightUp && g.product != GatedProduct::kWeightDown;
+  j.b_inner = g.product == GatedProduct::kUp || g.product == GatedProduct::kDown;
+  const GatedOperand a[2] = {g.a0, z.results * z.parts > 1 ? g.a1 : g.a0}, b[2] = {g.b0, z.gate || z.parts > 1 ? g.b1 : g.b0};
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && a[1].data == a[0].data && a[1].ld == a[0].ld) j.a[1] = j.a[0];
+    else if (!make_map(&j.a[i], a[i], j.a_inner ? z.depth : z.rows, j.a_inner ? z.rows : z.depth, j.a_inner ? Box::kInnerK : Box::kOwn, h.bf16))
+      return false;
+    if (i == 1 && b[1].data == b[0].data && b[1].ld == b[0].ld) j.b[1] = j.b[0];
+    else if (!make_map(&j.b[i], b[i], j.b_inner ? z.depth : z.cols, j.b_inner ? z.cols : z.depth, j.b_inner ? Box::kInnerK : Box::kOwn, h.bf16))
+      return false;
+  }
+  // h, dg and du have rows of whole groups; the others are a caller's
+  const bool between = g.product == GatedProduct::kUp || g.product == GatedProduct::kGate;
+  j.to[0] = g.out0;
+  j.to[1] = g.out1;
+  j.to[2] = g.out2;
+  j.rows = z.rows;
+  j.cols = between ? gated_pitch(h.hidden) : z.cols;
+  j.ldo = between ? j.cols : g.ldo;
+  j.wide = j.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out0) | reinterpret_cast<uintptr_t>(g.out1) | reinterpret_cast<uintptr_t>(g.out2)) % 16 == 0;
+  const int results = g.product == GatedProduct::kGate ? 3 : g.product == GatedProduct::kWeightUp ? 2 : 1;
+  for (int i = 0; i < 3; ++i) {
+    if ((i < results) != (j.to[i] != nullptr)) return false;
+    if (i < results && j.wide && !make_map(&j.out[i], {j.to[i], j.ldo}, j.cols, z.rows, Box::kResult, h.bf16)) return false;
+  }
+  return j.wide || !between;
 }
 
 }  // namespace
@@ -902,9 +1011,19 @@ int64_t gated_kept_bytes(const GatedShape& s) {
   const int64_t n = s.tokens * gated_pitch(s.hidden);
   return s.keep == GatedKeep::kNone ? 0 : s.keep == GatedKeep::kWide ? 6 * n : 2 * n + 8 * (n / kGroup8);
 }
-int64_t gated_partial_bytes(GatedProduct p, const GatedShape& s) {
-  const Plan l = plan_of(p, s);
-  return l.tail * l.splits * kTile * kTile * 4;
+int64_t gated_partial_bytes(const GatedProduct* p, int n, const GatedShape& s) {
+  Plan l[kMostJobs];
+  int order[kMostJobs];
+  int64_t parts = 0;
+  if (n > 1 && plan_together(p, s, n, l, order)) {
+    for (int i = 0; i < n; ++i) parts += l[i].tail * l[i].splits;
+  } else {
+    for (int i = 0; i < n; ++i) {
+      plan_one(p[i], s, l[i]);
+      parts = std::max(parts, l[i].tail * l[i].splits);
+    }
+  }
+  return parts * kTile * kTile * 4;
 }
 
 cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, cudaStream_t s) {
@@ -923,74 +1042,74 @@ cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s) {
-  const GatedShape& h = g.shape;
-  if (h.tokens <= 0 || h.width <= 0 || h.hidden <= 0 || encode_tiled() == nullptr) return cudaErrorInvalidValue;
-  const Sizes z = sizes_of(g.product, h);
-  const Plan l = plan_of(g.product, h);
-  if (l.tiles_i * l.tiles_j * 16 + 1 > 0x7FFFFFFF || z.depth > 0x3FFFFFFF) return cudaErrorInvalidValue;
+cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaStream_t s) {
+  const GatedShape& h = r.shape;
+  if (n < 1 || n > kMostJobs || h.tokens <= 0 || h.width <= 0 || h.hidden <= 0 || encode_tiled() == nullptr) return cudaErrorInvalidValue;
   // a thread that has made no call of the runtime yet, such as autograd's, has no context, and maps need one
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess) e = cudaSetDevice(device);
   if (e != cudaSuccess) return e;
-  Work w{};
-  const bool a_inner = g.product != GatedProduct::kWeightUp && g.product != GatedProduct::kWeightDown;
-  const bool b_inner = g.product == GatedProduct::kUp || g.product == GatedProduct::kDown;
-  const GatedOperand a[2] = {g.a0, z.results * z.parts > 1 ? g.a1 : g.a0}, b[2] = {g.b0, z.gate || z.parts > 1 ? g.b1 : g.b0};
-  for (int i = 0; i < 2; ++i) {
-    if (i == 1 && a[1].data == a[0].data && a[1].ld == a[0].ld) w.a[1] = w.a[0];
-    else if (!make_map(&w.a[i], a[i], a_inner ? z.depth : z.rows, a_inner ? z.rows : z.depth, a_inner ? Box::kInnerK : Box::kOwn, h.bf16))
-      return cudaErrorInvalidValue;
-    if (i == 1 && b[1].data == b[0].data && b[1].ld == b[0].ld) w.b[1] = w.b[0];
-    else if (!make_map(&w.b[i], b[i], b_inner ? z.depth : z.cols, b_inner ? z.cols : z.depth, b_inner ? Box::kInnerK : Box::kOwn, h.bf16))
-      return cudaErrorInvalidValue;
+  GatedProduct p[kMostJobs];
+  Plan l[kMostJobs];
+  int order[kMostJobs];
+  for (int i = 0; i < n; ++i) {
+    p[i] = g[i].product;
+    if (n > 1 && (p[i] == GatedProduct::kUp || p[i] == GatedProduct::kGate)) return cudaErrorInvalidValue;
   }
-  w.f.out0 = g.out0;
-  w.f.out1 = g.out1;
-  w.f.out2 = g.out2;
-  w.f.ldo = g.ldo;
-  // h, dg and du have rows of whole groups; the others are a caller's
-  const bool between = g.product == GatedProduct::kUp || g.product == GatedProduct::kGate;
-  const int64_t ldo = between ? gated_pitch(h.hidden) : g.ldo;
-  w.f.wide = ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out0) | reinterpret_cast<uintptr_t>(g.out1) | reinterpret_cast<uintptr_t>(g.out2)) % 16 == 0;
-  if (between && !w.f.wide) return cudaErrorInvalidValue;
-  void* const outs[3] = {g.out0, g.out1, g.out2};
-  for (int i = 0; i < 3; ++i)
-    if (w.f.wide && outs[i] != nullptr && !make_map(&w.out[i], {outs[i], ldo}, between ? ldo : z.cols, z.rows, Box::kResult, h.bf16)) return cudaErrorInvalidValue;
+  if (n == 1) {
+    plan_one(p[0], h, l[0]);
+    order[0] = 0;
+  } else if (!plan_together(p, h, n, l, order)) {
+    for (int i = 0; i < n && e == cudaSuccess; ++i) e = launch_gated(g + i, 1, r, s);
+    return e;
+  }
+  Work<kMostJobs> w{};
+  int64_t items = 0, parts = 0, joins = 0;
+  bool high = false;
+  for (int i = 0; i < n; ++i) {
+    const Plan& q = l[order[i]];
+    Job& j = w.job[i];
+    if (!make_job(j, g[order[i]], h) || q.stages > 0x3FFFFFFF) return cudaErrorInvalidValue;
+    j.tiles_i = static_cast<int>(q.tiles_i);
+    j.tiles_j = static_cast<int>(q.tiles_j);
+    j.rows_segment = static_cast<int>(q.tiles_i / (p[order[i]] == GatedProduct::kWeightUp ? 2 : 1));
+    j.stages = static_cast<int>(q.stages);
+    j.segment = static_cast<int>(q.segment);
+    j.first = static_cast<int>(items);
+    j.whole = static_cast<int>(q.whole);
+    j.splits = static_cast<int>(q.splits);
+    j.per_split = static_cast<int>(q.per_split);
+    j.part = static_cast<int>(parts);
+    j.join = static_cast<int>(joins);
+    items += q.whole + q.tail * q.splits;
+    parts += q.tail * q.splits;
+    joins += q.tail;
+    high = high || (q.tail > 0 && j.rows > kHalf);
+    if (items + kPairs > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  }
+  w.jobs = n;
+  w.items = static_cast<int>(items);
   w.f.bf16 = h.bf16;
   const double log2e = 1.4426950408889634, gelu = 1.5957691216057308;  // 2 sqrt(2 / pi)
   w.f.curve = h.activation == GatedActivation::kSilu ? Curve{static_cast<float>(-log2e), 0.f}
                                                      : Curve{static_cast<float>(-log2e * gelu), static_cast<float>(-log2e * gelu * 0.044715)};
-  w.f.kept = static_cast<char*>(g.kept);
-  w.f.rows = z.rows;
-  w.f.cols = z.cols;
+  w.f.kept = static_cast<char*>(r.kept);
+  w.f.rows = h.tokens;
   w.f.pitch = gated_pitch(h.hidden);
-  w.tiles_i = static_cast<int>(l.tiles_i);
-  w.tiles_j = static_cast<int>(l.tiles_j);
-  w.rows_segment = static_cast<int>(l.tiles_i / z.results);
-  w.stages = static_cast<int>(l.stages);
-  w.segment = static_cast<int>(l.segment);
-  w.whole = static_cast<int>(l.whole);
-  w.splits = static_cast<int>(l.splits);
-  w.per_split = static_cast<int>(l.per_split);
-  w.items = static_cast<int>(l.whole + l.tail * l.splits);
-  w.partial = g.partial;
-  w.failed = g.failed;
-  w.limit = g.wait_limit >= 0 ? g.wait_limit : kWaitLimit;
-  switch (g.product) {
+  w.partial = r.partial;
+  w.failed = r.failed;
+  w.limit = r.wait_limit >= 0 ? r.wait_limit : kWaitLimit;
+  switch (p[0]) {
     case GatedProduct::kUp:
       switch (h.keep) {
-        case GatedKeep::kNone: return run<true, true, kActivate, GatedKeep::kNone>(w, l.tail, s);
-        case GatedKeep::kWide: return run<true, true, kActivate, GatedKeep::kWide>(w, l.tail, s);
-        default: return run<true, true, kActivate, GatedKeep::kEight>(w, l.tail, s);
+        case GatedKeep::kNone: return run<kActivate, GatedKeep::kNone>(w, joins, high, s);
+        case GatedKeep::kWide: return run<kActivate, GatedKeep::kWide>(w, joins, high, s);
+        default: return run<kActivate, GatedKeep::kEight>(w, joins, high, s);
       }
-    case GatedProduct::kDown: return run<true, true, kStore, GatedKeep::kNone>(w, l.tail, s);
     case GatedProduct::kGate:
-      return h.keep == GatedKeep::kEight ? run<true, false, kDerive, GatedKeep::kEight>(w, l.tail, s)
-                                         : run<true, false, kDerive, GatedKeep::kWide>(w, l.tail, s);
-    case GatedProduct::kInput: return run<true, false, kStore, GatedKeep::kNone>(w, l.tail, s);
-    default: return run<false, false, kStore, GatedKeep::kNone>(w, l.tail, s);
+      return h.keep == GatedKeep::kEight ? run<kDerive, GatedKeep::kEight>(w, joins, high, s) : run<kDerive, GatedKeep::kWide>(w, joins, high, s);
+    default: return run<kStore, GatedKeep::kNone>(w, joins, high, s);
   }
 }
 

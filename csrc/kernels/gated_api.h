@@ -41,17 +41,20 @@ struct GatedOperand {
 };
 struct GatedArgs {
   GatedProduct product;
-  GatedShape shape;
   GatedOperand a0, a1, b0, b1;
   void *out0, *out1, *out2;
-  int64_t ldo;          // of the outputs
+  int64_t ldo;          // of the outputs; of h, dg and du gated_pitch
+};
+struct GatedLaunch {
+  GatedShape shape;
   void* kept;
   float* partial;       // gated_partial_bytes
   uint32_t* failed;     // set to 1 where a wait runs out, whose tiles then are NaN; or null
   int64_t wait_limit;   // cycles of a quarter of a wait; negative: about a second in all
 };
-int64_t gated_partial_bytes(GatedProduct p, const GatedShape& s);
-cudaError_t launch_gated(const GatedArgs& g, cudaStream_t s);
+// One product, or up to three of kDown, kInput, kWeightUp and kWeightDown: side by side where that is faster.
+int64_t gated_partial_bytes(const GatedProduct* p, int n, const GatedShape& s);
+cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaStream_t s);
 
 // Matrices of 16-bit numbers whose rows are not 16-byte aligned (or whose numbers do not lie side by side) copied to ones that are,
 // up to five in one launch.
@@ -79,10 +82,10 @@ struct GatedFew {
 };
 cudaError_t launch_gated_few(const GatedFew& g, cudaStream_t s);
 
-// The same in fp32, between products of their own (kernels/gate_f32.cu): h of n numbers g and u; with dh, their gradients too.
-cudaError_t launch_gate_f32(const float* g, const float* u, float* h, int64_t n, GatedActivation act, cudaStream_t s);
-cudaError_t launch_gate_f32_backward(const float* g, const float* u, const float* dh, float* dg, float* du, int64_t n, GatedActivation act,
-                                     cudaStream_t s);
+// The same in fp32, between products of their own (kernels/gate_f32.cu): rows of g and u, `ld` numbers apart, to rows of h; rows of
+// g with u behind them and dh to rows of dg with du behind them.
+cudaError_t launch_gate_f32(const float* g, const float* u, int64_t ld, float* h, int64_t rows, int64_t cols, GatedActivation act, cudaStream_t s);
+cudaError_t launch_gate_f32_backward(const float* gu, const float* dh, float* dgu, int64_t rows, int64_t cols, GatedActivation act, cudaStream_t s);
 
 }  // namespace kern
 }  // namespace mccl

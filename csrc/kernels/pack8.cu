@@ -12,50 +12,44 @@ namespace mccl {
 namespace kern {
 namespace {
 
-constexpr int kThreads = 256, kLanes = 4;       // threads of a block, and of a group: two runs of eight numbers each, 32 apart
+constexpr int kThreads = 256;
+
+// ---- rows that are whole groups, one behind the other, aligned: one long row --------------------------------------
+constexpr int kLanes = 4;                       // threads of a group: two runs of eight numbers each, 32 apart
 constexpr int kUnits = kThreads / kLanes;       // groups a block has in hand at a time
 constexpr int kDeep = 2;                        // groups of a thread in flight
 constexpr int kTurn = kUnits * kDeep;           // groups of a block's turn
 
-// Where a group lies.  Rows that are whole groups, one behind the other, are one row.
-struct Steps {
-  int64_t all, groups;    // of the whole, of a row
+// A group's scale, in the lane `sub` 0 of it, and what its numbers are multiplied with, from the bits of its largest magnitude: scale8
+// with its two quotients in two lanes.
+struct Shared8 {
+  float scale, inverse;
 };
-struct Place {
-  int64_t row;
-  int64_t col;
-  __device__ __forceinline__ Place(const Steps& t, int64_t unit, bool linear) {
-    if (linear) {
-      row = 0;
-      col = unit * kGroup8;
-    } else {
-      row = t.all <= 0xFFFFFFFFll ? static_cast<uint32_t>(unit) / static_cast<uint32_t>(t.groups) : unit / t.groups;
-      col = (unit - row * t.groups) * kGroup8;
-    }
-  }
-};
-__device__ __forceinline__ int present(int64_t cols, int64_t col, bool there) {
-  return there ? static_cast<int>(min(max(cols - col, static_cast<int64_t>(0)), static_cast<int64_t>(8))) : 0;
+template <int kOver>
+__device__ __forceinline__ Shared8 shared8(uint32_t bits, int sub) {
+#pragma unroll
+  for (int m = kOver / 2; m > 0; m /= 2) bits = max(bits, __shfl_xor_sync(0xFFFFFFFFu, bits, m));
+  const float most = __uint_as_float(bits);
+  const bool finite = most < INFINITY, kept = finite && most >= kTiny8;
+  const float quotient = __fdiv_rn(sub == 0 ? most : 127.f, sub == 0 ? 127.f : most);
+  const float inverse = __shfl_sync(0xFFFFFFFFu, quotient, 1, kOver);
+  return {kept ? quotient : finite ? 0.f : NAN, kept ? inverse : 0.f};
 }
 
 // Bound by memory: one pass, 2 (4) bytes read and 1 + 1/16 written for each number.  Four lanes share a group, so that few
 // instructions are spent on what a group needs once; kDeep groups of each are in flight before the first is looked at.
-template <typename T, bool kLinear>
-__global__ void __launch_bounds__(kThreads, 4) pack8_kernel(const T* __restrict__ x, int64_t ld, bool vec, const Packed8Rows p, const Steps t) {
+// 16384 x 5632 bf16 to codes 46 us, back 40 (B200; 5.9 and 6.7 TB/s).
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) pack8_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, int64_t all) {
   const int sub = threadIdx.x % kLanes;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTurn; base < t.all; base += static_cast<int64_t>(gridDim.x) * kTurn) {
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kTurn; base < all; base += static_cast<int64_t>(gridDim.x) * kTurn) {
     const int64_t unit = base + threadIdx.x / kLanes;
     float v[kDeep][2][8];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int64_t u = unit + d * kUnits;
-      const Place at(t, u < t.all ? u : 0, kLinear);
-      const int64_t col = at.col + sub * 8;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const T* from = x + at.row * ld + col + 32 * h;
-        load_run<T, 8>(from, kLinear ? (u < t.all ? 8 : 0) : present(p.cols, col + 32 * h, u < t.all), kLinear || vec, v[d][h]);
-      }
+      for (int h = 0; h < 2; ++h) load_run<T, 8>(x + u * kGroup8 + sub * 8 + 32 * h, u < all ? 8 : 0, true, v[d][h]);
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
@@ -64,92 +58,189 @@ __global__ void __launch_bounds__(kThreads, 4) pack8_kernel(const T* __restrict_
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 8; ++i) bits = most8(bits, v[d][h][i]);
-#pragma unroll
-      for (int m = kLanes / 2; m > 0; m /= 2) bits = max(bits, __shfl_xor_sync(0xFFFFFFFFu, bits, m));
-      // scale8, its two quotients in two lanes
-      const float most = __uint_as_float(bits);
-      const bool finite = most < INFINITY, kept = finite && most >= kTiny8;
-      const float quotient = __fdiv_rn(sub == 0 ? most : 127.f, sub == 0 ? 127.f : most);
-      const float shared = __shfl_sync(0xFFFFFFFFu, quotient, 1, kLanes), inverse = kept ? shared : 0.f;
+      const Shared8 s = shared8<kLanes>(bits, sub);
       const int64_t u = unit + d * kUnits;
-      if (u >= t.all) continue;
-      const Place at(t, u, kLinear);
-      const int64_t col = at.col + sub * 8;
+      if (u >= all) continue;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (kLinear || col + 32 * h < p.pitch)
-          *reinterpret_cast<uint2*>(p.codes + at.row * p.pitch + col + 32 * h) =
-              make_uint2(codes8(v[d][h][0], v[d][h][1], v[d][h][2], v[d][h][3], inverse), codes8(v[d][h][4], v[d][h][5], v[d][h][6], v[d][h][7], inverse));
-      if (sub == 0) p.scales[u] = kept ? quotient : finite ? 0.f : NAN;
+        *reinterpret_cast<uint2*>(codes + u * kGroup8 + sub * 8 + 32 * h) =
+            make_uint2(codes8(v[d][h][0], v[d][h][1], v[d][h][2], v[d][h][3], s.inverse), codes8(v[d][h][4], v[d][h][5], v[d][h][6], v[d][h][7], s.inverse));
+      if (sub == 0) scales[u] = s.scale;
     }
   }
 }
 
-template <typename T, bool kLinear>
-__global__ void __launch_bounds__(kThreads, 4) unpack8_kernel(const Packed8Rows p, T* __restrict__ x, int64_t ld, bool vec, const Steps t) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) unpack8_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ x, int64_t all) {
   const int sub = threadIdx.x % kLanes;
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kTurn + threadIdx.x / kLanes; unit < t.all; unit += static_cast<int64_t>(gridDim.x) * kTurn) {
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kTurn + threadIdx.x / kLanes; unit < all; unit += static_cast<int64_t>(gridDim.x) * kTurn) {
     uint2 word[kDeep][2];
     float scale[kDeep];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int64_t u = unit + d * kUnits;
-      const bool there = u < t.all;
-      const Place at(t, there ? u : 0, kLinear);
-      const int64_t col = at.col + sub * 8;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        word[d][h] = there && (kLinear || col + 32 * h < p.cols) ? __ldcs(reinterpret_cast<const uint2*>(p.codes + at.row * p.pitch + col + 32 * h))
-                                                                 : make_uint2(0u, 0u);
-      scale[d] = there ? p.scales[u] : 0.f;
+      for (int h = 0; h < 2; ++h) word[d][h] = u < all ? __ldcs(reinterpret_cast<const uint2*>(codes + u * kGroup8 + sub * 8 + 32 * h)) : make_uint2(0u, 0u);
+      scale[d] = u < all ? scales[u] : 0.f;
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int64_t u = unit + d * kUnits;
-      const Place at(t, u < t.all ? u : 0, kLinear);
-      const int64_t col = at.col + sub * 8;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = value8(i < 4 ? word[d][h].x : word[d][h].y, i & 3, scale[d]);
-        store_run<T, 8>(x + at.row * ld + col + 32 * h, kLinear ? (u < t.all ? 8 : 0) : present(p.cols, col + 32 * h, u < t.all), kLinear || vec, v);
+        store_run<T, 8>(x + u * kGroup8 + sub * 8 + 32 * h, u < all ? 8 : 0, true, v);
       }
     }
   }
 }
 
-constexpr int kSms = 148;
-struct Shape {
-  int blocks;
-  bool vec, linear;
-  Steps t;
+// ---- any rows -----------------------------------------------------------------------------------------------------
+// Sixteen lanes share a group and have every sixteenth of its numbers, so that neighbours read and write neighbours wherever a row
+// begins.  (Runs of eight a lane, one number at a time: 9349 x 2731 fp16 to codes and back 141 us.)
+constexpr int kWideLanes = 16, kEach = kGroup8 / kWideLanes, kWideUnits = kThreads / kWideLanes, kWideDeep = 4;
+
+// Where a group lies.  Steps from one to the next are divided by the groups of a row on the host.
+struct Place {
+  int64_t row;
+  int group;
 };
-// One row (`linear`) where rows are whole groups that follow each other, aligned: no division, no ends inside of a group.
-Shape shape_of(const Packed8Rows& p, const void* x, int64_t ld, size_t size) {
-  Shape s{};
-  s.vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * static_cast<int64_t>(size) % 16 == 0;
-  s.linear = s.vec && p.cols % kGroup8 == 0 && p.pitch == p.cols && (ld == p.cols || p.rows == 1);
-  s.t.groups = pack8_groups(p.cols);
-  s.t.all = p.rows * s.t.groups;
-  s.blocks = static_cast<int>(std::min<int64_t>((s.t.all + kTurn - 1) / kTurn, 32 * kSms));
-  return s;
+struct Steps {
+  int64_t all, groups;    // of the whole, of a row
+  int64_t unit_rows, turn_rows;
+  int unit_groups, turn_groups;   // from one of a thread's groups to the next, and from one of its turns
+};
+__device__ __forceinline__ Place onward(const Place& p, int64_t rows, int by, const Steps& t) {
+  Place n{p.row + rows, p.group + by};
+  if (n.group >= t.groups) {
+    n.group -= static_cast<int>(t.groups);
+    ++n.row;
+  }
+  return n;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pack8_rows_kernel(const T* __restrict__ x, int64_t ld, const Packed8Rows p, const Steps t) {
+  const int sub = threadIdx.x % kWideLanes;
+  constexpr int kStep = kWideUnits * kWideDeep;
+  int64_t unit = static_cast<int64_t>(blockIdx.x) * kStep + threadIdx.x / kWideLanes;
+  Place turn{unit / t.groups, 0};
+  turn.group = static_cast<int>(unit - turn.row * t.groups);
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kStep; base < t.all;
+       base += static_cast<int64_t>(gridDim.x) * kStep, unit += static_cast<int64_t>(gridDim.x) * kStep) {
+    float v[kWideDeep][kEach];
+    Place at = turn;
+#pragma unroll
+    for (int d = 0; d < kWideDeep; ++d) {
+      const int64_t col = at.group * static_cast<int64_t>(kGroup8) + sub;
+      const T* from = x + at.row * ld + col;
+      const int64_t left = unit + d * kWideUnits < t.all ? p.cols - col : 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) v[d][i] = kWideLanes * i < left ? Traits<T>::load(from[kWideLanes * i]) : 0.f;
+      at = onward(at, t.unit_rows, t.unit_groups, t);
+    }
+    at = turn;
+#pragma unroll
+    for (int d = 0; d < kWideDeep; ++d) {
+      uint32_t bits = 0u;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) bits = most8(bits, v[d][i]);
+      const Shared8 s = shared8<kWideLanes>(bits, sub);
+      const uint32_t word = codes8(v[d][0], v[d][1], v[d][2], v[d][3], s.inverse);
+      if (unit + d * kWideUnits < t.all) {
+        const int64_t col = at.group * static_cast<int64_t>(kGroup8) + sub;
+        int8_t* to = p.codes + at.row * p.pitch + col;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (col + kWideLanes * i < p.pitch) to[kWideLanes * i] = static_cast<int8_t>(word >> (8 * i));
+        if (sub == 0) p.scales[at.row * t.groups + at.group] = s.scale;
+      }
+      at = onward(at, t.unit_rows, t.unit_groups, t);
+    }
+    turn = onward(turn, t.turn_rows, t.turn_groups, t);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) unpack8_rows_kernel(const Packed8Rows p, T* __restrict__ x, int64_t ld, const Steps t) {
+  const int sub = threadIdx.x % kWideLanes;
+  constexpr int kStep = kWideUnits * kWideDeep;
+  int64_t unit = static_cast<int64_t>(blockIdx.x) * kStep + threadIdx.x / kWideLanes;
+  Place turn{unit / t.groups, 0};
+  turn.group = static_cast<int>(unit - turn.row * t.groups);
+  for (; unit < t.all; unit += static_cast<int64_t>(gridDim.x) * kStep) {
+    int8_t code[kWideDeep][kEach];
+    float scale[kWideDeep];
+    Place at = turn;
+#pragma unroll
+    for (int d = 0; d < kWideDeep; ++d) {
+      const int64_t col = at.group * static_cast<int64_t>(kGroup8) + sub, left = unit + d * kWideUnits < t.all ? p.cols - col : 0;
+      const int8_t* from = p.codes + at.row * p.pitch + col;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) code[d][i] = kWideLanes * i < left ? from[kWideLanes * i] : static_cast<int8_t>(0);
+      scale[d] = left > 0 ? p.scales[at.row * t.groups + at.group] : 0.f;
+      at = onward(at, t.unit_rows, t.unit_groups, t);
+    }
+    at = turn;
+#pragma unroll
+    for (int d = 0; d < kWideDeep; ++d) {
+      const int64_t col = at.group * static_cast<int64_t>(kGroup8) + sub, left = unit + d * kWideUnits < t.all ? p.cols - col : 0;
+      T* to = x + at.row * ld + col;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (kWideLanes * i < left) to[kWideLanes * i] = Traits<T>::store(static_cast<float>(code[d][i]) * scale[d]);
+      at = onward(at, t.unit_rows, t.unit_groups, t);
+    }
+    turn = onward(turn, t.turn_rows, t.turn_groups, t);
+  }
+}
+
+constexpr int kSms = 148;
+int blocks_for(int64_t all, int per) { return static_cast<int>(std::min<int64_t>((all + per - 1) / per, 32 * kSms)); }
+// Rows that are whole groups, follow each other and are aligned.
+bool one_row(const Packed8Rows& p, const void* x, int64_t ld, size_t size) {
+  return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && p.cols % kGroup8 == 0 && p.pitch == p.cols && (ld == p.cols || p.rows == 1) &&
+         p.cols * static_cast<int64_t>(size) % 16 == 0;
+}
+Steps steps_of(const Packed8Rows& p, int& blocks) {
+  Steps t{};
+  constexpr int kStep = kWideUnits * kWideDeep;
+  t.groups = pack8_groups(p.cols);
+  t.all = p.rows * t.groups;
+  blocks = blocks_for(t.all, kStep);
+  t.unit_rows = kWideUnits / t.groups;
+  t.unit_groups = static_cast<int>(kWideUnits % t.groups);
+  t.turn_rows = static_cast<int64_t>(blocks) * kStep / t.groups;
+  t.turn_groups = static_cast<int>(static_cast<int64_t>(blocks) * kStep % t.groups);
+  return t;
 }
 
 template <typename T>
 cudaError_t pack(const void* x, int64_t ld, const Packed8Rows& p, cudaStream_t s) {
-  const Shape h = shape_of(p, x, ld, sizeof(T));
   note_launch();
-  if (h.linear) pack8_kernel<T, true><<<h.blocks, kThreads, 0, s>>>(static_cast<const T*>(x), ld, h.vec, p, h.t);
-  else pack8_kernel<T, false><<<h.blocks, kThreads, 0, s>>>(static_cast<const T*>(x), ld, h.vec, p, h.t);
+  if (one_row(p, x, ld, sizeof(T))) {
+    const int64_t all = p.rows * pack8_groups(p.cols);
+    pack8_kernel<T><<<blocks_for(all, kTurn), kThreads, 0, s>>>(static_cast<const T*>(x), p.codes, p.scales, all);
+  } else {
+    int blocks = 0;
+    const Steps t = steps_of(p, blocks);
+    pack8_rows_kernel<T><<<blocks, kThreads, 0, s>>>(static_cast<const T*>(x), ld, p, t);
+  }
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t unpack(const Packed8Rows& p, void* x, int64_t ld, cudaStream_t s) {
-  const Shape h = shape_of(p, x, ld, sizeof(T));
   note_launch();
-  if (h.linear) unpack8_kernel<T, true><<<h.blocks, kThreads, 0, s>>>(p, static_cast<T*>(x), ld, h.vec, h.t);
-  else unpack8_kernel<T, false><<<h.blocks, kThreads, 0, s>>>(p, static_cast<T*>(x), ld, h.vec, h.t);
+  if (one_row(p, x, ld, sizeof(T))) {
+    const int64_t all = p.rows * pack8_groups(p.cols);
+    unpack8_kernel<T><<<blocks_for(all, kTurn), kThreads, 0, s>>>(p.codes, p.scales, static_cast<T*>(x), all);
+  } else {
+    int blocks = 0;
+    const Steps t = steps_of(p, blocks);
+    unpack8_rows_kernel<T><<<blocks, kThreads, 0, s>>>(p, static_cast<T*>(x), ld, t);
+  }
   return cudaGetLastError();
 }
 

@@ -102,8 +102,8 @@ def test_a_ddp_step_under_autocast_runs_on_the_kernels(checkpoint):
             with torch.autocast("cuda", dtype=torch.bfloat16):
                 loss = model(x, y)
             loss.backward()
-            # a layer's heads take three launches, its gated block six, packed rows three times two more
-            assert native._kernel_launches() - before >= 4 * (15 if checkpoint else 9)
+            # a layer's heads take three launches, its gated block four, packed rows three times two more
+            assert native._kernel_launches() - before >= 4 * (13 if checkpoint else 7)
             opt.step()
             losses.append(loss.item())
         assert losses[-1] < losses[0] - 2
