@@ -490,7 +490,12 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
 }
 // A pair of CTAs per tile of 256 x 256, tiles in turn: each CTA loads half of either operand's rows and has half of the
 // accumulator's; the first one issues the products of both.  Two accumulators, so that a tile is taken out while the next one
-// is multiplied.
+// is multiplied.  A stage is 64 KB for 8.4 million multiplications: what passes through the second-level cache, 13.5 TB/s of it, bounds
+// all of them.  8192 x 1024 x 2816 bf16 (B200, by itself): up 61 us without, 77 with three kept bytes, 70 with codes (1.55, 1.23, 1.35
+// PFLOP/s), down 33 (1.42), gate 75 and 70 (0.63: 12 or 8 bytes a number of its own beside the operands, 10.8 TB/s), the last three 168
+// (1.40); 16384 x 2048 x 5632 up 545 (1.39), down 240 (1.58), gate 379, the last three 1250 (1.51).
+// Left: 16 warps to take the accumulators out (no faster, 397 for 339 of the wide gate), what was kept asked for two runs ahead through
+// shared memory (72 for 75, but 418 for 379 of the wide one, which has then a stage less) or a tile ahead into the second-level cache.
 template <Out kOut, GatedKeep kKeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   constexpr int kDepths = kStages<kOut>, kOuts = kBoxes<kOut>;

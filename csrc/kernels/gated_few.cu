@@ -73,7 +73,7 @@ __device__ __forceinline__ uint4 eight(const T* row, int64_t at, int64_t depth, 
 // kGroups groups of 8 tokens (the last ones may be none).  kUp: gate and up and what follows them, else one product of h.
 template <typename T, int kGroups, bool kUp, bool kVec>
 __global__ void __launch_bounds__(kThreads, kGroups == 2 ? 3 : 2) few_kernel(const Few w) {
-  constexpr int kX = kUp ? 1 : 2, kW = kUp ? 2 : 1, kAhead = !kUp && kGroups == 1 ? 8 : 4;
+  constexpr int kX = kUp ? 1 : 2, kW = kUp ? 2 : 1, kAhead = !kUp && kGroups == 1 && kVec ? 8 : 4;
   constexpr int kHeld = kUp ? 4 : 2;  // accumulators of a lane and group that mean something
   __shared__ float part[kWarps][kGroups][kHeld][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;

@@ -7,7 +7,9 @@
 //
 // Bound by memory.  A team of lanes, 8 pairs each, has a row in registers; both members of a pair are in the same lane, so the
 // rotation moves nothing between lanes and the norm is the only sum over a team.  A team takes several heads of its token, for
-// which the angles stay in registers.
+// which the angles stay in registers.  32768 tokens of 40 heads of 128, bf16: forward 129 us (5.2 TB/s), backward, values copied, 269
+// (4.2); 8192 tokens of 32 heads of 64 15 and 37 us (B200; 4.6 and 3.6 TB/s).  Backward half of the issue slots are busy, half of the
+// time for want of numbers: its two rows and two gradients a lane in flight are what 128 registers hold.
 #include <algorithm>
 #include <type_traits>
 

@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from .. import require_native
+from ._native import native
 
 GROUP = 64
 _TINY = 2.0 ** -100
@@ -41,7 +41,7 @@ def pack8(x: torch.Tensor) -> Packed8:
     """``x`` in 8 bits.  Not differentiable: what is kept is no function of the graph."""
     _check(x)
     if x.is_cuda:
-        codes, scales = require_native()._pack8(x)
+        codes, scales = native()._pack8(x)
         return Packed8(codes, scales, tuple(x.shape), x.dtype)
     x = x.detach()
     cols = x.shape[-1] if x.dim() else 1
@@ -60,7 +60,7 @@ def pack8(x: torch.Tensor) -> Packed8:
 def unpack8(packed: Packed8) -> torch.Tensor:
     """The values, in the shape and type that they had."""
     if packed.codes.is_cuda:
-        return require_native()._unpack8(packed.codes, packed.scales, list(packed.shape), packed.dtype)
+        return native()._unpack8(packed.codes, packed.scales, list(packed.shape), packed.dtype)
     rows, pitch = packed.codes.shape
     cols = packed.shape[-1] if packed.shape else 1
     scale = packed.scales.repeat_interleave(GROUP, 1)[:, :cols]

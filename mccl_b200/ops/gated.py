@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .. import require_native
+from ._native import native
 from .checkpoint import Packed8, pack8, unpack8
 
 ACTIVATIONS = ("silu", "gelu_tanh")
@@ -41,8 +41,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
             to = torch.get_autocast_dtype("cuda")
             x, w_gate, w_up, w_down = x.to(to), w_gate.to(to), w_up.to(to), w_down.to(to)
             with torch.autocast("cuda", enabled=False):
-                return require_native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
-        return require_native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+                return native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+        return native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
     return _Plain.apply(x, w_gate, w_up, w_down, activation, checkpoint is not None)
 
 

@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .. import require_native
+from ._native import native
 
 
 def rotary_table(positions: int, rotary: int, *, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -36,7 +36,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weig
     ``positions``: int64 or int32, [tokens] or [batch, tokens]; 0, 1, ... in each batch without it.
     """
     if q.is_cuda:
-        return require_native()._norm_rotate(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+        return native()._norm_rotate(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     if not eps > 0:
         raise ValueError("eps must be positive")
     return (_plain(q, q_weight, table, positions, eps, interleaved), _plain(k, k_weight, table, positions, eps, interleaved))
@@ -48,7 +48,7 @@ def norm_rotate_packed(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
     """:func:`norm_rotate` of one projection [batch, tokens, (heads + 2 kv_heads) * dim]; also the view of its values."""
     kv_heads = heads if kv_heads is None else kv_heads
     if qkv.is_cuda:
-        return require_native()._norm_rotate_packed(qkv, q_weight, k_weight, table, positions, heads, kv_heads, eps, interleaved)
+        return native()._norm_rotate_packed(qkv, q_weight, k_weight, table, positions, heads, kv_heads, eps, interleaved)
     if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[-1] % (heads + 2 * kv_heads):
         raise ValueError(f"norm_rotate_packed: [batch, tokens, (heads + 2 kv_heads) dim] expected, got {tuple(qkv.shape)}")
     q, k, v = qkv.unflatten(-1, (heads + 2 * kv_heads, -1)).split((heads, kv_heads, kv_heads), 2)

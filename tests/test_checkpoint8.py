@@ -104,6 +104,18 @@ def test_another_stream_and_a_graph():
     assert torch.equal(again, -want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [65536, 65541])
+def test_more_than_two_to_the_31_numbers(cols):
+    rows = 33000
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = _data((3, cols), torch.bfloat16, "cuda", seed=4)
+    x[5] = 1
+    back = unpack8(pack8(x))
+    assert torch.equal(back[-3:], unpack8(pack8(x[-3:].clone()))) and not back[-4].any() and not back[6].any()
+    assert ((back[5] - 1).abs() <= 2.0 ** -8).all()
+
+
 def test_refusals_on_cpu():
     with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
         pack8(torch.zeros(3, dtype=torch.float64))

@@ -199,6 +199,19 @@ def test_many_tiles(tokens, width, hidden):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("eight", [None, "int8"])
+def test_what_is_kept_beyond_31_bits(eight):
+    tokens, width, hidden = 400_000 if eight is None else 1_100_000, 16, 1000
+    *args, dy = _inputs(tokens, width, hidden, torch.bfloat16)
+    last = [args[0][-300:].clone(), *args[1:]]
+    want = _want(*last, dy[-300:], "silu", eight is not None, Rounding(torch.bfloat16))
+    x = args[0].requires_grad_()
+    y = gated_feed_forward(x, *args[1:], checkpoint=eight)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    _check({"y": y[-300:], "dx": dx[-300:]}, {k: want[k] for k in ("y", "dx")})
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_gradients_asked_for_alone(dtype):
     *args, dy = _inputs(150, 72, 200, dtype)

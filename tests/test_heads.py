@@ -78,6 +78,7 @@ CASES = [
     (1, 40, 2, 2, 31, 14, True), (2, 5, 1, 1, 1, 0, False), (2, 5, 2, 1, 2, 2, True), (1, 33, 3, 3, 256, 256, False), (1, 33, 3, 1, 512, 256, True),
     (1, 7, 2, 2, 511, 400, False), (2, 11, 4, 2, 100, 50, False), (2, 11, 4, 2, 100, 100, True), (1, 1000, 16, 4, 64, 32, False),
     (5, 1, 32, 8, 128, 128, True), (1, 21, 2, 1, 48, 0, False), (1, 300, 7, 7, 32, 24, False), (2, 6, 2, 2, 300, 8, True),
+    (1, 9, 2, 1, 264, 264, False), (1, 9, 2, 1, 264, 264, True), (3, 500, 24, 24, 64, 64, False), (1, 3000, 2, 1, 128, 128, True),
 ]
 
 
@@ -274,6 +275,13 @@ def test_refusals():
             norm_rotate_packed(torch.zeros(1, 2, 8 * 64, device="cuda"), w, w, table, heads=heads, kv_heads=kv)
     with pytest.raises(RuntimeError, match="transforms"):
         torch.func.vmap(lambda a: norm_rotate(a, a, w, w, table)[0])(torch.zeros(2, 1, 3, 4, 64, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_tracing_is_refused():
+    q, w, table = torch.zeros(1, 3, 2, 64, device="cuda"), torch.ones(64, device="cuda"), rotary_table(4, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda a: norm_rotate(a, a, w, w, table)[0], (q,))
 
 
 @pytest.mark.parametrize("near", [False, True])
