@@ -441,6 +441,7 @@ constexpr int kStages = kOut == kDerive ? 4 : 6;
 template <Out kOut>
 constexpr int kSmem = kStages<kOut> * kStage + kOutWarps * kBoxes<kOut> * kBoxBytes + 1024;  // of 227 KB
 
+constexpr int kJoinThreads = 256;
 template <Out kOut, GatedKeep kKeep>
 constexpr int kJoinSmem = kTake<kOut, kKeep> * (kOut == kActivate ? 2 : 1) * kHalf * 4;
 
@@ -701,47 +702,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
 }
 
 // Adds up the parts of the tiles whose reduction was shared, in order, and finishes them.  A block has 16 (64) columns of half a
-// tile: its warps add up a column each, four rows a lane, and hand them over in shared memory to the thread that has the row.
+// tile: its warps add up two columns each, four rows a lane, and hand them over in shared memory to the thread that has the row.
 // (Each thread its own row's numbers: 14.5 us for 18 MB of parts, a quarter of it in flight.)
 template <Out kOut, GatedKeep kKeep>
-__global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
+__global__ void __launch_bounds__(kJoinThreads) gated_join_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kN = kTake<kOut, kKeep>, kAll = kN * (kOut == kActivate ? 2 : 1), kEach = kAll / 4, kParts = 4;
+  constexpr int kN = kTake<kOut, kKeep>, kAll = kN * (kOut == kActivate ? 2 : 1), kWarps = kJoinThreads / 32, kEach = kAll / kWarps, kAt = 2, kParts = 8;
   extern __shared__ float4 sums[];  // [kAll][32]
   int job = 0;
   while (job + 1 < w.jobs && static_cast<int>(blockIdx.x) >= w.job[job + 1].join) ++job;
   const Job& j = w.job[job];
-  const int tile = static_cast<int>(blockIdx.x) - j.join, c = blockIdx.z * kN, row = blockIdx.y * kHalf + threadIdx.x, lane = threadIdx.x % 32,
+  const int tile = static_cast<int>(blockIdx.x) - j.join, c = blockIdx.z * kN, row = blockIdx.y * kHalf + threadIdx.x % kHalf, lane = threadIdx.x % 32,
             warp = threadIdx.x / 32;
   int ti, tj;
   tile_place(j, j.whole + tile, ti, tj);
   const Finish& f = w.f;
   const Spot at = spot_of<kOut>(j, ti, tj, row);
   const int64_t left = j.cols - at.col - c;
-  if (left <= 0 || at.row - threadIdx.x >= j.rows) return;
+  if (left <= 0 || at.row - threadIdx.x % kHalf >= j.rows) return;
   const float* from = w.partial + (j.part + static_cast<int64_t>(tile) * j.splits) * (kTile * kTile) + blockIdx.y * kHalf + 4 * lane;
 #pragma unroll 1
-  for (int i0 = 0; i0 < kEach; i0 += 4) {
-    float4 sum[4];
-    const float* column[4];
+  for (int i0 = 0; i0 < kEach; i0 += kAt) {
+    float4 sum[kAt];
+    const float* column[kAt];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int col = warp + 4 * (i0 + i);
+    for (int i = 0; i < kAt; ++i) {
+      const int col = warp + kWarps * (i0 + i);
       column[i] = from + (col < kN ? c + col : kHalf + c + col - kN) * kTile;
       sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     for (int p = 0; p < j.splits; p += kParts) {
-      float4 x[4][kParts];
+      float4 x[kAt][kParts];
 #pragma unroll
       for (int q = 0; q < kParts; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i][q] = __ldcg(reinterpret_cast<const float4*>(column[i] + static_cast<int64_t>(min(p + q, j.splits - 1)) * (kTile * kTile)));
+        for (int i = 0; i < kAt; ++i)
+          if (p + q < j.splits) x[i][q] = __ldcg(reinterpret_cast<const float4*>(column[i] + static_cast<int64_t>(p + q) * (kTile * kTile)));
 #pragma unroll
       for (int q = 0; q < kParts; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kAt; ++i)
           if (p + q < j.splits) {
             sum[i].x += x[i][q].x;
             sum[i].y += x[i][q].y;
@@ -750,11 +751,12 @@ __global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant
           }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[(warp + 4 * (i0 + i)) * 32 + lane] = sum[i];
+    for (int i = 0; i < kAt; ++i) sums[(warp + kWarps * (i0 + i)) * 32 + lane] = sum[i];
   }
   __syncthreads();
+  const int mine = threadIdx.x % kHalf;  // the second half of the threads has no row
   auto fetch = [&](int col, float* v) {
-    const float* s = reinterpret_cast<const float*>(sums) + (col >= kHalf && kOut == kActivate ? kN : 0) * kHalf + threadIdx.x;
+    const float* s = reinterpret_cast<const float*>(sums) + (col >= kHalf && kOut == kActivate ? kN : 0) * kHalf + mine;
 #pragma unroll
     for (int i = 0; i < kN; ++i) v[i] = s[i * kHalf];
   };
@@ -765,18 +767,19 @@ __global__ void __launch_bounds__(kHalf) gated_join_kernel(const __grid_constant
       __syncthreads();
       uint32_t* rows = reinterpret_cast<uint32_t*>(sums);  // [128][9]
 #pragma unroll
-      for (int i = 0; i < kN; i += 2) rows[threadIdx.x * 9 + i / 2] = pack2(v[i], v[i + 1], f.bf16);
+      for (int i = 0; i < kN; i += 2)
+        if (threadIdx.x < kHalf) rows[mine * 9 + i / 2] = pack2(v[i], v[i + 1], f.bf16);
       __syncthreads();
-      const int64_t y = at.row - threadIdx.x;
+      const int64_t y = at.row - mine;
       uint16_t* to = static_cast<uint16_t*>(j.to[at.which]) + at.col + c;
-      for (int i = threadIdx.x; i < kHalf * kN; i += kHalf) {
+      for (int i = threadIdx.x; i < kHalf * kN; i += kJoinThreads) {
         const int r = i / kN, e = i % kN;
         if (y + r < j.rows && e < left) to[(y + r) * j.ldo + e] = static_cast<uint16_t>(rows[r * 9 + e / 2] >> (16 * (e % 2)));
       }
       return;
     }
   }
-  if (at.row >= j.rows) return;
+  if (threadIdx.x >= kHalf || at.row >= j.rows) return;
   Ahead<kOut, kKeep> ahead;
   ahead.load(f, at.row, at.col + c);
   const int64_t to = at.row * j.ldo + at.col + c;
@@ -973,7 +976,7 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
   e = cudaLaunchKernelEx(&cfg, kernel, w);
   if (e != cudaSuccess || tail == 0) return e;
   cfg.gridDim = dim3(static_cast<unsigned>(tail), high ? 2 : 1, (kOut == kActivate ? kHalf : kTile) / kTake<kOut, kKeep>);
-  cfg.blockDim = dim3(kHalf);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = kJoinSmem<kOut, kKeep>;
   note_launch();
   return cudaLaunchKernelEx(&cfg, gated_join_kernel<kOut, kKeep>, w);
