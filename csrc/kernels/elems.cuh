@@ -94,8 +94,12 @@ __device__ __forceinline__ uint32_t codes8(float x0, float x1, float x2, float x
   const uint32_t w = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
   return inverse == 0.f ? 0u : w;
 }
-__device__ __forceinline__ float value8(uint32_t word, int i, float scale) {
-  return static_cast<float>(static_cast<int8_t>(word >> (8 * i))) * scale;
+// The values of four codes: a code and 128 in the lowest byte of 2^23 is that float, less 2^23 + 128 the code, exactly.  (A conversion
+// has a quarter of an addition's rate.)
+__device__ __forceinline__ void values8(uint32_t word, float scale, float* v) {
+  const uint32_t w = word ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(__fadd_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + i)), -8388736.f), scale);
 }
 // The largest magnitude, as bits: those of a NaN are above those of all numbers.
 __device__ __forceinline__ uint32_t most8(uint32_t most, float x) { return max(most, __float_as_uint(x) & 0x7FFFFFFFu); }

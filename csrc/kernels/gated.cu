@@ -301,10 +301,8 @@ __device__ __forceinline__ void keep_wide(const Wide& k, int which, int64_t at, 
 __device__ __forceinline__ void take_wide(const uint4& up, const uint2& low, float* v) {
   const uint32_t u[4] = {up.x, up.y, up.z, up.w}, l[2] = {low.x, low.y};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t high = i % 2 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16;
-    v[i] = __uint_as_float(high | ((l[i / 4] >> (8 * (i % 4))) & 0xFFu) << 8);
-  }
+  for (int i = 0; i < 8; ++i)  // the two upper bytes, the lower one, and nothing
+    v[i] = __uint_as_float(__byte_perm(u[i / 2], l[i / 4], (i % 2 ? 0x3200 : 0x1000) | (4 + i % 4) << 4) & 0xFFFFFF00u);
 }
 
 // Where 8 numbers of a thread's row go, `i` columns from where it is: straight to memory, which costs a request for each row (the
@@ -401,12 +399,10 @@ struct Kept<GatedKeep::kEight> {
     }
   }
   __device__ __forceinline__ void value(int b, float* g, float* u) const {
-    const uint32_t p[2] = {b ? codes[0].z : codes[0].x, b ? codes[0].w : codes[0].y}, q[2] = {b ? codes[1].z : codes[1].x, b ? codes[1].w : codes[1].y};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      g[e] = value8(p[e / 4], e % 4, scale[0]);
-      u[e] = value8(q[e / 4], e % 4, scale[1]);
-    }
+    values8(b ? codes[0].z : codes[0].x, scale[0], g);
+    values8(b ? codes[0].w : codes[0].y, scale[0], g + 4);
+    values8(b ? codes[1].z : codes[1].x, scale[1], u);
+    values8(b ? codes[1].w : codes[1].y, scale[1], u + 4);
   }
 };
 // 16 columns of dh to h, dg and du.

@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(kThreads, 4) unpack8_kernel(const int8_t* __re
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = value8(i < 4 ? word[d][h].x : word[d][h].y, i & 3, scale[d]);
+        values8(word[d][h].x, scale[d], v);
+        values8(word[d][h].y, scale[d], v + 4);
         store_run<T, 8>(x + u * kGroup8 + sub * 8 + 32 * h, u < all ? 8 : 0, true, v);
       }
     }
