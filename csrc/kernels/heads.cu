@@ -7,9 +7,11 @@
 //
 // Bound by memory.  A team of lanes, 8 pairs each, has a row in registers; both members of a pair are in the same lane, so the
 // rotation moves nothing between lanes and the norm is the only sum over a team.  A team takes several heads of its token, for
-// which the angles stay in registers.  32768 tokens of 40 heads of 128, bf16: forward 129 us (5.2 TB/s), backward, values copied, 269
-// (4.2); 8192 tokens of 32 heads of 64 15 and 37 us (B200; 4.6 and 3.6 TB/s).  Backward half of the issue slots are busy, half of the
-// time for want of numbers: its two rows and two gradients a lane in flight are what 128 registers hold.
+// which the angles stay in registers.  32768 tokens of 40 heads of 128, bf16: forward 129 us (5.2 TB/s), backward, values copied, 262
+// (4.4); 8192 tokens of 32 heads of 64 15 and 37 us (B200; 4.6 and 3.6 TB/s).  Backward half of the issue slots are busy, half of the
+// time for want of numbers: its two rows and two gradients a lane in flight are what 128 registers hold; each is asked for again as
+// soon as its numbers are used, the next token's at a token's end (269 us when both were waited for together).  Forward, with four
+// rows, that gains nothing and costs 2 us of 8192 tokens.  Sums of two numbers by one instruction: 137 and 273 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -297,24 +299,25 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? kBackwardResident 
 #pragma unroll
     for (int i = 0; i < V; ++i) grad[k][0][i] = grad[k][1][i] = 0.f;
   const float inv = 1.f / static_cast<float>(s.dim);
+  Pairs<T, V, kNear> x[kRows][K], g[kRows][K];
+  auto load = [&](int j, const T* xs, const T* gs, int h, bool there) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const Lane<V, kNear> l(s, lane, k * w.team);
+      x[j][k].load(xs + h * d.x.head, l, there && h < d.heads);
+      g[j][k].load(gs + h * d.dy.head, l, there && h < d.heads);
+    }
+  };
+  Token next(d, s, walk.base + walk.mine);
+  const T *next_from = token_rows<T>(d.x, next), *next_gfrom = token_rows<T>(d.dy, next);
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) load(j, next_from, next_gfrom, j * step + next.first, next.there);
   for (int64_t base = walk.base; base < d.units; base += walk.step) {
-    const Token token(d, s, base + walk.mine);
-    const T *from = token_rows<T>(d.x, token), *gfrom = token_rows<T>(d.dy, token);
-    Pairs<T, V, kNear> x[kRows][K], g[kRows][K];
-    auto load = [&](int h0) {
-#pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int h = h0 + j * step + token.first;
-        const bool on = token.there && h < d.heads;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const Lane<V, kNear> l(s, lane, k * w.team);
-          x[j][k].load(from + h * d.x.head, l, on);
-          g[j][k].load(gfrom + h * d.dy.head, l, on);
-        }
-      }
-    };
-    load(0);
+    const Token token = next;
+    const T *from = next_from, *gfrom = next_gfrom;
+    next = Token(d, s, base + walk.step + walk.mine);
+    next_from = token_rows<T>(d.x, next);
+    next_gfrom = token_rows<T>(d.dy, next);
     const int64_t position = position_of(s, token.b, token.t);
     float weight[K][2][V], c[K][V], sn[K][V];
 #pragma unroll
@@ -325,7 +328,10 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? kBackwardResident 
     }
     T* to = reinterpret_cast<T*>(d.out) + token.at * d.out_token;
     for (int h0 = 0; h0 < d.heads; h0 += kRows * step) {
-      if (h0 > 0) load(h0);
+      const bool more = h0 + kRows * step < d.heads;
+      const T *then = more ? from : next_from, *gthen = more ? gfrom : next_gfrom;
+      const int then_h = more ? h0 + kRows * step + token.first : next.first;
+      const bool then_there = more ? token.there : next.there;
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
         const int h = h0 + j * step + token.first;
@@ -362,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, V > 1 && K == 1 ? kBackwardResident 
           y.set(ya, yb);
           y.store(to + static_cast<int64_t>(h) * s.dim, l, on);
         }
+        load(j, then, gthen, then_h + j * step, then_there);
       }
     }
   }
