@@ -508,7 +508,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * kDepths + b); };
   auto acc_free = [&](int b) { return bar0 + 8u * (2 * kDepths + 2 + b); };
   const uint32_t drained = bar0 + 8u * (2 * kDepths + 4);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int s = 0; s < kDepths; ++s) {
       bar_init(full(s), 1);
@@ -530,7 +529,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
   cluster_sync();
   fence_after();
   const uint32_t tmem = tmem_base;
+  // Only now, when all that came before is done: copies beside this (gated_copies_kernel) do not wait before they write.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   bool ok = true, issued = false;
 
   if (warp == kLoader) {
@@ -789,12 +790,17 @@ struct Copies {
   int64_t first[kGatedCopies + 1];  // blocks
 };
 constexpr int kCopyRows = 8, kCopyCols = 512;  // of a block; a warp has a row, two neighbours a lane and turn
-__global__ void __launch_bounds__(256) gated_copies_kernel(const Copies w) {
+constexpr int kCopyThreads = 32 * kCopyRows;
+// Ahead of the product that reads them, or beside the product before it.  (333 tokens of 1000 x 2731, w_down copied, 35 us ahead of
+// both products, 27 beside the first.)
+__global__ void __launch_bounds__(kCopyThreads) gated_copies_kernel(const Copies w) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int j = 0;
   while (static_cast<int64_t>(blockIdx.x) >= w.first[j + 1]) ++j;
   const GatedCopy& c = w.job[j];
   const int64_t across = (c.cols + kCopyCols - 1) / kCopyCols, block = blockIdx.x - w.first[j];
   const int64_t row = block / across * kCopyRows + threadIdx.x / 32, col = block % across * kCopyCols + threadIdx.x % 32 * 2;
+  // What waits for this grid waits for the product beside it too: one thread's wait is enough, the first one's, which has a row.
   if (row >= c.rows) return;
   const uint16_t* from = static_cast<const uint16_t*>(c.from) + row * c.row_stride;
   uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(c.to) + row * c.ld);
@@ -807,6 +813,7 @@ __global__ void __launch_bounds__(256) gated_copies_kernel(const Copies w) {
 #pragma unroll
   for (int i = 0; i < kCopyCols / 64; ++i)
     if (col + 64 * i < c.cols) to[(col + 64 * i) / 2] = v[i];
+  if (blockIdx.x == 0 && threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
@@ -1030,7 +1037,7 @@ int64_t gated_partial_bytes(const GatedProduct* p, int n, const GatedShape& s) {
   return parts * kTile * kTile * 4;
 }
 
-cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, cudaStream_t s) {
+cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, bool beside, cudaStream_t s) {
   if (n < 1 || n > kGatedCopies) return cudaErrorInvalidValue;
   Copies w{};
   for (int j = 0; j < kGatedCopies; ++j) {
@@ -1042,8 +1049,16 @@ cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, cudaStream_t s) {
   if (blocks == 0) return cudaSuccess;
   if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
   note_launch();
-  gated_copies_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(w);
-  return cudaGetLastError();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(kCopyThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, gated_copies_kernel, w);
 }
 
 cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaStream_t s) {

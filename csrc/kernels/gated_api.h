@@ -57,7 +57,7 @@ int64_t gated_partial_bytes(const GatedProduct* p, int n, const GatedShape& s);
 cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaStream_t s);
 
 // Matrices of 16-bit numbers whose rows are not 16-byte aligned (or whose numbers do not lie side by side) copied to ones that are,
-// up to five in one launch.
+// up to five in one launch.  `beside`: while the launch of this file before it runs, which neither reads `to` nor writes `from`.
 struct GatedCopy {
   const void* from;
   int64_t row_stride, col_stride, rows, cols;  // elements
@@ -66,7 +66,7 @@ struct GatedCopy {
 };
 inline int64_t gated_row(int64_t cols) { return (cols + 7) / 8 * 8; }
 constexpr int kGatedCopies = 5;
-cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, cudaStream_t s);
+cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, bool beside, cudaStream_t s);
 
 // A whole forward pass of few rows, two launches that read the weights at the rate of memory (kernels/gated_few.cu).  Rows of any
 // alignment.  `h`: scratch of 2 x tokens x gated_pitch(hidden) 16-bit numbers.

@@ -58,7 +58,9 @@ class Operands {
     }
     return n_++;
   }
-  void copy(const at::Tensor& like) {
+  bool any() const { return copied_ > 0; }
+  // Before what reads them; `beside` the product launched last, which doesn't.
+  void copy(const at::Tensor& like, bool beside = false) {
     if (copied_ == 0) return;
     held_ = at::empty({bytes_}, like.options().dtype(at::kByte));
     char* at = static_cast<char*>(held_.data_ptr());
@@ -67,7 +69,7 @@ class Operands {
       m_[of_[i]].data = at;
       at += (copies_[i].rows * copies_[i].ld * 2 + 255) / 256 * 256;
     }
-    OPS_CK(kern::launch_gated_copies(copies_, copied_, at::cuda::getCurrentCUDAStream()));
+    OPS_CK(kern::launch_gated_copies(copies_, copied_, beside, at::cuda::getCurrentCUDAStream()));
   }
   const kern::GatedOperand& operator[](int i) const { return m_[i]; }
 
@@ -122,13 +124,16 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
     return y;
   }
   Operands m;
-  const int ox = m.add(x), og = m.add(wg), ou = m.add(wu), od = m.add(wd);
-  m.copy(x);
+  const int ox = m.add(x), og = m.add(wg), ou = m.add(wu);
+  const bool first = m.any();  // else a copy of w_down has time until the second product
+  const int od = m.add(wd);
+  if (first) m.copy(x);
   const at::Tensor h = at::empty({s.tokens, kern::gated_pitch(s.hidden)}, x.options());
   Products run(s, x, wait_limit);
   run.r.kept = kept ? kept->data_ptr() : nullptr;
   const kern::GatedArgs up{GatedProduct::kUp, m[ox], {}, m[og], m[ou], h.data_ptr(), nullptr, nullptr, 0};
   run.launch(&up, 1, x);
+  if (!first) m.copy(x, true);
   const kern::GatedArgs down{GatedProduct::kDown, {h.const_data_ptr(), h.size(1)}, {}, m[od], {}, y.data_ptr(), nullptr, nullptr, s.width};
   run.launch(&down, 1, x);
   return y;

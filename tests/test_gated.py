@@ -364,6 +364,25 @@ def test_repeated_calls_are_bit_equal():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,width,hidden", [(333, 1000, 2731), (40, 520, 4001), (2000, 64, 130), (100, 999, 515)])
+def test_copied_rows_of_calls_one_after_another(tokens, width, hidden):
+    # what is copied for one call lies where an earlier one's copies, parts and h lay, which its kernels may still read
+    sets = [_inputs(tokens, width, hidden, torch.bfloat16, seed=i)[:4] for i in range(3)]
+    want = []
+    for args in sets:
+        want.append(gated_feed_forward(*args))
+        torch.cuda.synchronize()
+    got = [gated_feed_forward(*sets[i % 3]) for i in range(60)]
+    assert all(torch.equal(g, want[i % 3]) for i, g in enumerate(got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [gated_feed_forward(*args) for args in sets]
+    for _ in range(5):
+        graph.replay()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_waits_that_run_out_are_reported_and_leave_nan():
     # in a process of its own: the report is one for the whole device
     code = """
