@@ -186,6 +186,7 @@ struct Job {
   void* to[3];
   int64_t rows, cols, ldo;  // of one result; cols: of h, dg and du their pitch
   bool a_inner, b_inner;    // k innermost
+  uint32_t bytes;           // of a stage, that both CTAs load
   bool wide;                // there are maps of the results: their rows are aligned to 16 bytes
   int rows_segment;         // tiles of rows of the first of two results (dWg, then dWu); all of them where there is one
   int tiles_i, tiles_j;     // tiles_i: of all results
@@ -551,7 +552,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           const CUtensorMap* a = &j.a[i_second | k_second];
           const CUtensorMap* b = &j.b[kOut == kActivate ? rank : k_second];
           const uint32_t to = smem0 + s * kStage, bar = in_leader(full(s));
-          if (rank == 0) bar_expect(full(s), 2 * kStage);
+          if (rank == 0) bar_expect(full(s), j.bytes);
           if (a_inner) load_box(to, a, k0, i0, bar);
           else {
             load_box(to, a, i0, k0, bar);
@@ -930,13 +931,19 @@ EncodeTiled encode_tiled() {
   }();
   return fn;
 }
-// A matrix of `outer` rows of `inner` numbers, read in boxes of 64 of a row and of 128 rows (k innermost) or 64 (own index innermost),
-// or written in boxes of 64 of a row and of 32 rows.
-enum class Box { kInnerK, kOwn, kResult };
-bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t outer, Box kind, bool bf16) {
+// A matrix of `outer` rows of `inner` numbers in boxes of 64 of a row and of `box_rows` rows: read, of 128 (k innermost; of tokens fewer
+// where there are fewer: a box's rows beyond the matrix take time, 73 us for 67 of 12 tokens of 4096 x 10240, 279 for 236 of 3 of 8192 x
+// 24576; what lies below in shared memory are rows of nobody's) or 64 (own index innermost); written, of 32.
+constexpr uint32_t kOwnRows = 64, kResultRows = 32;
+uint32_t rows_read(int64_t rows) {
+  uint32_t n = 8;
+  while (n < rows && n < kHalf) n *= 2;
+  return n;
+}
+bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t outer, uint32_t box_rows, bool bf16) {
   if (m.data == nullptr || reinterpret_cast<uintptr_t>(m.data) % 16 != 0 || m.ld % 8 != 0 || m.ld < inner || inner > 0x7FFFFFFF || outer > 0x7FFFFFFF) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)}, strides[1] = {static_cast<cuuint64_t>(m.ld) * 2};
-  const cuuint32_t box[2] = {64, kind == Box::kResult ? 32u : kind == Box::kInnerK ? 128u : 64u}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {64, box_rows}, one[2] = {1, 1};
   return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(m.data), dims, strides, box, one,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -991,12 +998,14 @@ bool make_job(Job& j, const GatedArgs& g, const GatedShape& h) {
   j.a_inner = g.product != GatedProduct::kWeightUp && g.product != GatedProduct::kWeightDown;
   j.b_inner = g.product == GatedProduct::kUp || g.product == GatedProduct::kDown;
   const GatedOperand a[2] = {g.a0, z.results * z.parts > 1 ? g.a1 : g.a0}, b[2] = {g.b0, z.gate || z.parts > 1 ? g.b1 : g.b0};
+  const uint32_t a_rows = j.a_inner ? rows_read(z.rows) : kOwnRows;
+  j.bytes = 2 * ((j.a_inner ? a_rows * kDepth * 2 : kOperand) + kOperand);
   for (int i = 0; i < 2; ++i) {
     if (i == 1 && a[1].data == a[0].data && a[1].ld == a[0].ld) j.a[1] = j.a[0];
-    else if (!make_map(&j.a[i], a[i], j.a_inner ? z.depth : z.rows, j.a_inner ? z.rows : z.depth, j.a_inner ? Box::kInnerK : Box::kOwn, h.bf16))
+    else if (!make_map(&j.a[i], a[i], j.a_inner ? z.depth : z.rows, j.a_inner ? z.rows : z.depth, a_rows, h.bf16))
       return false;
     if (i == 1 && b[1].data == b[0].data && b[1].ld == b[0].ld) j.b[1] = j.b[0];
-    else if (!make_map(&j.b[i], b[i], j.b_inner ? z.depth : z.cols, j.b_inner ? z.cols : z.depth, j.b_inner ? Box::kInnerK : Box::kOwn, h.bf16))
+    else if (!make_map(&j.b[i], b[i], j.b_inner ? z.depth : z.cols, j.b_inner ? z.cols : z.depth, j.b_inner ? kHalf : kOwnRows, h.bf16))
       return false;
   }
   // h, dg and du have rows of whole groups; the others are a caller's
@@ -1011,7 +1020,7 @@ bool make_job(Job& j, const GatedArgs& g, const GatedShape& h) {
   const int results = g.product == GatedProduct::kGate ? 3 : g.product == GatedProduct::kWeightUp ? 2 : 1;
   for (int i = 0; i < 3; ++i) {
     if ((i < results) != (j.to[i] != nullptr)) return false;
-    if (i < results && j.wide && !make_map(&j.out[i], {j.to[i], j.ldo}, j.cols, z.rows, Box::kResult, h.bf16)) return false;
+    if (i < results && j.wide && !make_map(&j.out[i], {j.to[i], j.ldo}, j.cols, z.rows, kResultRows, h.bf16)) return false;
   }
   return j.wide || !between;
 }

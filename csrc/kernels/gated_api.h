@@ -71,9 +71,13 @@ cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, bool beside, cudaS
 // A whole forward pass of few rows, two launches that read the weights at the rate of memory (kernels/gated_few.cu).  Rows of any
 // alignment.  `h`: scratch of 2 x tokens x gated_pitch(hidden) 16-bit numbers.
 constexpr int64_t kFewTokens = 32;
-// Whether it is faster than the tiles: from 17 tokens on only where the block is narrow (32 tokens of 1024 x 2816 18.3 and 28 us, of
-// 2048 x 5632 40 and 37).
-inline bool gated_is_few(const GatedShape& s) { return s.tokens <= 16 || (s.tokens <= kFewTokens && s.width * s.hidden <= (8 << 20)); }
+// Whether it is faster than the tiles, whose matrix instructions cost the same for any number of tokens and whose launches cost more.
+// us, here and by tiles: 2 tokens 4096 x 10240 59 and 68, 5120 x 8192 64 and 59, 5120 x 13824 98 and 93; 8 tokens 4096 x 6144 40 and 44,
+// 5120 x 8192 70 and 59; 16 tokens 2048 x 4096 25 and 26, 2048 x 5632 32 and 30; 32 tokens 1024 x 2816 18 and 19, 1536 x 4096 27 and 25.
+inline bool gated_is_few(const GatedShape& s) {
+  const int64_t n = s.width * s.hidden;
+  return n <= (s.tokens <= 2 ? 48 << 20 : s.tokens <= 8 ? 32 << 20 : s.tokens <= 16 ? 8 << 20 : s.tokens <= kFewTokens ? 4 << 20 : 0);
+}
 struct GatedFew {
   GatedShape shape;
   GatedOperand x, w_gate, w_up, w_down;

@@ -5,9 +5,12 @@
 // and these are what it gives to the matrix instructions: which of the 32 numbers of a step is called k = 0 does not matter as long as
 // both operands agree, so nothing is rearranged.  The products are a few instructions a kilobyte; with multiplications and additions
 // instead 16 tokens of 1024 x 2816 took 78 us (the tokens' numbers came from the cache for every row), and the tiles of 256 rows of
-// gated.cu take 28 for any number of tokens up to 64.  h is the sum of two 16-bit numbers here, as good as in 32 bits.
+// gated.cu take 19 for any number of tokens up to 64.  h is the sum of two 16-bit numbers here, as good as in 32 bits.
 // us (B200, weights of six blocks in turn), 1, 8, 16, 32 tokens: 1024 x 2816 8.3, 9.4, 13.4, 18.3; 2048 x 5632 18.2 (69 MB: 3.8 TB/s),
-// 20.6, 31.6, 40.0.  A run of a block's rows ahead of the products, 4 or 16 warps a block, more of the row in flight: all slower.
+// 20.6, 31.6, 40.0; 4096 x 10240 56 (4.5 TB/s), 63, 100, 122.  A run of a block's rows ahead of the products, 4 or 16 warps a block, more
+// of the row in flight: all slower; so are weights through a ring in shared memory, 24 runs a thread on their way at any time (64 us of
+// 4096 x 10240 and 8 tokens: what is left of the first-level cache doesn't hold the tokens).  16 rows a block of the projection back: 59
+// of it, but 24 for 21 of 2048 x 5632.
 #include <type_traits>
 
 #include "kernels/elems.cuh"

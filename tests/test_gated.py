@@ -175,6 +175,15 @@ def test_few_tokens_match_64_bits(tokens, width, hidden, dtype, activation):
     _check({"y": same[-1:]}, {"y": tuple(t[:1] for t in want["y"])})
 
 
+# on both sides of the sizes at which a few tokens of wide blocks become tiles
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,width,hidden", [(1, 7168, 7000), (2, 7168, 7048), (3, 4096, 8100), (8, 4096, 8209), (16, 2048, 4096), (9, 2048, 4104),
+                                                 (32, 1024, 4096), (17, 1000, 4211)])
+def test_few_tokens_of_wide_blocks_match_64_bits(tokens, width, hidden):
+    x, wg, wu, wd, _ = _inputs(tokens, width, hidden, torch.bfloat16, seed=tokens)
+    _check({"y": gated_feed_forward(x, wg, wu, wd)}, _want(x, wg, wu, wd, None, "silu", False, Rounding(torch.bfloat16)))
+
+
 # what is launched before the kernels has written the weights they read
 @pytest.mark.gpu
 def test_few_tokens_see_new_weights():
