@@ -489,9 +489,9 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
 // A pair of CTAs per tile of 256 x 256, tiles in turn: each CTA loads half of either operand's rows and has half of the
 // accumulator's; the first one issues the products of both.  Two accumulators, so that a tile is taken out while the next one
 // is multiplied.  A stage is 64 KB for 8.4 million multiplications: what passes through the second-level cache, 13.5 TB/s of it, bounds
-// all of them.  8192 x 1024 x 2816 bf16 (B200, by itself): up 61 us without, 77 with three kept bytes, 70 with codes (1.55, 1.23, 1.35
-// PFLOP/s), down 33 (1.42), gate 75 and 70 (0.63: 12 or 8 bytes a number of its own beside the operands, 10.8 TB/s), the last three 168
-// (1.40); 16384 x 2048 x 5632 up 545 (1.39), down 240 (1.58), gate 379, the last three 1250 (1.51).
+// all of them.  8192 x 1024 x 2816 bf16 (B200, by itself): up 61 us without, 79 with three kept bytes, 71 with codes (1.55, 1.20, 1.33
+// PFLOP/s), down 34 (1.39), gate 75 and 67 (0.63 and 0.71: 12 or 8 bytes a number of its own beside the operands, 10.8 TB/s), the last three 168
+// (1.40); 16384 x 2048 x 5632 up 545 (1.39), down 240 (1.58), gate 366, the last three 1250 (1.51).
 // Left: 16 warps to take the accumulators out (no faster, 397 for 339 of the wide gate), what was kept asked for two runs ahead through
 // shared memory (72 for 75, but 418 for 379 of the wide one, which has then a stage less) or a tile ahead into the second-level cache.
 template <Out kOut, GatedKeep kKeep>
@@ -841,11 +841,12 @@ struct Plan {
   int64_t longest() const { return whole > 0 ? stages : per_split; }
 };
 constexpr double kStageUs = 0.37;
-// Whether sharing tiles along the reduction saves more than it costs: a partial sum is written and read at 4 TB/s, behind 4 us for
-// the launch that adds them up.
+// Whether sharing tiles along the reduction saves more than it costs: a partial sum is written and read at 6 TB/s, behind 2 us for
+// the launch that adds them up.  us, shared and not: down of 1024 tokens of 1024 x 2816 15.4 and 18.9, of 1000 of 768 x 2048 13.9 and 15.5;
+// up of 2048 tokens of 2048 x 4096 (which stays whole) 51.3 and 46.8.
 bool split_pays(const Plan& l, int64_t tiles, int64_t splits, int64_t per, int64_t rows) {
   const double saved = kStageUs * static_cast<double>(l.stages - per);
-  return saved > 4.0 + 8.0 * static_cast<double>(tiles * splits * kTile * std::min<int64_t>(kTile, rows)) / 4e6;
+  return saved > 2.0 + 8.0 * static_cast<double>(tiles * splits * kTile * std::min<int64_t>(kTile, rows)) / 6e6;
 }
 Plan plan_of(GatedProduct p, const GatedShape& s) {
   const Sizes z = sizes_of(p, s);
@@ -883,7 +884,7 @@ double stages_alone(const Plan& l) {
 }
 // Several products side by side: whole tiles, but for a product whose tiles are so few and long that the device would wait for them.
 // Whether that is faster than one after the other, of which each leaves part of the device idle in its last round: 8192 tokens of 1024 x
-// 2816 168 us and 183, 1024 33 and 48, 64 of 640 x 2112 16 and 26; 16384 of 2048 x 5632, fourteen rounds, 1302 and 1246, for what
+// 2816 168 us and 183, 1024 32 and 47, 64 of 640 x 2112 13 and 25; 16384 of 2048 x 5632, fourteen rounds, 1302 and 1246, for what
 // different operands in the second-level cache cost (a twentieth, taken into account).
 bool plan_together(const GatedProduct* p, const GatedShape& s, int n, Plan* l, int* order) {
   int64_t total = 0;
