@@ -247,17 +247,10 @@ __device__ __forceinline__ int item_of(int round, int pair, int pairs, int jobs)
 }
 
 // ---- after the product --------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
-  if (bf16) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&p);
-  }
-  const __half2 p = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-__device__ __forceinline__ void store16(void* row, int64_t col, const float* v, bool bf16) {  // 8 numbers
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + col) =
-      make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16), pack2(v[4], v[5], bf16), pack2(v[6], v[7], bf16));
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (kBf16) return store_pair<__nv_bfloat16>(a, b);
+  else return store_pair<__half>(a, b);
 }
 
 // Floats of three bytes: the upper 24 bits, rounded to nearest; infinities and NaN cut off.
@@ -310,23 +303,25 @@ __device__ __forceinline__ void take_wide(const uint4& up, const uint2& low, flo
 // joining kernel), or to the warp's boxes of 32 rows and 64 columns in shared memory, 128-byte swizzle,
 // which then leave as a whole.  (Straight to memory kGate took 99 us of 8192 x 1024 x 2816, bound by its requests.)
 constexpr int kTurn = 64, kBoxBytes = 32 * kTurn * 2;
+template <bool kBf16>
 struct Direct {
   uint16_t* out[3];
-  bool bf16;
   int64_t left;  // numbers of the row from here on, a multiple of 8
   __device__ __forceinline__ void put(int which, int i, const float* v) const {
-    if (i < left) store16(out[which], i, v, bf16);
+    if (i < left)
+      *reinterpret_cast<uint4*>(out[which] + i) =
+          make_uint4(pack2<kBf16>(v[0], v[1]), pack2<kBf16>(v[2], v[3]), pack2<kBf16>(v[4], v[5]), pack2<kBf16>(v[6], v[7]));
   }
 };
+template <bool kBf16>
 struct Staged {
   uint32_t row;       // of the first box
   int swizzle;
-  bool bf16;
-  __device__ __forceinline__ Staged(uint32_t boxes, int lane, bool half) : row(boxes + lane * 128), swizzle(lane & 7), bf16(half) {}
+  __device__ __forceinline__ Staged(uint32_t boxes, int lane) : row(boxes + lane * 128), swizzle(lane & 7) {}
   __device__ __forceinline__ void put(int which, int i, const float* v) const {
     const uint32_t to = row + which * kBoxBytes + ((i / 8) ^ swizzle) * 16;
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pack2(v[0], v[1], bf16)), "r"(pack2(v[2], v[3], bf16)),
-                 "r"(pack2(v[4], v[5], bf16)), "r"(pack2(v[6], v[7], bf16))
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pack2<kBf16>(v[0], v[1])), "r"(pack2<kBf16>(v[2], v[3])),
+                 "r"(pack2<kBf16>(v[4], v[5])), "r"(pack2<kBf16>(v[6], v[7]))
                  : "memory");
   }
 };
@@ -493,7 +488,8 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
 // PFLOP/s), down 34 (1.39), gate 75 and 67 (0.63 and 0.71: 12 or 8 bytes a number of its own beside the operands, 10.8 TB/s), the last three 168
 // (1.40); 16384 x 2048 x 5632 up 545 (1.39), down 240 (1.58), gate 366, the last three 1250 (1.51).
 // Left: 16 warps to take the accumulators out (no faster, 397 for 339 of the wide gate), what was kept asked for two runs ahead through
-// shared memory (72 for 75, but 418 for 379 of the wide one, which has then a stage less) or a tile ahead into the second-level cache.
+// shared memory (72 for 75, but 418 for 379 of the wide one, which has then a stage less) or a tile ahead into the second-level cache
+// (83 and 431).
 template <Out kOut, GatedKeep kKeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   constexpr int kDepths = kStages<kOut>, kOuts = kBoxes<kOut>;
@@ -635,7 +631,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
         for (int c = first; c < last; c += kTurn) {
           if (lane == 0) stores_left();
           __syncwarp();
-          finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged(boxes, lane, w.f.bf16));
+          if (w.f.bf16) finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged<true>(boxes, lane));
+          else finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged<false>(boxes, lane));
           if (kOut != kStore || j.wide) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -766,7 +763,7 @@ __global__ void __launch_bounds__(kJoinThreads) gated_join_kernel(const __grid_c
       uint32_t* rows = reinterpret_cast<uint32_t*>(sums);  // [128][9]
 #pragma unroll
       for (int i = 0; i < kN; i += 2)
-        if (threadIdx.x < kHalf) rows[mine * 9 + i / 2] = pack2(v[i], v[i + 1], f.bf16);
+        if (threadIdx.x < kHalf) rows[mine * 9 + i / 2] = f.bf16 ? pack2<true>(v[i], v[i + 1]) : pack2<false>(v[i], v[i + 1]);
       __syncthreads();
       const int64_t y = at.row - mine;
       uint16_t* to = static_cast<uint16_t*>(j.to[at.which]) + at.col + c;
@@ -781,8 +778,9 @@ __global__ void __launch_bounds__(kJoinThreads) gated_join_kernel(const __grid_c
   Ahead<kOut, kKeep> ahead;
   ahead.load(f, at.row, at.col + c);
   const int64_t to = at.row * j.ldo + at.col + c;
-  const Direct sink{{static_cast<uint16_t*>(j.to[at.which]) + to, static_cast<uint16_t*>(j.to[1]) + to, static_cast<uint16_t*>(j.to[2]) + to}, f.bf16, left};
-  finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, sink);
+  uint16_t* const out[3] = {static_cast<uint16_t*>(j.to[at.which]) + to, static_cast<uint16_t*>(j.to[1]) + to, static_cast<uint16_t*>(j.to[2]) + to};
+  if (f.bf16) finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, Direct<true>{{out[0], out[1], out[2]}, left});
+  else finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, Direct<false>{{out[0], out[1], out[2]}, left});
 }
 
 // ---- rows that are not aligned --------------------------------------------------------------------------------
