@@ -7,10 +7,11 @@
 // instead 16 tokens of 1024 x 2816 took 78 us (the tokens' numbers came from the cache for every row), and the tiles of 256 rows of
 // gated.cu take 19 for any number of tokens up to 64.  h is the sum of two 16-bit numbers here, as good as in 32 bits.
 // us (B200, weights of six blocks in turn), 1, 8, 16, 32 tokens: 1024 x 2816 8.3, 9.4, 13.4, 18.3; 2048 x 5632 18.2 (69 MB: 3.8 TB/s),
-// 20.6, 31.6, 40.0; 4096 x 10240 56 (4.5 TB/s), 63, 100, 122.  A run of a block's rows ahead of the products, 4 or 16 warps a block, more
-// of the row in flight: all slower; so are weights through a ring in shared memory, 24 runs a thread on their way at any time (64 us of
-// 4096 x 10240 and 8 tokens: what is left of the first-level cache doesn't hold the tokens).  16 rows a block of the projection back: 59
-// of it, but 24 for 21 of 2048 x 5632.
+// 20.6, 31.6, 40.0; 4096 x 10240 56 (4.5 TB/s), 63, 100, 122; 1000 x 2731, whose rows of w_down begin anywhere, 10.2, 10.9, 13.7, 20.9
+// (read in pairs from the first aligned number on 12.9, 17.3, 33, 42), 1723 x 5258, all rows, 37, 39, 48, 66 (47, 57, 86, 122).
+// A run of a block's rows ahead of the products, 4 or 16 warps a block, more of the row in flight: all slower; so are weights through a
+// ring in shared memory, 24 runs a thread on their way at any time (64 us of 4096 x 10240 and 8 tokens: what is left of the first-level
+// cache doesn't hold the tokens).  16 rows a block of the projection back: 59 of it, but 24 for 21 of 2048 x 5632.
 #include <type_traits>
 
 #include "kernels/elems.cuh"
@@ -47,36 +48,72 @@ __device__ __forceinline__ void multiply(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 8 numbers of a row from column `at` of `depth`; zeros beyond it.  Aligned rows are whole runs of 8, and no branch stands between
-// one load and the next.
-template <bool kVec, typename T>
-__device__ __forceinline__ uint4 eight(const T* row, int64_t at, int64_t depth, bool there) {
-  if constexpr (kVec) {
+// 8 numbers of a row from a column that is a multiple of 8; zeros beyond the row.  Rows that are aligned to 16 bytes are whole runs,
+// and no branch stands between one load and the next.
+enum class Rows { kWhole, kPadded, kAny };
+template <Rows kRows, typename T>
+struct Run {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* row, int64_t at, int64_t depth, bool there, const T*, const T*) {
     const bool in = there && at < depth;
-    const uint4 v = *reinterpret_cast<const uint4*>(row + (in ? at : 0));
-    return make_uint4(in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u);
+    v = *reinterpret_cast<const uint4*>(row + (in ? at : 0));
+    if (!in) v = make_uint4(0u, 0u, 0u, 0u);
   }
-  uint32_t v[4] = {0u, 0u, 0u, 0u};
-  const uint16_t* p = reinterpret_cast<const uint16_t*>(row + at);
-  if (there && at + 8 <= depth) {  // in pairs, from the first that is aligned on
-    if ((reinterpret_cast<uintptr_t>(p) & 2) == 0) {
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
-      return make_uint4(q[0], q[1], q[2], q[3]);
-    }
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(p + 1);
-    const uint32_t a = q[0], b = q[1], c = q[2];
-    return make_uint4(p[0] | a << 16, __funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), c >> 16 | static_cast<uint32_t>(p[7]) << 16);
+  __device__ __forceinline__ uint4 get(const T*) const { return v; }
+};
+// Aligned rows that can be read beyond their end, where there are no numbers.
+template <typename T>
+struct Run<Rows::kPadded, T> {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* row, int64_t at, int64_t depth, bool there, const T*, const T*) {
+    const bool in = there && at < depth;
+    v = *reinterpret_cast<const uint4*>(row + (in ? at : 0));
+    const int64_t n = in ? depth - at : 0;
+    v.x &= n > 1 ? 0xFFFFFFFFu : n > 0 ? 0xFFFFu : 0u;
+    v.y &= n > 3 ? 0xFFFFFFFFu : n > 2 ? 0xFFFFu : 0u;
+    v.z &= n > 5 ? 0xFFFFFFFFu : n > 4 ? 0xFFFFu : 0u;
+    v.w &= n > 7 ? 0xFFFFFFFFu : n > 6 ? 0xFFFFu : 0u;
   }
+  __device__ __forceinline__ uint4 get(const T*) const { return v; }
+};
+// Of other rows the two aligned runs that hold the 8, moved into place when they are used; one by one where these are not inside of
+// the matrix, `begin` to `end`, or the row ends.
+template <typename T>
+struct Run<Rows::kAny, T> {
+  uint4 v, behind;
+  bool moved;
+  __device__ __forceinline__ void load(const T* row, int64_t at, int64_t depth, bool there, const T* begin, const T* end) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row + at);
+    const uint16_t* base = p - reinterpret_cast<uintptr_t>(p) % 16 / 2;
+    moved = there && at + 8 <= depth && base >= reinterpret_cast<const uint16_t*>(begin) && base + 16 <= reinterpret_cast<const uint16_t*>(end);
+    if (moved) {
+      v = reinterpret_cast<const uint4*>(base)[0];
+      behind = reinterpret_cast<const uint4*>(base)[1];
+    } else {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (there && at + i < depth) v[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
+      for (int i = 0; i < 8; ++i)
+        if (there && at + i < depth) w[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i % 2));
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ uint4 get(const T* row) const {  // the row, for where it begins
+    const uint32_t m = moved ? reinterpret_cast<uintptr_t>(row) % 16 : 0;
+    uint32_t w[8] = {v.x, v.y, v.z, v.w, behind.x, behind.y, behind.z, behind.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = m & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = m & 4 ? w[i + 1] : w[i];
+    const uint32_t bits = m & 2 ? 16 : 0;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                      __funnelshift_r(w[3], w[4], bits));
+  }
+};
 
 // kGroups groups of 8 tokens (the last ones may be none).  kUp: gate and up and what follows them, else one product of h.
 template <typename T, int kGroups, bool kUp, bool kVec>
-__global__ void __launch_bounds__(kThreads, kGroups == 2 ? 3 : 2) few_kernel(const Few w) {
-  constexpr int kX = kUp ? 1 : 2, kW = kUp ? 2 : 1, kAhead = !kUp && kGroups == 1 && kVec ? 8 : 4;
+__global__ void __launch_bounds__(kThreads, kGroups == 2 && kVec ? 3 : 2) few_kernel(const Few w) {
+  constexpr int kX = kUp ? 1 : 2, kW = kUp ? 2 : 1, kAhead = !kVec ? (kUp || kGroups > 2 ? 2 : 5 - kGroups) : !kUp && kGroups == 1 ? 8 : 4;
   constexpr int kHeld = kUp ? 4 : 2;  // accumulators of a lane and group that mean something
   __shared__ float part[kWarps][kGroups][kHeld][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
@@ -86,12 +123,13 @@ __global__ void __launch_bounds__(kThreads, kGroups == 2 ? 3 : 2) few_kernel(con
 #pragma unroll
   for (int i = 0; i < kW; ++i) weight[i] = static_cast<const T*>(w.w[i]) + (there ? first + g : 0) * w.ldw[i];
   const int64_t begin = warp * kStep + t * 8, step = kWarps * kStep;
-  uint4 run[kAhead][kW];
+  Run<kVec ? Rows::kWhole : Rows::kAny, T> run[kAhead][kW];
   auto load = [&](int64_t at) {
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-      for (int i = 0; i < kW; ++i) run[a][i] = eight<kVec>(weight[i], at + a * step, w.depth, there);
+      for (int i = 0; i < kW; ++i)
+        run[a][i].load(weight[i], at + a * step, w.depth, there, static_cast<const T*>(w.w[i]), static_cast<const T*>(w.w[i]) + (w.rows - 1) * w.ldw[i] + w.depth);
   };
   // The second launch is let in behind the first one's wait: whatever wrote the weights is done by then, and their first runs are
   // asked for before h is there.
@@ -111,18 +149,26 @@ __global__ void __launch_bounds__(kThreads, kGroups == 2 ? 3 : 2) few_kernel(con
     for (int p = 0; p < kX; ++p) token[n][p] = static_cast<const T*>(w.x[p]) + (8 * n + g < w.tokens ? 8 * n + g : 0) * w.ldx;
   for (int64_t at = begin; at < w.depth + t * 8; at += kAhead * step) {  // alike in a warp's lanes
     if (at != begin) load(at);
-#pragma unroll
-    for (int n = 0; n < kGroups; ++n) {
-      uint4 b[kAhead][kX];
+    uint4 rows[kAhead][kW];  // moved once for all tokens
+    if constexpr (!kVec)
 #pragma unroll
       for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-        for (int p = 0; p < kX; ++p) b[a][p] = eight<kVec>(token[n][p], at + a * step, w.depth, true);
+        for (int i = 0; i < kW; ++i) rows[a][i] = run[a][i].get(weight[i]);
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) {
+      Run<kVec ? Rows::kWhole : kUp ? Rows::kAny : Rows::kPadded, T> b[kAhead][kX];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int p = 0; p < kX; ++p)
+          b[a][p].load(token[n][p], at + a * step, w.depth, true, static_cast<const T*>(w.x[p]), static_cast<const T*>(w.x[p]) + (w.tokens - 1) * w.ldx + w.depth);
 #pragma unroll
       for (int a = 0; a < kAhead; ++a)
 #pragma unroll
         for (int p = 0; p < kX; ++p) {
-          const uint4 a0 = run[a][0], a1 = kUp ? run[a][kW - 1] : make_uint4(0u, 0u, 0u, 0u), y = b[a][p];
+          const uint4 a0 = kVec ? run[a][0].v : rows[a][0], y = b[a][p].get(token[n][p]);
+          const uint4 a1 = !kUp ? make_uint4(0u, 0u, 0u, 0u) : kVec ? run[a][kW - 1].v : rows[a][kW - 1];
           multiply<T>(sum[n], a0.x, a1.x, a0.y, a1.y, y.x, y.y);
           multiply<T>(sum[n], a0.z, a1.z, a0.w, a1.w, y.z, y.w);
         }

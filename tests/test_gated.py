@@ -184,6 +184,22 @@ def test_few_tokens_of_wide_blocks_match_64_bits(tokens, width, hidden):
     _check({"y": gated_feed_forward(x, wg, wu, wd)}, _want(x, wg, wu, wd, None, "silu", False, Rounding(torch.bfloat16)))
 
 
+# rows at every distance from 16 bytes, among numbers that are not theirs
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,width,hidden", [(1, 1023, 515), (3, 70, 33), (8, 517, 1030), (13, 259, 771), (30, 333, 130)])
+@pytest.mark.parametrize("shift", range(8))
+def test_few_tokens_between_other_numbers(tokens, width, hidden, shift):
+    x, wg, wu, wd, _ = _inputs(tokens, width, hidden, torch.float16, seed=shift)
+    want = _want(x, wg, wu, wd, None, "silu", False, Rounding(torch.float16))
+
+    def among(t, pad):
+        big = torch.full((t.shape[0] + 2, t.shape[1] + shift + pad), float("nan"), dtype=t.dtype, device="cuda")
+        return big[1:-1, shift:shift + t.shape[1]].copy_(t)
+
+    for pad in (0, 8, 13):
+        _check({"y": gated_feed_forward(among(x, pad), among(wg, pad), among(wu, pad + 3), among(wd, pad))}, want)
+
+
 # what is launched before the kernels has written the weights they read
 @pytest.mark.gpu
 def test_few_tokens_see_new_weights():
