@@ -69,7 +69,7 @@ constexpr int kGatedCopies = 5;
 cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, bool beside, cudaStream_t s);
 
 // A whole forward pass of few rows, two launches that read the weights at the rate of memory (kernels/gated_few.cu).  Rows of any
-// alignment.  `h`: scratch of 2 x tokens x gated_pitch(hidden) 16-bit numbers.
+// alignment.  `h`: scratch of tokens x gated_pitch(hidden) x 4 bytes.
 constexpr int64_t kFewTokens = 32;
 // Whether it is faster than the tiles, whose matrix instructions cost the same for any number of tokens and whose launches cost more.
 // us, here and by tiles: 2 tokens 4096 x 10240 59 and 68, 5120 x 8192 64 and 59, 5120 x 13824 98 and 93; 8 tokens 4096 x 6144 40 and 44,
@@ -78,11 +78,15 @@ inline bool gated_is_few(const GatedShape& s) {
   const int64_t n = s.width * s.hidden;
   return n <= (s.tokens <= 2 ? 48 << 20 : s.tokens <= 8 ? 32 << 20 : s.tokens <= 16 ? 8 << 20 : s.tokens <= kFewTokens ? 4 << 20 : 0);
 }
+// fp32, against three products of the linear layer and the gate between them, us: 8 tokens 256 x 704 7 and 15, 1024 x 2816 20 and 40, 1481 x
+// 4108 53 and 55, 4096 x 10240 148 and 234; 16 tokens 10 and 23, 34 and 41, 93 and 56, 251 and 256.  (The host's part: 12 and 31.)
+inline bool gated_is_few_f32(const GatedShape& s) { return s.tokens <= 8 || (s.tokens <= 16 && s.width * s.hidden <= (4 << 20)); }
 struct GatedFew {
   GatedShape shape;
   GatedOperand x, w_gate, w_up, w_down;
   void* h;
   void* y;   // rows of `width`
+  bool f32;  // all of them, whatever `shape` says
 };
 cudaError_t launch_gated_few(const GatedFew& g, cudaStream_t s);
 

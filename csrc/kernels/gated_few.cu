@@ -204,8 +204,122 @@ __global__ void __launch_bounds__(kThreads, kGroups == 2 && kVec ? 3 : 2) few_ke
   }
 }
 
+// ---- fp32 ---------------------------------------------------------------------------------------------------
+// Multiplications and additions: a warp has four rows of weights (two of either projection) and up to four tokens, a lane four numbers
+// of each at a time; `share` warps of a block share the reduction, and neighbouring blocks have the next four tokens of the same rows.
+// One token is bound by memory, 1024 x 2816 8.0 us, 2048 x 5632 27 (138 MB: 5.1 TB/s), 4096 x 10240 79 (6.4); more by the loads of
+// tokens, 4 of them 14, 42 and 113 us, 8 20, 53 and 148.  Eight tokens a warp took 32, 78 and 224 (registers); three bf16 parts of each
+// number and the matrix instructions 24, 59 and 185 of any up to 8, bound by taking the numbers apart, with 5 times the error.
+constexpr int kWeights = 4, kLaneStep = 128;  // columns of a warp's step
+template <bool kVec>
+__device__ __forceinline__ float4 four(const float* row, int64_t at, int64_t depth) {
+  if constexpr (kVec) {  // rows of whole and aligned runs of four
+    const float4 v = *reinterpret_cast<const float4*>(row + (at < depth ? at : 0));
+    return at < depth ? v : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  return make_float4(at < depth ? row[at] : 0.f, at + 1 < depth ? row[at + 1] : 0.f, at + 2 < depth ? row[at + 2] : 0.f, at + 3 < depth ? row[at + 3] : 0.f);
+}
+template <int kM, bool kUp, bool kVec>
+__global__ void __launch_bounds__(kThreads, 2) few32_kernel(const Few w, int share, int groups) {
+  constexpr int kSet = kUp ? kWeights / 2 : kWeights, kAhead = 4, kSums = kWeights * kM;
+  __shared__ float part[kWarps][kSums];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, slice = warp % share, sets = kWarps / share;
+  const int token0 = static_cast<int>(blockIdx.x % groups) * kM;
+  const int64_t first = static_cast<int64_t>(blockIdx.x / groups) * sets * kSet, row0 = first + warp / share * kSet;
+  const float* weight[kWeights];
+#pragma unroll
+  for (int r = 0; r < kWeights; ++r) {
+    const int64_t row = row0 + r % kSet;  // of rows that there are not, the first one
+    weight[r] = static_cast<const float*>(w.w[r / kSet]) + (row < w.rows ? row : 0) * w.ldw[r / kSet];
+  }
+  const int64_t begin = slice * kLaneStep + lane * 4, step = share * kLaneStep;
+  float4 run[kAhead][kWeights];
+  auto load = [&](int64_t at) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int r = 0; r < kWeights; ++r) run[a][r] = four<kVec>(weight[r], at + a * step, w.depth);
+  };
+  if constexpr (!kUp) load(begin);  // as above
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (kUp) load(begin);
+  const float* token[kM];  // of tokens that there are not, the first one's
+#pragma unroll
+  for (int m = 0; m < kM; ++m) token[m] = static_cast<const float*>(w.x[0]) + (token0 + m < w.tokens ? token0 + m : 0) * w.ldx;
+  float sum[kSums];
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) sum[i] = 0.f;
+  for (int64_t at = begin; at < w.depth; at += kAhead * step) {
+    if (at != begin) load(at);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int m = 0; m < kM; ++m) {
+        const float4 x = four<kVec>(token[m], at + a * step, w.depth);
+#pragma unroll
+        for (int r = 0; r < kWeights; ++r) {
+          float& v = sum[r * kM + m];
+          v = fmaf(run[a][r].x, x.x, fmaf(run[a][r].y, x.y, fmaf(run[a][r].z, x.z, fmaf(run[a][r].w, x.w, v))));
+        }
+      }
+  }
+  // each lane hands on half of what it has, until it has one sum
+#pragma unroll
+  for (int o = 16, n = kSums; o > 0; o /= 2) {
+    if (n > 1) {
+      n /= 2;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float mine = lane & o ? sum[i + n] : sum[i], other = lane & o ? sum[i] : sum[i + n];
+        sum[i] = mine + __shfl_xor_sync(0xFFFFFFFFu, other, o);
+      }
+    } else {
+      sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], o);
+    }
+  }
+  if (lane % (32 / kSums) == 0) part[warp][lane / (32 / kSums)] = sum[0];
+  __syncthreads();
+  for (int item = threadIdx.x; item < sets * kSet * kM; item += kThreads) {
+    const int m = item % kM, r = item / kM % kSet, set = item / (kM * kSet);
+    const int64_t row = first + set * kSet + r;
+    if (token0 + m >= w.tokens || row >= w.rows) continue;
+    float v[2] = {0.f, 0.f};
+    for (int p = set * share; p < (set + 1) * share; ++p) {
+      v[0] += part[p][r * kM + m];
+      if constexpr (kUp) v[1] += part[p][(kSet + r) * kM + m];
+    }
+    static_cast<float*>(w.out[0])[(token0 + m) * w.ldo + row] = kUp ? v[0] * gate(v[0], w.c0, w.c1) * v[1] : v[0];
+  }
+}
+// Warps that share a reduction: as many as leave the device full, and each a step.
+template <bool kUp, bool kVec>
+cudaError_t run32(const Few& w, cudaStream_t s) {
+  constexpr int64_t kSet = kUp ? kWeights / 2 : kWeights, kFull = 148 * 16;
+  const int64_t sets = (w.rows + kSet - 1) / kSet;
+  int share = 1;
+  while (share < kWarps && sets * share < kFull && w.depth > share * kLaneStep) share *= 2;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  const int groups = static_cast<int>((w.tokens + 3) / 4);
+  cfg.gridDim = dim3(static_cast<unsigned>((sets * share + kWarps - 1) / kWarps * groups));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  note_launch();
+  if (w.tokens <= 1) return cudaLaunchKernelEx(&cfg, few32_kernel<1, kUp, kVec>, w, share, groups);
+  if (w.tokens <= 2) return cudaLaunchKernelEx(&cfg, few32_kernel<2, kUp, kVec>, w, share, groups);
+  return cudaLaunchKernelEx(&cfg, few32_kernel<4, kUp, kVec>, w, share, groups);
+}
+
 template <typename T, bool kUp, bool kVec>
 cudaError_t run(const Few& w, cudaStream_t s) {
+  if constexpr (std::is_same_v<T, float>) {
+    return run32<kUp, kVec>(w, s);
+  } else {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -219,15 +333,20 @@ cudaError_t run(const Few& w, cudaStream_t s) {
   if (w.tokens <= 8) return cudaLaunchKernelEx(&cfg, few_kernel<T, 1, kUp, kVec>, w);
   if (w.tokens <= 16) return cudaLaunchKernelEx(&cfg, few_kernel<T, 2, kUp, kVec>, w);
   return cudaLaunchKernelEx(&cfg, few_kernel<T, 4, kUp, kVec>, w);
+  }
 }
-bool aligned(const GatedOperand& m, int64_t rows) { return reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && (rows <= 1 || m.ld % 8 == 0); }
+template <typename T>
+bool aligned(const GatedOperand& m, int64_t rows) {
+  return reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && (rows <= 1 || m.ld * sizeof(T) % 16 == 0);
+}
 
 template <typename T>
 cudaError_t both(const GatedFew& g, cudaStream_t s) {
   const GatedShape& h = g.shape;
   const double log2e = 1.4426950408889634, gelu = 1.5957691216057308;  // 2 sqrt(2 / pi)
   const int64_t pitch = gated_pitch(h.hidden);
-  T* const parts[2] = {static_cast<T*>(g.h), static_cast<T*>(g.h) + h.tokens * pitch};
+  constexpr int kRun = 16 / sizeof(T);
+  T* const parts[2] = {static_cast<T*>(g.h), static_cast<T*>(g.h) + h.tokens * pitch};  // (fp32: the first alone)
   Few w{};
   w.c0 = static_cast<float>(h.activation == GatedActivation::kSilu ? -log2e : -log2e * gelu);
   w.c1 = h.activation == GatedActivation::kSilu ? 0.f : static_cast<float>(-log2e * gelu * 0.044715);
@@ -243,7 +362,7 @@ cudaError_t both(const GatedFew& g, cudaStream_t s) {
   w.ldo = pitch;
   w.rows = h.hidden;
   w.depth = h.width;
-  const bool whole = h.width % 8 == 0 && aligned(g.x, h.tokens) && aligned(g.w_gate, h.hidden) && aligned(g.w_up, h.hidden);
+  const bool whole = h.width % kRun == 0 && aligned<T>(g.x, h.tokens) && aligned<T>(g.w_gate, h.hidden) && aligned<T>(g.w_up, h.hidden);
   const cudaError_t e = whole ? run<T, true, true>(w, s) : run<T, true, false>(w, s);
   if (e != cudaSuccess) return e;
   w.x[0] = parts[0];
@@ -255,7 +374,7 @@ cudaError_t both(const GatedFew& g, cudaStream_t s) {
   w.ldo = h.width;
   w.rows = h.width;
   w.depth = h.hidden;
-  return h.hidden % 8 == 0 && aligned(g.w_down, h.width) ? run<T, false, true>(w, s) : run<T, false, false>(w, s);
+  return h.hidden % kRun == 0 && aligned<T>(g.w_down, h.width) ? run<T, false, true>(w, s) : run<T, false, false>(w, s);
 }
 
 }  // namespace
@@ -264,7 +383,7 @@ cudaError_t launch_gated_few(const GatedFew& g, cudaStream_t s) {
   const GatedShape& h = g.shape;
   if (h.tokens <= 0 || h.tokens > kFewTokens || h.width <= 0 || h.hidden <= 0 || reinterpret_cast<uintptr_t>(g.h) % 16 != 0) return cudaErrorInvalidValue;
   if (h.width > 0x7FFFFFFFll || h.hidden > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  return h.bf16 ? both<__nv_bfloat16>(g, s) : both<__half>(g, s);
+  return g.f32 ? both<float>(g, s) : h.bf16 ? both<__nv_bfloat16>(g, s) : both<__half>(g, s);
 }
 
 }  // namespace kern

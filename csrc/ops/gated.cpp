@@ -106,6 +106,15 @@ struct Products {
 
 at::Tensor few_rows(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
 
+void few(const kern::GatedShape& s, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, const at::Tensor& y) {
+  const at::Tensor rows[4] = {few_rows(x), few_rows(wg), few_rows(wu), few_rows(wd)};
+  const bool f32 = x.scalar_type() == at::kFloat;
+  const at::Tensor h = at::empty({f32 ? 1 : 2, s.tokens, kern::gated_pitch(s.hidden)}, x.options());
+  kern::GatedOperand m[4];
+  for (int i = 0; i < 4; ++i) m[i] = {rows[i].const_data_ptr(), row_stride(rows[i])};
+  OPS_CK(kern::launch_gated_few({s, m[0], m[1], m[2], m[3], h.data_ptr(), y.data_ptr(), f32}, at::cuda::getCurrentCUDAStream()));
+}
+
 // y of 16-bit rows; g and u to `kept` where there is one.
 at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, kern::GatedActivation act,
                      kern::GatedKeep keep, at::Tensor* kept, int64_t wait_limit = -1) {
@@ -116,11 +125,7 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
   if (keep != kern::GatedKeep::kNone) *kept = at::empty({kern::gated_kept_bytes(s)}, x.options().dtype(at::kByte));
   if (x.size(0) == 0) return y;
   if (keep == kern::GatedKeep::kNone && kern::gated_is_few(s) && wait_limit < 0) {
-    const at::Tensor rows[4] = {few_rows(x), few_rows(wg), few_rows(wu), few_rows(wd)};
-    const at::Tensor h = at::empty({2, s.tokens, kern::gated_pitch(s.hidden)}, x.options());
-    kern::GatedOperand m[4];
-    for (int i = 0; i < 4; ++i) m[i] = {rows[i].const_data_ptr(), row_stride(rows[i])};
-    OPS_CK(kern::launch_gated_few({s, m[0], m[1], m[2], m[3], h.data_ptr(), y.data_ptr()}, at::cuda::getCurrentCUDAStream()));
+    few(s, x, wg, wu, wd, y);
     return y;
   }
   Operands m;
@@ -189,7 +194,7 @@ Gradients backward16(const at::Tensor& dy, const at::Tensor& x, const at::Tensor
 // ---- fp32: the products of the linear layer -----------------------------------------------------------------------
 // With gradients both projections are one product of the two weights one behind the other: two thirds of the products of three
 // weights, and one sum for the gradient of x.  (Putting them together costs their size twice in traffic; 256 x 1024 x 2816, forward and
-// backward: 215 us without, 193 so.)  A forward pass alone leaves them where they are.
+// backward: 215 us without, 193 so.)  A forward pass alone leaves them where they are; of few tokens it has kernels of its own.
 at::Tensor joined(const at::Tensor& wg, const at::Tensor& wu) { return at::cat({wg, wu}, 0); }
 
 at::Tensor gate32(const at::Tensor& g, const at::Tensor& u, kern::GatedActivation act) {
@@ -207,6 +212,12 @@ at::Tensor forward32(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
   if (kept) {
     *kept = mccl::linear(x, joined(wg, wu), c10::nullopt);
     return mccl::linear(gate32(*kept, act), wd, c10::nullopt);
+  }
+  const kern::GatedShape s = shape_of(x, wg.size(0), act, kern::GatedKeep::kNone);
+  if (x.size(0) > 0 && kern::gated_is_few_f32(s)) {
+    const at::Tensor y = at::empty(x.sizes(), x.options());
+    few(s, x, wg, wu, wd, y);
+    return y;
   }
   return mccl::linear(gate32(mccl::linear(x, wg, c10::nullopt), mccl::linear(x, wu, c10::nullopt), act), wd, c10::nullopt);
 }

@@ -184,6 +184,29 @@ def test_few_tokens_of_wide_blocks_match_64_bits(tokens, width, hidden):
     _check({"y": gated_feed_forward(x, wg, wu, wd)}, _want(x, wg, wu, wd, None, "silu", False, Rounding(torch.bfloat16)))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("width,hidden", [(1024, 2816), (1000, 2731), (999, 514), (8, 24), (5, 3), (1, 1), (260, 136), (136, 9000), (3000, 1500)])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 13, 16, 17])
+def test_few_tokens_of_float32_match_64_bits(tokens, width, hidden, activation):
+    x, wg, wu, wd, _ = _inputs(tokens, width, hidden, torch.float32, seed=tokens)
+    want = _want(x, wg, wu, wd, None, activation, False, Rounding(torch.float32))
+    _check({"y": gated_feed_forward(x, wg, wu, wd, activation=activation)}, want)
+
+    def among(t, shift):
+        big = torch.full((t.shape[0] + 2, t.shape[1] + 5 + shift), float("nan"), device="cuda")
+        return big[1:-1, shift:shift + t.shape[1]].copy_(t)
+
+    for shift in range(4):
+        _check({"y": gated_feed_forward(among(x, shift), among(wg, 3 - shift), wu.t().contiguous().t(), among(wd, shift), activation=activation)}, want)
+    same = gated_feed_forward(x[:1].expand(tokens, width), wg, wu, wd, activation=activation)
+    _check({"y": same[-1:]}, {"y": tuple(t[:1] for t in want["y"])})
+    bad = x.clone()
+    bad[0, width // 2] = float("nan")
+    got = gated_feed_forward(bad, wg, wu, wd, activation=activation)
+    assert torch.isnan(got[0]).all() and torch.isfinite(got[1:]).all()
+
+
 # rows at every distance from 16 bytes, among numbers that are not theirs
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens,width,hidden", [(1, 1023, 515), (3, 70, 33), (8, 517, 1030), (13, 259, 771), (30, 333, 130)])
