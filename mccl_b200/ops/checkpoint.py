@@ -8,6 +8,7 @@ comes back as zeros.
 
 :func:`pack8` and :func:`unpack8` are the two halves, for a program's own layers; :func:`linear` is a linear layer whose input
 is kept so, and ``mccl_b200.ops.gated`` keeps its activations so on request, written and read inside of its products' kernels.
+CPU tensors, and calls under a dispatch mode (``make_fx``, flop counters), take the same formula in torch, bit for bit.
 """
 from __future__ import annotations
 
@@ -17,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from ._native import native
+from ._native import native, on_kernels
 
 GROUP = 64
 _TINY = 2.0 ** -100
@@ -40,13 +41,13 @@ def _check(x: torch.Tensor) -> None:
 def pack8(x: torch.Tensor) -> Packed8:
     """``x`` in 8 bits.  Not differentiable: what is kept is no function of the graph."""
     _check(x)
-    if x.is_cuda:
+    if on_kernels(x):
         codes, scales = native()._pack8(x)
         return Packed8(codes, scales, tuple(x.shape), x.dtype)
     x = x.detach()
     cols = x.shape[-1] if x.dim() else 1
     groups, rows = -(-cols // GROUP), math.prod(x.shape[:-1])
-    v = torch.zeros(rows, groups * GROUP)
+    v = torch.zeros(rows, groups * GROUP, device=x.device)
     v[:, :cols] = x.reshape(rows, cols)
     v = v.view(rows, groups, GROUP)
     most = v.abs().amax(-1, keepdim=True) if v.numel() else v[..., :1]
@@ -59,7 +60,7 @@ def pack8(x: torch.Tensor) -> Packed8:
 
 def unpack8(packed: Packed8) -> torch.Tensor:
     """The values, in the shape and type that they had."""
-    if packed.codes.is_cuda:
+    if on_kernels(packed.codes):
         return native()._unpack8(packed.codes, packed.scales, list(packed.shape), packed.dtype)
     rows, pitch = packed.codes.shape
     cols = packed.shape[-1] if packed.shape else 1

@@ -8,7 +8,8 @@ range becomes infinite there).  ``float32``: the products of ``mccl_b200.ops.lin
 What the backward pass needs of the two projections is kept with 16 significant bits (three bytes a number); with
 ``checkpoint="int8"`` it is kept, and the input too, as 8-bit codes with a scale for each group of 64 (see
 ``mccl_b200.ops.checkpoint``), and the gradients are those of the kept values.  The backward pass is not differentiable itself.
-CPU tensors take the same formulas in torch.
+CPU tensors, and calls under a dispatch mode (``make_fx``, flop counters), take the same formulas in torch; a backward pass takes
+the form that its forward pass took.
 """
 from __future__ import annotations
 
@@ -19,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._native import native
+from ._native import native, on_kernels
 from .checkpoint import Packed8, pack8, unpack8
 
 ACTIVATIONS = ("silu", "gelu_tanh")
@@ -41,9 +42,12 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
             to = torch.get_autocast_dtype("cuda")
             x, w_gate, w_up, w_down = x.to(to), w_gate.to(to), w_up.to(to), w_down.to(to)
             with torch.autocast("cuda", enabled=False):
-                return native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
-        return native()._gated_feed_forward(x, w_gate, w_up, w_down, activation, checkpoint is not None)
-    return _Plain.apply(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+                return _call(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+    return _call(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+
+
+def _call(x, *args):
+    return native()._gated_feed_forward(x, *args) if on_kernels(x) else _Plain.apply(x, *args)
 
 
 def _act(name, g):

@@ -8,7 +8,8 @@ The angles come from a table, :func:`rotary_table` or a program's own (scaled or
 rotary / 2]``, cosines and then sines.  A token whose position is outside of the table gets NaN in its rotated part.
 
 Gradients: of queries and keys (of the packed form one gradient of the projection, values included) and of the two weights,
-summed in a fixed order.  The backward pass is not differentiable itself.  CPU tensors take the same formulas in torch.
+summed in a fixed order.  The backward pass is not differentiable itself.  CPU tensors, and calls under a dispatch mode
+(``make_fx``, flop counters), take the same formulas in torch.
 """
 from __future__ import annotations
 
@@ -16,7 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._native import native
+from ._native import native, on_kernels
 
 
 def rotary_table(positions: int, rotary: int, *, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -35,7 +36,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weig
 
     ``positions``: int64 or int32, [tokens] or [batch, tokens]; 0, 1, ... in each batch without it.
     """
-    if q.is_cuda:
+    if on_kernels(q):
         return native()._norm_rotate(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     if not eps > 0:
         raise ValueError("eps must be positive")
@@ -47,7 +48,7 @@ def norm_rotate_packed(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
                        eps: float = 1e-6, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """:func:`norm_rotate` of one projection [batch, tokens, (heads + 2 kv_heads) * dim]; also the view of its values."""
     kv_heads = heads if kv_heads is None else kv_heads
-    if qkv.is_cuda:
+    if on_kernels(qkv):
         return native()._norm_rotate_packed(qkv, q_weight, k_weight, table, positions, heads, kv_heads, eps, interleaved)
     if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[-1] % (heads + 2 * kv_heads):
         raise ValueError(f"norm_rotate_packed: [batch, tokens, (heads + 2 kv_heads) dim] expected, got {tuple(qkv.shape)}")
