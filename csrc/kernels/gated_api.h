@@ -57,7 +57,9 @@ int64_t gated_partial_bytes(const GatedProduct* p, int n, const GatedShape& s);
 cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaStream_t s);
 
 // Matrices of 16-bit numbers whose rows are not 16-byte aligned (or whose numbers do not lie side by side) copied to ones that are,
-// up to five in one launch.  `beside`: while the launch of this file before it runs, which neither reads `to` nor writes `from`.
+// up to five in one launch.  `beside`: without waiting for the last launch_gated before it on this stream, nor for anything launched
+// behind that one; neither it nor these may read or write `to` or write `from`.  So `to` was allocated before that launch, at which all
+// earlier work on the stream is done: a block that the allocator hands out later may have been another thread's, whose kernels still run.
 struct GatedCopy {
   const void* from;
   int64_t row_stride, col_stride, rows, cols;  // elements

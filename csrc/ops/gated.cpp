@@ -59,10 +59,15 @@ class Operands {
     return n_++;
   }
   bool any() const { return copied_ > 0; }
-  // Before what reads them; `beside` the product launched last, which doesn't.
+  // The copies' memory.  What was freed before had its last use on this stream before now.
+  void reserve(const at::Tensor& like) {
+    if (copied_ > 0 && !held_.defined()) held_ = at::empty({bytes_}, like.options().dtype(at::kByte));
+  }
+  // Before what reads them.  `beside`: while the products launched since reserve() run, none of which reads them; the copies don't wait
+  // for these, nor for what another thread has launched on this stream since then, so no memory that was in use since may be theirs.
   void copy(const at::Tensor& like, bool beside = false) {
     if (copied_ == 0) return;
-    held_ = at::empty({bytes_}, like.options().dtype(at::kByte));
+    reserve(like);
     char* at = static_cast<char*>(held_.data_ptr());
     for (int i = 0; i < copied_; ++i) {
       copies_[i].to = at;
@@ -133,6 +138,7 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& wg, const at::Tensor
   const bool first = m.any();  // else a copy of w_down has time until the second product
   const int od = m.add(wd);
   if (first) m.copy(x);
+  else m.reserve(x);
   const at::Tensor h = at::empty({s.tokens, kern::gated_pitch(s.hidden)}, x.options());
   Products run(s, x, wait_limit);
   run.r.kept = kept ? kept->data_ptr() : nullptr;

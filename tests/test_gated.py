@@ -2,6 +2,7 @@
 import math
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
@@ -428,6 +429,54 @@ def test_copied_rows_of_calls_one_after_another(tokens, width, hidden):
     for _ in range(5):
         graph.replay()
     assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_memory_of_copies_beside_a_product_is_taken_before_it():
+    # these copies wait for nothing that runs, so a block that is freed after the product before them was launched may not be theirs
+    tokens, width, hidden = 333, 1024, 2731
+    x, wg, wu, wd = _inputs(tokens, width, hidden, torch.bfloat16)[:4]
+    gated_feed_forward(x, wg, wu, wd)
+    torch.cuda.synchronize()
+    torch.cuda.memory._record_memory_history(max_entries=1000)
+    try:
+        gated_feed_forward(x, wg, wu, wd)
+        trace = torch.cuda.memory._snapshot()["device_traces"][0]
+    finally:
+        torch.cuda.memory._record_memory_history(enabled=None)
+    sizes = [e["size"] for e in trace if e["action"] == "alloc"]
+    copies, h = width * 2736 * 2, tokens * 2752 * 2
+    assert sizes.count(copies) == 1 and sizes.count(h) == 1 and sizes.index(copies) < sizes.index(h)
+
+
+@pytest.mark.gpu
+def test_threads_that_share_a_stream():
+    from mccl_b200.ops.linear import linear
+    x, wg, wu, wd = _inputs(333, 1024, 2731, torch.bfloat16)[:4]    # w_down is copied beside the first product
+    y, vg, vu, vd = _inputs(1000, 640, 2112, torch.bfloat16, seed=1)[:4]  # reductions that pairs share: a launch that adds them up
+    a, b, _, _, _ = _inputs(64, 1024, 4096, torch.float32, seed=2)
+    calls = [lambda: gated_feed_forward(x, wg, wu, wd), lambda: gated_feed_forward(y, vg, vu, vd), lambda: linear(a, b)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    stream, wrong, ready = torch.cuda.current_stream(), [], threading.Barrier(len(calls))
+
+    def work(i):
+        try:
+            with torch.no_grad(), torch.cuda.stream(stream):
+                ready.wait()
+                for _ in range(40):
+                    got = [calls[i]() for _ in range(10)]
+                    if not all(torch.equal(g, want[i]) for g in got):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 @pytest.mark.gpu
