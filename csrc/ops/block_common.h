@@ -38,6 +38,18 @@ inline void check_block_tensor(const at::Tensor& t, const char* what) {
   MCCL_CHECK_T(TensorError, ordinary(t), what << ": tensor subclasses, transforms and forward-mode tangents are not supported");
   MCCL_CHECK_T(DeviceError, device_fits(t.get_device()), what << ": built for compute capability 10.0");
 }
+// A tensor that was saved for the backward pass, as it comes back: a hook of the caller's may have laid it out anew, but may not have made
+// another one of it, whose memory the kernels would run out of.
+inline void check_saved(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& device, const char* what) {
+  check_block_tensor(t, what);
+  MCCL_CHECK_T(TensorError, t.sizes() == sizes && t.scalar_type() == type && t.device() == device,
+               what << ": a tensor saved for the backward pass came back as " << t.scalar_type() << " " << t.sizes() << " on " << t.device());
+}
+// Its numbers one behind the other from a multiple of 16 bytes on, as they were saved.
+inline at::Tensor packed_again(const at::Tensor& t) {
+  const at::Tensor r = t.contiguous();
+  return reinterpret_cast<uintptr_t>(r.const_data_ptr()) % 16 == 0 ? r : r.clone();
+}
 // `t` as rows along its last dimension: a view where its layout allows it, else a copy.
 inline at::Tensor rows_of(const at::Tensor& t) {
   const int64_t cols = t.dim() ? t.size(-1) : 1;

@@ -18,9 +18,9 @@ std::tuple<at::Tensor, at::Tensor> pack8(const at::Tensor& x) {
   return {codes, scales};
 }
 
-at::Tensor unpack8(const at::Tensor& codes, const at::Tensor& scales, at::IntArrayRef shape, at::ScalarType type) {
-  check_block_tensor(codes, "unpack8");
-  check_block_tensor(scales, "unpack8");
+at::Tensor unpack8(const at::Tensor& codes_in, const at::Tensor& scales_in, at::IntArrayRef shape, at::ScalarType type) {
+  check_block_tensor(codes_in, "unpack8");
+  check_block_tensor(scales_in, "unpack8");
   int64_t rows = 1;
   for (size_t d = 0; d < shape.size(); ++d) {
     MCCL_CHECK_T(TensorError, shape[d] >= 0, "unpack8: negative size");
@@ -28,12 +28,12 @@ at::Tensor unpack8(const at::Tensor& codes, const at::Tensor& scales, at::IntArr
   }
   const int64_t cols = shape.empty() ? 1 : shape.back();
   MCCL_CHECK_T(TensorError,
-               codes.scalar_type() == at::kChar && scales.scalar_type() == at::kFloat && codes.is_contiguous() && scales.is_contiguous() &&
-                   codes.dim() == 2 && scales.dim() == 2 && codes.size(0) == rows && scales.size(0) == rows &&
-                   codes.size(1) == kern::pack8_pitch(cols) && scales.size(1) == kern::pack8_groups(cols) && codes.device() == scales.device() &&
-                   reinterpret_cast<uintptr_t>(codes.const_data_ptr()) % 8 == 0,
+               codes_in.scalar_type() == at::kChar && scales_in.scalar_type() == at::kFloat && codes_in.dim() == 2 && scales_in.dim() == 2 &&
+                   codes_in.size(0) == rows && scales_in.size(0) == rows && codes_in.size(1) == kern::pack8_pitch(cols) &&
+                   scales_in.size(1) == kern::pack8_groups(cols) && codes_in.device() == scales_in.device(),
                "unpack8: codes and scales are not those of pack8 for this shape");
-  c10::cuda::CUDAGuard guard(codes.device());
+  c10::cuda::CUDAGuard guard(codes_in.device());
+  const at::Tensor codes = packed_again(codes_in), scales = packed_again(scales_in);
   at::Tensor x = at::empty(shape, codes.options().dtype(type));
   const kern::Packed8Rows p{const_cast<int8_t*>(codes.const_data_ptr<int8_t>()), const_cast<float*>(scales.const_data_ptr<float>()), rows, cols,
                             kern::pack8_pitch(cols)};

@@ -249,16 +249,11 @@ Gradients backward32(const at::Tensor& dy, const at::Tensor& x, const at::Tensor
 }
 
 // ---- autograd -----------------------------------------------------------------------------------------------------
-// What is packed, to rows of a matrix; to rows that the products can read.
+// What is packed, to rows of a matrix.
 void unpack_to(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales) {
   const kern::Packed8Rows p{const_cast<int8_t*>(codes.const_data_ptr<int8_t>()), const_cast<float*>(scales.const_data_ptr<float>()), x.size(0), x.size(1),
                             kern::pack8_pitch(x.size(1))};
   OPS_CK(kern::launch_unpack8(p, x.data_ptr(), elem_of(x, kWhat), x.stride(0), at::cuda::getCurrentCUDAStream()));
-}
-at::Tensor unpacked(const at::Tensor& codes, const at::Tensor& scales, int64_t rows, int64_t cols, const at::TensorOptions& like) {
-  const at::Tensor x = at::empty({rows, kern::gated_row(cols)}, like).narrow(1, 0, cols);
-  unpack_to(x, codes, scales);
-  return x;
 }
 
 struct GatedFn : torch::autograd::Function<GatedFn> {
@@ -269,6 +264,8 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     ctx->saved_data["act"] = act;
     ctx->saved_data["eight"] = eight;
     ctx->saved_data["rows"] = x.size(0);
+    ctx->saved_data["width"] = wg.size(1);
+    ctx->saved_data["hidden"] = wg.size(0);
     std::vector<at::Tensor> saved{wg, wu, wd};
     at::Tensor y;
     if (x.scalar_type() == at::kFloat) {
@@ -304,30 +301,47 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     const at::Tensor &wg = saved[0], &wu = saved[1], &wd = saved[2];
     const auto act = static_cast<kern::GatedActivation>(ctx->saved_data["act"].toInt());
     const bool eight = ctx->saved_data["eight"].toBool();
-    const int64_t rows = ctx->saved_data["rows"].toInt(), width = wg.size(1), hidden = wg.size(0);
+    const int64_t rows = ctx->saved_data["rows"].toInt(), width = ctx->saved_data["width"].toInt(), hidden = ctx->saved_data["hidden"].toInt();
     check_block_tensor(dy, kWhat);
-    MCCL_CHECK_T(TensorError, dy.dim() == 2 && dy.size(0) == rows && dy.size(1) == width && dy.scalar_type() == wg.scalar_type() && dy.device() == wg.device(),
-                 kWhat << ": not a gradient of its result");
+    MCCL_CHECK_T(TensorError, dy.dim() == 2 && dy.size(0) == rows && dy.size(1) == width, kWhat << ": not a gradient of its result");
+    const auto type = dy.scalar_type();
+    auto back = [&](const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType of) -> const at::Tensor& {
+      check_saved(t, sizes, of, dy.device(), kWhat);
+      return t;
+    };
+    back(wg, {hidden, width}, type);
+    back(wu, {hidden, width}, type);
+    back(wd, {width, hidden}, type);
     c10::cuda::CUDAGuard guard(dy.device());
+    // codes and scales of `cols` columns from saved[i] on, to rows of x
+    auto unpack = [&](const at::Tensor& x, size_t i) {
+      unpack_to(x, packed_again(back(saved[i], {rows, kern::pack8_pitch(x.size(1))}, at::kChar)),
+                packed_again(back(saved[i + 1], {rows, kern::pack8_groups(x.size(1))}, at::kFloat)));
+    };
+    auto kept_x = [&] {
+      if (!eight) return back(saved[3], {rows, width}, type);
+      const at::Tensor x = at::empty({rows, kern::gated_row(width)}, dy.options()).narrow(1, 0, width);
+      unpack(x, 3);
+      return x;
+    };
     const Needs need{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3)};
     const bool need_up = need.gate || need.up;
     Gradients r;
-    if (wg.scalar_type() == at::kFloat) {
+    if (type == at::kFloat) {
       dy = dy.contiguous();
-      at::Tensor x, gu;
+      at::Tensor gu;
       if (eight) {
-        x = need_up ? unpacked(saved[3], saved[4], rows, width, wg.options()) : at::empty({rows, width}, wg.options());
-        gu = at::empty({rows, 2 * hidden}, wg.options());
-        unpack_to(gu.narrow(1, 0, hidden), saved[5], saved[6]);
-        unpack_to(gu.narrow(1, hidden, hidden), saved[7], saved[8]);
+        gu = at::empty({rows, 2 * hidden}, dy.options());
+        unpack(gu.narrow(1, 0, hidden), 5);
+        unpack(gu.narrow(1, hidden, hidden), 7);
       } else {
-        x = saved[3];
-        gu = saved[4];
+        gu = back(saved[4], {rows, 2 * hidden}, type).contiguous();
       }
-      r = backward32(dy, x, wg, wu, wd, gu, act, need);
+      r = backward32(dy, need_up ? kept_x() : at::empty({rows, width}, dy.options()), wg, wu, wd, gu, act, need);
     } else {
-      const at::Tensor x = !need_up || rows == 0 ? at::Tensor() : eight ? unpacked(saved[3], saved[4], rows, width, wg.options()) : saved[3];
-      r = backward16(dy, x, wg, wu, wd, saved.back(), act, eight ? kern::GatedKeep::kEight : kern::GatedKeep::kWide, need);
+      const auto keep = eight ? kern::GatedKeep::kEight : kern::GatedKeep::kWide;
+      const at::Tensor kept = packed_again(back(saved.back(), {kern::gated_kept_bytes(shape_of(dy, hidden, act, keep))}, at::kByte));
+      r = backward16(dy, need_up && rows > 0 ? kept_x() : at::Tensor(), wg, wu, wd, kept, act, keep, need);
     }
     return {r.x, need.gate ? r.gate : at::Tensor(), need.up ? r.up : at::Tensor(), r.down, {}, {}};
   }

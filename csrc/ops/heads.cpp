@@ -94,7 +94,7 @@ std::tuple<at::Tensor, at::Tensor> forward_of(const kern::HeadsShape& s, const k
 // A gradient as the kernels read it; none is zeros.
 at::Tensor grad_for(const at::Tensor& g, const at::Tensor& like, at::IntArrayRef sizes) {
   if (!g.defined()) return at::zeros(sizes, like.options());
-  MCCL_CHECK_T(TensorError, ordinary(g) && g.scalar_type() == like.scalar_type() && g.sizes() == sizes, "norm_rotate: not a gradient of its results");
+  MCCL_CHECK_T(TensorError, ordinary(g) && g.scalar_type() == like.scalar_type() && g.device() == like.device() && g.sizes() == sizes, "norm_rotate: not a gradient of its results");
   return side_by_side(g);
 }
 
@@ -169,9 +169,10 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_second("norm_rotate");
     const auto saved = ctx->get_saved_variables();
+    heads_of(saved[0], saved[1]);
     c10::cuda::CUDAGuard guard(saved[0].device());
     const at::Tensor q = side_by_side(saved[0]), k = side_by_side(saved[1]);
-    const Kept kept{saved[2], saved[3], saved[4], saved[5]};
+    const Kept kept{saved[2].contiguous(), saved[3].contiguous(), saved[4].contiguous(), saved[5]};
     const at::Tensor dq = grad_for(g[0], q, q.sizes()), dk = grad_for(g[1], k, k.sizes());
     at::Tensor dqo = out_like(q), dko = out_like(k);
     kern::HeadsBackward a{};
@@ -205,8 +206,12 @@ struct NormRotatePacked : torch::autograd::Function<NormRotatePacked> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_second("norm_rotate_packed");
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor& qkv = saved[0];
-    const Kept kept{saved[1], saved[2], saved[3], saved[4]};
+    check_block_tensor(saved[0], kWhat);
+    const int64_t kinds = ctx->saved_data["heads"].toInt() + 2 * ctx->saved_data["kv_heads"].toInt();
+    MCCL_CHECK_T(TensorError, saved[0].dim() == 3 && saved[0].size(2) > 0 && saved[0].size(2) % kinds == 0,
+                 "norm_rotate_packed: a tensor saved for the backward pass came back as " << saved[0].sizes());
+    const at::Tensor qkv = saved[0].size(2) == 1 || saved[0].stride(2) == 1 ? saved[0] : saved[0].contiguous();
+    const Kept kept{saved[1].contiguous(), saved[2].contiguous(), saved[3].contiguous(), saved[4]};
     c10::cuda::CUDAGuard guard(qkv.device());
     const Packed p = packed_of(qkv, ctx->saved_data["heads"].toInt(), ctx->saved_data["kv_heads"].toInt());
     at::Tensor out = at::empty(qkv.sizes(), qkv.options());
