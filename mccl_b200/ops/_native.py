@@ -5,6 +5,9 @@ import torch
 
 from .. import require_native
 
+_included = torch._C._dispatch_tls_is_dispatch_key_included
+_PYTHON, _PRE_DISPATCH = torch._C.DispatchKey.Python, torch._C.DispatchKey.PreDispatch
+
 
 def native():
     """The library; refuses under ``torch.jit.trace``, which would record a call's results as constants."""
@@ -19,6 +22,16 @@ def on_kernels(x: torch.Tensor) -> bool:
     Not under a mode that has to see the operators of torch that a call is made of (``make_fx``, which would record a result of the
     kernels as an empty tensor, flop counters, selective recomputation): the formulas in torch answer there.
     """
-    key = torch._C.DispatchKey
-    included = torch._C._dispatch_tls_is_dispatch_key_included
-    return x.is_cuda and not (included(key.Python) or included(key.PreDispatch))
+    return x.is_cuda and not (_included(_PYTHON) or _included(_PRE_DISPATCH))
+
+
+def autocast_of(x: torch.Tensor):
+    """The device type whose autocast is on for a call on ``x``, or None."""
+    device = "cuda" if x.is_cuda else x.device.type
+    return device if torch.is_autocast_enabled(device) else None
+
+
+def cast(device: str, *tensors):
+    """The tensors as that autocast casts a product's."""
+    to = torch.get_autocast_dtype(device)
+    return [None if t is None else t.to(to) for t in tensors]

@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from ._native import native, on_kernels
+from ._native import autocast_of, cast, native, on_kernels
 
 GROUP = 64
 _TINY = 2.0 ** -100
@@ -94,9 +94,9 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
     Under autocast the three are cast first, as ``torch.nn.functional.linear`` casts them.
     """
-    if input.is_cuda and torch.is_autocast_enabled("cuda"):
-        to = torch.get_autocast_dtype("cuda")
-        input, weight, bias = input.to(to), weight.to(to), None if bias is None else bias.to(to)
-        with torch.autocast("cuda", enabled=False):
+    device = autocast_of(input)
+    if device is not None:
+        input, weight, bias = cast(device, input, weight, bias)
+        with torch.autocast(device, enabled=False):
             return _Linear8.apply(input, weight, bias)
     return _Linear8.apply(input, weight, bias)

@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._native import native, on_kernels
+from ._native import autocast_of, cast, native, on_kernels
 from .checkpoint import Packed8, pack8, unpack8
 
 ACTIVATIONS = ("silu", "gelu_tanh")
@@ -37,12 +37,11 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
         raise ValueError(f"activation is one of {ACTIVATIONS}, got {activation!r}")
     if checkpoint not in (None, "int8"):
         raise ValueError(f"checkpoint is None or 'int8', got {checkpoint!r}")
-    if x.is_cuda:
-        if torch.is_autocast_enabled("cuda"):
-            to = torch.get_autocast_dtype("cuda")
-            x, w_gate, w_up, w_down = x.to(to), w_gate.to(to), w_up.to(to), w_down.to(to)
-            with torch.autocast("cuda", enabled=False):
-                return _call(x, w_gate, w_up, w_down, activation, checkpoint is not None)
+    device = autocast_of(x)
+    if device is not None:
+        x, w_gate, w_up, w_down = cast(device, x, w_gate, w_up, w_down)
+        with torch.autocast(device, enabled=False):
+            return _call(x, w_gate, w_up, w_down, activation, checkpoint is not None)
     return _call(x, w_gate, w_up, w_down, activation, checkpoint is not None)
 
 

@@ -534,3 +534,17 @@ def test_cpu_form(activation, eight):
     block(x).sum().backward()
     assert x.grad.shape == x.shape and block.w_down.grad.shape == (70, 130) and "hidden=130" in repr(block)
     assert mccl_b200.__version__
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_autocast_is_a_call_with_tensors_of_its_type(checkpoint, device):
+    *args, dy = _inputs(13, 72, 130, torch.float32, device=device)
+    low = [t.bfloat16().requires_grad_() for t in args]
+    y = gated_feed_forward(*low, checkpoint=checkpoint)
+    want = torch.autograd.grad(y, low, dy.bfloat16())
+    args = [t.requires_grad_() for t in args]
+    with torch.autocast(device, dtype=torch.bfloat16):
+        z = gated_feed_forward(*args, checkpoint=checkpoint)
+    got = torch.autograd.grad(z, args, dy.bfloat16())
+    assert torch.equal(y, z) and all(g.dtype == torch.float32 and torch.equal(g, w.float()) for g, w in zip(got, want))

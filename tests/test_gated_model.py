@@ -39,6 +39,24 @@ def test_learns_one_batch(checkpoint, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_gradients_under_autocast(checkpoint, dtype, device):
+    torch.manual_seed(0)
+    model = gated_tiny(checkpoint=checkpoint).to(device)
+    x, y = _batch(device)
+    model(x, y).backward()
+    want = [p.grad for p in model.parameters()]
+    model.zero_grad()
+    with torch.autocast(device, dtype=dtype):
+        loss = model(x, y)
+    (loss * 256).backward()
+    for (name, p), w in zip(model.named_parameters(), want):
+        # some thirty roundings to 2^-8 (2^-11) one behind the other, of either sign; codes of 8 bits in both or in neither
+        assert p.grad.dtype == torch.float32 and (p.grad / 256 - w).norm() <= (0.25 if dtype == torch.bfloat16 else 0.06) * w.norm(), name
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_decoding_with_a_cache_is_the_whole_sequence_again(device):
     torch.manual_seed(1)
     model = gated_tiny().to(device)
