@@ -38,6 +38,7 @@
 #include "ops/gated.h"
 #include "ops/heads.h"
 #include "ops/linear.h"
+#include "ops/ordinary.h"
 #include "optim/adamw_plan.h"
 #include "optim/bucket_hook.h"
 #include "runtime/arena.h"
@@ -874,13 +875,36 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("_linear_native", &linear_native, py::arg("input"), py::arg("weight"), py::arg("bias") = py::none());
 
   // ---- operators of a decoder block ---------------------------------------------------------------------
-  m.def("_pack8", &pack8, py::call_guard<py::gil_scoped_release>());
-  m.def("_unpack8", [](const at::Tensor& codes, const at::Tensor& scales, const std::vector<int64_t>& shape, at::ScalarType type) {
+  // None under a mode that has to see the operators of torch that a call is made of (make_fx, flop counters, selective recomputation).
+  m.def("_pack8", [](const at::Tensor& x) -> std::optional<std::tuple<at::Tensor, at::Tensor>> {
     py::gil_scoped_release free;
+    if (dispatch_modes()) return std::nullopt;
+    return pack8(x);
+  });
+  m.def("_unpack8", [](const at::Tensor& codes, const at::Tensor& scales, const std::vector<int64_t>& shape,
+                       at::ScalarType type) -> std::optional<at::Tensor> {
+    py::gil_scoped_release free;
+    if (dispatch_modes()) return std::nullopt;
     return unpack8(codes, scales, shape, type);
   });
-  m.def("_gated_feed_forward", &gated_feed_forward, py::call_guard<py::gil_scoped_release>());
+  m.def("_gated_feed_forward", [](const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, const at::Tensor& w_down,
+                                  const std::string& activation, bool eight_bits) -> std::optional<at::Tensor> {
+    py::gil_scoped_release free;
+    if (dispatch_modes()) return std::nullopt;
+    return gated_feed_forward(x, w_gate, w_up, w_down, activation, eight_bits);
+  });
   m.def("_gated_with_limit", &gated_with_limit);
-  m.def("_norm_rotate", &norm_rotate, py::call_guard<py::gil_scoped_release>());
-  m.def("_norm_rotate_packed", &norm_rotate_packed, py::call_guard<py::gil_scoped_release>());
+  m.def("_norm_rotate", [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight, const at::Tensor& k_weight, const at::Tensor& table,
+                           const c10::optional<at::Tensor>& positions, double eps, bool interleaved) -> std::optional<std::tuple<at::Tensor, at::Tensor>> {
+    py::gil_scoped_release free;
+    if (dispatch_modes()) return std::nullopt;
+    return norm_rotate(q, k, q_weight, k_weight, table, positions, eps, interleaved);
+  });
+  m.def("_norm_rotate_packed", [](const at::Tensor& qkv, const at::Tensor& q_weight, const at::Tensor& k_weight, const at::Tensor& table,
+                                  const c10::optional<at::Tensor>& positions, int64_t heads, int64_t kv_heads, double eps,
+                                  bool interleaved) -> std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> {
+    py::gil_scoped_release free;
+    if (dispatch_modes()) return std::nullopt;
+    return norm_rotate_packed(qkv, q_weight, k_weight, table, positions, heads, kv_heads, eps, interleaved);
+  });
 }

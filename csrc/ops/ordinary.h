@@ -15,4 +15,10 @@ inline bool ordinary(const at::Tensor& t) {
 // No mode that wants to see the operators (Python modes, functorch transforms, functionalization).
 inline bool no_modes() { return (c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty(); }
 
+// A Python mode over the operators themselves, of a trace before or behind autograd.
+inline bool dispatch_modes() {
+  const auto included = c10::impl::tls_local_dispatch_key_set().included_;
+  return included.has(c10::DispatchKey::Python) || included.has(c10::DispatchKey::PreDispatch);
+}
+
 }  // namespace mccl

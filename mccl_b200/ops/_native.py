@@ -5,24 +5,12 @@ import torch
 
 from .. import require_native
 
-_included = torch._C._dispatch_tls_is_dispatch_key_included
-_PYTHON, _PRE_DISPATCH = torch._C.DispatchKey.Python, torch._C.DispatchKey.PreDispatch
-
 
 def native():
     """The library; refuses under ``torch.jit.trace``, which would record a call's results as constants."""
     if torch._C._get_tracing_state() is not None:
         raise RuntimeError("this operator cannot be traced: it is no operator of torch's")
     return require_native()
-
-
-def on_kernels(x: torch.Tensor) -> bool:
-    """Whether a call on ``x`` is the kernels'.
-
-    Not under a mode that has to see the operators of torch that a call is made of (``make_fx``, which would record a result of the
-    kernels as an empty tensor, flop counters, selective recomputation): the formulas in torch answer there.
-    """
-    return x.is_cuda and not (_included(_PYTHON) or _included(_PRE_DISPATCH))
 
 
 def autocast_of(x: torch.Tensor):

@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from ._native import autocast_of, cast, native, on_kernels
+from ._native import autocast_of, cast, native
 
 GROUP = 64
 _TINY = 2.0 ** -100
@@ -41,9 +41,10 @@ def _check(x: torch.Tensor) -> None:
 def pack8(x: torch.Tensor) -> Packed8:
     """``x`` in 8 bits.  Not differentiable: what is kept is no function of the graph."""
     _check(x)
-    if on_kernels(x):
-        codes, scales = native()._pack8(x)
-        return Packed8(codes, scales, tuple(x.shape), x.dtype)
+    if x.is_cuda:
+        packed = native()._pack8(x)
+        if packed is not None:
+            return Packed8(*packed, tuple(x.shape), x.dtype)
     x = x.detach()
     cols = x.shape[-1] if x.dim() else 1
     groups, rows = -(-cols // GROUP), math.prod(x.shape[:-1])
@@ -60,8 +61,10 @@ def pack8(x: torch.Tensor) -> Packed8:
 
 def unpack8(packed: Packed8) -> torch.Tensor:
     """The values, in the shape and type that they had."""
-    if on_kernels(packed.codes):
-        return native()._unpack8(packed.codes, packed.scales, list(packed.shape), packed.dtype)
+    if packed.codes.is_cuda:
+        x = native()._unpack8(packed.codes, packed.scales, list(packed.shape), packed.dtype)
+        if x is not None:
+            return x
     rows, pitch = packed.codes.shape
     cols = packed.shape[-1] if packed.shape else 1
     scale = packed.scales.repeat_interleave(GROUP, 1)[:, :cols]

@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._native import autocast_of, cast, native, on_kernels
+from ._native import autocast_of, cast, native
 from .checkpoint import Packed8, pack8, unpack8
 
 ACTIVATIONS = ("silu", "gelu_tanh")
@@ -46,7 +46,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 
 
 def _call(x, *args):
-    return native()._gated_feed_forward(x, *args) if on_kernels(x) else _Plain.apply(x, *args)
+    y = native()._gated_feed_forward(x, *args) if x.is_cuda else None
+    return _Plain.apply(x, *args) if y is None else y
 
 
 def _act(name, g):

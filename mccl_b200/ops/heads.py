@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._native import native, on_kernels
+from ._native import native
 
 
 def rotary_table(positions: int, rotary: int, *, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -36,8 +36,10 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weig
 
     ``positions``: int64 or int32, [tokens] or [batch, tokens]; 0, 1, ... in each batch without it.
     """
-    if on_kernels(q):
-        return native()._norm_rotate(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    if q.is_cuda:
+        out = native()._norm_rotate(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+        if out is not None:
+            return out
     if not eps > 0:
         raise ValueError("eps must be positive")
     return (_plain(q, q_weight, table, positions, eps, interleaved), _plain(k, k_weight, table, positions, eps, interleaved))
@@ -48,8 +50,10 @@ def norm_rotate_packed(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
                        eps: float = 1e-6, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """:func:`norm_rotate` of one projection [batch, tokens, (heads + 2 kv_heads) * dim]; also the view of its values."""
     kv_heads = heads if kv_heads is None else kv_heads
-    if on_kernels(qkv):
-        return native()._norm_rotate_packed(qkv, q_weight, k_weight, table, positions, heads, kv_heads, eps, interleaved)
+    if qkv.is_cuda:
+        out = native()._norm_rotate_packed(qkv, q_weight, k_weight, table, positions, heads, kv_heads, eps, interleaved)
+        if out is not None:
+            return out
     if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[-1] % (heads + 2 * kv_heads):
         raise ValueError(f"norm_rotate_packed: [batch, tokens, (heads + 2 kv_heads) dim] expected, got {tuple(qkv.shape)}")
     q, k, v = qkv.unflatten(-1, (heads + 2 * kv_heads, -1)).split((heads, kv_heads, kv_heads), 2)
