@@ -20,6 +20,6 @@ def autocast_of(x: torch.Tensor):
 
 
 def cast(device: str, *tensors):
-    """The tensors as that autocast casts a product's."""
+    """The tensors as that autocast casts a product's: float64 stays what it is."""
     to = torch.get_autocast_dtype(device)
-    return [None if t is None else t.to(to) for t in tensors]
+    return [t if t is None or t.dtype is torch.float64 else t.to(to) for t in tensors]

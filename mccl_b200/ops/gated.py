@@ -31,7 +31,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     """``x`` [..., width], ``w_gate`` and ``w_up`` [hidden, width], ``w_down`` [width, hidden], all of one type.
 
     ``activation``: ``"silu"`` or ``"gelu_tanh"``.  ``checkpoint``: ``None`` or ``"int8"``.  Under autocast all four are cast
-    to its type first.
+    to its type first, in every call, as ``torch.nn.functional.linear`` casts them (float64, which the kernels refuse, is not).
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {ACTIVATIONS}, got {activation!r}")

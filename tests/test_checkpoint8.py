@@ -182,3 +182,19 @@ def test_linear_under_autocast():
     want = torch.ones(64, 96, device="cuda", dtype=torch.double).T @ seen
     # a bf16 product of 64 terms that are added up in fp32 and rounded once
     assert ((w.grad.double() - want).abs() <= want.abs() * 2.0 ** -8 + seen.abs().sum(0) * 66 * 2.0 ** -23).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_autocast_leaves_float64(device):
+    from mccl_b200.ops.gated import gated_feed_forward
+    x, w = _data((4, 8), torch.float32, device).double(), _data((6, 8), torch.float32, device, seed=1).double()
+    want = x @ w.t()
+    with torch.autocast(device, dtype=torch.bfloat16):
+        with torch.no_grad():
+            assert torch.nn.functional.linear(x, w).dtype == torch.float64
+            assert torch.allclose(checkpoint.linear(x, w), want, rtol=1e-12, atol=1e-12)
+            if device == "cpu":
+                assert gated_feed_forward(x, w, w, w.t()).dtype == torch.float64
+            else:
+                with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+                    gated_feed_forward(x, w, w, w.t())
