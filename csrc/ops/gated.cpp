@@ -297,6 +297,8 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     MCCL_CHECK_T(TensorError, !at::GradMode::is_enabled(), kWhat << ": the backward pass is not differentiable (create_graph)");
     at::Tensor dy = grads[0];
     if (!dy.defined()) return variable_list(6);
+    // products that are torch's are of the tensors' types, also where this is called inside of an autocast region
+    c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &wg = saved[0], &wu = saved[1], &wd = saved[2];
     const auto act = static_cast<kern::GatedActivation>(ctx->saved_data["act"].toInt());

@@ -1,6 +1,8 @@
 """The native library for operators that torch cannot look into."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import require_native
@@ -23,3 +25,18 @@ def cast(device: str, *tensors):
     """The tensors as that autocast casts a product's: float64 stays what it is."""
     to = torch.get_autocast_dtype(device)
     return [t if t is None or t.dtype is torch.float64 else t.to(to) for t in tensors]
+
+
+def without_autocast(backward):
+    """A backward pass whose products are of its tensors' types, also where it is called inside of an autocast region."""
+    @functools.wraps(backward)
+    def run(ctx, grad):
+        device = autocast_of(grad)
+        if device is None:
+            return backward(ctx, grad)
+        torch.set_autocast_enabled(device, False)
+        try:
+            return backward(ctx, grad)
+        finally:
+            torch.set_autocast_enabled(device, True)
+    return run

@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from ._native import autocast_of, cast, native
+from ._native import autocast_of, cast, native, without_autocast
 
 GROUP = 64
 _TINY = 2.0 ** -100
@@ -81,6 +81,7 @@ class _Linear8(torch.autograd.Function):
 
     @staticmethod
     @torch.autograd.function.once_differentiable
+    @without_autocast
     def backward(ctx, grad):
         weight, *kept = ctx.saved_tensors
         dx = grad.matmul(weight) if ctx.needs_input_grad[0] else None

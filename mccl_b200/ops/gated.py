@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._native import autocast_of, cast, native
+from ._native import autocast_of, cast, native, without_autocast
 from .checkpoint import Packed8, pack8, unpack8
 
 ACTIVATIONS = ("silu", "gelu_tanh")
@@ -69,6 +69,7 @@ class _Plain(torch.autograd.Function):
 
     @staticmethod
     @torch.autograd.function.once_differentiable
+    @without_autocast
     def backward(ctx, dy):
         w_gate, w_up, w_down, *kept = ctx.saved_tensors
         if ctx.kept_as is not None:

@@ -198,3 +198,15 @@ def test_autocast_leaves_float64(device):
             else:
                 with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
                     gated_feed_forward(x, w, w, w.t())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_inside_of_an_autocast_region(dtype, device):
+    x, w = _data((37, 130), dtype, device).requires_grad_(), _data((50, 130), dtype, device, seed=1).requires_grad_()
+    y = checkpoint.linear(x, w)
+    dy = _data((37, 50), dtype, device, seed=2)
+    want = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        got = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

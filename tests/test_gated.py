@@ -548,3 +548,18 @@ def test_autocast_is_a_call_with_tensors_of_its_type(checkpoint, device):
         z = gated_feed_forward(*args, checkpoint=checkpoint)
     got = torch.autograd.grad(z, args, dy.bfloat16())
     assert torch.equal(y, z) and all(g.dtype == torch.float32 and torch.equal(g, w.float()) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("tokens,width,hidden", [(5, 8, 24), (256, 512, 704)])
+def test_backward_inside_of_an_autocast_region(tokens, width, hidden, checkpoint, dtype, device):
+    *args, dy = _inputs(tokens, width, hidden, dtype, device=device)
+    args = [t.requires_grad_() for t in args]
+    y = gated_feed_forward(*args, checkpoint=checkpoint)
+    want = torch.autograd.grad(y, args, dy, retain_graph=True)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        got = torch.autograd.grad(y, args, dy)
+        assert torch.is_autocast_enabled(device)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
