@@ -13,11 +13,14 @@ summed in a fixed order.  The backward pass is not differentiable itself.  CPU t
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
 
 from ._native import native
+
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def rotary_table(positions: int, rotary: int, *, theta: float = 10000.0, device=None) -> torch.Tensor:
@@ -40,8 +43,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weig
         out = native()._norm_rotate(q, k, q_weight, k_weight, table, positions, eps, interleaved)
         if out is not None:
             return out
-    if not eps > 0:
-        raise ValueError("eps must be positive")
+    _check(q, k, q_weight, k_weight, table, positions, eps)
     return (_plain(q, q_weight, table, positions, eps, interleaved), _plain(k, k_weight, table, positions, eps, interleaved))
 
 
@@ -61,10 +63,34 @@ def norm_rotate_packed(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
     return q, k, v
 
 
+def _check(q, k, q_weight, k_weight, table, positions, eps):
+    """Refuses what the kernels refuse."""
+    def need(ok, what):
+        if not ok:
+            raise ValueError(f"norm_rotate: {what}")
+
+    need(q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3] and q.shape[2] > 0 and k.shape[2] > 0,
+         f"queries [batch, tokens, heads, dim] and keys [batch, tokens, kv heads, dim] expected, got {tuple(q.shape)} and {tuple(k.shape)}")
+    dim, alike = q.shape[3], lambda t: t.device == q.device
+    need(q.dtype in _TYPES and k.dtype == q.dtype and alike(k), "queries and keys of one of float32, float16 and bfloat16 on one device expected")
+    need(0 < dim <= 512, f"head sizes up to 512, got {dim}")
+    need(all(w.shape == (dim,) and w.is_contiguous() and alike(w) and w.dtype == q_weight.dtype for w in (q_weight, k_weight))
+         and q_weight.dtype in (torch.float32, q.dtype), f"weights are {dim} numbers of float32 or of the queries' type, on their device, both alike")
+    need(table.dim() == 3 and table.shape[1] == 2 and table.dtype == torch.float32 and table.is_contiguous() and alike(table)
+         and not table.requires_grad and 2 * table.shape[2] <= dim,
+         f"a contiguous float32 table [positions, 2, rotary / 2] without gradient expected, rotary at most {dim}")
+    need(0 < eps < math.inf, "eps must be positive")
+    need(positions is None or (positions.dtype in (torch.int64, torch.int32) and alike(positions) and positions.dim() in (1, 2)
+                               and positions.shape[-1] == q.shape[1] and (positions.dim() == 1 or positions.shape[0] in (1, q.shape[0]))),
+         "positions are int64 or int32, [tokens] or [batch, tokens]")
+
+
 def _plain(x, weight, table, positions, eps, interleaved):
     if positions is None:
         positions = torch.arange(x.shape[1], device=x.device)
     inside = (positions >= 0) & (positions < table.shape[0])
+    if table.shape[0] == 0:  # all are outside; a row to look them up in
+        table = table.new_zeros((1, *table.shape[1:]))
     cs = table[positions.clamp(0, table.shape[0] - 1).long()].masked_fill(~inside[..., None, None], float("nan"))
     cos, sin = cs[..., None, 0, :], cs[..., None, 1, :]   # one head for all
     half = table.shape[-1]

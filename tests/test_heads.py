@@ -310,3 +310,31 @@ def test_cpu_form_and_its_gradient(near):
     with pytest.raises(ValueError):
         rotary_table(4, 3)
     assert math.isnan(norm_rotate(rows[:1, :1].float(), rows[:1, :1].float(), *w, table, torch.tensor([99]))[0].detach().sum())
+
+
+def test_the_cpu_form_refuses_what_the_kernels_refuse():
+    q, k, w = torch.zeros(2, 3, 4, 64), torch.zeros(2, 3, 2, 64), torch.ones(64)
+    table, pos = rotary_table(16, 64), torch.zeros(2, 3, dtype=torch.long)
+    norm_rotate(q, k, w, w, table, pos), norm_rotate(q, k, w, w, table, pos[0].int()), norm_rotate(q.half(), k.half(), w.half(), w.half(), table, pos[:1])
+    bad = [
+        (q[0], k, w, w, table, pos), (q, k[:1], w, w, table, pos), (q, k[..., :32], w, w, table, pos), (q, k.half(), w, w, table, pos),
+        (q.double(), k.double(), w, w, table, pos), (q, k, w[:32], w, table, pos), (q, k, w[:1], w[:1], table, pos), (q, k, w, w.half(), table, pos),
+        (q, k, w.half(), w.half(), table, pos), (q, k, w, w, table.half(), pos), (q, k, w, w, table.bfloat16(), pos), (q, k, w, w, table.double(), pos),
+        (q, k, w, w, table[:, :1], pos), (q, k, w, w, table.clone().requires_grad_(), pos), (q, k, w, w, rotary_table(16, 66), pos),
+        (q, k, w, w, table, pos.float()), (q, k, w, w, table, pos[:, :2]), (q, k, w, w, table, pos[:, 0]), (q[:, :, :0], k, w, w, table, pos),
+        (torch.zeros(1, 1, 1, 600),) * 2 + (torch.ones(600),) * 2 + (table, None), (torch.zeros(1, 1, 1, 65),) * 2 + (torch.ones(65),) * 2 + (rotary_table(4, 128), None),
+    ]
+    for args in bad:
+        with pytest.raises(ValueError, match="norm_rotate"):
+            norm_rotate(*args)
+    for eps in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            norm_rotate(q, k, w, w, table, pos, eps=eps)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_an_empty_table_has_no_position(device):
+    x, w = torch.ones(1, 2, 1, 8, device=device), torch.ones(8, device=device)
+    for pos in (None, torch.tensor([0, 5], device=device)):
+        y = norm_rotate(x, x, w, w, rotary_table(0, 4, device=device), pos)[0]
+        assert torch.isnan(y[..., :4]).all() and torch.isfinite(y[..., 4:]).all()
