@@ -47,7 +47,19 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 
 def _call(x, *args):
     y = native()._gated_feed_forward(x, *args) if x.is_cuda else None
-    return _Plain.apply(x, *args) if y is None else y
+    if y is None:
+        _check(x, *args[:3])
+        y = _Plain.apply(x, *args)
+    return y
+
+
+def _check(x, w_gate, w_up, w_down):
+    """Refuses what the kernels refuse, but for types that torch's products take."""
+    if any(t.dtype != x.dtype or t.device != x.device for t in (w_gate, w_up, w_down)):
+        raise ValueError("gated_feed_forward: tensors differ in type or device")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.numel() == 0 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1] or x.shape[-1] != w_gate.shape[1]:
+        raise ValueError("gated_feed_forward: x [..., width], w_gate and w_up [hidden, width] and w_down [width, hidden] expected, got "
+                         + ", ".join(str(tuple(t.shape)) for t in (x, w_gate, w_up, w_down)))
 
 
 def _act(name, g):

@@ -563,3 +563,12 @@ def test_backward_inside_of_an_autocast_region(tokens, width, hidden, checkpoint
         got = torch.autograd.grad(y, args, dy)
         assert torch.is_autocast_enabled(device)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_cpu_form_refuses_what_the_kernels_refuse():
+    x, wg, wu, wd, _ = _inputs(4, 16, 24, torch.float32, device="cpu")
+    gated_feed_forward(x[0], wg, wu, wd), gated_feed_forward(x.double(), wg.double(), wu.double(), wd.double())
+    for args in ((x.half(), wg, wu, wd), (x, wg[:, :8], wu, wd), (x, wg[:8], wu, wd), (x, wg, wu[:1], wd), (x, wg[:1], wu, wd), (x, wg, wu, wd[:5]), (x, wg, wu, wd.t()),
+                 (x, wg[0], wu, wd), (x[:, :0], wg[:, :0], wu[:, :0], wd[:0]), (x, wg[:0], wu[:0], wd[:, :0]), (x.sum(), wg, wu, wd)):
+        with pytest.raises(ValueError, match="gated_feed_forward"):
+            gated_feed_forward(*args)
