@@ -65,8 +65,11 @@ def unpack8(packed: Packed8) -> torch.Tensor:
         x = native()._unpack8(packed.codes, packed.scales, list(packed.shape), packed.dtype)
         if x is not None:
             return x
-    rows, pitch = packed.codes.shape
-    cols = packed.shape[-1] if packed.shape else 1
+    cols, rows = packed.shape[-1] if packed.shape else 1, math.prod(packed.shape[:-1])
+    if (any(n < 0 for n in packed.shape) or packed.dtype not in _TYPES or packed.codes.dtype != torch.int8 or packed.scales.dtype != torch.float32
+            or packed.codes.device != packed.scales.device or packed.codes.shape != (rows, -(-cols // 16) * 16)
+            or packed.scales.shape != (rows, -(-cols // GROUP))):
+        raise ValueError("unpack8: codes and scales are not those of pack8 for this shape")
     scale = packed.scales.repeat_interleave(GROUP, 1)[:, :cols]
     return (packed.codes[:, :cols].float() * scale).to(packed.dtype).view(packed.shape)
 

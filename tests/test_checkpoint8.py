@@ -210,3 +210,12 @@ def test_backward_inside_of_an_autocast_region(dtype, device):
     with torch.autocast(device, dtype=torch.bfloat16):
         got = torch.autograd.grad(y, (x, w), dy)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_cpu_form_refuses_what_the_kernels_refuse():
+    p = pack8(torch.ones(4, 100))
+    for broken in (p._replace(shape=(5, 100)), p._replace(shape=(4, 99 + 30)), p._replace(shape=(8, 50)), p._replace(scales=p.scales[:3]),
+                   p._replace(scales=p.scales[:1]), p._replace(codes=p.codes[:, :96]), p._replace(codes=p.codes[:1]), p._replace(codes=p.codes.to(torch.uint8)),
+                   p._replace(scales=p.scales.double()), p._replace(shape=(4, -100)), p._replace(dtype=torch.float64)):
+        with pytest.raises(ValueError, match="unpack8"):
+            unpack8(broken)
