@@ -59,6 +59,13 @@ class GatedDecoder(nn.Module):
             if p.dim() == 2:  # scaled residual projections, as in GPT-2
                 nn.init.normal_(p, std=0.02 / math.sqrt(2 * layers) if name.endswith(("proj.weight", "w_down")) else 0.02)
 
+    def _apply(self, fn, recurse=True):
+        table = self.table
+        super()._apply(fn, recurse)
+        if self.table.dtype != torch.float32:  # cosines of 8 bits are no angles: `to` another type leaves them alone
+            self.table = table.to(self.table.device)
+        return self
+
     def _trunk(self, idx, positions, caches: Optional[List] = None):
         x, out = self.wte(idx), []
         for i, b in enumerate(self.blocks):

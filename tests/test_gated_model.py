@@ -73,6 +73,30 @@ def test_decoding_with_a_cache_is_the_whole_sequence_again(device):
         model(torch.zeros(1, 129, dtype=torch.long, device=device))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_a_model_of_another_type(checkpoint, dtype, device):
+    torch.manual_seed(4)
+    model = gated_tiny(checkpoint=checkpoint)
+    table, (x, y) = model.table.clone(), _batch(device)
+    with torch.no_grad():
+        want = model.to(device)(x)
+    model = model.to(dtype)
+    assert model.table.dtype == torch.float32 and torch.equal(model.table.cpu(), table) and "table" not in model.state_dict()
+    assert model.table.device == model.wte.weight.device and torch.equal(model.cpu().float().table, table)
+    if dtype == torch.float64:  # no type of the operators
+        return
+    model = model.to(device, dtype)
+    logits = model(x)
+    # some thirty roundings one behind the other, of either sign
+    assert logits.dtype == dtype and (logits.float() - want).norm() <= (0.1 if dtype == torch.bfloat16 else 0.02) * want.norm()
+    model(x, y).backward()
+    assert all(p.grad.dtype == dtype and torch.isfinite(p.grad).all() for p in model.parameters())
+    got = model.generate(x[:, :9], 3)
+    assert got.shape == (2, 12) and torch.equal(got[:, :9], x[:, :9])
+
+
 def test_refusals():
     with pytest.raises(ValueError):
         GatedBlock(128, 3, 1, 256, None)
