@@ -19,31 +19,36 @@ from ..ops.gated import GatedFeedForward
 from ..ops.heads import norm_rotate_packed, rotary_table
 
 
+class _Kept8Linear(nn.Linear):
+    """A linear layer that keeps its input in 8 bits."""
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        return ckpt.linear(input, self.weight, self.bias)
+
+
 class GatedBlock(nn.Module):
     def __init__(self, d: int, heads: int, kv_heads: int, hidden: int, checkpoint: Optional[str]):
         super().__init__()
         if d % heads or heads % kv_heads:
             raise ValueError(f"width {d}, heads {heads} and kv heads {kv_heads} do not divide each other")
         self.heads, self.kv_heads, self.dim, self.checkpoint = heads, kv_heads, d // heads, checkpoint
+        linear = _Kept8Linear if checkpoint else nn.Linear
         self.norm1, self.norm2 = nn.RMSNorm(d, eps=1e-6), nn.RMSNorm(d, eps=1e-6)
-        self.qkv = nn.Linear(d, (heads + 2 * kv_heads) * self.dim, bias=False)
+        self.qkv = linear(d, (heads + 2 * kv_heads) * self.dim, bias=False)
         self.q_norm, self.k_norm = nn.Parameter(torch.ones(self.dim)), nn.Parameter(torch.ones(self.dim))
-        self.proj = nn.Linear(d, d, bias=False)
+        self.proj = linear(d, d, bias=False)
         self.ff = GatedFeedForward(d, hidden, checkpoint=checkpoint)
-
-    def _linear(self, layer: nn.Linear, x: torch.Tensor) -> torch.Tensor:
-        return ckpt.linear(x, layer.weight) if self.checkpoint else layer(x)
 
     def forward(self, x, table, positions, cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
         B, T, D = x.shape
-        q, k, v = norm_rotate_packed(self._linear(self.qkv, self.norm1(x)), self.q_norm, self.k_norm, table, positions, heads=self.heads,
+        q, k, v = norm_rotate_packed(self.qkv(self.norm1(x)), self.q_norm, self.k_norm, table, positions, heads=self.heads,
                                      kv_heads=self.kv_heads)
         q, k, v = (t.transpose(1, 2) for t in (q, k, v))
         if cache is not None:
             k, v = torch.cat((cache[0], k), 2), torch.cat((cache[1], v), 2)
         # one token sees all of the cache; several at once come with none behind them
         a = F.scaled_dot_product_attention(q, k, v, is_causal=T > 1, enable_gqa=self.heads != self.kv_heads)
-        x = x + self._linear(self.proj, a.transpose(1, 2).reshape(B, T, D))
+        x = x + self.proj(a.transpose(1, 2).reshape(B, T, D))
         return x + self.ff(self.norm2(x)), (k, v)
 
 

@@ -97,6 +97,36 @@ def test_a_model_of_another_type(checkpoint, dtype, device):
     assert got.shape == (2, 12) and torch.equal(got[:, :9], x[:, :9])
 
 
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_projections_are_called_as_layers(checkpoint):
+    torch.manual_seed(5)
+    model, seen = gated_tiny(checkpoint=checkpoint), []
+    block = model.blocks[0]
+    for name in ("qkv", "proj"):
+        getattr(block, name).register_forward_hook(lambda *a, name=name: seen.append(name))
+    x, _ = _batch("cpu")
+    model(x)
+    assert seen == ["qkv", "proj"]
+
+    class Twice(torch.nn.Module):
+        def __init__(self, layer):
+            super().__init__()
+            self.layer, self.weight = layer, layer.weight
+
+        def forward(self, t):
+            return 2 * self.layer(t)
+
+    with torch.no_grad():
+        for b in model.blocks:
+            b.proj = Twice(b.proj)
+        replaced = model(x)
+        for b in model.blocks:
+            b.proj = b.proj.layer
+            b.proj.weight.mul_(2)
+        assert torch.equal(model(x), replaced)
+    assert gated_tiny(checkpoint="int8").state_dict().keys() == gated_tiny().state_dict().keys()
+
+
 def test_refusals():
     with pytest.raises(ValueError):
         GatedBlock(128, 3, 1, 256, None)
