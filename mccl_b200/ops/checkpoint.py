@@ -101,6 +101,8 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
     Under autocast the three are cast first, as ``torch.nn.functional.linear`` casts them.
     """
+    if not torch.is_grad_enabled():  # nothing is kept
+        return F.linear(input, weight, bias)
     device = autocast_of(input)
     if device is not None:
         input, weight, bias = cast(device, input, weight, bias)

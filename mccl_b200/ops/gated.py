@@ -49,7 +49,8 @@ def _call(x, *args):
     y = native()._gated_feed_forward(x, *args) if x.is_cuda else None
     if y is None:
         _check(x, *args[:3])
-        y = _Plain.apply(x, *args)
+        *tensors, activation, eight = (x, *args)
+        y = _Plain.apply(*tensors, activation, eight and torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
     return y
 
 

@@ -219,3 +219,32 @@ def test_the_cpu_form_refuses_what_the_kernels_refuse():
                    p._replace(scales=p.scales.double()), p._replace(shape=(4, -100)), p._replace(dtype=torch.float64)):
         with pytest.raises(ValueError, match="unpack8"):
             unpack8(broken)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_nothing_is_packed_where_no_gradient_can_follow(device, monkeypatch):
+    from mccl_b200.models import gated_tiny
+    from mccl_b200.ops import gated
+    packed = []
+
+    def counted(x):
+        packed.append(x.shape)
+        return pack8(x)
+
+    monkeypatch.setattr(checkpoint, "pack8", counted)
+    monkeypatch.setattr(gated, "pack8", counted)
+    model = gated_tiny(checkpoint="int8").to(device)
+    ids = torch.randint(0, 1024, (2, 5), device=device)
+    model.generate(ids, 2)
+    with torch.no_grad(), torch.autocast(device, dtype=torch.bfloat16):
+        model(ids)
+    model.requires_grad_(False)
+    model(ids)
+    x, w = _data((7, 64), torch.float32, device), _data((5, 64), torch.float32, device, seed=1)
+    with torch.inference_mode():
+        want = checkpoint.linear(x, w.requires_grad_())
+    assert not packed
+    assert torch.equal(checkpoint.linear(x, w), want) and packed == [(7, 64)]
+    # of types that the codes don't have, too
+    with torch.no_grad():
+        assert checkpoint.linear(x.double(), w.double()).dtype == torch.float64
