@@ -1,8 +1,9 @@
 // What stands between the fp32 products of a gated feed-forward block (sm_100a): h = act(g) u, and dg = dh u act'(g),
-// du = dh act(g), in one pass each.  act(z) = z s(z), see gated.cu; here with exponential and quotient to the last bits.
+// du = dh act(g), in one pass each.  act(z) = z s(z), see gate.cuh.
 // Bound by memory: 12 and 20 bytes a number.
 #include <algorithm>
 
+#include "kernels/gate.cuh"
 #include "kernels/gated_api.h"
 #include "kernels/launch_count.h"
 
@@ -11,9 +12,6 @@ namespace kern {
 namespace {
 
 constexpr int kThreads = 256, kSms = 148;
-constexpr float kGelu = 1.5957691216057308f, kCubic = 0.044715f;  // 2 sqrt(2 / pi)
-
-__device__ __forceinline__ float gate_of(float z, bool silu) { return 1.f / (1.f + expf(-(silu ? z : kGelu * (z + kCubic * z * z * z)))); }
 
 // Rows of g and of u, `ld` numbers apart, `cols` of each; h and dh have theirs one behind the other.
 struct Rows {

@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "kernels/elems.cuh"
+#include "kernels/gate.cuh"
 #include "kernels/gated_api.h"
 #include "kernels/launch_count.h"
 
@@ -31,7 +32,8 @@ struct Few {
   int64_t ldx, ldw[2], ldo;
   int64_t rows, depth; // of the weights
   int tokens;
-  float c0, c1;        // the curve, see gated.cu
+  float c0, c1;        // the curve, see gated.cu; fp32 asks for gate.cuh's
+  bool silu;
 };
 
 __device__ __forceinline__ float gate(float z, float c0, float c1) {
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) few32_kernel(const Few w, int sha
       v[0] += part[p][r * kM + m];
       if constexpr (kUp) v[1] += part[p][(kSet + r) * kM + m];
     }
-    static_cast<float*>(w.out[0])[(token0 + m) * w.ldo + row] = kUp ? v[0] * gate(v[0], w.c0, w.c1) * v[1] : v[0];
+    static_cast<float*>(w.out[0])[(token0 + m) * w.ldo + row] = kUp ? v[0] * gate_of(v[0], w.silu) * v[1] : v[0];
   }
 }
 // Warps that share a reduction: as many as leave the device full, and each a step.
@@ -349,6 +351,7 @@ cudaError_t both(const GatedFew& g, cudaStream_t s) {
   T* const parts[2] = {static_cast<T*>(g.h), static_cast<T*>(g.h) + h.tokens * pitch};  // (fp32: the first alone)
   Few w{};
   w.c0 = static_cast<float>(h.activation == GatedActivation::kSilu ? -log2e : -log2e * gelu);
+  w.silu = h.activation == GatedActivation::kSilu;
   w.c1 = h.activation == GatedActivation::kSilu ? 0.f : static_cast<float>(-log2e * gelu * 0.044715);
   w.tokens = static_cast<int>(h.tokens);
   w.x[0] = g.x.data;

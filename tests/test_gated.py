@@ -572,3 +572,16 @@ def test_the_cpu_form_refuses_what_the_kernels_refuse():
                  (x, wg[0], wu, wd), (x[:, :0], wg[:, :0], wu[:, :0], wd[:0]), (x, wg[:0], wu[:0], wd[:, :0]), (x.sum(), wg, wu, wd)):
         with pytest.raises(ValueError, match="gated_feed_forward"):
             gated_feed_forward(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 4, 8, 40])
+def test_float32_gates_far_out(tokens):
+    # h = silu(z), of its own kernels for few tokens and between two products.  The exponential is within 2 units in the last place, 4
+    # times 2^-24; its sum with one, the quotient and the product with z round once each; the other products are with ones and zeros.
+    z = torch.linspace(-85, 85, 960, device="cuda")
+    eye, up = torch.eye(2, device="cuda"), torch.tensor([[0.0, 1.0], [0.0, 1.0]], device="cuda")
+    x = torch.stack((z, torch.ones_like(z)), 1)
+    got = torch.cat([gated_feed_forward(x[i:i + tokens], eye, up, eye) for i in range(0, 960, tokens)])[:, 0].double()
+    want = z.double() * torch.sigmoid(z.double())
+    assert ((got - want).abs() <= want.abs() * 8 * 2.0 ** -24).all()
