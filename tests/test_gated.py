@@ -585,3 +585,22 @@ def test_float32_gates_far_out(tokens):
     got = torch.cat([gated_feed_forward(x[i:i + tokens], eye, up, eye) for i in range(0, 960, tokens)])[:, 0].double()
     want = z.double() * torch.sigmoid(z.double())
     assert ((got - want).abs() <= want.abs() * 8 * 2.0 ** -24).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
+def test_gradients_at_a_gate_of_one(activation, dtype):
+    # z = 1: the gradient of x's first number is act'(1), of its second act(1)
+    x = torch.tensor([[1.0, 1.0]], dtype=dtype, device="cuda")
+    gate, up = torch.tensor([[1.0, 0.0]], dtype=dtype, device="cuda"), torch.tensor([[0.0, 1.0]], dtype=dtype, device="cuda")
+    down = torch.ones(2, 1, dtype=dtype, device="cuda")
+    args = [t.requires_grad_() for t in (x, gate, up, down)]
+    got = _pass(args, torch.tensor([[1.0, 0.0]], dtype=dtype, device="cuda"), activation=activation)
+    a, slope = (v.item() for v in _act(activation, torch.ones((), dtype=torch.double)))
+    # two roundings of the type at most (an operand's and the result's), the gate's 2^-16 (fp32 2^-20)
+    near = 2.5 * ROUNDOFF[dtype] + (2.0 ** -16 if dtype != torch.float32 else 2.0 ** -20)
+    for value, want in ((got["y"][0, 0], a), (got["y"][0, 1], a), (got["dx"][0, 0], slope), (got["dx"][0, 1], a), (got["dw_gate"][0, 0], slope),
+                        (got["dw_gate"][0, 1], slope), (got["dw_up"][0, 0], a), (got["dw_down"][0, 0], a)):
+        assert abs(value.item() - want) <= near * want
+    assert got["dw_down"][1, 0].item() == 0
