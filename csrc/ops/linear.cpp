@@ -24,6 +24,12 @@ bool blackwell(int device) {
   return p->major == 10 && p->minor == 0;
 }
 
+// A program that lets torch round its fp32 products has asked for something else (the getter that torch's products use: the older one
+// throws where the newer setting has been used).
+bool torch_rounds() {
+  return at::globalContext().float32Precision(at::Float32Backend::CUDA, at::Float32Op::MATMUL) == at::Float32Precision::TF32;
+}
+
 kern::MatrixF32 matrix(const at::Tensor& t) {
   return {t.const_data_ptr<float>(), t.size(0) == 1 ? std::max(t.stride(0), t.size(1)) : t.stride(0), t.size(0), t.size(1)};
 }
@@ -190,9 +196,7 @@ bool linear_native(const at::Tensor& x, const at::Tensor& w, const c10::optional
   if (bias && bias->defined() &&
       (!ordinary(*bias) || bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != w.size(0) || bias->stride(0) != 1 || bias->device() != x.device()))
     return false;
-  // a program that lets torch round its fp32 products has asked for something else (the getter that torch's products use: the
-  // older one throws where the newer setting has been used)
-  if (at::globalContext().float32Precision(at::Float32Backend::CUDA, at::Float32Op::MATMUL) == at::Float32Precision::TF32 || at::autocast::is_autocast_enabled(at::kCUDA)) return false;
+  if (torch_rounds() || at::autocast::is_autocast_enabled(at::kCUDA)) return false;
   return blackwell(x.get_device()) && kern::gemm_pays(kern::Product::kForward, x.size(0), w.size(1), w.size(0));
 }
 
@@ -208,7 +212,7 @@ std::vector<at::Tensor> linear_with_limit(const at::Tensor& x, const at::Tensor&
 
 std::tuple<at::Tensor, at::Tensor> linear_gradients(const at::Tensor& grad, const at::Tensor& x, const at::Tensor& w, bool need_x, bool need_w) {
   const at::Tensor g = rows_ok(grad) ? grad : grad.contiguous();
-  if (!rows_ok(g) || !rows_ok(x) || !rows_ok(w)) return {need_x ? g.mm(w) : at::Tensor(), need_w ? g.t().mm(x) : at::Tensor()};
+  if (torch_rounds() || !rows_ok(g) || !rows_ok(x) || !rows_ok(w)) return {need_x ? g.mm(w) : at::Tensor(), need_w ? g.t().mm(x) : at::Tensor()};
   const Gradients r = backward_products(g, x, w, need_x, need_w, false);
   return {r.x, r.w};
 }

@@ -604,3 +604,23 @@ def test_gradients_at_a_gate_of_one(activation, dtype):
                         (got["dw_gate"][0, 1], slope), (got["dw_up"][0, 0], a), (got["dw_down"][0, 0], a)):
         assert abs(value.item() - want) <= near * want
     assert got["dw_down"][1, 0].item() == 0
+
+
+@pytest.mark.gpu
+def test_float32_products_are_torchs_where_tf32_is_allowed():
+    native = mccl_b200.require_native()
+    *args, dy = _inputs(256, 1024, 2816, torch.float32)
+    args = [t.requires_grad_() for t in args]
+    was = torch.backends.cuda.matmul.allow_tf32
+    counts = []
+    try:
+        for allowed in (False, True):
+            torch.backends.cuda.matmul.allow_tf32 = allowed
+            y = gated_feed_forward(*args)
+            before = native._kernel_launches()
+            torch.autograd.grad(y, args, dy)
+            counts.append(native._kernel_launches() - before)
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = was
+    # what stands between the products is two launches; each product has others of its own
+    assert counts[0] > 2 and counts[1] == 2
