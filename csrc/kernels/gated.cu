@@ -156,7 +156,8 @@ __device__ __forceinline__ bool elect() {
 
 // ---- what a launch is told ----------------------------------------------------------------------------------
 // act(z) = z s(z), s = 1 / (1 + 2^(z (c0 + c1 z^2))): silu has c0 = -log2(e) and c1 = 0, gelu 2 sqrt(2/pi) times as much and
-// 0.044715 of that.  Exponential and quotient are within 2^-21 of theirs, which 16 bits do not show.
+// 0.044715 of that.  The exponent is rounded too: s is within 2^-21 + |t| 2^-22 of its size, t the logistic function's argument, the second
+// only where s is small; that is 2^-15 at t = -87, where fp32 ends, and 16 bits, rounded by 2^-8 or 2^-11, do not show it.
 struct Curve {
   float c0, c1;
   __device__ __forceinline__ float square(float z) const { return fminf(z * z, 1e30f); }  // no infinity for c1 = 0 to meet

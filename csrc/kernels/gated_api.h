@@ -74,6 +74,8 @@ cudaError_t launch_gated_copies(const GatedCopy* jobs, int n, bool beside, cudaS
 // alignment.  `h`: scratch of tokens x gated_pitch(hidden) x 4 bytes.
 constexpr int64_t kFewTokens = 32;
 // Whether it is faster than the tiles, whose matrix instructions cost the same for any number of tokens and whose launches cost more.
+// By the weights' size alone, which near the limits is as often a little wrong as right: for 2 tokens the kernels here gain 9 us of 4096 x
+// 10240 and lose 5 of 5120 x 8192, just as many numbers.
 // us, here and by tiles: 2 tokens 4096 x 10240 59 and 68, 5120 x 8192 64 and 59, 5120 x 13824 98 and 93; 8 tokens 4096 x 6144 40 and 44,
 // 5120 x 8192 70 and 59; 16 tokens 2048 x 4096 25 and 26, 2048 x 5632 32 and 30; 32 tokens 1024 x 2816 18 and 19, 1536 x 4096 27 and 25.
 inline bool gated_is_few(const GatedShape& s) {

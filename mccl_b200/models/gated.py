@@ -3,7 +3,8 @@
 Per layer: RMS norm, one projection to queries, keys and values, ``ops.heads.norm_rotate_packed``, causal attention with
 shared key heads, projection; RMS norm, ``ops.gated``.  ``checkpoint="int8"`` keeps what the gated blocks and the attention's
 projections need for their backward pass in 8 bits (``ops.checkpoint``).  Trains like the other models (``wrap_ddp``,
-``FusedAdamW``, autocast); :meth:`GatedDecoder.generate` decodes token by token over a cache of keys and values.
+``FusedAdamW``, autocast); :meth:`GatedDecoder.generate` decodes token by token over a cache of keys and values.  In a 16-bit type
+(``model.bfloat16()``) a token takes two thirds of what it takes under autocast, which casts the weights in every call.
 """
 from __future__ import annotations
 

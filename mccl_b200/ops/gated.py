@@ -3,11 +3,12 @@
 Both projections, the activation and the product are one kernel on the tensor cores, the projection back a second one; the
 backward pass takes four.  ``float16`` and ``bfloat16``: sums in fp32; ``h``, the result of activation and product, and the
 gradients of its two factors are rounded to 16 bits once, as operands of the next product (in ``float16`` what is beyond its
-range becomes infinite there).  ``float32``: the products of ``mccl_b200.ops.linear``, with one pass between them.
+range becomes infinite there).  ``float32``: the products of ``mccl_b200.ops.linear`` (torch's where TF32 is allowed), with one pass
+between them; a few tokens without gradients have kernels of their own, in full fp32 whatever is allowed.
 
 What the backward pass needs of the two projections is kept with 16 significant bits (three bytes a number); with
 ``checkpoint="int8"`` it is kept, and the input too, as 8-bit codes with a scale for each group of 64 (see
-``mccl_b200.ops.checkpoint``), and the gradients are those of the kept values.  The backward pass is not differentiable itself.
+``mccl_b200.ops.checkpoint``), and the gradients are those of the kept values (of the input as ``unpack8`` gives it, in its type).  The backward pass is not differentiable itself.
 CPU tensors, and calls under a dispatch mode (``make_fx``, flop counters), take the same formulas in torch; a backward pass takes
 the form that its forward pass took.
 """
