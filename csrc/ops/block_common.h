@@ -3,6 +3,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <atomic>
@@ -37,6 +38,12 @@ inline void check_block_tensor(const at::Tensor& t, const char* what) {
   MCCL_CHECK_T(TensorError, t.defined() && t.is_cuda() && t.layout() == at::kStrided, what << ": a dense CUDA tensor expected");
   MCCL_CHECK_T(TensorError, ordinary(t), what << ": tensor subclasses, transforms and forward-mode tangents are not supported");
   MCCL_CHECK_T(DeviceError, device_fits(t.get_device()), what << ": built for compute capability 10.0");
+}
+// A backward pass of kernels under a trace would leave its results in it as empty tensors.
+inline void check_not_traced(const char* what) {
+  const bool traced = c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+                      c10::impl::tls_local_dispatch_key_set().included_.has(c10::DispatchKey::PreDispatch);
+  MCCL_CHECK_T(TensorError, !traced, what << ": the backward pass of a call outside of the trace cannot be traced");
 }
 // A tensor that was saved for the backward pass, as it comes back: a hook of the caller's may have laid it out anew, but may not have made
 // another one of it, whose memory the kernels would run out of.

@@ -297,6 +297,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     MCCL_CHECK_T(TensorError, !at::GradMode::is_enabled(), kWhat << ": the backward pass is not differentiable (create_graph)");
     at::Tensor dy = grads[0];
     if (!dy.defined()) return variable_list(6);
+    check_not_traced(kWhat);
     // products that are torch's are of the tensors' types, also where this is called inside of an autocast region
     c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
     const auto saved = ctx->get_saved_variables();

@@ -138,6 +138,7 @@ variable_list backward_of(kern::HeadsBackward& a, const at::Tensor& like, const 
 
 void no_second(const char* what) {
   MCCL_CHECK_T(TensorError, !at::GradMode::is_enabled(), what << ": the backward pass is not differentiable (create_graph)");
+  check_not_traced(what);
 }
 
 std::tuple<at::Tensor, at::Tensor> plain_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw, const at::Tensor& table,

@@ -10,7 +10,7 @@ What the backward pass needs of the two projections is kept with 16 significant 
 ``checkpoint="int8"`` it is kept, and the input too, as 8-bit codes with a scale for each group of 64 (see
 ``mccl_b200.ops.checkpoint``), and the gradients are those of the kept values (of the input as ``unpack8`` gives it, in its type).  The backward pass is not differentiable itself.
 CPU tensors, and calls under a dispatch mode (``make_fx``, flop counters), take the same formulas in torch; a backward pass takes
-the form that its forward pass took.
+the form that its forward pass took, and one of the kernels cannot be traced by itself.
 """
 from __future__ import annotations
 

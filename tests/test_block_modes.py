@@ -105,3 +105,19 @@ def test_outside_of_modes_the_kernels_answer():
     with torch.device("cuda"):  # a mode of functions, not of operators
         gated_feed_forward(x, w, w, d), unpack8(pack8(x))
     assert native._kernel_launches() >= before + 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pre_dispatch", [False, True])
+def test_a_trace_of_a_backward_pass_alone_is_refused(pre_dispatch):
+    rand = _gen("cuda")
+    x, w, d, dy = rand(9, 24).requires_grad_(), rand(40, 24), rand(24, 40), rand(9, 24)
+    y = gated_feed_forward(x, w, w, d)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda t: torch.autograd.grad(y, x, t, retain_graph=True)[0], pre_dispatch=pre_dispatch)(dy)
+    q, ones, table = rand(1, 5, 2, 16).requires_grad_(), torch.ones(16, device="cuda"), rotary_table(8, 16, device="cuda")
+    r, _ = norm_rotate(q, q, ones, ones, table)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda t: torch.autograd.grad(r, q, t, retain_graph=True)[0], pre_dispatch=pre_dispatch)(torch.ones_like(r))
+    with FlopCounterMode(display=False):  # what a mode cannot see does no harm elsewhere
+        torch.autograd.grad(y, x, dy)
