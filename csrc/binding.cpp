@@ -353,6 +353,12 @@ at::Tensor topk_select(const at::Tensor& grad, at::Tensor residual, double ratio
   return pairs;
 }
 
+// (scale of exp_avg, scale of exp_avg_sq, lower bits of the parameter), each or none.
+using ExtraTensors = std::tuple<std::optional<at::Tensor>, std::optional<at::Tensor>, std::optional<at::Tensor>>;
+AdamWExtra adamw_extra(const ExtraTensors& x) {
+  return {std::get<0>(x).value_or(at::Tensor()), std::get<1>(x).value_or(at::Tensor()), std::get<2>(x).value_or(at::Tensor())};
+}
+
 // One optimizer step of a parameter group, checks included, if `plan` covers exactly `params` and everything is as
 // the kernel wants it; false, with nothing done, otherwise (the caller then goes through the parameters one by one).
 // `steps`: the parameters' step counters, host tensors that agree; all are advanced.
@@ -369,7 +375,7 @@ bool adamw_step_group(AdamWPlan& plan, const py::list& params, const py::list& s
     const at::Tensor& p = THPVariable_Unpack(py::handle(params[i]).ptr());
     const at::Tensor& c = THPVariable_Unpack(py::handle(steps[i]).ptr());
     auto dense_floats = [&](const at::Tensor& t) {
-      return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == at::kFloat &&
+      return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == own[i].scalar_type() &&
              t.is_contiguous() && t.numel() == own[i].numel();
     };
     if (!dense_floats(p) || p.data_ptr() != own[i].data_ptr() || !dense_floats(p.grad())) return false;
@@ -669,8 +675,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 
   // ---- fused optimizer -------------------------------------------------------------------
   py::class_<AdamWPlan>(m, "AdamWPlan")
-      .def(py::init<std::vector<at::Tensor>, std::vector<at::Tensor>, std::vector<at::Tensor>>(), py::arg("params"),
-           py::arg("exp_avg"), py::arg("exp_avg_sq"))
+      .def(py::init([](std::vector<at::Tensor> params, std::vector<at::Tensor> exp_avg, std::vector<at::Tensor> exp_avg_sq,
+                       const std::vector<ExtraTensors>& extra) {
+             std::vector<AdamWExtra> e;
+             for (const ExtraTensors& x : extra) e.push_back(adamw_extra(x));
+             return std::make_unique<AdamWPlan>(std::move(params), std::move(exp_avg), std::move(exp_avg_sq), std::move(e));
+           }),
+           py::arg("params"), py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("extra") = std::vector<ExtraTensors>{})
       .def("step", &AdamWPlan::step, py::arg("grads"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"),
            py::arg("eps"), py::arg("weight_decay"), py::arg("step"), py::arg("grad_scale") = 1.0)
       .def("step_group", &adamw_step_group, py::arg("params"), py::arg("steps"), py::arg("lr"), py::arg("beta1"),
@@ -682,8 +693,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
              return std::make_shared<BucketOptimizerState>(std::move(pg), scale);
            }),
            py::arg("backend"), py::arg("scale"))
-      .def("add_param", &BucketOptimizerState::add_param, py::arg("param"), py::arg("exp_avg"), py::arg("exp_avg_sq"),
-           py::arg("group"))
+      .def("add_param",
+           [](BucketOptimizerState& st, const at::Tensor& p, const at::Tensor& m, const at::Tensor& v, int group, const std::optional<ExtraTensors>& extra) {
+             st.add_param(p, m, v, group, extra ? std::optional<AdamWExtra>(adamw_extra(*extra)) : std::nullopt);
+           },
+           py::arg("param"), py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("group"), py::arg("extra") = py::none())
       .def("set_hyper", &BucketOptimizerState::set_hyper, py::arg("group"), py::arg("lr"), py::arg("beta1"),
            py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"))
       .def("set_step", &BucketOptimizerState::set_step)

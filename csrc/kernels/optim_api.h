@@ -39,5 +39,33 @@ struct AdamWHyper {
 // kernels (a bucket's update during backward) can be kept to a share of the SMs and of HBM bandwidth.
 cudaError_t launch_adamw_multi(const AdamWTable& tab, const AdamWHyper& h, cudaStream_t s, int max_ctas = 0);
 
+// ---- tensors of several kinds (kernels/adamw_kinds.cu) ---------------------------------------------
+// Moments that share one scale where they are kept in 8 bits.
+constexpr int kMomentGroup = 256;
+static_assert(kAdamWChunk % kMomentGroup == 0, "a CTA has whole groups");
+
+// One tensor, in device memory.
+struct AdamWTensor {
+  void* param;              // fp32 or, `half`, bf16
+  void* exp_avg;            // fp32 or, `eight`, e4m3 padded to whole groups
+  void* exp_avg_sq;         // fp32 or e5m2, alike
+  float* exp_avg_scale;     // of each group
+  float* exp_avg_sq_scale;
+  int16_t* low;             // what a bf16 parameter leaves of its fp32 value's bits
+  int64_t size;
+  int32_t half, eight, aligned, unused;  // aligned: all but the gradient begin at multiples of 16 bytes
+};
+// The hyper-parameters of one step, each rounded from 64 bits once.
+struct AdamWStep {
+  float beta1, one_less_beta1, beta2, one_less_beta2, eps;
+  float decay;           // 1 - lr wd
+  float step_size;       // lr / (1 - beta1^t)
+  float inv_sqrt_bias2;  // 1 / sqrt(1 - beta2^t)
+  float grad_scale;
+  uint32_t step_word;    // t times the golden ratio's digits, for the dither
+};
+cudaError_t launch_adamw_kinds(const AdamWTensor* tensors, const uint64_t* grads, const int2* chunks, int num_chunks, const AdamWStep& h, cudaStream_t s,
+                               int max_ctas = 0);
+
 }  // namespace kern
 }  // namespace mccl

@@ -21,6 +21,7 @@
 #include <map>
 #include <memory>
 #include <mutex>
+#include <optional>
 #include <unordered_map>
 #include <vector>
 
@@ -36,6 +37,7 @@ struct BucketOptimizerState {
   };
   struct ParamEntry {
     at::Tensor p, m, v;
+    std::optional<AdamWExtra> extra;
     int group = 0;  // negative: its update is left to optimizer.step()
   };
   struct BucketPlan {
@@ -47,9 +49,9 @@ struct BucketOptimizerState {
 
   BucketOptimizerState(c10::intrusive_ptr<ProcessGroupMCCL> pg_, double scale_) : pg(std::move(pg_)), scale(scale_) {}
 
-  void add_param(const at::Tensor& p, const at::Tensor& m, const at::Tensor& v, int group) {
+  void add_param(const at::Tensor& p, const at::Tensor& m, const at::Tensor& v, int group, std::optional<AdamWExtra> extra) {
     std::lock_guard<std::mutex> g(mu);
-    params[reinterpret_cast<int64_t>(p.data_ptr())] = ParamEntry{p, m, v, group};
+    params[reinterpret_cast<int64_t>(p.data_ptr())] = ParamEntry{p, m, v, std::move(extra), group};
     buckets.clear();
   }
   void set_hyper(int group, double lr, double b1, double b2, double eps, double wd) {
@@ -103,13 +105,18 @@ class BucketOptimizerHook : public c10d::CommHookInterface {
       }
       for (auto& kv : by_group) {
         std::vector<at::Tensor> ps, ms, vs;
+        std::vector<AdamWExtra> extra;
+        bool kinds = false;
         for (size_t i : kv.second) {
           const auto& e = st.params.at(sig[i]);
           ps.push_back(e.p);
           ms.push_back(e.m);
           vs.push_back(e.v);
+          extra.push_back(e.extra.value_or(AdamWExtra{}));
+          kinds = kinds || e.extra.has_value();
         }
-        bp.plans.push_back(std::make_unique<AdamWPlan>(ps, ms, vs));
+        if (!kinds) extra.clear();
+        bp.plans.push_back(std::make_unique<AdamWPlan>(ps, ms, vs, extra));
         bp.groups.push_back(kv.first);
         bp.positions.push_back(kv.second);
       }

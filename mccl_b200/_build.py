@@ -59,6 +59,7 @@ CUDA_SOURCES = [
     "kernels/topk_cluster.cu",
     "kernels/stft.cu",
     "kernels/adamw.cu",
+    "kernels/adamw_kinds.cu",
     "kernels/gemm_f32.cu",
     "kernels/pack8.cu",
     "kernels/heads.cu",

@@ -7,6 +7,12 @@ parameter, the HBM floor of the update.  State is kept in the standard
 interchangeable with ``torch.optim.AdamW`` (checkpoints load either way).
 ``grad_scale`` lets a caller fold a deferred gradient scaling (for example the
 1/world of a summed allreduce) into the update instead of a separate pass.
+
+``state_bits=8`` keeps the moments in 8 bits (``mccl_b200.optim.moments``): ``exp_avg`` and ``exp_avg_sq`` are then padded float8
+tensors with ``exp_avg_scale`` and ``exp_avg_sq_scale`` beside them, 2.03 bytes a parameter instead of 8, and a step streams 16 bytes
+instead of 28.  ``bfloat16`` parameters are the upper half of an fp32 value that the update is made on; the lower half is their
+state ``low`` (int16), so that no update is too small for them.  Checkpoints of either kind, and ``torch.optim.AdamW``'s, load
+into the other; :meth:`FusedAdamW.moments` gives a parameter's moments as fp32 numbers.
 """
 from __future__ import annotations
 
@@ -15,14 +21,26 @@ from typing import Iterable
 import torch
 
 from .. import require_native
+from .moments import GROUP, pack_moment, padded, unpack_moment
+
+_TYPES = (torch.float32, torch.bfloat16)
+_EXTRAS = ("exp_avg_scale", "exp_avg_sq_scale", "low")
+_REFUSED = "FusedAdamW handles contiguous float32 or bfloat16 CUDA parameters"
+
+
+def _handled(p: torch.Tensor) -> bool:
+    return p.is_cuda and p.dtype in _TYPES and p.is_contiguous()
 
 
 class FusedAdamW(torch.optim.Optimizer):
     def __init__(self, params: Iterable, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 1e-2):
+                 weight_decay: float = 1e-2, *, state_bits: int = 32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits is 8 or 32, got {state_bits!r}")
         if lr < 0 or eps < 0 or weight_decay < 0 or not (0 <= betas[0] < 1) or not (0 <= betas[1] < 1):
             raise ValueError("invalid AdamW hyper-parameters")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits = state_bits
         self._plans = {}
         # DDP hands back bucket parameters as tensors that may be fresh Python objects: find ours by address
         self._by_ptr = {}
@@ -46,9 +64,29 @@ class FusedAdamW(torch.optim.Optimizer):
         st = self.state[p]
         if "exp_avg" not in st:
             st["step"] = torch.tensor(0.0)
-            st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            if self.state_bits == 8:
+                n = padded(p.numel())
+                for name, kind in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
+                    st[name] = torch.zeros(n, dtype=torch.uint8, device=p.device).view(kind)
+                    st[name + "_scale"] = torch.zeros(n // GROUP, device=p.device)
+            else:
+                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format, dtype=torch.float32)
+                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format, dtype=torch.float32)
+        if p.dtype is torch.bfloat16 and "low" not in st:
+            st["low"] = torch.zeros_like(p, dtype=torch.int16)
         return st
+
+    @staticmethod
+    def _extra_of(st):
+        """What the kernel for several kinds is given beside the moments; None where fp32 is all there is."""
+        extra = tuple(st.get(name) for name in _EXTRAS)
+        return None if all(e is None for e in extra) else extra
+
+    def moments(self, p: torch.Tensor):
+        """``(exp_avg, exp_avg_sq)`` of a parameter as float32 numbers of its shape, whatever they are kept as."""
+        st = self._state_of(p)
+        return tuple(unpack_moment(st[name], st[name + "_scale"], p.shape) if name + "_scale" in st else st[name].clone()
+                     for name in ("exp_avg", "exp_avg_sq"))
 
     def _by_step(self, params):
         """``{step number of the coming update: its parameters}``; one entry unless some parameter missed a step."""
@@ -66,12 +104,14 @@ class FusedAdamW(torch.optim.Optimizer):
         plan = self._plans.get(gi)
         if plan is None or plan[0] != key:
             native = require_native()
-            ms, vs = [], []
+            ms, vs, extra = [], [], []
             for p in params:
                 st = self._state_of(p)
                 ms.append(st["exp_avg"])
                 vs.append(st["exp_avg_sq"])
-            plan = (key, native.AdamWPlan([p.data for p in params], ms, vs))
+                extra.append(self._extra_of(st))
+            extra = [e or (None, None, None) for e in extra] if any(extra) else []
+            plan = (key, native.AdamWPlan([p.data for p in params], ms, vs, extra))
             self._plans[gi] = plan
         return plan[1]
 
@@ -106,9 +146,8 @@ class FusedAdamW(torch.optim.Optimizer):
             params = [p for p in group["params"] if p.grad is not None and id(p) not in self._bw_done]
             if not params:
                 continue
-            if not all(p.is_cuda and p.dtype == torch.float32 and p.is_contiguous() for p in params):
-                raise RuntimeError("FusedAdamW handles contiguous float32 CUDA parameters "
-                                   "(see mccl_b200.params.ensure_contiguous_parameters)")
+            if not all(_handled(p) for p in params):
+                raise RuntimeError(_REFUSED + " (see mccl_b200.params.ensure_contiguous_parameters)")
             b1, b2 = group["betas"]
             # the bias corrections are those of a parameter's own counter: one launch for each value among them
             for part, (step, own) in enumerate(self._by_step(params).items()):
@@ -188,10 +227,10 @@ class FusedAdamW(torch.optim.Optimizer):
         here = self._on_shared_step([p for g in self.param_groups for p in g["params"]])
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
-                if not (p.is_cuda and p.dtype == torch.float32 and p.is_contiguous()):
-                    raise RuntimeError("FusedAdamW handles contiguous float32 CUDA parameters")
+                if not _handled(p):
+                    raise RuntimeError(_REFUSED)
                 st = self.state[p]
-                hook_state.add_param(p.data, st["exp_avg"], st["exp_avg_sq"], gi if id(p) in here else -1)
+                hook_state.add_param(p.data, st["exp_avg"], st["exp_avg_sq"], gi if id(p) in here else -1, self._extra_of(st))
         self._native_hook = hook_state
         self.sync_native_hook()
 
@@ -212,8 +251,40 @@ class FusedAdamW(torch.optim.Optimizer):
         self._bw_touched.append(own)
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+        loaded = []
+        last = self.register_load_state_dict_pre_hook(lambda _, d: loaded.append(d))  # what the program's own hooks make of it
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
+        saved, own = ([i for g in groups for i in g["params"]] for groups in (loaded[0]["param_groups"], self.param_groups))
+        for i, p in zip(saved, own):
+            if i in loaded[0]["state"]:
+                self._adopt(p, loaded[0]["state"][i])
         self._plans.clear()  # state tensors were replaced
         self._bw_cache.clear()
         if self._native_hook is not None:
             self.attach_native_hook(self._native_hook)
+
+    def _adopt(self, p, saved) -> None:
+        """A parameter's saved state as this optimizer keeps it; the base class has cast every tensor to the parameter's type."""
+        if "exp_avg" not in saved or "exp_avg_sq" not in saved:
+            return
+        if self.state_bits == 32 and p.dtype is torch.float32 and "exp_avg_scale" not in saved:
+            return  # as it came
+        st = self.state[p]
+        for name, kind in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
+            moment, scale = saved[name].to(p.device), saved.get(name + "_scale")
+            scale = scale if scale is None else scale.to(p.device)
+            if (scale is not None) == (self.state_bits == 8):
+                st[name] = moment if scale is not None else moment.float()
+                if scale is not None:
+                    st[name + "_scale"] = scale
+            elif scale is None:
+                st[name], st[name + "_scale"] = pack_moment(moment, kind)
+            else:
+                st[name] = unpack_moment(moment, scale, p.shape)
+                st.pop(name + "_scale", None)
+        st.pop("low", None)
+        if p.dtype is torch.bfloat16 and "low" in saved:
+            st["low"] = saved["low"].to(p.device)
