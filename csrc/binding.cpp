@@ -687,6 +687,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("step_group", &adamw_step_group, py::arg("params"), py::arg("steps"), py::arg("lr"), py::arg("beta1"),
            py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("grad_scale"))
       .def_property_readonly("num_chunks", &AdamWPlan::num_chunks);
+  m.def("_test_root_quotient", [](const at::Tensor& a, const at::Tensor& b) {
+    for (const at::Tensor* t : {&a, &b})
+      MCCL_CHECK_TENSOR(t->is_cuda() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == a.numel() && t->device() == a.device(),
+                        "_test_root_quotient: float32 CUDA tensors of one size");
+    c10::cuda::CUDAGuard guard(a.device());
+    at::Tensor root = at::empty_like(a), quotient = at::empty_like(a);
+    CK(kern::launch_root_quotient(a.const_data_ptr<float>(), b.const_data_ptr<float>(), root.data_ptr<float>(), quotient.data_ptr<float>(), a.numel(),
+                                  at::cuda::getCurrentCUDAStream()));
+    return std::make_tuple(root, quotient);
+  });
   // ---- native DDP hook: allreduce + AdamW per bucket, registered on the C++ reducer ----
   py::class_<BucketOptimizerState, std::shared_ptr<BucketOptimizerState>>(m, "BucketOptimizerState")
       .def(py::init([](c10::intrusive_ptr<ProcessGroupMCCL> pg, double scale) {

@@ -62,10 +62,13 @@ struct AdamWStep {
   float step_size;       // lr / (1 - beta1^t)
   float inv_sqrt_bias2;  // 1 / sqrt(1 - beta2^t)
   float grad_scale;
+  uint32_t ordinary;     // eps and inv_sqrt_bias2 are far from either end of fp32's range
   uint32_t step_word;    // t times the golden ratio's digits, for the dither
 };
 cudaError_t launch_adamw_kinds(const AdamWTensor* tensors, const uint64_t* grads, const int2* chunks, int num_chunks, const AdamWStep& h, cudaStream_t s,
                                int max_ctas = 0);
+// For tests: the step's root of each b and its quotients a / b.
+cudaError_t launch_root_quotient(const float* a, const float* b, float* root, float* quotient, int64_t n, cudaStream_t s);
 
 }  // namespace kern
 }  // namespace mccl

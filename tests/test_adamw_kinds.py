@@ -193,6 +193,25 @@ def test_steps_are_the_formula_bit_for_bit(cuda_device, dtype, bits):
 
 
 @pytest.mark.gpu
+def test_roots_and_quotients_are_correctly_rounded(cuda_device):
+    import mccl_b200
+    native = mccl_b200.require_native()
+    # every number of two neighbouring binades: a root's digits depend on no more, and a reciprocal's on one of them
+    b = torch.arange(1 << 24, dtype=torch.int32, device=cuda_device).add_(0x3F800000).view(torch.float32)
+    root, quotient = native._test_root_quotient(torch.ones_like(b), b)
+    assert torch.equal(root, torch.sqrt(b.double()).float()) and torch.equal(quotient, torch.ones_like(b) / b)
+    gen = torch.Generator(device=cuda_device).manual_seed(1)
+    for near in (False, True):  # numerators of every kind, and ones beside a multiple of the denominator
+        for scale in (2.0 ** -58, 2.0 ** -31, 1.0, 2.0 ** 25):
+            a = torch.randn(b.shape, generator=gen, device=cuda_device) * scale
+            a = b * (torch.randint(1, 1 << 24, b.shape, generator=gen, device=cuda_device).float() * 2.0 ** -23) * scale if near else a
+            inside = (a.abs() >= 2.0 ** -60) & (a.abs() <= 2.0 ** 60)
+            assert torch.equal(torch.where(inside, native._test_root_quotient(a, b)[1], 0), torch.where(inside, a / b, 0))
+    small = b * 2.0 ** -60
+    assert torch.equal(native._test_root_quotient(b, small)[0], torch.sqrt(small.double()).float())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,bits", KINDS)
 def test_tensors_that_are_not_aligned(cuda_device, dtype, bits):
     torch.manual_seed(12)
