@@ -38,6 +38,7 @@
 #include "ops/gated.h"
 #include "ops/heads.h"
 #include "ops/linear.h"
+#include "ops/norm.h"
 #include "ops/ordinary.h"
 #include "optim/adamw_plan.h"
 #include "optim/bucket_hook.h"
@@ -930,5 +931,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     py::gil_scoped_release free;
     if (dispatch_modes()) return std::nullopt;
     return norm_rotate_packed(qkv, q_weight, k_weight, table, positions, heads, kv_heads, eps, interleaved);
+  });
+  m.def("_layer_norm", [](const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias, double eps,
+                          const std::optional<at::Tensor>& residual, const py::object& dtype) -> std::optional<std::vector<at::Tensor>> {
+    std::optional<at::ScalarType> type;
+    if (!dtype.is_none()) type = dtype.cast<at::ScalarType>();
+    py::gil_scoped_release free;
+    if (dispatch_modes()) return std::nullopt;
+    return layer_norm(x, weight, bias, eps, residual, type);
   });
 }

@@ -46,6 +46,7 @@ CPP_SOURCES = [
     "ops/checkpoint.cpp",
     "ops/heads.cpp",
     "ops/gated.cpp",
+    "ops/norm.cpp",
     "p2p/nccl_p2p.cpp",
 ]
 CUDA_SOURCES = [
@@ -66,6 +67,7 @@ CUDA_SOURCES = [
     "kernels/gated.cu",
     "kernels/gated_few.cu",
     "kernels/gate_f32.cu",
+    "kernels/norm.cu",
     "kernels/noalloc.cu",
 ]
 
