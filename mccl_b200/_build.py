@@ -67,7 +67,8 @@ CUDA_SOURCES = [
     "kernels/gated.cu",
     "kernels/gated_few.cu",
     "kernels/gate_f32.cu",
-    "kernels/norm.cu",
+    "kernels/norm_forward.cu",
+    "kernels/norm_backward.cu",
     "kernels/noalloc.cu",
 ]
 
