@@ -35,6 +35,7 @@
 #include "kernels/stft_api.h"
 #include "kernels/topk_api.h"
 #include "ops/checkpoint.h"
+#include "ops/fused_linear.h"
 #include "ops/gated.h"
 #include "ops/heads.h"
 #include "ops/linear.h"
@@ -940,4 +941,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     if (dispatch_modes()) return std::nullopt;
     return layer_norm(x, weight, bias, eps, residual, type);
   });
+  m.def("_fused_linear", [](const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias, const std::string& activation,
+                            const std::optional<at::Tensor>& residual) -> std::optional<at::Tensor> {
+    py::gil_scoped_release free;
+    if (dispatch_modes()) return std::nullopt;
+    return fused_linear(x, weight, bias, activation, residual);
+  });
+  m.def("_fused_linear_with_limit", &fused_linear_with_limit);
 }

@@ -1,12 +1,13 @@
-// Products of a gated feed-forward block on the fifth-generation tensor cores (sm_100a).
+// Products of a gated feed-forward block, and of a linear layer, on the fifth-generation tensor cores (sm_100a).
 //
-// One kernel for all six: c(i, j) = sum over k of a(i, k) b(j, k) of 16-bit numbers, added up in fp32, with what follows the
+// One kernel for all: c(i, j) = sum over k of a(i, k) b(j, k) of 16-bit numbers, added up in fp32, with what follows the
 // product done on the accumulators: the activation and the product of g and u behind the first, its derivative behind the
 // gradient of h.  act(z) = z s(z) with s the logistic function of z (silu) or of 2 sqrt(2/pi) (z + 0.044715 z^3) (gelu, tanh form).
 //
 // Rounding: h, dg and du are operands of the next product and rounded to 16 bits once.  g and u are kept for the backward pass
 // with 16 significant bits (three bytes; rounded to bf16 they would put two more roundings into every gradient: 2.0 times the
-// error of a result that is rounded once, where it is 1.4 so) or, where asked for, as 8-bit codes.
+// error of a result that is rounded once, where it is 1.4 so) or, where asked for, as 8-bit codes.  A linear layer keeps z = x W^T + b in 16
+// bits: only the activation's slope is taken of it, which moves less than z does (1.45 times the error for 1.41).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -18,6 +19,7 @@
 #include "kernels/elems.cuh"
 #include "kernels/gated_api.h"
 #include "kernels/launch_count.h"
+#include "kernels/layer_act.cuh"
 
 namespace mccl {
 namespace kern {
@@ -173,13 +175,27 @@ struct Curve {
   }
 };
 
-enum Out { kStore, kActivate, kDerive };  // what follows the product
+// What follows the product.  kLayer..: bias, activation and residual of a linear layer, whose result is in 16 or in 32 bits, and z kept or not.
+enum Out { kStore, kActivate, kDerive, kLayer, kLayerKeep, kLayer32, kLayer32Keep };
+template <Out kOut>
+constexpr bool kIsLayer = kOut >= kLayer;
+template <Out kOut>
+constexpr bool kKeepsZ = kOut == kLayerKeep || kOut == kLayer32Keep;
+template <Out kOut>
+constexpr bool kWideY = kOut == kLayer32 || kOut == kLayer32Keep;
 
+struct Layer {
+  LayerActivation activation;
+  const char *bias, *residual;
+  int64_t ldr, cols;
+  bool bias_vec, residual_vec;  // aligned to 16 bytes, whole runs of them
+};
 struct Finish {
   bool bf16;
   Curve curve;
   char* kept;
   int64_t rows, pitch;    // of what is kept, and of h, dg and du
+  Layer layer;
 };
 // One product: tiles, and how they become items of work.
 struct Job {
@@ -325,7 +341,130 @@ struct Staged {
                  "r"(pack2<kBf16>(v[4], v[5])), "r"(pack2<kBf16>(v[6], v[7]))
                  : "memory");
   }
+  // In 32 bits: boxes of 32 columns, from the `which`th on.
+  __device__ __forceinline__ void put_f32(int which, int i, const float* v) const {
+    const uint32_t box = row + (which + i / 32) * kBoxBytes;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + ((((i % 32) + e) / 4) ^ swizzle) * 16), "f"(v[e]), "f"(v[e + 1]), "f"(v[e + 2]),
+                   "f"(v[e + 3])
+                   : "memory");
+  }
 };
+// The joining kernel's of a linear layer: number by number where rows are not aligned.
+template <bool kBf16, bool kKeep>
+struct DirectLayer {
+  uint16_t* z;
+  void* y;
+  int64_t left, left_z;  // numbers of the row from here on
+  bool wide;
+  __device__ __forceinline__ void put(int which, int i, const float* v) const {
+    const bool of_z = kKeep && which == 0;
+    uint16_t* to = (of_z ? z : static_cast<uint16_t*>(y)) + i;
+    const int64_t here = (of_z ? left_z : left) - i;
+    if (of_z || wide) {
+      if (here > 0) *reinterpret_cast<uint4*>(to) = make_uint4(pack2<kBf16>(v[0], v[1]), pack2<kBf16>(v[2], v[3]), pack2<kBf16>(v[4], v[5]), pack2<kBf16>(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < here) to[e] = static_cast<uint16_t>(pack2<kBf16>(v[e], v[e]));
+    }
+  }
+  __device__ __forceinline__ void put_f32(int, int i, const float* v) const {
+    float* to = static_cast<float*>(y) + i;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < left) to[e] = v[e];
+  }
+};
+// What 16 columns of a linear layer's result need from memory: the bias, which is the same for all rows, and a row's residual, as they lie there.
+template <bool kWide>
+struct LayerAhead {
+  uint4 bias[2], residual[kWide ? 4 : 2];
+  // 16 bytes from the number `at` on, of `n` that there are, of 2 or 4 bytes each.
+  template <int kSize>
+  static __device__ __forceinline__ uint4 run(const char* from, int64_t n, bool vec) {
+    constexpr int kPer = 16 / kSize;
+    if (vec) return n > 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i < n) {
+        if constexpr (kSize == 4) w[i] = reinterpret_cast<const uint32_t*>(from)[i];
+        else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[i]) << (16 * (i % 2));
+      }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void load(const Finish& f, int64_t row, int64_t col) {
+    const Layer& l = f.layer;
+    const int64_t n = l.cols - col;
+    if (l.bias != nullptr)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) bias[i] = run<2>(l.bias + 2 * (col + 8 * i), n - 8 * i, l.bias_vec);
+    if (l.residual != nullptr) {
+      constexpr int kSize = kWide ? 4 : 2, kPer = 16 / kSize;
+#pragma unroll
+      for (int i = 0; i < 16 / kPer; ++i) residual[i] = run<kSize>(l.residual + kSize * (row * l.ldr + col + kPer * i), n - kPer * i, l.residual_vec);
+    }
+  }
+};
+template <bool kBf16>
+__device__ __forceinline__ void halves(const uint4& raw, float* v) {  // 8 numbers of 16 bits
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = kBf16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+// 16 columns of x W^T to z and y.
+template <bool kKeep, bool kWide, bool kBf16, typename Sink>
+__device__ __forceinline__ void finish_layer(const Finish& f, const float* v, const LayerAhead<kWide>& now, const Sink& sink, int i0) {
+  const Layer& l = f.layer;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    float z[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = v[8 * b + e];
+    if (l.bias != nullptr) {
+      float bias[8];
+      halves<kBf16>(now.bias[b], bias);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] += bias[e];
+    }
+    if constexpr (kKeep) {
+      if constexpr (kBf16) {
+        sink.put(0, i0 + 8 * b, z);
+      } else {  // beyond fp16's range slopes are what they are at its end
+        float kept[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) kept[e] = z[e] != z[e] ? z[e] : fminf(fmaxf(z[e], -65504.f), 65504.f);
+        sink.put(0, i0 + 8 * b, kept);
+      }
+    }
+    with_activation(l.activation, [&](auto act) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = Act16::value<decltype(act)::kValue>(z[e]);
+    });
+    if (l.residual != nullptr) {
+      float r[8];
+      if constexpr (kWide) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4& w = now.residual[2 * b + h];
+          r[4 * h] = __uint_as_float(w.x), r[4 * h + 1] = __uint_as_float(w.y), r[4 * h + 2] = __uint_as_float(w.z), r[4 * h + 3] = __uint_as_float(w.w);
+        }
+      } else {
+        halves<kBf16>(now.residual[b], r);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] += r[e];
+    }
+    if constexpr (kWide) sink.put_f32(kKeep ? 1 : 0, i0 + 8 * b, z);
+    else sink.put(kKeep ? 1 : 0, i0 + 8 * b, z);
+  }
+}
 // kN columns of g and u to h and to what is kept.
 template <GatedKeep kKeep, int kN, typename Sink>
 __device__ __forceinline__ void finish_activate(const Finish& f, int64_t row, int64_t col, const float* g, const float* u, const Sink& sink, int i0) {
@@ -428,9 +567,9 @@ __device__ __forceinline__ void finish_derive(const Finish& f, const float* dh, 
 template <Out kOut, GatedKeep kKeep>
 constexpr int kTake = kOut == kActivate && kKeep == GatedKeep::kEight ? 64 : 16;
 template <Out kOut>
-constexpr int kBoxes = kOut == kDerive ? 3 : 1;
+constexpr int kBoxes = kOut == kDerive ? 3 : kIsLayer<kOut> ? (kKeepsZ<kOut> ? 1 : 0) + (kWideY<kOut> ? 2 : 1) : 1;
 template <Out kOut>
-constexpr int kStages = kOut == kDerive ? 4 : 6;
+constexpr int kStages = kBoxes<kOut> == 1 ? 6 : kBoxes<kOut> == 2 ? 5 : 4;
 template <Out kOut>
 constexpr int kSmem = kStages<kOut> * kStage + kOutWarps * kBoxes<kOut> * kBoxBytes + 1024;  // of 227 KB
 
@@ -444,7 +583,7 @@ struct Nothing {
   __device__ __forceinline__ void load(const Finish&, int64_t, int64_t) {}
 };
 template <Out kOut, GatedKeep kKeep>
-using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, Nothing>;
+using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, std::conditional_t<kIsLayer<kOut>, LayerAhead<kWideY<kOut>>, Nothing>>;
 
 // A thread's row and columns of a tile: `row` of the result that the tile is of, its columns from `col` on.
 struct Spot {
@@ -457,7 +596,7 @@ __device__ __forceinline__ Spot spot_of(const Job& j, int ti, int tj, int row_in
   return {static_cast<int64_t>(second ? ti - j.rows_segment : ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * (kOut == kActivate ? kHalf : kTile), second};
 }
 // kCols columns from `c` of the tile on, into a sink.
-template <Out kOut, GatedKeep kKeep, int kCols, typename Fetch, typename Sink>
+template <Out kOut, GatedKeep kKeep, bool kBf16, int kCols, typename Fetch, typename Sink>
 __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int c, int last, Ahead<kOut, kKeep>& ahead, const Fetch& fetch, const Sink& sink) {
   constexpr int kN = kTake<kOut, kKeep>;
 #pragma unroll 1
@@ -474,6 +613,11 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
         if (c + i + kN < last) ahead.load(f, min(at.row, f.rows - 1), at.col + c + i + kN);
         fetch(c + i, v);
         finish_derive<kKeep>(f, v, now, sink, i);
+      } else if constexpr (kIsLayer<kOut>) {
+        const LayerAhead<kWideY<kOut>> now = ahead;
+        if (c + i + kN < last) ahead.load(f, min(at.row, f.rows - 1), at.col + c + i + kN);
+        fetch(c + i, v);
+        finish_layer<kKeepsZ<kOut>, kWideY<kOut>, kBf16>(f, v, now, sink, i);
       } else {
         fetch(c + i, v);
 #pragma unroll
@@ -632,9 +776,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
         for (int c = first; c < last; c += kTurn) {
           if (lane == 0) stores_left();
           __syncwarp();
-          if (w.f.bf16) finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged<true>(boxes, lane));
-          else finish_turn<kOut, kKeep, kTurn>(w.f, at, c, last, ahead, fetch, Staged<false>(boxes, lane));
-          if (kOut != kStore || j.wide) {
+          if (w.f.bf16) finish_turn<kOut, kKeep, true, kTurn>(w.f, at, c, last, ahead, fetch, Staged<true>(boxes, lane));
+          else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, fetch, Staged<false>(boxes, lane));
+          if constexpr (kIsLayer<kOut>) {
+            constexpr int kFirst = kKeepsZ<kOut> ? 1 : 0;  // y's boxes behind z's
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (y < j.rows) {
+                const int x = static_cast<int>(at.col) + c;
+                if constexpr (kKeepsZ<kOut>) store_box(&j.out[1], boxes, x, static_cast<int>(y));
+                if (j.wide) {
+                  store_box(&j.out[0], boxes + kFirst * kBoxBytes, x, static_cast<int>(y));
+                  if (kWideY<kOut> && c + 32 < last) store_box(&j.out[0], boxes + (kFirst + 1) * kBoxBytes, x + 32, static_cast<int>(y));
+                }
+              }
+              stores_commit();
+            }
+            if (!j.wide) {  // rows that are not aligned: two numbers a lane, row by row
+              const int n = static_cast<int>(min(static_cast<int64_t>(32), j.rows - y)), here = last - c - 2 * lane;
+              char* to = static_cast<char*>(j.to[0]) + (y * j.ldo + at.col + c + 2 * lane) * (kWideY<kOut> ? 4 : 2);
+#pragma unroll 4
+              for (int r = 0; r < n; ++r, to += j.ldo * (kWideY<kOut> ? 4 : 2)) {
+                uint32_t v[2];
+                if constexpr (kWideY<kOut>) {
+                  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1])
+                               : "r"(boxes + (kFirst + lane / 16) * kBoxBytes + r * 128 + ((lane % 16 / 2) ^ (r & 7)) * 16 + lane % 2 * 8));
+                  if (here > 0) reinterpret_cast<uint32_t*>(to)[0] = v[0];
+                  if (here > 1) reinterpret_cast<uint32_t*>(to)[1] = v[1];
+                } else {
+                  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(boxes + kFirst * kBoxBytes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
+                  if (here > 0) reinterpret_cast<uint16_t*>(to)[0] = static_cast<uint16_t>(v[0]);
+                  if (here > 1) reinterpret_cast<uint16_t*>(to)[1] = static_cast<uint16_t>(v[0] >> 16);
+                }
+              }
+              __syncwarp();
+            }
+          } else if (kOut != kStore || j.wide) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
@@ -778,10 +956,17 @@ __global__ void __launch_bounds__(kJoinThreads) gated_join_kernel(const __grid_c
   if (threadIdx.x >= kHalf || at.row >= j.rows) return;
   Ahead<kOut, kKeep> ahead;
   ahead.load(f, at.row, at.col + c);
-  const int64_t to = at.row * j.ldo + at.col + c;
-  uint16_t* const out[3] = {static_cast<uint16_t*>(j.to[at.which]) + to, static_cast<uint16_t*>(j.to[1]) + to, static_cast<uint16_t*>(j.to[2]) + to};
-  if (f.bf16) finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, Direct<true>{{out[0], out[1], out[2]}, left});
-  else finish_turn<kOut, kKeep, kN>(f, at, c, c + kN, ahead, fetch, Direct<false>{{out[0], out[1], out[2]}, left});
+  if constexpr (kIsLayer<kOut>) {
+    uint16_t* const z = kKeepsZ<kOut> ? static_cast<uint16_t*>(j.to[1]) + at.row * f.pitch + at.col + c : nullptr;
+    void* const y = static_cast<char*>(j.to[0]) + (at.row * j.ldo + at.col + c) * (kWideY<kOut> ? 4 : 2);
+    if (f.bf16) finish_turn<kOut, kKeep, true, kN>(f, at, c, c + kN, ahead, fetch, DirectLayer<true, kKeepsZ<kOut>>{z, y, left, f.pitch - at.col - c, j.wide});
+    else finish_turn<kOut, kKeep, false, kN>(f, at, c, c + kN, ahead, fetch, DirectLayer<false, kKeepsZ<kOut>>{z, y, left, f.pitch - at.col - c, j.wide});
+  } else {
+    const int64_t to = at.row * j.ldo + at.col + c;
+    uint16_t* const out[3] = {static_cast<uint16_t*>(j.to[at.which]) + to, static_cast<uint16_t*>(j.to[1]) + to, static_cast<uint16_t*>(j.to[2]) + to};
+    if (f.bf16) finish_turn<kOut, kKeep, true, kN>(f, at, c, c + kN, ahead, fetch, Direct<true>{{out[0], out[1], out[2]}, left});
+    else finish_turn<kOut, kKeep, false, kN>(f, at, c, c + kN, ahead, fetch, Direct<false>{{out[0], out[1], out[2]}, left});
+  }
 }
 
 // ---- rows that are not aligned --------------------------------------------------------------------------------
@@ -831,6 +1016,8 @@ Sizes sizes_of(GatedProduct p, const GatedShape& s) {
     case GatedProduct::kGate: return {s.tokens, s.hidden, s.width, 1, 1, false};
     case GatedProduct::kInput: return {s.tokens, s.width, s.hidden, 1, 2, false};
     case GatedProduct::kWeightUp: return {s.hidden, s.width, s.tokens, 2, 1, false};
+    case GatedProduct::kLayer: return {s.tokens, s.width, s.hidden, 1, 1, false};
+    case GatedProduct::kBack: return {s.tokens, s.hidden, s.width, 1, 1, false};
     default: return {s.width, s.hidden, s.tokens, 1, 1, false};
   }
 }
@@ -940,11 +1127,12 @@ uint32_t rows_read(int64_t rows) {
   while (n < rows && n < kHalf) n *= 2;
   return n;
 }
-bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t outer, uint32_t box_rows, bool bf16) {
-  if (m.data == nullptr || reinterpret_cast<uintptr_t>(m.data) % 16 != 0 || m.ld % 8 != 0 || m.ld < inner || inner > 0x7FFFFFFF || outer > 0x7FFFFFFF) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)}, strides[1] = {static_cast<cuuint64_t>(m.ld) * 2};
-  const cuuint32_t box[2] = {64, box_rows}, one[2] = {1, 1};
-  return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(m.data), dims, strides, box, one,
+bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t outer, uint32_t box_rows, bool bf16, bool f32 = false) {
+  const int64_t size = f32 ? 4 : 2;
+  if (m.data == nullptr || reinterpret_cast<uintptr_t>(m.data) % 16 != 0 || m.ld * size % 16 != 0 || m.ld < inner || inner > 0x7FFFFFFF || outer > 0x7FFFFFFF) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)}, strides[1] = {static_cast<cuuint64_t>(m.ld * size)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), box_rows}, one[2] = {1, 1};
+  return encode_tiled()(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(m.data), dims, strides, box, one,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -993,10 +1181,10 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
 }
 
 // A product's maps and shape.
-bool make_job(Job& j, const GatedArgs& g, const GatedShape& h) {
+bool make_job(Job& j, const GatedArgs& g, const GatedShape& h, const LayerFinish* layer) {
   const Sizes z = sizes_of(g.product, h);
   j.a_inner = g.product != GatedProduct::kWeightUp && g.product != GatedProduct::kWeightDown;
-  j.b_inner = g.product == GatedProduct::kUp || g.product == GatedProduct::kDown;
+  j.b_inner = g.product == GatedProduct::kUp || g.product == GatedProduct::kDown || g.product == GatedProduct::kLayer;
   const GatedOperand a[2] = {g.a0, z.results * z.parts > 1 ? g.a1 : g.a0}, b[2] = {g.b0, z.gate || z.parts > 1 ? g.b1 : g.b0};
   const uint32_t a_rows = j.a_inner ? rows_read(z.rows) : kOwnRows;
   j.bytes = 2 * ((j.a_inner ? a_rows * kDepth * 2 : kOperand) + kOperand);
@@ -1016,6 +1204,12 @@ bool make_job(Job& j, const GatedArgs& g, const GatedShape& h) {
   j.rows = z.rows;
   j.cols = between ? gated_pitch(h.hidden) : z.cols;
   j.ldo = between ? j.cols : g.ldo;
+  if (g.product == GatedProduct::kLayer) {
+    const int64_t size = layer->y_f32 ? 4 : 2;
+    j.wide = j.ldo * size % 16 == 0 && reinterpret_cast<uintptr_t>(g.out0) % 16 == 0;
+    return g.out0 != nullptr && (!j.wide || make_map(&j.out[0], {g.out0, j.ldo}, j.cols, z.rows, kResultRows, h.bf16, layer->y_f32)) &&
+           (g.out1 == nullptr || make_map(&j.out[1], {g.out1, gated_row(h.width)}, gated_row(h.width), z.rows, kResultRows, h.bf16));
+  }
   j.wide = j.ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out0) | reinterpret_cast<uintptr_t>(g.out1) | reinterpret_cast<uintptr_t>(g.out2)) % 16 == 0;
   const int results = g.product == GatedProduct::kGate ? 3 : g.product == GatedProduct::kWeightUp ? 2 : 1;
   for (int i = 0; i < 3; ++i) {
@@ -1083,7 +1277,8 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
   int order[kMostJobs];
   for (int i = 0; i < n; ++i) {
     p[i] = g[i].product;
-    if (n > 1 && (p[i] == GatedProduct::kUp || p[i] == GatedProduct::kGate)) return cudaErrorInvalidValue;
+    if (n > 1 && (p[i] == GatedProduct::kUp || p[i] == GatedProduct::kGate || p[i] == GatedProduct::kLayer)) return cudaErrorInvalidValue;
+    if ((p[i] == GatedProduct::kLayer) != (r.layer != nullptr)) return cudaErrorInvalidValue;
   }
   if (n == 1) {
     plan_one(p[0], h, l[0]);
@@ -1098,7 +1293,7 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
   for (int i = 0; i < n; ++i) {
     const Plan& q = l[order[i]];
     Job& j = w.job[i];
-    if (!make_job(j, g[order[i]], h) || q.stages > 0x3FFFFFFF) return cudaErrorInvalidValue;
+    if (!make_job(j, g[order[i]], h, r.layer) || q.stages > 0x3FFFFFFF) return cudaErrorInvalidValue;
     j.tiles_i = static_cast<int>(q.tiles_i);
     j.tiles_j = static_cast<int>(q.tiles_j);
     j.rows_segment = static_cast<int>(q.tiles_i / (p[order[i]] == GatedProduct::kWeightUp ? 2 : 1));
@@ -1125,6 +1320,19 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
   w.f.kept = static_cast<char*>(r.kept);
   w.f.rows = h.tokens;
   w.f.pitch = gated_pitch(h.hidden);
+  if (r.layer != nullptr) {
+    const LayerFinish& f = *r.layer;
+    const int64_t size = f.y_f32 ? 4 : 2;
+    w.f.pitch = gated_row(h.width);
+    Layer& l = w.f.layer;
+    l.activation = f.activation;
+    l.bias = static_cast<const char*>(f.bias);
+    l.residual = static_cast<const char*>(f.residual);
+    l.ldr = f.ldr;
+    l.cols = h.width;
+    l.bias_vec = h.width % 8 == 0 && reinterpret_cast<uintptr_t>(f.bias) % 16 == 0;
+    l.residual_vec = h.width * size % 16 == 0 && f.ldr * size % 16 == 0 && reinterpret_cast<uintptr_t>(f.residual) % 16 == 0;
+  }
   w.partial = r.partial;
   w.failed = r.failed;
   w.limit = r.wait_limit >= 0 ? r.wait_limit : kWaitLimit;
@@ -1137,6 +1345,9 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
       }
     case GatedProduct::kGate:
       return h.keep == GatedKeep::kEight ? run<kDerive, GatedKeep::kEight>(w, joins, high, s) : run<kDerive, GatedKeep::kWide>(w, joins, high, s);
+    case GatedProduct::kLayer:
+      if (r.layer->y_f32) return g[0].out1 != nullptr ? run<kLayer32Keep, GatedKeep::kNone>(w, joins, high, s) : run<kLayer32, GatedKeep::kNone>(w, joins, high, s);
+      return g[0].out1 != nullptr ? run<kLayerKeep, GatedKeep::kNone>(w, joins, high, s) : run<kLayer, GatedKeep::kNone>(w, joins, high, s);
     default: return run<kStore, GatedKeep::kNone>(w, joins, high, s);
   }
 }

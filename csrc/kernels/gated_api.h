@@ -1,13 +1,19 @@
-// Launchers of the gated feed-forward block's products (plain C++ header).
+// Launchers of the gated feed-forward block's products (plain C++ header), and of a linear layer's, which are of the same kind.
 //
 //     g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
 //
 // of `tokens` rows, `width` numbers in and out, `hidden` between.  Six products; what stands between them is inside of them.
+//
+//     y = act(x W^T + b) + r
+//
+// of `tokens` rows, `hidden` numbers in and `width` out: its product is kDown's with what follows it, and its gradients are kBack and kWeightDown.
 #pragma once
 
 #include <cuda_runtime_api.h>
 
 #include <cstdint>
+
+#include "kernels/pack8_api.h"
 
 namespace mccl {
 namespace kern {
@@ -19,6 +25,8 @@ enum class GatedProduct {
   kInput,       // a0 = dg, a1 = du, b0 = Wg, b1 = Wu: dx to out0
   kWeightUp,    // a0 = dg, a1 = du, b0 = x: dWg to out0, dWu to out1
   kWeightDown,  // a0 = dy, b0 = h: dWd to out0
+  kLayer,       // a0 = x, b0 = W: y to out0, x W^T + b to out1 (rows of gated_row(width)) where it is kept
+  kBack,        // a0 = dz, b0 = W: dx to out0
 };
 enum class GatedActivation { kSilu, kGeluTanh };
 // How g and u wait for the backward pass: not at all, as floats of three bytes, as codes of 8 bits.
@@ -45,14 +53,24 @@ struct GatedArgs {
   void *out0, *out1, *out2;
   int64_t ldo;          // of the outputs; of h, dg and du gated_pitch
 };
+// What follows the product of a linear layer.
+enum class LayerActivation { kNone, kRelu, kSilu, kGelu, kGeluTanh };
+struct LayerFinish {
+  LayerActivation activation;
+  const void* bias;      // `width` numbers of the operands' type, or null
+  const void* residual;  // rows of y's type, `ldr` numbers apart, or null
+  int64_t ldr;
+  bool y_f32;            // else of the operands' type
+};
 struct GatedLaunch {
   GatedShape shape;
+  const LayerFinish* layer;  // of kLayer, or null
   void* kept;
   float* partial;       // gated_partial_bytes
   uint32_t* failed;     // set to 1 where a wait runs out, whose tiles then are NaN; or null
   int64_t wait_limit;   // cycles of a quarter of a wait; negative: about a second in all
 };
-// One product, or up to three of kDown, kInput, kWeightUp and kWeightDown: side by side where that is faster.
+// One product, or up to three of kDown, kInput, kWeightUp, kWeightDown and kBack: side by side where that is faster.
 int64_t gated_partial_bytes(const GatedProduct* p, int n, const GatedShape& s);
 cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaStream_t s);
 
@@ -98,6 +116,46 @@ cudaError_t launch_gated_few(const GatedFew& g, cudaStream_t s);
 // g with u behind them and dh to rows of dg with du behind them.
 cudaError_t launch_gate_f32(const float* g, const float* u, int64_t ld, float* h, int64_t rows, int64_t cols, GatedActivation act, cudaStream_t s);
 cudaError_t launch_gate_f32_backward(const float* gu, const float* dh, float* dgu, int64_t rows, int64_t cols, GatedActivation act, cudaStream_t s);
+
+// ---- linear layer -------------------------------------------------------------------------------------------
+// A layer of few rows, one launch that reads the weights at the rate of memory (kernels/linear_few.cu).  Rows of any alignment.
+// us, here and by tiles: TIMES
+inline bool layer_is_few(int64_t tokens, int64_t in, int64_t out) {
+  const int64_t n = in * out;
+  return n <= (tokens <= 2 ? 48 << 20 : tokens <= 8 ? 32 << 20 : tokens <= 16 ? 8 << 20 : tokens <= kFewTokens ? 4 << 20 : 0);
+}
+struct LayerFew {
+  int64_t tokens, in, out;
+  bool bf16;  // else fp16
+  GatedOperand x, weight;
+  LayerFinish finish;
+  void* y;  // rows of `out`
+};
+cudaError_t launch_layer_few(const LayerFew& g, cudaStream_t s);
+
+// What stands around the products, in one pass each (kernels/linear_pass.cu).  Rows `ld` numbers apart of one type.
+struct LayerRows {
+  const void* data;
+  int64_t ld;
+  Elem type;
+};
+// y = act(z) + residual, of fp32 rows one behind the other (`residual.data` null without one).
+cudaError_t launch_layer_finish(const float* z, const LayerRows& residual, float* y, int64_t rows, int64_t cols, LayerActivation act, cudaStream_t s);
+// dz = dy act'(z) to rows of `dz_ld` numbers (null: only the sums), and the sums of dy act'(z) over the rows, before it is rounded, to `bias`
+// (null: none), in a fixed order.  `z.data` null: dz = dy.
+struct LayerDerive {
+  int64_t rows, cols;
+  LayerRows dy, z;
+  LayerActivation activation;
+  void* dz;
+  int64_t dz_ld;
+  Elem dz_type;
+  void* bias;
+  Elem bias_type;
+  float* partial;  // layer_partial_bytes
+};
+int64_t layer_partial_bytes(int64_t rows, int64_t cols);
+cudaError_t launch_layer_derive(const LayerDerive& g, cudaStream_t s);
 
 }  // namespace kern
 }  // namespace mccl

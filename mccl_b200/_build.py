@@ -46,6 +46,7 @@ CPP_SOURCES = [
     "ops/checkpoint.cpp",
     "ops/heads.cpp",
     "ops/gated.cpp",
+    "ops/fused_linear.cpp",
     "ops/norm.cpp",
     "p2p/nccl_p2p.cpp",
 ]
@@ -67,6 +68,8 @@ CUDA_SOURCES = [
     "kernels/gated.cu",
     "kernels/gated_few.cu",
     "kernels/gate_f32.cu",
+    "kernels/linear_few.cu",
+    "kernels/linear_pass.cu",
     "kernels/norm_forward.cu",
     "kernels/norm_backward.cu",
     "kernels/noalloc.cu",

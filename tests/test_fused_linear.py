@@ -1,0 +1,429 @@
+"""The linear layer with bias, activation and residual against its formulas in 64 bits."""
+import math
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
+
+from mccl_b200.ops.fused_linear import FusedLinear, fused_linear
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+ROUNDOFF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+SMALLEST = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+U = 2.0 ** -24
+ACTIVATIONS = [None, "relu", "silu", "gelu", "gelu_tanh"]
+
+
+def _act(name, z):
+    if name is None:
+        return z, torch.ones_like(z)
+    if name == "relu":
+        return torch.relu(z), (z > 0).to(z.dtype)
+    if name == "gelu":
+        return z * torch.special.ndtr(z), torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    c = 2 * math.sqrt(2 / math.pi)
+    s = torch.sigmoid(z if name == "silu" else c * (z + 0.044715 * z ** 3))
+    return z * s, s + z * s * (1 - s) * (1 if name == "silu" else c * (1 + 3 * 0.044715 * z * z))
+
+
+def _sum(dtype, depth):
+    """Products of 16-bit numbers are exact in fp32; the tensor cores cut each sum of (at least) 8 of them off at 2^-23 of what it adds
+    up.  fp32 products are six bf16 products (2^-20) or sums of a library kernel (2^-24 a term)."""
+    return (depth / 8 + 4) * 2.0 ** -23 if dtype != torch.float32 else 2.0 ** -20 + (depth + 2) * U
+
+
+def _inputs(tokens, width, out, dtype, residual, bias, device, seed=0, scale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    randn = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    t = {"x": (randn(tokens, width) * scale).to(dtype), "weight": (randn(out, width) * width ** -0.5).to(dtype)}
+    if bias:
+        t["bias"] = (randn(out) * 0.5).to(dtype)
+    if residual is not None:
+        t["residual"] = (2 * randn(tokens, out)).to(residual)
+    t["dy"] = randn(tokens, out).to(residual or dtype)
+    return {k: v.to(device) for k, v in t.items()}
+
+
+def _leaves(t):
+    return [t[k] for k in ("x", "weight", "bias", "residual") if k in t]
+
+
+def _call(t, activation, grad=True):
+    if not grad:
+        return [fused_linear(t["x"].detach(), t["weight"].detach(), None if "bias" not in t else t["bias"].detach(), activation=activation,
+                             residual=None if "residual" not in t else t["residual"].detach())]
+    for leaf in _leaves(t):
+        leaf.requires_grad_()
+    y = fused_linear(t["x"], t["weight"], t.get("bias"), activation=activation, residual=t.get("residual"))
+    return [y.detach(), *torch.autograd.grad(y, _leaves(t), t["dy"])]
+
+
+def _check(t, activation, got):
+    dtype = t["x"].dtype
+    t = {k: v.detach().cpu() for k, v in t.items()}
+    u, least, act_off = ROUNDOFF[dtype], SMALLEST[dtype], 2.0 ** -16 if dtype != torch.float32 else 2.0 ** -20
+    x, w, dy = (t[k].double() for k in ("x", "weight", "dy"))
+    bias = t["bias"].double() if "bias" in t else torch.zeros(w.shape[0], dtype=torch.float64)
+    z = x @ w.T + bias
+    ez = x.abs() @ w.abs().T * _sum(dtype, x.shape[1]) + U * (z.abs() + bias.abs())
+    a, slope = _act(activation, z)
+
+    def result(v, e, to):  # rounded once
+        return e + (v.abs() + e) * ROUNDOFF[to] + SMALLEST[to]
+
+    def near(g, want, bound, what):
+        assert g.shape == want.shape, what
+        g = g.double().cpu()
+        worst = float(((g - want).abs() - bound).max()) if want.numel() else 0.0
+        assert worst <= 0 and torch.isfinite(g).all(), (what, worst)
+
+    # slopes are below 1.13, second derivatives below 1
+    ea = 1.13 * ez + a.abs() * act_off
+    y = a
+    if "residual" in t:
+        y = a + t["residual"].double()
+        ea = ea + U * y.abs()
+    y_type = t["residual"].dtype if "residual" in t else dtype
+    assert got[0].dtype is y_type
+    near(got[0], y, result(y, ea, y_type), "y")
+    if len(got) == 1:
+        return
+    # z as it is kept, and its slope; where relu's corner is within reach it may be either
+    kept = (z.abs() + ez) * u + least if activation is not None and dtype != torch.float32 else 0.0
+    es = 0.0 if activation is None else (z.abs() <= ez).double() if activation == "relu" else ez + kept + (1 + slope.abs()) * act_off
+    dz = dy * slope
+    edz = dy.abs() * es + dz.abs() * 2 * U
+    got = got[1:]
+    db, edb = dz.sum(0), (edz + (dz.abs() + edz) * U * (64 + dz.shape[0] / 32)).sum(0)
+    if dtype != torch.float32:
+        edz = edz + (dz.abs() + edz) * u + least  # an operand
+
+    def product(m, em, r):
+        return m @ r, em @ r.abs() + (m.abs() + em) @ r.abs() * _sum(dtype, m.shape[1])
+
+    for name, v, e in (("dx", *product(dz, edz, w)), ("dw", *product(dz.T, edz.T, x))):
+        near(got[0], v, result(v, e, dtype), name)
+        got = got[1:]
+    if "bias" in t:
+        near(got[0], db, result(db, edb, dtype), "db")
+        got = got[1:]
+    if "residual" in t:
+        assert torch.equal(got[0].cpu(), t["dy"])
+
+
+SIZES = [(1, 8, 8), (1, 64, 72), (3, 24, 40), (5, 1, 1), (7, 33, 1), (2, 1, 50), (33, 100, 60), (130, 264, 520), (257, 72, 1000), (300, 200, 731),
+         (513, 64, 300), (100, 1024, 256), (70, 1000, 333), (300, 2048, 520)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tokens,width,out", SIZES)
+@pytest.mark.parametrize("dtype,activation,residual", [(torch.bfloat16, "gelu_tanh", None), (torch.float16, "gelu", torch.float16),
+                                                       (torch.bfloat16, None, torch.float32), (torch.float32, "silu", torch.float32)])
+def test_matches_64_bits(device, tokens, width, out, dtype, activation, residual):
+    t = _inputs(tokens, width, out, dtype, residual, True, device)
+    _check(t, activation, _call(t, activation))
+    _check(t, activation, _call(t, activation, grad=False))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("residual", [None, "same", torch.float32])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("tokens,width,out", [(40, 72, 136), (9, 31, 45)])
+def test_types_and_activations(device, dtype, activation, residual, bias, tokens, width, out):
+    t = _inputs(tokens, width, out, dtype, dtype if residual == "same" else residual, bias, device, seed=1, scale=2.0)
+    _check(t, activation, _call(t, activation))
+    _check(t, activation, _call(t, activation, grad=False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 16, 17, 32, 33])
+@pytest.mark.parametrize("width,out", [(512, 256), (1000, 2731), (264, 9480), (8, 9472), (33, 9500), (4096, 64)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_few_tokens(tokens, width, out, dtype):
+    t = _inputs(tokens, width, out, dtype, dtype, True, "cuda", seed=tokens)
+    _check(t, "gelu_tanh", _call(t, "gelu_tanh", grad=False))
+    t = _inputs(tokens, width, out, dtype, torch.float32, False, "cuda", seed=tokens)
+    _check(t, None, _call(t, None, grad=False))
+
+
+@pytest.mark.gpu
+def test_few_tokens_between_other_numbers():
+    base = torch.full((40, 300), math.nan, device="cuda", dtype=torch.bfloat16)
+    weights = torch.full((90, 301), math.nan, device="cuda", dtype=torch.bfloat16)
+    out = torch.full((20, 90), math.nan, device="cuda", dtype=torch.bfloat16)
+    for shift in range(0, 9):
+        t = _inputs(5, 200, 77, torch.bfloat16, torch.bfloat16, True, "cuda", seed=shift)
+        x, w, r = base[3:8, shift:shift + 200], weights[5:82, shift:shift + 200], out[2:7, shift:shift + 77]
+        x.copy_(t["x"]), w.copy_(t["weight"]), r.copy_(t["residual"])
+        t.update(x=x, weight=w, residual=r)
+        _check(t, "silu", _call(t, "silu", grad=False))
+        base.fill_(math.nan), weights.fill_(math.nan), out.fill_(math.nan)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,width,out,dtype,residual", [(2048, 1024, 1024, torch.bfloat16, torch.float32), (1500, 520, 4096, torch.float16, None),
+                                                             (5000, 264, 2056, torch.bfloat16, torch.bfloat16), (1000, 1024, 1024, torch.float32, torch.float32)])
+def test_many_tiles(tokens, width, out, dtype, residual):
+    t = _inputs(tokens, width, out, dtype, residual, True, "cuda", seed=3)
+    _check(t, "gelu", _call(t, "gelu"))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_of_the_gradients_alone(device, dtype):
+    t = _inputs(40, 64, 72, dtype, torch.float32, True, device)
+    full = _call(t, "gelu")[1:]
+    for i, name in enumerate(("x", "weight", "bias", "residual")):
+        for k in ("x", "weight", "bias", "residual"):
+            t[k] = t[k].detach().requires_grad_(k == name)
+        y = fused_linear(t["x"], t["weight"], t["bias"], activation="gelu", residual=t["residual"])
+        (g,) = torch.autograd.grad(y, [t[name]], [t["dy"]])
+        # (products side by side or alone add up alike here: no reduction is shared)
+        assert torch.equal(g, full[i]), name
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_layouts(device, dtype):
+    gen = torch.Generator().manual_seed(4)
+    base = torch.randn(4, 6, 211, generator=gen).to(device, dtype)
+    weight = torch.randn(90, 211, generator=gen).to(device, dtype)
+
+    def both(x, w, r, dy, b):
+        x, w, r, b = (v.detach().requires_grad_() for v in (x, w, r, b))
+        y = fused_linear(x, w, b, activation="gelu", residual=r)
+        return [y.detach(), *torch.autograd.grad(y, (x, w, r, b), dy)]
+
+    for x in (base[..., :100], base[..., 1:101], base[..., 0:200:2], base.transpose(0, 1)[..., :100].transpose(0, 1), base[:1, :1, 4:104].expand(4, 6, 100)):
+        for w in (weight[:, :100], weight[:, 3:103], weight[:, 0:200:2], weight.t()[:100].t(), weight[:1, :100].expand(90, 100)):
+            r, dy, b = base[..., 7:97], base[..., 11:101], weight[:, 5]
+            want = both(*(v.contiguous().clone() for v in (x, w, r, dy, b)))
+            got = both(x, w, r, dy, b)
+            # 100 terms of size one or so with other terms before or behind them
+            assert all(torch.allclose(a.double(), c.double(), rtol=2 * ROUNDOFF[dtype], atol=200 * (U if dtype == torch.float32 else 2.0 ** -11) * 10) for a, c in zip(got, want))
+    x = base[0, 0, :100]
+    assert fused_linear(x, weight[:, :100]).shape == (90,)
+    xs, w = base[..., :100].detach().requires_grad_(), weight[:, :100]
+    g1 = torch.autograd.grad(fused_linear(xs, w, activation="relu").sum(), xs)[0]  # a gradient of stride zero
+    g2 = torch.autograd.grad(fused_linear(xs, w, activation="relu"), xs, torch.ones(4, 6, 90, device=device, dtype=dtype))[0]
+    assert torch.equal(g1, g2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_infinities_nan_and_no_rows(device, dtype):
+    x, w = torch.randn(6, 40, device=device).to(dtype), torch.randn(24, 40, device=device).to(dtype)
+    x[1, 3], x[2, 5] = math.nan, math.inf
+    for act in ACTIVATIONS:
+        y = fused_linear(x, w, activation=act)
+        assert torch.isnan(y[1]).all() and not torch.isfinite(y[2]).all() and torch.isfinite(y[[0, 3, 4, 5]]).all()
+    for act in (None, "gelu"):
+        t = {k: v.requires_grad_() for k, v in (("x", torch.zeros(0, 40, device=device, dtype=dtype)), ("w", w.clone()), ("b", torch.zeros(24, device=device, dtype=dtype)))}
+        y = fused_linear(t["x"], t["w"], t["b"], activation=act)
+        gx, gw, gb = torch.autograd.grad(y.sum(), list(t.values()))
+        assert y.shape == (0, 24) and gx.shape == (0, 40) and float(gw.abs().sum()) == 0 and float(gb.abs().sum()) == 0 and gb.shape == (24,)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("activation", ["relu", "silu", "gelu", "gelu_tanh"])
+def test_far_out(device, dtype, activation):
+    # one weight of one: z is x.  Slopes are 0 and 1 far out, also where z is beyond fp16's range.
+    ends = [-6e4, -300.0, -88.0, -30.0, 30.0, 88.0, 300.0, 6e4]
+    x = torch.tensor(ends, device=device).to(dtype)[:, None].requires_grad_()
+    w = torch.ones(1, 1, device=device, dtype=dtype)
+    b = torch.zeros(1, device=device, dtype=dtype)
+    y = fused_linear(x, w, b, activation=activation)
+    (g,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    # (silu's slope at -30 is 29 exp(-30), 2.8e-12, below zero)
+    assert ((g[:, 0].float().cpu() - torch.tensor([0.0] * 4 + [1.0] * 4)).abs() <= 3e-12).all() and torch.equal(y[4:], x.detach()[4:]) and (y[:4].float().abs() < 1e-10).all()
+    x = torch.full((3, 2), 5e4, device=device).to(dtype).requires_grad_()
+    y = fused_linear(x, torch.ones(1, 2, device=device, dtype=dtype), activation=activation, residual=torch.zeros(3, 1, device=device))
+    assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], torch.ones_like(x))
+    assert (y == 2 * x.detach()[:, :1].float()).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_are_those_of_differences(device):
+    t = _inputs(6, 30, 20, torch.float32, torch.float32, True, device, seed=5)
+    gen = torch.Generator().manual_seed(8)
+    for activation in ("silu", "gelu", "gelu_tanh", None):
+        grads = _call(t, activation)[1:]
+        for name, grad in zip(("x", "weight", "bias", "residual"), grads):
+            way = torch.randn(t[name].shape, generator=gen).to(device)
+            h = 2.0 ** -8
+
+            def value(sign):
+                moved = {k: v.detach() for k, v in t.items()}
+                moved[name] = moved[name] + sign * h * way
+                return float((_call(moved, activation, grad=False)[0].double() * t["dy"].double()).sum())
+
+            got, want = (value(1) - value(-1)) / (2 * h), float((grad.double() * way.double()).sum())
+            # 120 results, each off by some 50 roundings of its size of a few, over h; third derivatives (below 2) of steps of up to
+            # 5 h each, cubed and weighted with dy
+            assert abs(got - want) <= 120 * 4 * 50 * U / h + 120 * 2 * 125 * h * h / 6
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_module_autocast_and_modes(device):
+    torch.manual_seed(2)
+    m = FusedLinear(48, 40, activation="gelu").to(device)
+    ref = torch.nn.Linear(48, 40).to(device)
+    ref.load_state_dict(m.state_dict())
+    m.requires_grad_(False), ref.requires_grad_(False)
+    x, other, r = torch.randn(7, 48, device=device), torch.randn(7, 48, device=device), torch.randn(7, 40, device=device)
+    assert torch.allclose(m(x, r), torch.nn.functional.gelu(ref(x)) + r, rtol=0, atol=1e-5)
+    with torch.autocast(device, dtype=torch.bfloat16):
+        y, y32 = m(x), m(x, r)
+    assert y.dtype is torch.bfloat16 and y32.dtype is torch.float32
+    lone = [t.bfloat16() for t in (x, m.weight, m.bias)]
+    assert torch.equal(y, fused_linear(*lone, activation="gelu")) and torch.equal(y32, fused_linear(*lone, activation="gelu", residual=r))
+    w = m.weight.clone().requires_grad_()
+    with torch.autocast(device, dtype=torch.bfloat16):
+        z = fused_linear(x, w, m.bias, activation="silu")
+        (g,) = torch.autograd.grad(z, w, torch.ones_like(z))
+    assert g.dtype is torch.float32
+    for pre in (False, True):
+        traced = make_fx(lambda t: fused_linear(t, m.weight, m.bias, activation="gelu"), pre_dispatch=pre)(x)
+        assert torch.allclose(traced(other), m(other), rtol=0, atol=1e-5)
+    with FlopCounterMode(display=False) as count:
+        y = fused_linear(x.requires_grad_(), w, m.bias, activation="gelu")
+        torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert count.get_total_flops() == 3 * 2 * 7 * 48 * 40
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    x, w, b = torch.randn(4, 16, device=device).half(), torch.randn(24, 16, device=device).half(), torch.randn(24, device=device).half()
+    kind = ValueError if device == "cpu" else RuntimeError
+    r = torch.randn(4, 24, device=device)
+    for args, kw in [((x.float(), w), {}), ((x, w, b.float()), {}), ((x, w[:, :8]), {}), ((x, w, b[:8]), {}), ((x, w[0]), {}), ((x, w[:0]), {}), ((x[:, :0], w[:, :0]), {}),
+                     ((x[0, 0], w), {}), ((x, w, b[None]), {}), ((x, w), dict(residual=r[:2])), ((x, w), dict(residual=r.bfloat16())), ((x, w), dict(residual=r[:, :1])),
+                     ((x, w), dict(residual=r.double()))]:
+        with pytest.raises(kind, match="fused_linear"):
+            fused_linear(*args, **kw)
+    for bad in ("tanh", "none", "GELU"):
+        with pytest.raises(ValueError, match="activation"):
+            fused_linear(x, w, activation=bad)
+    with pytest.raises(ValueError, match="activation"):
+        FusedLinear(4, 4, activation="tanh")
+
+
+@pytest.mark.gpu
+def test_refusals_of_the_kernels(cuda_device):
+    x, w = torch.randn(4, 16, device=cuda_device, requires_grad=True), torch.randn(24, 16, device=cuda_device)
+    with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+        fused_linear(x.double(), w.double())
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        fused_linear(x, w.cpu())
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(fused_linear(x, w, activation="gelu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="fused_linear"):
+        torch.func.vmap(lambda t: fused_linear(t[None], w))(x.detach())
+    y = fused_linear(x, w)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda t: torch.autograd.grad(y, x, t, retain_graph=True)[0])(torch.ones_like(y))
+    for change in (lambda t: t.double(), lambda t: t[:2], lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            y = fused_linear(x, w, activation="relu")
+        with pytest.raises(RuntimeError, match="fused_linear: a (tensor saved for the backward pass|dense CUDA tensor)"):
+            torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_saved_tensors_that_come_back_laid_out_anew(cuda_device, dtype):
+    t = _inputs(70, 40, 56, dtype, None, True, cuda_device)
+    want = _call(t, "gelu")
+    for hooks in ((lambda v: v, lambda v: v.t().contiguous().t() if v.dim() == 2 else v), (lambda v: v.cpu(), lambda v: v.to(cuda_device))):
+        with torch.autograd.graph.saved_tensors_hooks(*hooks):
+            y = fused_linear(*_leaves(t), activation="gelu")
+        got = [y.detach(), *torch.autograd.grad(y, _leaves(t), t["dy"])]
+        assert all(torch.allclose(a.double(), b.double(), rtol=2 * ROUNDOFF[dtype], atol=1e-4) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_the_run(cuda_device):
+    t = _inputs(3000, 264, 1032, torch.bfloat16, torch.float32, True, cuda_device)
+    first = _call(t, "gelu_tanh")
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, _call(t, "gelu_tanh")))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_captured_replayed_and_on_another_stream(cuda_device, tokens):
+    t = _inputs(tokens, 200, 136, torch.bfloat16, torch.float32, True, cuda_device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            out = _call(t, "gelu")
+            few = _call(t, "gelu", grad=False)
+    torch.cuda.current_stream().wait_stream(side)
+    _check(t, "gelu", out), _check(t, "gelu", few)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _call(t, "gelu")
+        few = _call(t, "gelu", grad=False)
+    other = _inputs(tokens, 200, 136, torch.bfloat16, torch.float32, True, cuda_device, seed=8)
+    with torch.no_grad():
+        for k, v in other.items():
+            t[k].copy_(v)
+    graph.replay()
+    _check(t, "gelu", out), _check(t, "gelu", few)
+
+
+@pytest.mark.gpu
+def test_waits_that_run_out_are_reported_and_leave_nan():
+    # in a process of its own: the report is one for the whole device
+    code = """
+import torch, mccl_b200
+from mccl_b200.ops.fused_linear import fused_linear
+native = mccl_b200.require_native()
+x, w = (torch.randn(*s, device="cuda").bfloat16() for s in ((300, 256), (512, 256)))
+y = native._fused_linear_with_limit(x, w, 0)
+torch.cuda.synchronize()
+assert torch.isnan(y).all()
+try:
+    fused_linear(x, w)
+except RuntimeError as e:
+    assert "ran out" in str(e)
+else:
+    raise AssertionError("not reported")
+assert torch.isfinite(fused_linear(x, w)).all()
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation,residual", [("gelu", None), (None, torch.float32)])
+def test_places_beyond_32_bits(cuda_device, activation, residual):
+    tokens, out, width = 70000, 32776, 24
+    gen = torch.Generator(device=cuda_device).manual_seed(2)
+    x, w = (torch.randn(*s, generator=gen, device=cuda_device).bfloat16() for s in ((tokens, width), (out, width)))
+    r = None
+    if residual is not None:
+        r = torch.empty(tokens, out, device=cuda_device, dtype=residual).normal_(generator=gen)
+    x.requires_grad_()
+    y = fused_linear(x, w, activation=activation, residual=r)
+    ends = torch.tensor([0, 1, 65535, 65536, tokens - 2, tokens - 1], device=cuda_device)
+    part = x.detach()[ends].requires_grad_()
+    want = fused_linear(part, w, activation=activation, residual=None if r is None else r[ends])
+    # (few tokens that keep nothing have a kernel of their own, with another order of the sums)
+    size = x.detach()[ends].abs().double() @ w.abs().double().T
+    off = (y.detach()[ends].double() - want.detach().double()).abs()
+    assert (off == 0).all() if residual is None else (off <= 2 * _sum(torch.bfloat16, width) * size + 2 * U * want.detach().abs().double()).all()
+    dy = y.detach()
+    (g,) = torch.autograd.grad(y, x, dy)
+    (few,) = torch.autograd.grad(want, part, dy[ends])
+    # (a sum of 32776 terms whose order and parts may differ)
+    size = dy[ends].abs().double() @ w.abs().double()
+    assert ((g[ends].double() - few.double()).abs() <= few.abs().double() * 2.0 ** -7 + size * (out / 8 + 40) * 2.0 ** -22).all()
