@@ -377,10 +377,10 @@ struct DirectLayer {
       if (i + e < left) to[e] = v[e];
   }
 };
-// What 16 columns of a linear layer's result need from memory: the bias, which is the same for all rows, and a row's residual, as they lie there.
-template <bool kWide>
+// What kN columns of a linear layer's result need from memory: the bias, which is the same for all rows, and a row's residual, as they lie there.
+template <bool kWide, int kN>
 struct LayerAhead {
-  uint4 bias[2], residual[kWide ? 4 : 2];
+  uint4 bias[kN / 8], residual[kN / (kWide ? 4 : 8)];
   // 16 bytes from the number `at` on, of `n` that there are, of 2 or 4 bytes each.
   template <int kSize>
   static __device__ __forceinline__ uint4 run(const char* from, int64_t n, bool vec) {
@@ -400,11 +400,11 @@ struct LayerAhead {
     const int64_t n = l.cols - col;
     if (l.bias != nullptr)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) bias[i] = run<2>(l.bias + 2 * (col + 8 * i), n - 8 * i, l.bias_vec);
+      for (int i = 0; i < kN / 8; ++i) bias[i] = run<2>(l.bias + 2 * (col + 8 * i), n - 8 * i, l.bias_vec);
     if (l.residual != nullptr) {
       constexpr int kSize = kWide ? 4 : 2, kPer = 16 / kSize;
 #pragma unroll
-      for (int i = 0; i < 16 / kPer; ++i) residual[i] = run<kSize>(l.residual + kSize * (row * l.ldr + col + kPer * i), n - kPer * i, l.residual_vec);
+      for (int i = 0; i < kN / kPer; ++i) residual[i] = run<kSize>(l.residual + kSize * (row * l.ldr + col + kPer * i), n - kPer * i, l.residual_vec);
     }
   }
 };
@@ -418,36 +418,37 @@ __device__ __forceinline__ void halves(const uint4& raw, float* v) {  // 8 numbe
     v[2 * i + 1] = f.y;
   }
 }
-// 16 columns of x W^T to z and y.
-template <bool kKeep, bool kWide, bool kBf16, typename Sink>
-__device__ __forceinline__ void finish_layer(const Finish& f, const float* v, const LayerAhead<kWide>& now, const Sink& sink, int i0) {
+// kN columns of x W^T to z and y.
+template <bool kKeep, bool kWide, bool kBf16, int kN, typename Sink>
+__device__ __forceinline__ void finish_layer(const Finish& f, float* z, const LayerAhead<kWide, kN>& now, const Sink& sink, int i0) {
   const Layer& l = f.layer;
+  if (l.bias != nullptr)
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    float z[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = v[8 * b + e];
-    if (l.bias != nullptr) {
+    for (int b = 0; b < kN / 8; ++b) {
       float bias[8];
       halves<kBf16>(now.bias[b], bias);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] += bias[e];
+      for (int e = 0; e < 8; ++e) z[8 * b + e] += bias[e];
     }
-    if constexpr (kKeep) {
+  if constexpr (kKeep)
+#pragma unroll
+    for (int b = 0; b < kN; b += 8) {
       if constexpr (kBf16) {
-        sink.put(0, i0 + 8 * b, z);
+        sink.put(0, i0 + b, z + b);
       } else {  // beyond fp16's range slopes are what they are at its end
         float kept[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) kept[e] = z[e] != z[e] ? z[e] : fminf(fmaxf(z[e], -65504.f), 65504.f);
-        sink.put(0, i0 + 8 * b, kept);
+        for (int e = 0; e < 8; ++e) kept[e] = z[b + e] != z[b + e] ? z[b + e] : fminf(fmaxf(z[b + e], -65504.f), 65504.f);
+        sink.put(0, i0 + b, kept);
       }
     }
-    with_activation(l.activation, [&](auto act) {
+  with_activation(l.activation, [&](auto act) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = Act16::value<decltype(act)::kValue>(z[e]);
-    });
-    if (l.residual != nullptr) {
+    for (int e = 0; e < kN; ++e) z[e] = Act16::value<decltype(act)::kValue>(z[e]);
+  });
+  if (l.residual != nullptr)
+#pragma unroll
+    for (int b = 0; b < kN / 8; ++b) {
       float r[8];
       if constexpr (kWide) {
 #pragma unroll
@@ -459,10 +460,12 @@ __device__ __forceinline__ void finish_layer(const Finish& f, const float* v, co
         halves<kBf16>(now.residual[b], r);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] += r[e];
+      for (int e = 0; e < 8; ++e) z[8 * b + e] += r[e];
     }
-    if constexpr (kWide) sink.put_f32(kKeep ? 1 : 0, i0 + 8 * b, z);
-    else sink.put(kKeep ? 1 : 0, i0 + 8 * b, z);
+#pragma unroll
+  for (int b = 0; b < kN; b += 8) {
+    if constexpr (kWide) sink.put_f32(kKeep ? 1 : 0, i0 + b, z + b);
+    else sink.put(kKeep ? 1 : 0, i0 + b, z + b);
   }
 }
 // kN columns of g and u to h and to what is kept.
@@ -565,7 +568,7 @@ __device__ __forceinline__ void finish_derive(const Finish& f, const float* dh, 
 // The columns that a thread takes out of the accumulator at a time (of h for kActivate: of c two each; an 8-bit group is one
 // thread's).  64 columns leave together.
 template <Out kOut, GatedKeep kKeep>
-constexpr int kTake = kOut == kActivate && kKeep == GatedKeep::kEight ? 64 : 16;
+constexpr int kTake = kOut == kActivate && kKeep == GatedKeep::kEight ? 64 : kIsLayer<kOut> ? 32 : 16;
 template <Out kOut>
 constexpr int kBoxes = kOut == kDerive ? 3 : kIsLayer<kOut> ? (kKeepsZ<kOut> ? 1 : 0) + (kWideY<kOut> ? 2 : 1) : 1;
 template <Out kOut>
@@ -583,7 +586,7 @@ struct Nothing {
   __device__ __forceinline__ void load(const Finish&, int64_t, int64_t) {}
 };
 template <Out kOut, GatedKeep kKeep>
-using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, std::conditional_t<kIsLayer<kOut>, LayerAhead<kWideY<kOut>>, Nothing>>;
+using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, std::conditional_t<kIsLayer<kOut>, LayerAhead<kWideY<kOut>, kTake<kOut, kKeep>>, Nothing>>;
 
 // A thread's row and columns of a tile: `row` of the result that the tile is of, its columns from `col` on.
 struct Spot {
@@ -614,10 +617,10 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
         fetch(c + i, v);
         finish_derive<kKeep>(f, v, now, sink, i);
       } else if constexpr (kIsLayer<kOut>) {
-        const LayerAhead<kWideY<kOut>> now = ahead;
+        const Ahead<kOut, kKeep> now = ahead;
         if (c + i + kN < last) ahead.load(f, min(at.row, f.rows - 1), at.col + c + i + kN);
         fetch(c + i, v);
-        finish_layer<kKeepsZ<kOut>, kWideY<kOut>, kBf16>(f, v, now, sink, i);
+        finish_layer<kKeepsZ<kOut>, kWideY<kOut>, kBf16, kN>(f, v, now, sink, i);
       } else {
         fetch(c + i, v);
 #pragma unroll

@@ -19,7 +19,11 @@ struct Act16 {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
   }
-  static __device__ __forceinline__ float logistic(float t) { return reciprocal(1.f + exp2_of(-1.4426950408889634f * t)); }
+  // The logistic function of z, or of 2 sqrt(2 / pi) (z + 0.044715 z^3): s = 1 / (1 + 2^(z (c0 + c1 z^2))).  (Where the square overflows the
+  // exponent does, to the right end.)
+  static constexpr float kC0 = -1.4426950408889634f;
+  static __device__ __forceinline__ float logistic(float z) { return reciprocal(1.f + exp2_of(kC0 * z)); }
+  static __device__ __forceinline__ float cubic(float z, float square) { return reciprocal(1.f + exp2_of(z * fmaf(kC0 * kGelu * kCubic, square, kC0 * kGelu))); }
   // The normal distribution up to z, and its density times z.  The tail is t P(t) exp(-z^2 / 2) / 2 with t = 1 / (1 + |z| / sqrt(8)) and a polynomial
   // fitted to erfc(x) exp(x^2) / t by reweighted least squares, 2^-19.5 of its size off at most between x = 0 and 10.
   struct Normal {
@@ -37,13 +41,12 @@ struct Act16 {
     const float tail = 0.5f * t * p * e;
     return {z < 0.f ? tail : 1.f - tail, z * (0.3989422804014327f * e)};
   }
-  static __device__ __forceinline__ float cubic(float z) { return kGelu * fmaf(kCubic * z, fminf(z * z, 1e30f), z); }
   template <LayerActivation kAct>
   static __device__ __forceinline__ float value(float z) {
     if constexpr (kAct == LayerActivation::kRelu) return z > 0.f || z != z ? z : 0.f;
     else if constexpr (kAct == LayerActivation::kSilu) return z * logistic(z);
     else if constexpr (kAct == LayerActivation::kGelu) return z * normal(z).share;
-    else if constexpr (kAct == LayerActivation::kGeluTanh) return z * logistic(cubic(z));
+    else if constexpr (kAct == LayerActivation::kGeluTanh) return z * cubic(z, z * z);
     else return z;
   }
   template <LayerActivation kAct>
@@ -52,13 +55,13 @@ struct Act16 {
       return z > 0.f ? 1.f : z != z ? z : 0.f;
     } else if constexpr (kAct == LayerActivation::kSilu) {
       const float s = logistic(z);
-      return fmaf(z, s - s * s, s);
+      return fmaf(z, fmaf(-s, s, s), s);
     } else if constexpr (kAct == LayerActivation::kGelu) {
       const Normal n = normal(z);
       return n.share + n.slope;
     } else if constexpr (kAct == LayerActivation::kGeluTanh) {
-      const float s = logistic(cubic(z));
-      return fmaf(z * (s - s * s), kGelu * fmaf(3.f * kCubic, fminf(z * z, 1e30f), 1.f), s);
+      const float square = fminf(z * z, 1e30f), s = cubic(z, square);
+      return fmaf(z * fmaf(-s, s, s), fmaf(kGelu * 3.f * kCubic, square, kGelu), s);
     } else {
       return 1.f;
     }

@@ -42,9 +42,23 @@ __global__ void __launch_bounds__(kThreads) layer_finish_kernel(const Finish w) 
 }
 
 // ---- dz and the bias's gradient ---------------------------------------------------------------------------------
-// T: the operands' type; D: of dy.  A warp has kV columns a lane, and every kWarps-th row of its block's.
+// kV numbers of a row, as they lie in memory.
+template <typename T, int kV>
+struct RawRun {
+  static constexpr int kBytes = kV * sizeof(T);
+  using Word = std::conditional_t<kBytes >= 16, uint4, std::conditional_t<kBytes == 8, uint2, T>>;
+  Word w[kBytes >= 16 ? kBytes / 16 : 1];
+  __device__ __forceinline__ void load(const T* p) {
+    const Word* f = reinterpret_cast<const Word*>(p);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(w) / sizeof(Word)); ++i) w[i] = f[i];
+  }
+  __device__ __forceinline__ float operator[](int i) const { return Traits<T>::load(reinterpret_cast<const T*>(w)[i]); }
+};
+// T: the operands' type; D: of dy.  A warp has kV columns a lane, and every kWarps-th row of its block's; kRowsAhead of them are asked for while the
+// ones before are worked on.
 template <typename T, typename D, LayerActivation kAct, int kV>
-__global__ void __launch_bounds__(kThreads) layer_derive_kernel(const LayerDerive g, int64_t rows_each) {
+__global__ void __launch_bounds__(kThreads, 2) layer_derive_kernel(const LayerDerive g, int64_t rows_each) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using Act = std::conditional_t<std::is_same_v<T, float>, Act32, Act16>;
   constexpr bool kSlope = kAct != LayerActivation::kNone;
@@ -58,27 +72,34 @@ __global__ void __launch_bounds__(kThreads) layer_derive_kernel(const LayerDeriv
     const D* dy = static_cast<const D*>(g.dy.data) + col;
     const T* z = static_cast<const T*>(g.z.data) + col;
     T* dz = static_cast<T*>(g.dz) + col;
+    RawRun<D, kV> next_d[kRowsAhead];
+    RawRun<T, kV> next_z[kRowsAhead];
+    auto ask = [&](int r, int64_t at) {
+      if (at >= end) return;
+      next_d[r].load(dy + at * g.dy.ld);
+      if constexpr (kSlope) next_z[r].load(z + at * g.z.ld);
+    };
+#pragma unroll
+    for (int r = 0; r < kRowsAhead; ++r) ask(r, begin + warp + r * kWarps);
 #pragma unroll 1
     for (int64_t row = begin + warp; row < end; row += kRowsAhead * kWarps) {
-      float d[kRowsAhead][kV], v[kRowsAhead][kV];
 #pragma unroll
-      for (int r = 0; r < kRowsAhead; ++r) {
-        const int64_t at = row + r * kWarps;
-        if (at < end) {
-          load_run<D, kV>(dy + at * g.dy.ld, kV, true, d[r]);
-          if constexpr (kSlope) load_run<T, kV>(z + at * g.z.ld, kV, true, v[r]);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < kRowsAhead; ++r) {
+      for (int r = 0; r < kRowsAhead; ++r) {  // each place is asked for again as soon as its numbers are in registers of their own
         const int64_t at = row + r * kWarps;
         if (at >= end) break;
+        float d[kV], v[kV];
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
-          if constexpr (kSlope) d[r][i] *= Act::template slope<kAct>(v[r][i]);
-          sum[i] += d[r][i];
+          d[i] = next_d[r][i];
+          if constexpr (kSlope) v[i] = next_z[r][i];
         }
-        if (g.dz != nullptr) store_run<T, kV>(dz + at * g.dz_ld, kV, true, d[r]);
+        ask(r, at + kRowsAhead * kWarps);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          if constexpr (kSlope) d[i] *= Act::template slope<kAct>(v[i]);
+          sum[i] += d[i];
+        }
+        if (g.dz != nullptr) store_run<T, kV>(dz + at * g.dz_ld, kV, true, d);
       }
     }
   }
@@ -115,7 +136,7 @@ __global__ void __launch_bounds__(kJoinThreads) layer_join_kernel(const float* p
   bias[c] = Traits<T>::store(sum);
 }
 
-int64_t parts_of(int64_t rows, int64_t cols) { return std::clamp<int64_t>(ceil_div(6 * kSms, ceil_div(cols, 256)), 1, std::max<int64_t>(1, ceil_div(rows, 4 * kWarps))); }
+int64_t parts_of(int64_t rows, int64_t cols) { return std::clamp<int64_t>(ceil_div(4 * kSms, ceil_div(cols, 256)), 1, std::max<int64_t>(1, ceil_div(rows, 4 * kWarps))); }
 
 template <typename T, typename D, int kV>
 cudaError_t derive(const LayerDerive& g, cudaStream_t s) {
