@@ -184,6 +184,17 @@ constexpr bool kKeepsZ = kOut == kLayerKeep || kOut == kLayer32Keep;
 template <Out kOut>
 constexpr bool kWideY = kOut == kLayer32 || kOut == kLayer32Keep;
 
+// Sums that leave in 32 bits are taken out of tensor memory every kChunk stages (512 of the reduction) and added in registers, rounded to nearest:
+// the tensor cores cut theirs off, 16 products at a time, each time towards zero.  A result is 5e-7 of its size off so, whatever its terms, and 1e-6
+// for each 1024 of them without; of 16 bits it does not show.  The 128 numbers a thread are what the first four warps hand over of their registers:
+// at launch a thread has 168 (three warps of a quarter SM's 512 a lane), four warps go down to 56 and eight up to 224, as many in all.
+template <Out kOut>
+constexpr bool kAddsUp = kWideY<kOut>;
+template <Out kOut>
+constexpr int kChunk = kAddsUp<kOut> ? 8 : 1 << 30;
+constexpr int kLaunched = 168, kKept = 56, kTaken = 224;
+static_assert(4 * kKept + kOutWarps * kTaken <= (kFirstOut + kOutWarps) * kLaunched, "a split of more than there are waits forever");
+
 struct Layer {
   LayerActivation activation;
   const char *bias, *residual;
@@ -348,6 +359,14 @@ struct Staged {
     for (int e = 0; e < 8; e += 4)
       asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + ((((i % 32) + e) / 4) ^ swizzle) * 16), "f"(v[e]), "f"(v[e + 1]), "f"(v[e + 2]),
                    "f"(v[e + 3])
+                   : "memory");
+  }
+  __device__ __forceinline__ void get_f32(int which, int i, float* v) const {  // as they were put
+    const uint32_t box = row + (which + i / 32) * kBoxBytes;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[e]), "=f"(v[e + 1]), "=f"(v[e + 2]), "=f"(v[e + 3])
+                   : "r"(box + ((((i % 32) + e) / 4) ^ swizzle) * 16)
                    : "memory");
   }
 };
@@ -568,7 +587,7 @@ __device__ __forceinline__ void finish_derive(const Finish& f, const float* dh, 
 // The columns that a thread takes out of the accumulator at a time (of h for kActivate: of c two each; an 8-bit group is one
 // thread's).  64 columns leave together.
 template <Out kOut, GatedKeep kKeep>
-constexpr int kTake = kOut == kActivate && kKeep == GatedKeep::kEight ? 64 : kIsLayer<kOut> ? 32 : 16;
+constexpr int kTake = kOut == kActivate && kKeep == GatedKeep::kEight ? 64 : kIsLayer<kOut> && !kAddsUp<kOut> ? 32 : 16;
 template <Out kOut>
 constexpr int kBoxes = kOut == kDerive ? 3 : kIsLayer<kOut> ? (kKeepsZ<kOut> ? 1 : 0) + (kWideY<kOut> ? 2 : 1) : 1;
 template <Out kOut>
@@ -629,6 +648,44 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
     }
   }
 }
+// The boxes of 64 columns from `c` of the tile on, of the warp's rows from `y` on, to z and y.
+template <Out kOut>
+__device__ __forceinline__ void flush_layer(const Job& j, const Spot& at, int c, int last, int64_t y, uint32_t boxes, int lane) {
+              constexpr int kFirst = kKeepsZ<kOut> ? 1 : 0;  // y's boxes behind z's
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) {
+                if (y < j.rows) {
+                  const int x = static_cast<int>(at.col) + c;
+                  if constexpr (kKeepsZ<kOut>) store_box(&j.out[1], boxes, x, static_cast<int>(y));
+                  if (j.wide) {
+                    store_box(&j.out[0], boxes + kFirst * kBoxBytes, x, static_cast<int>(y));
+                    if (kWideY<kOut> && c + 32 < last) store_box(&j.out[0], boxes + (kFirst + 1) * kBoxBytes, x + 32, static_cast<int>(y));
+                  }
+                }
+                stores_commit();
+              }
+              if (!j.wide) {  // rows that are not aligned: two numbers a lane, row by row
+                const int n = static_cast<int>(min(static_cast<int64_t>(32), j.rows - y)), here = last - c - 2 * lane;
+                char* to = static_cast<char*>(j.to[0]) + (y * j.ldo + at.col + c + 2 * lane) * (kWideY<kOut> ? 4 : 2);
+#pragma unroll 4
+                for (int r = 0; r < n; ++r, to += j.ldo * (kWideY<kOut> ? 4 : 2)) {
+                  uint32_t v[2];
+                  if constexpr (kWideY<kOut>) {
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1])
+                                 : "r"(boxes + (kFirst + lane / 16) * kBoxBytes + r * 128 + ((lane % 16 / 2) ^ (r & 7)) * 16 + lane % 2 * 8));
+                    if (here > 0) reinterpret_cast<uint32_t*>(to)[0] = v[0];
+                    if (here > 1) reinterpret_cast<uint32_t*>(to)[1] = v[1];
+                  } else {
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(boxes + kFirst * kBoxBytes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
+                    if (here > 0) reinterpret_cast<uint16_t*>(to)[0] = static_cast<uint16_t>(v[0]);
+                    if (here > 1) reinterpret_cast<uint16_t*>(to)[1] = static_cast<uint16_t>(v[0] >> 16);
+                  }
+                }
+                __syncwarp();
+              }
+}
+
 // A pair of CTAs per tile of 256 x 256, tiles in turn: each CTA loads half of either operand's rows and has half of the
 // accumulator's; the first one issues the products of both.  Two accumulators, so that a tile is taken out while the next one
 // is multiplied.  A stage is 64 KB for 8.4 million multiplications: what passes through the second-level cache, 13.5 TB/s of it, bounds
@@ -679,86 +736,143 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   bool ok = true, issued = false;
 
-  if (warp == kLoader) {
-    if (elect()) {
-      int s = 0, turn = 0;
-      for (int round = 0, item = pair; ok && item < w.items; item = item_of(++round, pair, pairs, w.jobs)) {
-        const Item t(w, item);
-        const Job& j = w.job[t.job];
-        const int i_second = t.ti >= j.rows_segment, i0 = (i_second ? t.ti - j.rows_segment : t.ti) * kTile + rank * kHalf;
-        // g and u side by side: one CTA has the rows of Wg, the other those of Wu
-        const int j0 = kOut == kActivate ? t.tj * kHalf : t.tj * kTile + rank * kHalf;
-        const bool a_inner = j.a_inner, b_inner = j.b_inner;
-        for (int c = t.c0; ok && c < t.c1; ++c) {
+  if (warp < kFirstOut) {
+    if constexpr (kAddsUp<kOut>) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKept));
+    if (warp == kLoader) {
+      if (elect()) {
+        int s = 0, turn = 0;
+        for (int round = 0, item = pair; ok && item < w.items; item = item_of(++round, pair, pairs, w.jobs)) {
+          const Item t(w, item);
+          const Job& j = w.job[t.job];
+          const int i_second = t.ti >= j.rows_segment, i0 = (i_second ? t.ti - j.rows_segment : t.ti) * kTile + rank * kHalf;
+          // g and u side by side: one CTA has the rows of Wg, the other those of Wu
+          const int j0 = kOut == kActivate ? t.tj * kHalf : t.tj * kTile + rank * kHalf;
+          const bool a_inner = j.a_inner, b_inner = j.b_inner;
+          for (int c = t.c0; ok && c < t.c1; ++c) {
+            ok = bar_wait(empty(s), (turn & 1) ^ 1, w.limit);
+            if (!ok) break;
+            const int k_second = c >= j.segment, k0 = (k_second ? c - j.segment : c) * kDepth;
+            const CUtensorMap* a = &j.a[i_second | k_second];
+            const CUtensorMap* b = &j.b[kOut == kActivate ? rank : k_second];
+            const uint32_t to = smem0 + s * kStage, bar = in_leader(full(s));
+            if (rank == 0) bar_expect(full(s), j.bytes);
+            if (a_inner) load_box(to, a, k0, i0, bar);
+            else {
+              load_box(to, a, i0, k0, bar);
+              load_box(to + kOperand / 2, a, i0 + 64, k0, bar);
+            }
+            if (b_inner) load_box(to + kOperand, b, k0, j0, bar);
+            else {
+              load_box(to + kOperand, b, j0, k0, bar);
+              load_box(to + kOperand + kOperand / 2, b, j0 + 64, k0, bar);
+            }
+            if (++s == kDepths) s = 0, ++turn;
+          }
+        }
+        // the products' last arrivals, before the barriers are another's
+        for (int left = 0; ok && left < kDepths; ++left) {
           ok = bar_wait(empty(s), (turn & 1) ^ 1, w.limit);
-          if (!ok) break;
-          const int k_second = c >= j.segment, k0 = (k_second ? c - j.segment : c) * kDepth;
-          const CUtensorMap* a = &j.a[i_second | k_second];
-          const CUtensorMap* b = &j.b[kOut == kActivate ? rank : k_second];
-          const uint32_t to = smem0 + s * kStage, bar = in_leader(full(s));
-          if (rank == 0) bar_expect(full(s), j.bytes);
-          if (a_inner) load_box(to, a, k0, i0, bar);
-          else {
-            load_box(to, a, i0, k0, bar);
-            load_box(to + kOperand / 2, a, i0 + 64, k0, bar);
-          }
-          if (b_inner) load_box(to + kOperand, b, k0, j0, bar);
-          else {
-            load_box(to + kOperand, b, j0, k0, bar);
-            load_box(to + kOperand + kOperand / 2, b, j0 + 64, k0, bar);
-          }
           if (++s == kDepths) s = 0, ++turn;
         }
       }
-      // the products' last arrivals, before the barriers are another's
-      for (int left = 0; ok && left < kDepths; ++left) {
-        ok = bar_wait(empty(s), (turn & 1) ^ 1, w.limit);
-        if (++s == kDepths) s = 0, ++turn;
-      }
-    }
-    __syncwarp();
-  } else if (warp == kIssuer) {
-    if (rank == 0 && elect()) {
-      issued = true;
-      ok = w.limit > 0;  // a limit of zero, of tests: no product is issued, and all others wait in vain
-      int s = 0, turn = 0, done = 0;
-      for (int round = 0, item = pair; ok && item < w.items; item = item_of(++round, pair, pairs, w.jobs), ++done) {
-        const Item t(w, item);
-        const bool a_inner = w.job[t.job].a_inner, b_inner = w.job[t.job].b_inner;
-        const uint32_t idesc = make_idesc(w.f.bf16, a_inner, b_inner), step_a = step_of(a_inner), step_b = step_of(b_inner);
-        const uint64_t a0 = make_desc(smem0, a_inner), b0 = make_desc(smem0 + kOperand, b_inner);
-        const int buffer = done & 1;
-        ok = bar_wait(acc_free(buffer), ((done >> 1) & 1) ^ 1, w.limit);
-        fence_after();
-        const uint32_t acc = tmem + buffer * kTile;
-        for (int c = t.c0; ok && c < t.c1; ++c) {
-          ok = bar_wait(full(s), turn & 1, w.limit);
-          if (!ok) break;
-          fence_after();
-          const uint64_t a = a0 + s * (kStage >> 4), b = b0 + s * (kStage >> 4);
+      __syncwarp();
+    } else if (warp == kIssuer) {
+      if (rank == 0 && elect()) {
+        issued = true;
+        ok = w.limit > 0;  // a limit of zero, of tests: no product is issued, and all others wait in vain
+        int s = 0, turn = 0, done = 0;
+        for (int round = 0, item = pair; ok && item < w.items; item = item_of(++round, pair, pairs, w.jobs)) {
+          const Item t(w, item);
+          const bool a_inner = w.job[t.job].a_inner, b_inner = w.job[t.job].b_inner;
+          const uint32_t idesc = make_idesc(w.f.bf16, a_inner, b_inner), step_a = step_of(a_inner), step_b = step_of(b_inner);
+          const uint64_t a0 = make_desc(smem0, a_inner), b0 = make_desc(smem0 + kOperand, b_inner);
+          for (int c = t.c0; ok && c < t.c1; ++done) {
+            const int buffer = done & 1, begin = c, end = min(t.c1, c + min(kChunk<kOut>, t.c1 - c));
+            ok = bar_wait(acc_free(buffer), ((done >> 1) & 1) ^ 1, w.limit);
+            fence_after();
+            const uint32_t acc = tmem + buffer * kTile;
+            for (; ok && c < end; ++c) {
+              ok = bar_wait(full(s), turn & 1, w.limit);
+              if (!ok) break;
+              fence_after();
+              const uint64_t a = a0 + s * (kStage >> 4), b = b0 + s * (kStage >> 4);
 #pragma unroll
-          for (int k = 0; k < kDepth / 16; ++k) mma(acc, a + k * step_a, b + k * step_b, idesc, c > t.c0 || k > 0);
-          mma_commit(empty(s));
-          if (++s == kDepths) s = 0, ++turn;
+              for (int k = 0; k < kDepth / 16; ++k) mma(acc, a + k * step_a, b + k * step_b, idesc, c > begin || k > 0);
+              mma_commit(empty(s));
+              if (++s == kDepths) s = 0, ++turn;
+            }
+            if (ok) mma_commit(acc_full(buffer));
+          }
         }
-        if (ok) mma_commit(acc_full(buffer));
       }
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp >= kFirstOut) {
+  } else {
+    if constexpr (kAddsUp<kOut>) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTaken));
     // lanes 32 q .. 32 q + 31 of tensor memory are open to the warps with warp % 4 == q, which share the columns
     constexpr int kN = kTake<kOut, kKeep>, kShares = kOutWarps / 4, kShare = (kOut == kActivate ? kHalf : kTile) / kShares;
     const int q = warp & 3, share = (warp - kFirstOut) >> 2;
     const int row = rank * kHalf + 32 * q + lane;
     const uint32_t boxes = smem0 + kDepths * kStage + (warp - kFirstOut) * (kOuts * kBoxBytes);
     int done = 0;
-    for (int round = 0, item = pair; item < w.items; item = item_of(++round, pair, pairs, w.jobs), ++done) {
+    for (int round = 0, item = pair; item < w.items; item = item_of(++round, pair, pairs, w.jobs), done += kAddsUp<kOut> ? 0 : 1) {
       const Item t(w, item);
       const Job& j = w.job[t.job];
       const int buffer = done & 1;
       const Spot at = spot_of<kOut>(j, t.ti, t.tj, row);
       Ahead<kOut, kKeep> ahead;
       if (t.part < 0 && at.col + share * kShare < j.cols) ahead.load(w.f, min(at.row, w.f.rows - 1), at.col + share * kShare);
+      if constexpr (kAddsUp<kOut>) {
+        float sum[kShare];
+#pragma unroll
+        for (int i = 0; i < kShare; ++i) sum[i] = 0.f;
+        for (int c = t.c0; c < t.c1; c += kChunk<kOut>, ++done) {
+          if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_full(done & 1), (done >> 1) & 1, w.limit));
+          fence_after();
+          const uint32_t from = tmem + (done & 1) * kTile + share * kShare + (static_cast<uint32_t>(32 * q) << 16);
+#pragma unroll
+          for (int i = 0; i < kShare; i += kN) {
+            float v[kN];
+            if (ok) {
+              tmem_load<kN>(from + i, v);
+              tmem_wait<kN>(v);
+            }
+#pragma unroll
+            for (int e = 0; e < kN; ++e) sum[i + e] += ok ? v[e] : NAN;  // no number that looks like a result
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0 && ok) bar_arrive_cluster(in_leader(acc_free(done & 1)));
+        }
+        if (t.part < 0) {
+          const int first = share * kShare, last = static_cast<int>(min(static_cast<int64_t>(first + kShare), j.cols - at.col));
+#pragma unroll
+          for (int turn = 0; turn < kShare; turn += kTurn) {
+            const int c = first + turn;
+            if (c >= last) break;
+            if (lane == 0) stores_left();
+            __syncwarp();
+            // the sums wait in y's boxes, so that what follows is one loop and not eight copies of it
+            constexpr int kY = kKeepsZ<kOut> ? 1 : 0;
+            const Staged<true> own(boxes, lane);
+#pragma unroll
+            for (int i = 0; i < kTurn; i += 8) own.put_f32(kY, i, sum + turn + i);
+            auto taken = [&](int col, float* v) {
+#pragma unroll
+              for (int e = 0; e < kN; e += 8) own.get_f32(kY, col - c + e, v + e);
+            };
+            if (w.f.bf16) finish_turn<kOut, kKeep, true, kTurn>(w.f, at, c, last, ahead, taken, Staged<true>(boxes, lane));
+            else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, taken, Staged<false>(boxes, lane));
+            flush_layer<kOut>(j, at, c, last, at.row - lane, boxes, lane);
+          }
+        } else if (at.row < j.rows) {
+          float* to = w.partial + static_cast<int64_t>(t.part) * (kTile * kTile) + row + static_cast<int64_t>(share) * kShare * kTile;
+#pragma unroll
+          for (int i = 0; i < kShare; ++i) __stcg(to + static_cast<int64_t>(i) * kTile, sum[i]);
+        }
+        __syncwarp();
+        continue;
+      }
       if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_full(buffer), (done >> 1) & 1, w.limit));
       fence_after();
       const uint32_t from = tmem + buffer * kTile + (static_cast<uint32_t>(32 * q) << 16);
@@ -782,39 +896,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           if (w.f.bf16) finish_turn<kOut, kKeep, true, kTurn>(w.f, at, c, last, ahead, fetch, Staged<true>(boxes, lane));
           else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, fetch, Staged<false>(boxes, lane));
           if constexpr (kIsLayer<kOut>) {
-            constexpr int kFirst = kKeepsZ<kOut> ? 1 : 0;  // y's boxes behind z's
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-              if (y < j.rows) {
-                const int x = static_cast<int>(at.col) + c;
-                if constexpr (kKeepsZ<kOut>) store_box(&j.out[1], boxes, x, static_cast<int>(y));
-                if (j.wide) {
-                  store_box(&j.out[0], boxes + kFirst * kBoxBytes, x, static_cast<int>(y));
-                  if (kWideY<kOut> && c + 32 < last) store_box(&j.out[0], boxes + (kFirst + 1) * kBoxBytes, x + 32, static_cast<int>(y));
-                }
-              }
-              stores_commit();
-            }
-            if (!j.wide) {  // rows that are not aligned: two numbers a lane, row by row
-              const int n = static_cast<int>(min(static_cast<int64_t>(32), j.rows - y)), here = last - c - 2 * lane;
-              char* to = static_cast<char*>(j.to[0]) + (y * j.ldo + at.col + c + 2 * lane) * (kWideY<kOut> ? 4 : 2);
-#pragma unroll 4
-              for (int r = 0; r < n; ++r, to += j.ldo * (kWideY<kOut> ? 4 : 2)) {
-                uint32_t v[2];
-                if constexpr (kWideY<kOut>) {
-                  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1])
-                               : "r"(boxes + (kFirst + lane / 16) * kBoxBytes + r * 128 + ((lane % 16 / 2) ^ (r & 7)) * 16 + lane % 2 * 8));
-                  if (here > 0) reinterpret_cast<uint32_t*>(to)[0] = v[0];
-                  if (here > 1) reinterpret_cast<uint32_t*>(to)[1] = v[1];
-                } else {
-                  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(boxes + kFirst * kBoxBytes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
-                  if (here > 0) reinterpret_cast<uint16_t*>(to)[0] = static_cast<uint16_t>(v[0]);
-                  if (here > 1) reinterpret_cast<uint16_t*>(to)[1] = static_cast<uint16_t>(v[0] >> 16);
-                }
-              }
-              __syncwarp();
-            }
+            flush_layer<kOut>(j, at, c, last, y, boxes, lane);
           } else if (kOut != kStore || j.wide) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -1161,6 +1243,12 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(gated_join_kernel<kOut, kKeep>, cudaFuncAttributeMaxDynamicSharedMemorySize, kJoinSmem<kOut, kKeep>);
     if (e != cudaSuccess) return e;
+    if constexpr (kAddsUp<kOut>) {  // the split of registers is one of as many as the launch has
+      cudaFuncAttributes at{};
+      e = cudaFuncGetAttributes(&at, kernel);
+      if (e != cudaSuccess) return e;
+      if (at.numRegs < kLaunched) return cudaErrorInvalidConfiguration;
+    }
     smem_set.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchAttribute attr[1];
