@@ -352,6 +352,13 @@ struct Staged {
                  "r"(pack2<kBf16>(v[4], v[5])), "r"(pack2<kBf16>(v[6], v[7]))
                  : "memory");
   }
+  __device__ __forceinline__ uint4 get(int which, int i) const {  // 8 numbers as they were put
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(row + which * kBoxBytes + ((i / 8) ^ swizzle) * 16)
+                 : "memory");
+    return v;
+  }
   // In 32 bits: boxes of 32 columns, from the `which`th on.
   __device__ __forceinline__ void put_f32(int which, int i, const float* v) const {
     const uint32_t box = row + (which + i / 32) * kBoxBytes;
@@ -396,35 +403,101 @@ struct DirectLayer {
       if (i + e < left) to[e] = v[e];
   }
 };
-// What kN columns of a linear layer's result need from memory: the bias, which is the same for all rows, and a row's residual, as they lie there.
-template <bool kWide, int kN>
-struct LayerAhead {
-  uint4 bias[kN / 8], residual[kN / (kWide ? 4 : 8)];
-  // 16 bytes from the number `at` on, of `n` that there are, of 2 or 4 bytes each.
-  template <int kSize>
-  static __device__ __forceinline__ uint4 run(const char* from, int64_t n, bool vec) {
-    constexpr int kPer = 16 / kSize;
-    if (vec) return n > 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
+// 16 bytes from `from` on, numbers of kSize bytes of which there are `n`.
+template <int kSize>
+__device__ __forceinline__ uint4 run_of(const char* from, int64_t n, bool vec) {
+  constexpr int kPer = 16 / kSize;
+  if (vec) return n > 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i < n) {
-        if constexpr (kSize == 4) w[i] = reinterpret_cast<const uint32_t*>(from)[i];
-        else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[i]) << (16 * (i % 2));
-      }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  __device__ __forceinline__ void load(const Finish& f, int64_t row, int64_t col) {
-    const Layer& l = f.layer;
-    const int64_t n = l.cols - col;
-    if (l.bias != nullptr)
-#pragma unroll
-      for (int i = 0; i < kN / 8; ++i) bias[i] = run<2>(l.bias + 2 * (col + 8 * i), n - 8 * i, l.bias_vec);
-    if (l.residual != nullptr) {
-      constexpr int kSize = kWide ? 4 : 2, kPer = 16 / kSize;
-#pragma unroll
-      for (int i = 0; i < kN / kPer; ++i) residual[i] = run<kSize>(l.residual + kSize * (row * l.ldr + col + kPer * i), n - kPer * i, l.residual_vec);
+  for (int i = 0; i < kPer; ++i)
+    if (i < n) {
+      if constexpr (kSize == 4) w[i] = reinterpret_cast<const uint32_t*>(from)[i];
+      else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[i]) << (16 * (i % 2));
     }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The bias of kN columns, which is the same for all rows, as it lies in memory.
+template <int kN>
+struct LayerAhead {
+  uint4 bias[kN / 8];
+  __device__ __forceinline__ void load(const Finish& f, int64_t, int64_t col) {
+    const Layer& l = f.layer;
+    if (l.bias == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < kN / 8; ++i) bias[i] = run_of<2>(l.bias + 2 * (col + 8 * i), l.cols - col - 8 * i, l.bias_vec);
+  }
+};
+// A warp's residual of a turn, 32 rows of 64 columns, by whole runs of the rows, where a thread's own row would take 32 requests for each of its
+// runs (8192 x 1024 x 4096 with an fp32 residual 98 us so, MEASURED).  Its place in y's boxes is where y's numbers go.
+template <bool kWide>
+struct LayerResidual {
+  static constexpr int kWords = kWide ? 64 : 32, kSize = kWide ? 4 : 2;
+  static constexpr int kLanes = kTurn * kSize / 16, kRowsAt = 32 / kLanes;  // lanes of a row, and rows a request, of aligned ones
+  uint32_t w[kWords];
+  // Rows from `row` on of `rows`, columns from `col` on.
+  __device__ __forceinline__ void load(const Layer& l, int64_t row, int64_t rows, int64_t col, int lane) {
+    const char* from = l.residual + kSize * (row * l.ldr + col);
+    const int64_t n = l.cols - col, high = rows - row;
+    if (l.residual_vec) {
+      const int at = lane % kLanes * (16 / kSize);
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const int r = i * kRowsAt + lane / kLanes;
+        const uint4 v = r < high && at < n ? __ldcs(reinterpret_cast<const uint4*>(from + kSize * (r * l.ldr + at))) : make_uint4(0u, 0u, 0u, 0u);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else {
+      const char* to = from + 2 * kSize * lane;  // two neighbours
+      const bool one = 2 * lane < n, two = 2 * lane + 1 < n;
+#pragma unroll
+      for (int r = 0; r < 32; ++r, to += kSize * l.ldr) {
+        if constexpr (kWide) {
+          w[2 * r] = r < high && one ? reinterpret_cast<const uint32_t*>(to)[0] : 0u;
+          w[2 * r + 1] = r < high && two ? reinterpret_cast<const uint32_t*>(to)[1] : 0u;
+        } else {
+          const uint32_t a = r < high && one ? reinterpret_cast<const uint16_t*>(to)[0] : 0u, b = r < high && two ? reinterpret_cast<const uint16_t*>(to)[1] : 0u;
+          w[r] = a | b << 16;
+        }
+      }
+    }
+  }
+  // Calls `f` with each run's place behind the first of y's boxes and its words: 4 of them, 2 or 1.
+  template <typename Call>
+  __device__ __forceinline__ void places(bool vec, int lane, Call f) const {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const int r = i * kRowsAt + lane / kLanes, run = lane % kLanes;
+        f(static_cast<uint32_t>(run / 8 * kBoxBytes + r * 128 + ((run % 8) ^ (r & 7)) * 16), w + 4 * i, std::integral_constant<int, 4>());
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        if constexpr (kWide) f(static_cast<uint32_t>(lane / 16 * kBoxBytes + r * 128 + ((lane % 16 / 2) ^ (r & 7)) * 16 + lane % 2 * 8), w + 2 * r, std::integral_constant<int, 2>());
+        else f(static_cast<uint32_t>(r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4), w + r, std::integral_constant<int, 1>());
+      }
+    }
+  }
+  __device__ __forceinline__ void put(bool vec, int lane, uint32_t box) const {
+    places(vec, lane, [&](uint32_t at, const uint32_t* v, auto n) {
+      if constexpr (decltype(n)::value == 4) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+      else if constexpr (decltype(n)::value == 2) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(box + at), "r"(v[0]), "r"(v[1]) : "memory");
+      else asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + at), "r"(v[0]) : "memory");
+    });
+  }
+  // In 32 bits: added to what is there.
+  __device__ __forceinline__ void add(bool vec, int lane, uint32_t box) const {
+    places(vec, lane, [&](uint32_t at, const uint32_t* v, auto n) {
+      constexpr int kN = decltype(n)::value;
+      float y[4];
+      if constexpr (kN == 4) asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(box + at) : "memory");
+      else asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(y[0]), "=f"(y[1]) : "r"(box + at) : "memory");
+#pragma unroll
+      for (int e = 0; e < kN; ++e) y[e] += __uint_as_float(v[e]);
+      if constexpr (kN == 4) asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + at), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]) : "memory");
+      else asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(box + at), "f"(y[0]), "f"(y[1]) : "memory");
+    });
   }
 };
 template <bool kBf16>
@@ -437,9 +510,9 @@ __device__ __forceinline__ void halves(const uint4& raw, float* v) {  // 8 numbe
     v[2 * i + 1] = f.y;
   }
 }
-// kN columns of x W^T to z and y.
-template <bool kKeep, bool kWide, bool kBf16, int kN, typename Sink>
-__device__ __forceinline__ void finish_layer(const Finish& f, float* z, const LayerAhead<kWide, kN>& now, const Sink& sink, int i0) {
+// kN columns of x W^T to z and y.  `more`: adds the residual of 8 columns.
+template <bool kKeep, bool kWide, bool kBf16, int kN, typename Sink, typename More>
+__device__ __forceinline__ void finish_layer(const Finish& f, float* z, const LayerAhead<kN>& now, const Sink& sink, int i0, const More& more) {
   const Layer& l = f.layer;
   if (l.bias != nullptr)
 #pragma unroll
@@ -465,22 +538,8 @@ __device__ __forceinline__ void finish_layer(const Finish& f, float* z, const La
 #pragma unroll
     for (int e = 0; e < kN; ++e) z[e] = Act16::value<decltype(act)::kValue>(z[e]);
   });
-  if (l.residual != nullptr)
 #pragma unroll
-    for (int b = 0; b < kN / 8; ++b) {
-      float r[8];
-      if constexpr (kWide) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4& w = now.residual[2 * b + h];
-          r[4 * h] = __uint_as_float(w.x), r[4 * h + 1] = __uint_as_float(w.y), r[4 * h + 2] = __uint_as_float(w.z), r[4 * h + 3] = __uint_as_float(w.w);
-        }
-      } else {
-        halves<kBf16>(now.residual[b], r);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[8 * b + e] += r[e];
-    }
+  for (int b = 0; b < kN; b += 8) more(i0 + b, z + b);
 #pragma unroll
   for (int b = 0; b < kN; b += 8) {
     if constexpr (kWide) sink.put_f32(kKeep ? 1 : 0, i0 + b, z + b);
@@ -605,7 +664,7 @@ struct Nothing {
   __device__ __forceinline__ void load(const Finish&, int64_t, int64_t) {}
 };
 template <Out kOut, GatedKeep kKeep>
-using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, std::conditional_t<kIsLayer<kOut>, LayerAhead<kWideY<kOut>, kTake<kOut, kKeep>>, Nothing>>;
+using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, std::conditional_t<kIsLayer<kOut>, LayerAhead<kTake<kOut, kKeep>>, Nothing>>;
 
 // A thread's row and columns of a tile: `row` of the result that the tile is of, its columns from `col` on.
 struct Spot {
@@ -618,8 +677,12 @@ __device__ __forceinline__ Spot spot_of(const Job& j, int ti, int tj, int row_in
   return {static_cast<int64_t>(second ? ti - j.rows_segment : ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * (kOut == kActivate ? kHalf : kTile), second};
 }
 // kCols columns from `c` of the tile on, into a sink.
-template <Out kOut, GatedKeep kKeep, bool kBf16, int kCols, typename Fetch, typename Sink>
-__device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int c, int last, Ahead<kOut, kKeep>& ahead, const Fetch& fetch, const Sink& sink) {
+struct NoMore {
+  __device__ __forceinline__ void operator()(int, float*) const {}
+};
+template <Out kOut, GatedKeep kKeep, bool kBf16, int kCols, typename Fetch, typename Sink, typename More = NoMore>
+__device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int c, int last, Ahead<kOut, kKeep>& ahead, const Fetch& fetch, const Sink& sink,
+                                            const More& more = More()) {
   constexpr int kN = kTake<kOut, kKeep>;
 #pragma unroll 1
   for (int i = 0; i < kCols; i += kN) {
@@ -639,7 +702,7 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
         const Ahead<kOut, kKeep> now = ahead;
         if (c + i + kN < last) ahead.load(f, min(at.row, f.rows - 1), at.col + c + i + kN);
         fetch(c + i, v);
-        finish_layer<kKeepsZ<kOut>, kWideY<kOut>, kBf16, kN>(f, v, now, sink, i);
+        finish_layer<kKeepsZ<kOut>, kWideY<kOut>, kBf16, kN>(f, v, now, sink, i, more);
       } else {
         fetch(c + i, v);
 #pragma unroll
@@ -822,6 +885,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
       const Spot at = spot_of<kOut>(j, t.ti, t.tj, row);
       Ahead<kOut, kKeep> ahead;
       if (t.part < 0 && at.col + share * kShare < j.cols) ahead.load(w.f, min(at.row, w.f.rows - 1), at.col + share * kShare);
+      [[maybe_unused]] LayerResidual<false> residual;
+      if constexpr (kAddsUp<kOut>) {
+        // (the residual itself has no registers before the sums are done: it comes nearer)
+        const Layer& l = w.f.layer;
+        if (t.part < 0 && l.residual != nullptr && at.row < w.f.rows)
+#pragma unroll
+          for (int i = 0; i < kShare; i += 32)
+            if (at.col + share * kShare + i < l.cols)
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(l.residual + 4 * (at.row * l.ldr + at.col + share * kShare + i)));
+      }
+      if constexpr (kIsLayer<kOut> && !kAddsUp<kOut>)
+        if (t.part < 0 && w.f.layer.residual != nullptr) residual.load(w.f.layer, at.row - lane, w.f.rows, at.col + share * kShare, lane);
       if constexpr (kAddsUp<kOut>) {
         float sum[kShare];
 #pragma unroll
@@ -861,8 +936,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
 #pragma unroll
               for (int e = 0; e < kN; e += 8) own.get_f32(kY, col - c + e, v + e);
             };
+            LayerResidual<true> residual;
+            if (w.f.layer.residual != nullptr) residual.load(w.f.layer, at.row - lane, w.f.rows, at.col + c, lane);
             if (w.f.bf16) finish_turn<kOut, kKeep, true, kTurn>(w.f, at, c, last, ahead, taken, Staged<true>(boxes, lane));
             else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, taken, Staged<false>(boxes, lane));
+            if (w.f.layer.residual != nullptr) {
+              __syncwarp();
+              residual.add(w.f.layer.residual_vec, lane, boxes + kY * kBoxBytes);
+            }
             flush_layer<kOut>(j, at, c, last, at.row - lane, boxes, lane);
           }
         } else if (at.row < j.rows) {
@@ -893,8 +974,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
         for (int c = first; c < last; c += kTurn) {
           if (lane == 0) stores_left();
           __syncwarp();
-          if (w.f.bf16) finish_turn<kOut, kKeep, true, kTurn>(w.f, at, c, last, ahead, fetch, Staged<true>(boxes, lane));
-          else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, fetch, Staged<false>(boxes, lane));
+          if constexpr (kIsLayer<kOut> && !kAddsUp<kOut>) {
+            constexpr int kY = kKeepsZ<kOut> ? 1 : 0;
+            const Layer& l = w.f.layer;
+            if (l.residual != nullptr) {
+              residual.put(l.residual_vec, lane, boxes + kY * kBoxBytes);
+              __syncwarp();
+              if (c + kTurn < last) residual.load(l, y, w.f.rows, at.col + c + kTurn, lane);
+            }
+            auto run = [&](auto bf16) {
+              constexpr bool kBf16 = decltype(bf16)::value;
+              const Staged<kBf16> sink(boxes, lane);
+              finish_turn<kOut, kKeep, kBf16, kTurn>(w.f, at, c, last, ahead, fetch, sink, [&](int i, float* v) {
+                if (l.residual == nullptr) return;
+                float r[8];
+                halves<kBf16>(sink.get(kY, i), r);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += r[e];
+              });
+            };
+            if (w.f.bf16) run(std::true_type());
+            else run(std::false_type());
+          } else {
+            if (w.f.bf16) finish_turn<kOut, kKeep, true, kTurn>(w.f, at, c, last, ahead, fetch, Staged<true>(boxes, lane));
+            else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, fetch, Staged<false>(boxes, lane));
+          }
           if constexpr (kIsLayer<kOut>) {
             flush_layer<kOut>(j, at, c, last, y, boxes, lane);
           } else if (kOut != kStore || j.wide) {
@@ -1044,8 +1148,29 @@ __global__ void __launch_bounds__(kJoinThreads) gated_join_kernel(const __grid_c
   if constexpr (kIsLayer<kOut>) {
     uint16_t* const z = kKeepsZ<kOut> ? static_cast<uint16_t*>(j.to[1]) + at.row * f.pitch + at.col + c : nullptr;
     void* const y = static_cast<char*>(j.to[0]) + (at.row * j.ldo + at.col + c) * (kWideY<kOut> ? 4 : 2);
-    if (f.bf16) finish_turn<kOut, kKeep, true, kN>(f, at, c, c + kN, ahead, fetch, DirectLayer<true, kKeepsZ<kOut>>{z, y, left, f.pitch - at.col - c, j.wide});
-    else finish_turn<kOut, kKeep, false, kN>(f, at, c, c + kN, ahead, fetch, DirectLayer<false, kKeepsZ<kOut>>{z, y, left, f.pitch - at.col - c, j.wide});
+    auto run = [&](auto bf16) {
+      constexpr bool kBf16 = decltype(bf16)::value;
+      finish_turn<kOut, kKeep, kBf16, kN>(f, at, c, c + kN, ahead, fetch, DirectLayer<kBf16, kKeepsZ<kOut>>{z, y, left, f.pitch - at.col - c, j.wide}, [&](int i, float* v) {
+        const Layer& l = f.layer;
+        if (l.residual == nullptr) return;
+        constexpr int kSize = kWideY<kOut> ? 4 : 2;
+        const char* from = l.residual + kSize * (at.row * l.ldr + at.col + c + i);
+        float r[8];
+        if constexpr (kWideY<kOut>) {
+#pragma unroll
+          for (int h = 0; h < 8; h += 4) {
+            const uint4 x = run_of<4>(from + 4 * h, left - i - h, l.residual_vec);
+            r[h] = __uint_as_float(x.x), r[h + 1] = __uint_as_float(x.y), r[h + 2] = __uint_as_float(x.z), r[h + 3] = __uint_as_float(x.w);
+          }
+        } else {
+          halves<kBf16>(run_of<2>(from, left - i, l.residual_vec), r);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += r[e];
+      });
+    };
+    if (f.bf16) run(std::true_type());
+    else run(std::false_type());
   } else {
     const int64_t to = at.row * j.ldo + at.col + c;
     uint16_t* const out[3] = {static_cast<uint16_t*>(j.to[at.which]) + to, static_cast<uint16_t*>(j.to[1]) + to, static_cast<uint16_t*>(j.to[2]) + to};
