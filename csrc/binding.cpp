@@ -389,7 +389,10 @@ bool adamw_step_group(AdamWPlan& plan, const py::list& params, const py::list& s
   }
   const int64_t step = static_cast<int64_t>(*counters[0].data_ptr<float>()) + 1;
   plan.step(grads, lr, beta1, beta2, eps, weight_decay, step, grad_scale);
-  for (at::Tensor& c : counters) c.fill_(static_cast<double>(step));
+  for (at::Tensor& c : counters) {  // (a dispatched fill_ each is most of a step over many small tensors)
+    *c.mutable_data_ptr<float>() = static_cast<float>(step);
+    if (!c.is_inference()) c.unsafeGetTensorImpl()->bump_version();
+  }
   return true;
 }
 

@@ -8,7 +8,8 @@ Flags follow reference examples/ddp_dummy_train.py:45-70 (``--backend``, ``--bas
 ``--steps``, ``--batch-size`` per rank, ``--bucket-mb``, ``--stress-model``, ``--fp16``,
 ``--save-stats``, ``--warmup``) plus ``--model`` (heavy | mlp | resnet50 | gpt2-medium | gpt2-tiny |
 gated-medium | gated-tiny, the decoders of gated blocks; ``--checkpoint int8`` keeps their activations in 8 bits),
-``--compression`` (none | fp16 | topk) and ``--fused-optim``.  AdamW lr 1e-4 wd 0.01 by
+``--compression`` (none | fp16 | topk), ``--fused-blocks`` (GPT-2 on this package's operators), ``--fused-optim`` and
+``--moment-bits`` (8: its moments in 8 bits).  AdamW lr 1e-4 wd 0.01 by
 default; after the run the first weights are broadcast from rank 0 and compared on every
 rank (replicas must be identical).
 """
@@ -43,6 +44,8 @@ def parse():
     ap.add_argument("--checkpoint", default=None, choices=["int8"], help="activations of the gated models in 8 bits")
     ap.add_argument("--topk-ratio", type=float, default=0.01)
     ap.add_argument("--fused-optim", action="store_true", help="use the fused AdamW kernel")
+    ap.add_argument("--moment-bits", type=int, default=32, choices=[8, 32], help="of the fused AdamW's moments")
+    ap.add_argument("--fused-blocks", action="store_true", help="GPT-2 blocks on this package's layer norm and linear layers")
     ap.add_argument("--lr", type=float, default=1e-4)
     ap.add_argument("--save-stats", default="")
     ap.add_argument("--cpu", action="store_true", help="CPU tensors (host transport)")
@@ -59,12 +62,12 @@ def build(args, device):
     if args.model == "resnet50":
         return models.ResNet50().to(device), "image"
     if args.model == "gpt2-medium":
-        return models.gpt2_medium().to(device), "tokens"
+        return models.gpt2_medium(fused=args.fused_blocks).to(device), "tokens"
     if args.model == "gated-medium":
         return models.gated_medium(checkpoint=args.checkpoint).to(device), "tokens"
     if args.model == "gated-tiny":
         return models.gated_tiny(checkpoint=args.checkpoint).to(device), "tokens-tiny"
-    return models.gpt2_tiny().to(device), "tokens-tiny"
+    return models.gpt2_tiny(fused=args.fused_blocks).to(device), "tokens-tiny"
 
 
 def make_batch(kind, n, ds, device):
@@ -110,7 +113,7 @@ def main():
                                             bucket_cap_mb=args.bucket_mb)
     if args.fused_optim and use_cuda:
         from mccl_b200.optim import FusedAdamW
-        opt = FusedAdamW(model.parameters(), lr=args.lr, weight_decay=0.01)
+        opt = FusedAdamW(model.parameters(), lr=args.lr, weight_decay=0.01, state_bits=args.moment_bits)
     else:
         opt = torch.optim.AdamW(model.parameters(), lr=args.lr, weight_decay=0.01)
     from mccl_b200.utils import SyntheticDataset, write_training_stats

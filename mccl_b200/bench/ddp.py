@@ -32,6 +32,8 @@ def main(argv=None):
     ap.add_argument("--bucket-mb", type=int, default=25)
     ap.add_argument("--batch", type=int, default=0, help="per-GPU batch (0: the config's default)")
     ap.add_argument("--curve-points", type=int, default=10, help="how many points of the loss curve to print")
+    ap.add_argument("--fused-blocks", action="store_true", help="GPT-2 blocks on this package's layer norm and linear layers")
+    ap.add_argument("--moment-bits", type=int, default=32, choices=[8, 32], help="of AdamW's moments")
     ap.add_argument("--optim-in-backward", action="store_true", help="AdamW per bucket behind its allreduce (native hook)")
     args = ap.parse_args(argv)
 
@@ -55,7 +57,7 @@ def main(argv=None):
                          torch.randint(0, 1000, (bs,), device=dev))
     else:
         big = args.model == "gpt2-medium"
-        model, bs, autocast = (models.gpt2_medium() if big else models.gpt2_tiny()).to(dev), args.batch or 8, True
+        model, bs, autocast = (models.gpt2_medium if big else models.gpt2_tiny)(fused=args.fused_blocks).to(dev), args.batch or 8, True
         vocab, seq = (50257, 1024) if big else (1024, 64)
 
         def batch():
@@ -65,7 +67,7 @@ def main(argv=None):
     pre_opt = None
     if args.impl == "mccl":
         if args.optim_in_backward and args.model != "resnet50" and args.compression == "none":
-            pre_opt = FusedAdamW(model.parameters(), lr=1e-3 if args.model == "mlp" else 3e-4)
+            pre_opt = FusedAdamW(model.parameters(), lr=1e-3 if args.model == "mlp" else 3e-4, state_bits=args.moment_bits)
         ddp = wrap_ddp(model, device_ids=[local], bucket_cap_mb=args.bucket_mb, compression=args.compression,
                        optimizer_in_backward=pre_opt)
         if args.compression == "topk":
@@ -79,7 +81,7 @@ def main(argv=None):
     elif pre_opt is not None:
         opt = pre_opt
     elif args.impl == "mccl":
-        opt = FusedAdamW(ddp.parameters(), lr=1e-3 if args.model == "mlp" else 3e-4)
+        opt = FusedAdamW(ddp.parameters(), lr=1e-3 if args.model == "mlp" else 3e-4, state_bits=args.moment_bits)
     else:
         opt = torch.optim.AdamW(ddp.parameters(), lr=1e-3 if args.model == "mlp" else 3e-4, fused=True)
     data = [batch() for _ in range(4)]
