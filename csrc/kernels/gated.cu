@@ -84,6 +84,12 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, in
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// Into this CTA's own shared memory, for this CTA alone.
+__device__ __forceinline__ void load_own_box(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x),
+               "r"(y), "r"(bar)
+               : "memory");
+}
 __device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t from, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(from) : "memory");
 }
@@ -428,78 +434,71 @@ struct LayerAhead {
     for (int i = 0; i < kN / 8; ++i) bias[i] = run_of<2>(l.bias + 2 * (col + 8 * i), l.cols - col - 8 * i, l.bias_vec);
   }
 };
-// A warp's residual of a turn, 32 rows of 64 columns, by whole runs of the rows, where a thread's own row would take 32 requests for each of its
-// runs (8192 x 1024 x 4096 with an fp32 residual 98 us so, MEASURED).  Its place in y's boxes is where y's numbers go.
-template <bool kWide>
+// A warp's residual of a turn, 32 rows of 64 columns, by whole runs of the rows, where a thread's own row would take 32 requests for each of its runs.
+// Its place in y's boxes is where y's numbers go.  In 16 bits it waits in registers until the boxes are free; in 32, where sums have the
+// registers, aligned rows come by themselves (load_own_box), others through here.
 struct LayerResidual {
-  static constexpr int kWords = kWide ? 64 : 32, kSize = kWide ? 4 : 2;
-  static constexpr int kLanes = kTurn * kSize / 16, kRowsAt = 32 / kLanes;  // lanes of a row, and rows a request, of aligned ones
+  static constexpr int kWords = 32, kLanes = kTurn * 2 / 16, kRowsAt = 32 / kLanes;  // lanes of a row, and rows a request, of aligned ones
   uint32_t w[kWords];
   // Rows from `row` on of `rows`, columns from `col` on.
   __device__ __forceinline__ void load(const Layer& l, int64_t row, int64_t rows, int64_t col, int lane) {
-    const char* from = l.residual + kSize * (row * l.ldr + col);
-    const int64_t n = l.cols - col, high = rows - row;
+    const char* from = l.residual + 2 * (row * l.ldr + col);
+    const int64_t n = l.cols - col;
+    const int high = static_cast<int>(min(rows - row, static_cast<int64_t>(32)));
     if (l.residual_vec) {
-      const int at = lane % kLanes * (16 / kSize);
+      const int at = lane % kLanes * 8, left = at < n ? high - lane / kLanes : 0;
+      const char* to = from + 2 * (lane / kLanes * l.ldr + at);
 #pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const int r = i * kRowsAt + lane / kLanes;
-        const uint4 v = r < high && at < n ? __ldcs(reinterpret_cast<const uint4*>(from + kSize * (r * l.ldr + at))) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < kWords / 4; ++i, to += 2 * kRowsAt * l.ldr) {
+        const uint4 v = i * kRowsAt < left ? __ldcs(reinterpret_cast<const uint4*>(to)) : make_uint4(0u, 0u, 0u, 0u);
         w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
       }
     } else {
-      const char* to = from + 2 * kSize * lane;  // two neighbours
+      const char* to = from + 4 * lane;  // two neighbours
       const bool one = 2 * lane < n, two = 2 * lane + 1 < n;
 #pragma unroll
-      for (int r = 0; r < 32; ++r, to += kSize * l.ldr) {
-        if constexpr (kWide) {
-          w[2 * r] = r < high && one ? reinterpret_cast<const uint32_t*>(to)[0] : 0u;
-          w[2 * r + 1] = r < high && two ? reinterpret_cast<const uint32_t*>(to)[1] : 0u;
-        } else {
-          const uint32_t a = r < high && one ? reinterpret_cast<const uint16_t*>(to)[0] : 0u, b = r < high && two ? reinterpret_cast<const uint16_t*>(to)[1] : 0u;
-          w[r] = a | b << 16;
-        }
-      }
-    }
-  }
-  // Calls `f` with each run's place behind the first of y's boxes and its words: 4 of them, 2 or 1.
-  template <typename Call>
-  __device__ __forceinline__ void places(bool vec, int lane, Call f) const {
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const int r = i * kRowsAt + lane / kLanes, run = lane % kLanes;
-        f(static_cast<uint32_t>(run / 8 * kBoxBytes + r * 128 + ((run % 8) ^ (r & 7)) * 16), w + 4 * i, std::integral_constant<int, 4>());
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        if constexpr (kWide) f(static_cast<uint32_t>(lane / 16 * kBoxBytes + r * 128 + ((lane % 16 / 2) ^ (r & 7)) * 16 + lane % 2 * 8), w + 2 * r, std::integral_constant<int, 2>());
-        else f(static_cast<uint32_t>(r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4), w + r, std::integral_constant<int, 1>());
+      for (int r = 0; r < 32; ++r, to += 2 * l.ldr) {
+        const uint32_t a = r < high && one ? reinterpret_cast<const uint16_t*>(to)[0] : 0u, b = r < high && two ? reinterpret_cast<const uint16_t*>(to)[1] : 0u;
+        w[r] = a | b << 16;
       }
     }
   }
   __device__ __forceinline__ void put(bool vec, int lane, uint32_t box) const {
-    places(vec, lane, [&](uint32_t at, const uint32_t* v, auto n) {
-      if constexpr (decltype(n)::value == 4) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-      else if constexpr (decltype(n)::value == 2) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(box + at), "r"(v[0]), "r"(v[1]) : "memory");
-      else asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + at), "r"(v[0]) : "memory");
-    });
-  }
-  // In 32 bits: added to what is there.
-  __device__ __forceinline__ void add(bool vec, int lane, uint32_t box) const {
-    places(vec, lane, [&](uint32_t at, const uint32_t* v, auto n) {
-      constexpr int kN = decltype(n)::value;
-      float y[4];
-      if constexpr (kN == 4) asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(box + at) : "memory");
-      else asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(y[0]), "=f"(y[1]) : "r"(box + at) : "memory");
+    if (vec) {
 #pragma unroll
-      for (int e = 0; e < kN; ++e) y[e] += __uint_as_float(v[e]);
-      if constexpr (kN == 4) asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + at), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]) : "memory");
-      else asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(box + at), "f"(y[0]), "f"(y[1]) : "memory");
-    });
+      for (int i = 0; i < kWords / 4; ++i) {
+        const int r = i * kRowsAt + lane / kLanes;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + r * 128 + ((lane % kLanes) ^ (r & 7)) * 16), "r"(w[4 * i]), "r"(w[4 * i + 1]),
+                     "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
+                     : "memory");
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4), "r"(w[r]) : "memory");
+    }
   }
 };
+// In 32 bits, rows that are not aligned: two neighbours a lane, eight rows at a time.
+__device__ __forceinline__ void put_residual(const Layer& l, int64_t row, int64_t rows, int64_t col, int lane, uint32_t box) {
+  const char* to = l.residual + 4 * (row * l.ldr + col + 2 * lane);
+  const int64_t n = l.cols - col - 2 * lane;
+  const int high = static_cast<int>(min(rows - row, static_cast<int64_t>(32)));
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    uint32_t v[16];
+#pragma unroll
+    for (int r = 0; r < 8; ++r, to += 4 * l.ldr) {
+      v[2 * r] = r0 + r < high && n > 0 ? reinterpret_cast<const uint32_t*>(to)[0] : 0u;
+      v[2 * r + 1] = r0 + r < high && n > 1 ? reinterpret_cast<const uint32_t*>(to)[1] : 0u;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(box + lane / 16 * kBoxBytes + (r0 + r) * 128 + ((lane % 16 / 2) ^ r) * 16 + lane % 2 * 8), "r"(v[2 * r]),
+                   "r"(v[2 * r + 1])
+                   : "memory");
+  }
+  __syncwarp();
+}
 template <bool kBf16>
 __device__ __forceinline__ void halves(const uint4& raw, float* v) {  // 8 numbers of 16 bits
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -508,6 +507,18 @@ __device__ __forceinline__ void halves(const uint4& raw, float* v) {  // 8 numbe
     const float2 f = kBf16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     v[2 * i] = f.x;
     v[2 * i + 1] = f.y;
+  }
+}
+// 8 columns of z as they are kept: beyond fp16's range slopes are what they are at its end.
+template <bool kBf16, typename Sink>
+__device__ __forceinline__ void put_z(const Sink& sink, int i, const float* z) {
+  if constexpr (kBf16) {
+    sink.put(0, i, z);
+  } else {
+    float kept[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) kept[e] = z[e] != z[e] ? z[e] : fminf(fmaxf(z[e], -65504.f), 65504.f);
+    sink.put(0, i, kept);
   }
 }
 // kN columns of x W^T to z and y.  `more`: adds the residual of 8 columns.
@@ -524,16 +535,7 @@ __device__ __forceinline__ void finish_layer(const Finish& f, float* z, const La
     }
   if constexpr (kKeep)
 #pragma unroll
-    for (int b = 0; b < kN; b += 8) {
-      if constexpr (kBf16) {
-        sink.put(0, i0 + b, z + b);
-      } else {  // beyond fp16's range slopes are what they are at its end
-        float kept[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) kept[e] = z[b + e] != z[b + e] ? z[b + e] : fminf(fmaxf(z[b + e], -65504.f), 65504.f);
-        sink.put(0, i0 + b, kept);
-      }
-    }
+    for (int b = 0; b < kN; b += 8) put_z<kBf16>(sink, i0 + b, z + b);
   with_activation(l.activation, [&](auto act) {
 #pragma unroll
     for (int e = 0; e < kN; ++e) z[e] = Act16::value<decltype(act)::kValue>(z[e]);
@@ -762,7 +764,7 @@ template <Out kOut, GatedKeep kKeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   constexpr int kDepths = kStages<kOut>, kOuts = kBoxes<kOut>;
   extern __shared__ char raw[];
-  __shared__ alignas(8) uint64_t bars[2 * kDepths + 5];
+  __shared__ alignas(8) uint64_t bars[2 * kDepths + 5 + (kAddsUp<kOut> ? kOutWarps : 0)];
   __shared__ uint32_t tmem_base;
   const uint32_t smem0 = (smem_addr(raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -783,6 +785,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
       bar_init(acc_free(b), 2 * kOutWarps);
     }
     bar_init(drained, 1);
+    if constexpr (kAddsUp<kOut>)
+      for (int i = 0; i < kOutWarps; ++i) bar_init(drained + 8u * (1 + i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kOwner) {
@@ -878,6 +882,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
     const int row = rank * kHalf + 32 * q + lane;
     const uint32_t boxes = smem0 + kDepths * kStage + (warp - kFirstOut) * (kOuts * kBoxBytes);
     int done = 0;
+    [[maybe_unused]] uint32_t phase = 0;  // of the residual's barrier
     for (int round = 0, item = pair; item < w.items; item = item_of(++round, pair, pairs, w.jobs), done += kAddsUp<kOut> ? 0 : 1) {
       const Item t(w, item);
       const Job& j = w.job[t.job];
@@ -885,26 +890,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
       const Spot at = spot_of<kOut>(j, t.ti, t.tj, row);
       Ahead<kOut, kKeep> ahead;
       if (t.part < 0 && at.col + share * kShare < j.cols) ahead.load(w.f, min(at.row, w.f.rows - 1), at.col + share * kShare);
-      [[maybe_unused]] LayerResidual<false> residual;
-      if constexpr (kAddsUp<kOut>) {
-        // (the residual itself has no registers before the sums are done: it comes nearer)
-        const Layer& l = w.f.layer;
-        if (t.part < 0 && l.residual != nullptr && at.row < w.f.rows)
-#pragma unroll
-          for (int i = 0; i < kShare; i += 32)
-            if (at.col + share * kShare + i < l.cols)
-              asm volatile("prefetch.global.L2 [%0];" ::"l"(l.residual + 4 * (at.row * l.ldr + at.col + share * kShare + i)));
-      }
+      [[maybe_unused]] LayerResidual residual;
       if constexpr (kIsLayer<kOut> && !kAddsUp<kOut>)
         if (t.part < 0 && w.f.layer.residual != nullptr) residual.load(w.f.layer, at.row - lane, w.f.rows, at.col + share * kShare, lane);
       if constexpr (kAddsUp<kOut>) {
+        constexpr int kY = kKeepsZ<kOut> ? 1 : 0;
+        const Layer& l = w.f.layer;
+        const int first = share * kShare, last = static_cast<int>(min(static_cast<int64_t>(first + kShare), j.cols - at.col));
+        const int64_t y = at.row - lane;  // the warp's first row
+        const uint32_t came = drained + 8u * (1 + warp - kFirstOut), y_boxes = boxes + kY * kBoxBytes;
+        // The residual of 64 columns to where y's numbers will be; the first ones' while the products still run.
+        auto ask = [&](int c) {
+          if (lane == 0) {
+            stores_left();
+            if (l.residual_vec && y < j.rows) {
+              const int x = static_cast<int>(at.col) + c, two = c + 32 < last;
+              bar_expect(came, (1 + two) * kBoxBytes);
+              load_own_box(y_boxes, &j.out[2], x, static_cast<int>(y), came);
+              if (two) load_own_box(y_boxes + kBoxBytes, &j.out[2], x + 32, static_cast<int>(y), came);
+            }
+          }
+          __syncwarp();
+          if (!l.residual_vec) put_residual(l, y, j.rows, at.col + c, lane, y_boxes);
+        };
+        if (t.part < 0 && first < last) ask(first);
         float sum[kShare];
 #pragma unroll
         for (int i = 0; i < kShare; ++i) sum[i] = 0.f;
         for (int c = t.c0; c < t.c1; c += kChunk<kOut>, ++done) {
           if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_full(done & 1), (done >> 1) & 1, w.limit));
           fence_after();
-          const uint32_t from = tmem + (done & 1) * kTile + share * kShare + (static_cast<uint32_t>(32 * q) << 16);
+          const uint32_t from = tmem + (done & 1) * kTile + first + (static_cast<uint32_t>(32 * q) << 16);
 #pragma unroll
           for (int i = 0; i < kShare; i += kN) {
             float v[kN];
@@ -920,34 +936,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           if (lane == 0 && ok) bar_arrive_cluster(in_leader(acc_free(done & 1)));
         }
         if (t.part < 0) {
-          const int first = share * kShare, last = static_cast<int>(min(static_cast<int64_t>(first + kShare), j.cols - at.col));
+          const Staged<true> own(boxes, lane);
 #pragma unroll
           for (int turn = 0; turn < kShare; turn += kTurn) {
             const int c = first + turn;
             if (c >= last) break;
-            if (lane == 0) stores_left();
-            __syncwarp();
-            // the sums wait in y's boxes, so that what follows is one loop and not eight copies of it
-            constexpr int kY = kKeepsZ<kOut> ? 1 : 0;
-            const Staged<true> own(boxes, lane);
+            if (turn > 0) ask(c);
+            float* const v = sum + turn;
+            if (l.bias != nullptr)
 #pragma unroll
-            for (int i = 0; i < kTurn; i += 8) own.put_f32(kY, i, sum + turn + i);
-            auto taken = [&](int col, float* v) {
+              for (int i = 0; i < kTurn; i += 8) {
+                float bias[8];
+                const uint4 raw = run_of<2>(l.bias + 2 * (at.col + c + i), l.cols - at.col - c - i, l.bias_vec);
+                if (w.f.bf16) halves<true>(raw, bias);
+                else halves<false>(raw, bias);
 #pragma unroll
-              for (int e = 0; e < kN; e += 8) own.get_f32(kY, col - c + e, v + e);
-            };
-            LayerResidual<true> residual;
-            if (w.f.layer.residual != nullptr) residual.load(w.f.layer, at.row - lane, w.f.rows, at.col + c, lane);
-            if (w.f.bf16) finish_turn<kOut, kKeep, true, kTurn>(w.f, at, c, last, ahead, taken, Staged<true>(boxes, lane));
-            else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, taken, Staged<false>(boxes, lane));
-            if (w.f.layer.residual != nullptr) {
-              __syncwarp();
-              residual.add(w.f.layer.residual_vec, lane, boxes + kY * kBoxBytes);
+                for (int e = 0; e < 8; ++e) v[i + e] += bias[e];
+              }
+            if constexpr (kKeepsZ<kOut>)
+#pragma unroll
+              for (int i = 0; i < kTurn; i += 8) {
+                if (w.f.bf16) put_z<true>(Staged<true>(boxes, lane), i, v + i);
+                else put_z<false>(Staged<false>(boxes, lane), i, v + i);
+              }
+            if (l.activation != LayerActivation::kNone)
+              with_activation(l.activation, [&](auto act) {
+#pragma unroll
+                for (int e = 0; e < kTurn; ++e) v[e] = Act16::value<decltype(act)::kValue>(v[e]);
+              });
+            if (l.residual_vec && y < j.rows) {
+              ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(came, phase, w.limit));
+              phase ^= 1;
             }
-            flush_layer<kOut>(j, at, c, last, at.row - lane, boxes, lane);
+#pragma unroll
+            for (int i = 0; i < kTurn; i += 8) {
+              float r[8];
+              own.get_f32(kY, i, r);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) r[e] = ok ? v[i + e] + r[e] : NAN;
+              own.put_f32(kY, i, r);
+            }
+            flush_layer<kOut>(j, at, c, last, y, boxes, lane);
           }
         } else if (at.row < j.rows) {
-          float* to = w.partial + static_cast<int64_t>(t.part) * (kTile * kTile) + row + static_cast<int64_t>(share) * kShare * kTile;
+          float* to = w.partial + static_cast<int64_t>(t.part) * (kTile * kTile) + row + static_cast<int64_t>(first) * kTile;
 #pragma unroll
           for (int i = 0; i < kShare; ++i) __stcg(to + static_cast<int64_t>(i) * kTile, sum[i]);
         }
@@ -1396,6 +1428,10 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
   return cudaLaunchKernelEx(&cfg, gated_join_kernel<kOut, kKeep>, w);
 }
 
+bool residual_aligned(const LayerFinish& f, int64_t cols) {
+  const int64_t size = f.y_f32 ? 4 : 2;
+  return cols * size % 16 == 0 && f.ldr * size % 16 == 0 && (!f.y_f32 || f.ldr >= cols) && reinterpret_cast<uintptr_t>(f.residual) % 16 == 0;
+}
 // A product's maps and shape.
 bool make_job(Job& j, const GatedArgs& g, const GatedShape& h, const LayerFinish* layer) {
   const Sizes z = sizes_of(g.product, h);
@@ -1423,6 +1459,10 @@ bool make_job(Job& j, const GatedArgs& g, const GatedShape& h, const LayerFinish
   if (g.product == GatedProduct::kLayer) {
     const int64_t size = layer->y_f32 ? 4 : 2;
     j.wide = j.ldo * size % 16 == 0 && reinterpret_cast<uintptr_t>(g.out0) % 16 == 0;
+    if (layer->y_f32 && layer->residual == nullptr) return false;
+    if (layer->y_f32 && residual_aligned(*layer, h.width) &&
+        !make_map(&j.out[2], {layer->residual, layer->ldr}, j.cols, z.rows, kResultRows, h.bf16, true))
+      return false;
     return g.out0 != nullptr && (!j.wide || make_map(&j.out[0], {g.out0, j.ldo}, j.cols, z.rows, kResultRows, h.bf16, layer->y_f32)) &&
            (g.out1 == nullptr || make_map(&j.out[1], {g.out1, gated_row(h.width)}, gated_row(h.width), z.rows, kResultRows, h.bf16));
   }
@@ -1538,7 +1578,6 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
   w.f.pitch = gated_pitch(h.hidden);
   if (r.layer != nullptr) {
     const LayerFinish& f = *r.layer;
-    const int64_t size = f.y_f32 ? 4 : 2;
     w.f.pitch = gated_row(h.width);
     Layer& l = w.f.layer;
     l.activation = f.activation;
@@ -1547,7 +1586,7 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
     l.ldr = f.ldr;
     l.cols = h.width;
     l.bias_vec = h.width % 8 == 0 && reinterpret_cast<uintptr_t>(f.bias) % 16 == 0;
-    l.residual_vec = h.width * size % 16 == 0 && f.ldr * size % 16 == 0 && reinterpret_cast<uintptr_t>(f.residual) % 16 == 0;
+    l.residual_vec = residual_aligned(f, h.width);
   }
   w.partial = r.partial;
   w.failed = r.failed;
