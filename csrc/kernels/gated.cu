@@ -8,7 +8,6 @@
 // with 16 significant bits (three bytes; rounded to bf16 they would put two more roundings into every gradient: 2.0 times the
 // error of a result that is rounded once, where it is 1.4 so) or, where asked for, as 8-bit codes.  A linear layer keeps z = x W^T + b in 16
 // bits: only the activation's slope is taken of it, which moves less than z does (1.45 times the error for 1.41).
-#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -19,7 +18,7 @@
 #include "kernels/elems.cuh"
 #include "kernels/gated_api.h"
 #include "kernels/launch_count.h"
-#include "kernels/layer_act.cuh"
+#include "kernels/layer_epilogue.cuh"
 
 namespace mccl {
 namespace kern {
@@ -34,41 +33,11 @@ constexpr int kColumns = 512;            // of tensor memory: two accumulators
 // warp 0 loads, warp 1 issues products, warp 2 has the tensor memory, the warps from 4 on take the accumulators out
 constexpr int kLoader = 0, kIssuer = 1, kOwner = 2, kFirstOut = 4, kOutWarps = 8, kThreads = 32 * (kFirstOut + kOutWarps);
 
-// ---- PTX ----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
+// ---- PTX of pairs of CTAs (tensor_pipe.cuh has the rest) ------------------------------------------------------
 // (What it orders is tensor memory, for which there are fences of its own: a release at cluster scope would wait for all of the
 // warp's stores, a microsecond or two a tile.)
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-// Waits for the phase of that parity, for four times `limit` cycles at most.  A pause of the whole device (another process has it, a
-// debugger stopped it) uses up one of the four.
-constexpr long long kWaitLimit = 500000000ll, kLanding = 2000000ll;  // about a quarter of a second and a millisecond
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long long limit) {
-  if (bar_try(bar, parity)) return true;
-#pragma unroll 1
-  for (int left = 4; left > 0; --left) {
-    const long long begin = clock64();
-    do {
-      if (bar_try(bar, parity)) return true;
-    } while (clock64() - begin <= limit);
-  }
-  return false;
 }
 __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
   uint32_t r;
@@ -84,27 +53,6 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, in
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-// Into this CTA's own shared memory, for this CTA alone.
-__device__ __forceinline__ void load_own_box(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x),
-               "r"(y), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t from, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(from) : "memory");
-}
-__device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// All of this thread's groups have left shared memory; are done.
-__device__ __forceinline__ void stores_left() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-// Shared-memory matrix descriptors, 128-byte swizzle.  k innermost: rows of 128 bytes (64 k), 1024 bytes per eight rows.  Own
-// index innermost: rows of 128 bytes (64 of the index, one k), 1024 bytes per eight k, 8192 from 64 of the index to the next.
-__device__ __forceinline__ uint64_t make_desc(uint32_t addr, bool inner) {
-  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(inner ? 1 : 8192 >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// from 16 k to the next, in descriptor units
-__device__ __forceinline__ uint32_t step_of(bool inner) { return (inner ? 32 : 2048) >> 4; }
 __device__ __forceinline__ uint32_t make_idesc(bool bf16, bool a_inner, bool b_inner) {
   const uint32_t type = bf16 ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | (a_inner ? 0u : 1u << 15) | (b_inner ? 0u : 1u << 16) |
@@ -122,44 +70,6 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
                "h"(static_cast<uint16_t>(3))
                : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// kN consecutive columns of the calling thread's lane, which are there behind the wait: its operands keep whatever uses them from
-// moving before it.
-template <int kN>
-__device__ __forceinline__ void tmem_load(uint32_t addr, float* v) {
-  static_assert(kN == 16 || kN % 32 == 0, "runs of 16 or 32 columns");
-  if constexpr (kN == 16) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-                   "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-                 : "r"(addr));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kN; i += 32, v += 32)
-      asm volatile(
-          "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-          "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-          : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-            "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]),
-            "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]),
-            "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-          : "r"(addr + i));
-  }
-}
-template <int kN>
-__device__ __forceinline__ void tmem_wait(float* v) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < kN; i += 16, v += 16)
-    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
-                     "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
-}
-__device__ __forceinline__ bool elect() {
-  uint32_t one;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
-  return one != 0;
 }
 
 // ---- what a launch is told ----------------------------------------------------------------------------------
@@ -201,12 +111,6 @@ constexpr int kChunk = kAddsUp<kOut> ? 8 : 1 << 30;
 constexpr int kLaunched = 168, kKept = 56, kTaken = 224;
 static_assert(4 * kKept + kOutWarps * kTaken <= (kFirstOut + kOutWarps) * kLaunched, "a split of more than there are waits forever");
 
-struct Layer {
-  LayerActivation activation;
-  const char *bias, *residual;
-  int64_t ldr, cols;
-  bool bias_vec, residual_vec;  // aligned to 16 bytes, whole runs of them
-};
 struct Finish {
   bool bf16;
   Curve curve;
@@ -281,12 +185,6 @@ __device__ __forceinline__ int item_of(int round, int pair, int pairs, int jobs)
 }
 
 // ---- after the product --------------------------------------------------------------------------------------
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (kBf16) return store_pair<__nv_bfloat16>(a, b);
-  else return store_pair<__half>(a, b);
-}
-
 // Floats of three bytes: the upper 24 bits, rounded to nearest; infinities and NaN cut off.
 __device__ __forceinline__ uint32_t three_bytes(float x) {
   const uint32_t b = __float_as_uint(x);
@@ -336,7 +234,6 @@ __device__ __forceinline__ void take_wide(const uint4& up, const uint2& low, flo
 // Where 8 numbers of a thread's row go, `i` columns from where it is: straight to memory, which costs a request for each row (the
 // joining kernel), or to the warp's boxes of 32 rows and 64 columns in shared memory, 128-byte swizzle,
 // which then leave as a whole.  (Straight to memory kGate took 99 us of 8192 x 1024 x 2816, bound by its requests.)
-constexpr int kTurn = 64, kBoxBytes = 32 * kTurn * 2;
 template <bool kBf16>
 struct Direct {
   uint16_t* out[3];
@@ -345,42 +242,6 @@ struct Direct {
     if (i < left)
       *reinterpret_cast<uint4*>(out[which] + i) =
           make_uint4(pack2<kBf16>(v[0], v[1]), pack2<kBf16>(v[2], v[3]), pack2<kBf16>(v[4], v[5]), pack2<kBf16>(v[6], v[7]));
-  }
-};
-template <bool kBf16>
-struct Staged {
-  uint32_t row;       // of the first box
-  int swizzle;
-  __device__ __forceinline__ Staged(uint32_t boxes, int lane) : row(boxes + lane * 128), swizzle(lane & 7) {}
-  __device__ __forceinline__ void put(int which, int i, const float* v) const {
-    const uint32_t to = row + which * kBoxBytes + ((i / 8) ^ swizzle) * 16;
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pack2<kBf16>(v[0], v[1])), "r"(pack2<kBf16>(v[2], v[3])),
-                 "r"(pack2<kBf16>(v[4], v[5])), "r"(pack2<kBf16>(v[6], v[7]))
-                 : "memory");
-  }
-  __device__ __forceinline__ uint4 get(int which, int i) const {  // 8 numbers as they were put
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(row + which * kBoxBytes + ((i / 8) ^ swizzle) * 16)
-                 : "memory");
-    return v;
-  }
-  // In 32 bits: boxes of 32 columns, from the `which`th on.
-  __device__ __forceinline__ void put_f32(int which, int i, const float* v) const {
-    const uint32_t box = row + (which + i / 32) * kBoxBytes;
-#pragma unroll
-    for (int e = 0; e < 8; e += 4)
-      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + ((((i % 32) + e) / 4) ^ swizzle) * 16), "f"(v[e]), "f"(v[e + 1]), "f"(v[e + 2]),
-                   "f"(v[e + 3])
-                   : "memory");
-  }
-  __device__ __forceinline__ void get_f32(int which, int i, float* v) const {  // as they were put
-    const uint32_t box = row + (which + i / 32) * kBoxBytes;
-#pragma unroll
-    for (int e = 0; e < 8; e += 4)
-      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[e]), "=f"(v[e + 1]), "=f"(v[e + 2]), "=f"(v[e + 3])
-                   : "r"(box + ((((i % 32) + e) / 4) ^ swizzle) * 16)
-                   : "memory");
   }
 };
 // The joining kernel's of a linear layer: number by number where rows are not aligned.
@@ -409,20 +270,6 @@ struct DirectLayer {
       if (i + e < left) to[e] = v[e];
   }
 };
-// 16 bytes from `from` on, numbers of kSize bytes of which there are `n`.
-template <int kSize>
-__device__ __forceinline__ uint4 run_of(const char* from, int64_t n, bool vec) {
-  constexpr int kPer = 16 / kSize;
-  if (vec) return n > 0 ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (i < n) {
-      if constexpr (kSize == 4) w[i] = reinterpret_cast<const uint32_t*>(from)[i];
-      else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[i]) << (16 * (i % 2));
-    }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 // The bias of kN columns, which is the same for all rows, as it lies in memory.
 template <int kN>
 struct LayerAhead {
@@ -434,93 +281,6 @@ struct LayerAhead {
     for (int i = 0; i < kN / 8; ++i) bias[i] = run_of<2>(l.bias + 2 * (col + 8 * i), l.cols - col - 8 * i, l.bias_vec);
   }
 };
-// A warp's residual of a turn, 32 rows of 64 columns, by whole runs of the rows, where a thread's own row would take 32 requests for each of its runs.
-// Its place in y's boxes is where y's numbers go.  In 16 bits it waits in registers until the boxes are free; in 32, where sums have the
-// registers, aligned rows come by themselves (load_own_box), others through here.
-struct LayerResidual {
-  static constexpr int kWords = 32, kLanes = kTurn * 2 / 16, kRowsAt = 32 / kLanes;  // lanes of a row, and rows a request, of aligned ones
-  uint32_t w[kWords];
-  // Rows from `row` on of `rows`, columns from `col` on.
-  __device__ __forceinline__ void load(const Layer& l, int64_t row, int64_t rows, int64_t col, int lane) {
-    const char* from = l.residual + 2 * (row * l.ldr + col);
-    const int64_t n = l.cols - col;
-    const int high = static_cast<int>(min(rows - row, static_cast<int64_t>(32)));
-    if (l.residual_vec) {
-      const int at = lane % kLanes * 8, left = at < n ? high - lane / kLanes : 0;
-      const char* to = from + 2 * (lane / kLanes * l.ldr + at);
-#pragma unroll
-      for (int i = 0; i < kWords / 4; ++i, to += 2 * kRowsAt * l.ldr) {
-        const uint4 v = i * kRowsAt < left ? __ldcs(reinterpret_cast<const uint4*>(to)) : make_uint4(0u, 0u, 0u, 0u);
-        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-      }
-    } else {
-      const char* to = from + 4 * lane;  // two neighbours
-      const bool one = 2 * lane < n, two = 2 * lane + 1 < n;
-#pragma unroll
-      for (int r = 0; r < 32; ++r, to += 2 * l.ldr) {
-        const uint32_t a = r < high && one ? reinterpret_cast<const uint16_t*>(to)[0] : 0u, b = r < high && two ? reinterpret_cast<const uint16_t*>(to)[1] : 0u;
-        w[r] = a | b << 16;
-      }
-    }
-  }
-  __device__ __forceinline__ void put(bool vec, int lane, uint32_t box) const {
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const int r = i * kRowsAt + lane / kLanes;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + r * 128 + ((lane % kLanes) ^ (r & 7)) * 16), "r"(w[4 * i]), "r"(w[4 * i + 1]),
-                     "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
-                     : "memory");
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 32; ++r) asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4), "r"(w[r]) : "memory");
-    }
-  }
-};
-// In 32 bits, rows that are not aligned: two neighbours a lane, eight rows at a time.
-__device__ __forceinline__ void put_residual(const Layer& l, int64_t row, int64_t rows, int64_t col, int lane, uint32_t box) {
-  const char* to = l.residual + 4 * (row * l.ldr + col + 2 * lane);
-  const int64_t n = l.cols - col - 2 * lane;
-  const int high = static_cast<int>(min(rows - row, static_cast<int64_t>(32)));
-#pragma unroll 1
-  for (int r0 = 0; r0 < 32; r0 += 8) {
-    uint32_t v[16];
-#pragma unroll
-    for (int r = 0; r < 8; ++r, to += 4 * l.ldr) {
-      v[2 * r] = r0 + r < high && n > 0 ? reinterpret_cast<const uint32_t*>(to)[0] : 0u;
-      v[2 * r + 1] = r0 + r < high && n > 1 ? reinterpret_cast<const uint32_t*>(to)[1] : 0u;
-    }
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(box + lane / 16 * kBoxBytes + (r0 + r) * 128 + ((lane % 16 / 2) ^ r) * 16 + lane % 2 * 8), "r"(v[2 * r]),
-                   "r"(v[2 * r + 1])
-                   : "memory");
-  }
-  __syncwarp();
-}
-template <bool kBf16>
-__device__ __forceinline__ void halves(const uint4& raw, float* v) {  // 8 numbers of 16 bits
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = kBf16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-// 8 columns of z as they are kept: beyond fp16's range slopes are what they are at its end.
-template <bool kBf16, typename Sink>
-__device__ __forceinline__ void put_z(const Sink& sink, int i, const float* z) {
-  if constexpr (kBf16) {
-    sink.put(0, i, z);
-  } else {
-    float kept[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) kept[e] = z[e] != z[e] ? z[e] : fminf(fmaxf(z[e], -65504.f), 65504.f);
-    sink.put(0, i, kept);
-  }
-}
 // kN columns of x W^T to z and y.  `more`: adds the residual of 8 columns.
 template <bool kKeep, bool kWide, bool kBf16, int kN, typename Sink, typename More>
 __device__ __forceinline__ void finish_layer(const Finish& f, float* z, const LayerAhead<kN>& now, const Sink& sink, int i0, const More& more) {
@@ -713,44 +473,6 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
     }
   }
 }
-// The boxes of 64 columns from `c` of the tile on, of the warp's rows from `y` on, to z and y.
-template <Out kOut>
-__device__ __forceinline__ void flush_layer(const Job& j, const Spot& at, int c, int last, int64_t y, uint32_t boxes, int lane) {
-              constexpr int kFirst = kKeepsZ<kOut> ? 1 : 0;  // y's boxes behind z's
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0) {
-                if (y < j.rows) {
-                  const int x = static_cast<int>(at.col) + c;
-                  if constexpr (kKeepsZ<kOut>) store_box(&j.out[1], boxes, x, static_cast<int>(y));
-                  if (j.wide) {
-                    store_box(&j.out[0], boxes + kFirst * kBoxBytes, x, static_cast<int>(y));
-                    if (kWideY<kOut> && c + 32 < last) store_box(&j.out[0], boxes + (kFirst + 1) * kBoxBytes, x + 32, static_cast<int>(y));
-                  }
-                }
-                stores_commit();
-              }
-              if (!j.wide) {  // rows that are not aligned: two numbers a lane, row by row
-                const int n = static_cast<int>(min(static_cast<int64_t>(32), j.rows - y)), here = last - c - 2 * lane;
-                char* to = static_cast<char*>(j.to[0]) + (y * j.ldo + at.col + c + 2 * lane) * (kWideY<kOut> ? 4 : 2);
-#pragma unroll 4
-                for (int r = 0; r < n; ++r, to += j.ldo * (kWideY<kOut> ? 4 : 2)) {
-                  uint32_t v[2];
-                  if constexpr (kWideY<kOut>) {
-                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1])
-                                 : "r"(boxes + (kFirst + lane / 16) * kBoxBytes + r * 128 + ((lane % 16 / 2) ^ (r & 7)) * 16 + lane % 2 * 8));
-                    if (here > 0) reinterpret_cast<uint32_t*>(to)[0] = v[0];
-                    if (here > 1) reinterpret_cast<uint32_t*>(to)[1] = v[1];
-                  } else {
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(boxes + kFirst * kBoxBytes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
-                    if (here > 0) reinterpret_cast<uint16_t*>(to)[0] = static_cast<uint16_t>(v[0]);
-                    if (here > 1) reinterpret_cast<uint16_t*>(to)[1] = static_cast<uint16_t>(v[0] >> 16);
-                  }
-                }
-                __syncwarp();
-              }
-}
-
 // A pair of CTAs per tile of 256 x 256, tiles in turn: each CTA loads half of either operand's rows and has half of the
 // accumulator's; the first one issues the products of both.  Two accumulators, so that a tile is taken out while the next one
 // is multiplied.  A stage is 64 KB for 8.4 million multiplications: what passes through the second-level cache, 13.5 TB/s of it, bounds
@@ -976,7 +698,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
               for (int e = 0; e < 8; ++e) r[e] = ok ? v[i + e] + r[e] : NAN;
               own.put_f32(kY, i, r);
             }
-            flush_layer<kOut>(j, at, c, last, y, boxes, lane);
+            flush_layer<kKeepsZ<kOut>, kWideY<kOut>>(LayerTarget{&j.out[0], &j.out[1], j.to[0], j.ldo, j.rows, j.wide}, at.col + c, last - c, y, boxes, lane);
           }
         } else if (at.row < j.rows) {
           float* to = w.partial + static_cast<int64_t>(t.part) * (kTile * kTile) + row + static_cast<int64_t>(first) * kTile;
@@ -1032,7 +754,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
             else finish_turn<kOut, kKeep, false, kTurn>(w.f, at, c, last, ahead, fetch, Staged<false>(boxes, lane));
           }
           if constexpr (kIsLayer<kOut>) {
-            flush_layer<kOut>(j, at, c, last, y, boxes, lane);
+            flush_layer<kKeepsZ<kOut>, kWideY<kOut>>(LayerTarget{&j.out[0], &j.out[1], j.to[0], j.ldo, j.rows, j.wide}, at.col + c, last - c, y, boxes, lane);
           } else if (kOut != kStore || j.wide) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -1349,36 +1071,6 @@ bool plan_together(const GatedProduct* p, const GatedShape& s, int n, Plan* l, i
   return 1.05 * static_cast<double>(most) + (joins ? 12.0 : 4.0) / kStageUs < alone;
 }
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return fn;
-}
-// A matrix of `outer` rows of `inner` numbers in boxes of 64 of a row and of `box_rows` rows: read, of 128 (k innermost; of tokens fewer
-// where there are fewer: a box's rows beyond the matrix take time, 73 us for 67 of 12 tokens of 4096 x 10240, 279 for 236 of 3 of 8192 x
-// 24576; what lies below in shared memory are rows of nobody's) or 64 (own index innermost); written, of 32.
-constexpr uint32_t kOwnRows = 64, kResultRows = 32;
-uint32_t rows_read(int64_t rows) {
-  uint32_t n = 8;
-  while (n < rows && n < kHalf) n *= 2;
-  return n;
-}
-bool make_map(CUtensorMap* map, const GatedOperand& m, int64_t inner, int64_t outer, uint32_t box_rows, bool bf16, bool f32 = false) {
-  const int64_t size = f32 ? 4 : 2;
-  if (m.data == nullptr || reinterpret_cast<uintptr_t>(m.data) % 16 != 0 || m.ld * size % 16 != 0 || m.ld < inner || inner > 0x7FFFFFFF || outer > 0x7FFFFFFF) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)}, strides[1] = {static_cast<cuuint64_t>(m.ld * size)};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), box_rows}, one[2] = {1, 1};
-  return encode_tiled()(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(m.data), dims, strides, box, one,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <Out kOut, GatedKeep kKeep>
 cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_t s) {
   Work<kJobs<kOut>> w;
@@ -1428,10 +1120,6 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
   return cudaLaunchKernelEx(&cfg, gated_join_kernel<kOut, kKeep>, w);
 }
 
-bool residual_aligned(const LayerFinish& f, int64_t cols) {
-  const int64_t size = f.y_f32 ? 4 : 2;
-  return cols * size % 16 == 0 && f.ldr * size % 16 == 0 && (!f.y_f32 || f.ldr >= cols) && reinterpret_cast<uintptr_t>(f.residual) % 16 == 0;
-}
 // A product's maps and shape.
 bool make_job(Job& j, const GatedArgs& g, const GatedShape& h, const LayerFinish* layer) {
   const Sizes z = sizes_of(g.product, h);
@@ -1577,16 +1265,8 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
   w.f.rows = h.tokens;
   w.f.pitch = gated_pitch(h.hidden);
   if (r.layer != nullptr) {
-    const LayerFinish& f = *r.layer;
     w.f.pitch = gated_row(h.width);
-    Layer& l = w.f.layer;
-    l.activation = f.activation;
-    l.bias = static_cast<const char*>(f.bias);
-    l.residual = static_cast<const char*>(f.residual);
-    l.ldr = f.ldr;
-    l.cols = h.width;
-    l.bias_vec = h.width % 8 == 0 && reinterpret_cast<uintptr_t>(f.bias) % 16 == 0;
-    l.residual_vec = residual_aligned(f, h.width);
+    w.f.layer = layer_of(*r.layer, h.width);
   }
   w.partial = r.partial;
   w.failed = r.failed;

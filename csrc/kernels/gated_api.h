@@ -133,6 +133,20 @@ struct LayerFew {
 };
 cudaError_t launch_layer_few(const LayerFew& g, cudaStream_t s);
 
+// A layer of some tens or hundreds of rows, on smaller tiles (kernels/linear_tiles.cu).  layer_tile: their columns, or 0 where they would be more than
+// one for each SM and launch_gated's kLayer takes the product.
+int layer_tile(int64_t tokens, int64_t in, int64_t out);
+struct LayerTiles {
+  int64_t tokens, in, out;
+  bool bf16;  // else fp16
+  GatedOperand x, weight;  // aligned to 16 bytes
+  LayerFinish finish;
+  void *y, *z;            // as kLayer's
+  uint32_t* failed;
+  int64_t wait_limit;
+};
+cudaError_t launch_layer_tiles(const LayerTiles& g, cudaStream_t s);
+
 // What stands around the products, in one pass each (kernels/linear_pass.cu).  Rows `ld` numbers apart of one type.
 struct LayerRows {
   const void* data;

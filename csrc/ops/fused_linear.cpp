@@ -77,6 +77,11 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
   Operands m;
   const int ox = m.add(x), ow = m.add(w);
   m.copy(x);
+  if (kern::layer_tile(tokens, w.size(1), out) > 0) {
+    const kern::LayerTiles tiles{tokens, w.size(1), out, s.bf16, m[ox], m[ow], finish, y.data_ptr(), z != nullptr ? z->data_ptr() : nullptr, wait_status(x), wait_limit};
+    OPS_CK(kern::launch_layer_tiles(tiles, at::cuda::getCurrentCUDAStream()));
+    return y;
+  }
   Products run(s, x, wait_limit);
   run.r.layer = &finish;
   const kern::GatedArgs g{GatedProduct::kLayer, m[ox], {}, m[ow], {}, y.data_ptr(), z != nullptr ? z->data_ptr() : nullptr, nullptr, out};

@@ -70,6 +70,7 @@ CUDA_SOURCES = [
     "kernels/gate_f32.cu",
     "kernels/linear_few.cu",
     "kernels/linear_pass.cu",
+    "kernels/linear_tiles.cu",
     "kernels/norm_forward.cu",
     "kernels/norm_backward.cu",
     "kernels/noalloc.cu",
