@@ -18,15 +18,19 @@ namespace {
 constexpr int kRows = 128, kDepth = 64, kSms = 148;     // of a tile; k per stage
 constexpr int kRowBytes = kRows * kDepth * 2;           // of x's part of a stage
 constexpr int kChunk = 8;                               // stages that are added up in tensor memory
-constexpr int kOutWarps = 4, kFirstOut = 2, kThreads = 32 * (kFirstOut + kOutWarps);
+constexpr int kFirstOut = 2;
+template <int kN>
+constexpr int kOutWarps = kRows / 32 * (kN / kTurn);         // each has 32 rows and 64 columns
+template <int kN>
+constexpr int kThreads = 32 * (kFirstOut + kOutWarps<kN>);
 template <int kN>
 constexpr int kStageBytes = kRowBytes + kN * kDepth * 2;
 template <bool kKeep, bool kWide>
 constexpr int kBoxes = (kKeep ? 1 : 0) + (kWide ? 2 : 1);
 template <int kN, bool kKeep, bool kWide>
-constexpr int kStages = (226 * 1024 - kOutWarps * kBoxes<kKeep, kWide> * kBoxBytes) / kStageBytes<kN>;  // as many as there is room for
+constexpr int kStages = (226 * 1024 - kOutWarps<kN> * kBoxes<kKeep, kWide> * kBoxBytes) / kStageBytes<kN>;  // as many as there is room for
 template <int kN, bool kKeep, bool kWide>
-constexpr int kSmem = kStages<kN, kKeep, kWide> * kStageBytes<kN> + kOutWarps * kBoxes<kKeep, kWide> * kBoxBytes + 1024;
+constexpr int kSmem = kStages<kN, kKeep, kWide> * kStageBytes<kN> + kOutWarps<kN> * kBoxes<kKeep, kWide> * kBoxBytes + 1024;
 
 struct Tiles {
   CUtensorMap x, w, y, z, residual;
@@ -54,10 +58,10 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 template <int kN, bool kKeep, bool kWide, bool kBf16>
-__global__ void __launch_bounds__(kThreads, 1) layer_tiles_kernel(const __grid_constant__ Tiles w) {
+__global__ void __launch_bounds__(kThreads<kN>, 1) layer_tiles_kernel(const __grid_constant__ Tiles w) {
   constexpr int kDepths = kStages<kN, kKeep, kWide>, kStage = kStageBytes<kN>, kOuts = kBoxes<kKeep, kWide>, kY = kKeep ? 1 : 0, kColumns = 2 * kN;
   extern __shared__ char raw[];
-  __shared__ alignas(8) uint64_t bars[2 * kDepths + 5 + kOutWarps];
+  __shared__ alignas(8) uint64_t bars[2 * kDepths + 5 + kOutWarps<kN>];
   __shared__ uint32_t tmem_base;
   const uint32_t smem0 = (smem_addr(raw) + 1023u) & ~1023u, bar0 = smem_addr(bars);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -73,9 +77,9 @@ __global__ void __launch_bounds__(kThreads, 1) layer_tiles_kernel(const __grid_c
     }
     for (int b = 0; b < 2; ++b) {
       bar_init(acc_full(b), 1);
-      bar_init(acc_free(b), kOutWarps);
+      bar_init(acc_free(b), kOutWarps<kN>);
     }
-    for (int i = 0; i <= kOutWarps; ++i) bar_init(drained + 8u * i, 1);
+    for (int i = 0; i <= kOutWarps<kN>; ++i) bar_init(drained + 8u * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -140,71 +144,58 @@ __global__ void __launch_bounds__(kThreads, 1) layer_tiles_kernel(const __grid_c
     // lanes 32 q .. 32 q + 31 of tensor memory are open to the warps with warp % 4 == q
     const int q = warp & 3;
     const Layer& l = w.layer;
-    const int64_t col0 = static_cast<int64_t>(tj) * kN, y = static_cast<int64_t>(ti) * kRows + 32 * q, rows = w.target.rows;
-    const int last = static_cast<int>(min(static_cast<int64_t>(kN), w.cols - col0));
+    const int share = (warp - kFirstOut) / 4 * kTurn;
+    const int64_t col = static_cast<int64_t>(tj) * kN + share, y = static_cast<int64_t>(ti) * kRows + 32 * q, rows = w.target.rows;
+    const int left = static_cast<int>(min(static_cast<int64_t>(kTurn), w.cols - col));
     const uint32_t boxes = smem0 + kDepths * kStage + (warp - kFirstOut) * (kOuts * kBoxBytes), came = drained + 8u * (1 + warp - kFirstOut);
-    const bool more = l.residual != nullptr && y < rows;
-    uint32_t phase = 0;
-    // The residual of 64 columns to where y's numbers will be; the first ones' while the products still run.
-    auto ask = [&](int c) {
+    const bool more = l.residual != nullptr && y < rows && left > 0;
+    // the residual to where y's numbers will be, while the products still run
+    if (more && l.residual_vec) {
       if (lane == 0) {
-        stores_left();
-        if (more && l.residual_vec) {
-          const int x = static_cast<int>(col0) + c, two = kWide && c + 32 < last;
-          bar_expect(came, (1 + two) * kBoxBytes);
-          load_own_box(boxes + kY * kBoxBytes, &w.residual, x, static_cast<int>(y), came);
-          if (two) load_own_box(boxes + (kY + 1) * kBoxBytes, &w.residual, x + 32, static_cast<int>(y), came);
-        }
+        const bool two = kWide && left > 32;
+        bar_expect(came, (two ? 2 : 1) * kBoxBytes);
+        load_own_box(boxes + kY * kBoxBytes, &w.residual, static_cast<int>(col), static_cast<int>(y), came);
+        if (two) load_own_box(boxes + (kY + 1) * kBoxBytes, &w.residual, static_cast<int>(col) + 32, static_cast<int>(y), came);
       }
-      __syncwarp();
-      if (more && !l.residual_vec) {
-        if constexpr (kWide) {
-          put_residual(l, y, rows, col0 + c, lane, boxes + kY * kBoxBytes);
-        } else {
-          LayerResidual r;
-          r.load(l, y, rows, col0 + c, lane);
-          r.put(false, lane, boxes + kY * kBoxBytes);
-          __syncwarp();
-        }
+    } else if (more) {
+      if constexpr (kWide) {
+        put_residual(l, y, rows, col, lane, boxes + kY * kBoxBytes);
+      } else {
+        LayerResidual r;
+        r.load(l, y, rows, col, lane);
+        r.put(false, lane, boxes + kY * kBoxBytes);
       }
-    };
-    ask(0);
-    float sum[kN];
+    }
+    __syncwarp();
+    float v[kTurn];
 #pragma unroll
-    for (int i = 0; i < kN; ++i) sum[i] = 0.f;
+    for (int i = 0; i < kTurn; ++i) v[i] = 0.f;
     int done = 0;
     for (int c = 0; c < w.stages; c += kChunk, ++done) {
       if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_full(done & 1), (done >> 1) & 1, w.limit));
       fence_after();
-      const uint32_t from = tmem + (done & 1) * kN + (static_cast<uint32_t>(32 * q) << 16);
+      const uint32_t from = tmem + (done & 1) * kN + share + (static_cast<uint32_t>(32 * q) << 16);
 #pragma unroll
-      for (int i = 0; i < kN; i += 32) {
-        float v[32];
+      for (int i = 0; i < kTurn; i += 32) {
+        float part[32];
         if (ok) {
-          tmem_load<32>(from + i, v);
-          tmem_wait<32>(v);
+          tmem_load<32>(from + i, part);
+          tmem_wait<32>(part);
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) sum[i + e] += ok ? v[e] : NAN;  // no number that looks like a result
+        for (int e = 0; e < 32; ++e) v[i + e] += ok ? part[e] : NAN;  // no number that looks like a result
       }
       fence_before();
       __syncwarp();
       if (lane == 0 && ok) bar_arrive(acc_free(done & 1));
     }
-    const Staged<kBf16> own(boxes, lane);
-    LayerTarget target = w.target;
-    target.y_map = &w.y;
-    target.z_map = &w.z;
-#pragma unroll
-    for (int c = 0; c < kN; c += kTurn) {
-      if (c >= last) break;
-      if (c > 0) ask(c);
-      float* const v = sum + c;
+    if (left > 0) {
+      const Staged<kBf16> own(boxes, lane);
       if (l.bias != nullptr)
 #pragma unroll
         for (int i = 0; i < kTurn; i += 8) {
           float bias[8];
-          halves<kBf16>(run_of<2>(l.bias + 2 * (col0 + c + i), w.cols - col0 - c - i, l.bias_vec), bias);
+          halves<kBf16>(run_of<2>(l.bias + 2 * (col + i), w.cols - col - i, l.bias_vec), bias);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[i + e] += bias[e];
         }
@@ -216,10 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) layer_tiles_kernel(const __grid_c
 #pragma unroll
           for (int e = 0; e < kTurn; ++e) v[e] = Act16::value<decltype(act)::kValue>(v[e]);
         });
-      if (more && l.residual_vec) {
-        ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(came, phase, w.limit));
-        phase ^= 1;
-      }
+      if (more && l.residual_vec) ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(came, 0, w.limit));
 #pragma unroll
       for (int i = 0; i < kTurn; i += 8) {
         float r[8];
@@ -232,7 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1) layer_tiles_kernel(const __grid_c
         if constexpr (kWide) own.put_f32(kY, i, r);
         else own.put(kY, i, r);
       }
-      flush_layer<kKeep, kWide>(target, col0 + c, last - c, y, boxes, lane);
+      LayerTarget target = w.target;
+      target.y_map = &w.y;
+      target.z_map = &w.z;
+      flush_layer<kKeep, kWide>(target, col, left, y, boxes, lane);
     }
     if (lane == 0) stores_done();
     __syncwarp();
@@ -274,7 +265,7 @@ cudaError_t run(const Tiles& w, int blocks, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kThreads<kN>);
   cfg.dynamicSmemBytes = kSmem<kN, kKeep, kWide>;
   cfg.stream = s;
   cfg.attrs = attr;
