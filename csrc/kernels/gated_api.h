@@ -118,11 +118,13 @@ cudaError_t launch_gate_f32(const float* g, const float* u, int64_t ld, float* h
 cudaError_t launch_gate_f32_backward(const float* gu, const float* dh, float* dgu, int64_t rows, int64_t cols, GatedActivation act, cudaStream_t s);
 
 // ---- linear layer -------------------------------------------------------------------------------------------
-// A layer of few rows, one launch that reads the weights at the rate of memory (kernels/linear_few.cu).  Rows of any alignment.
-// us, here and by tiles: TIMES
-inline bool layer_is_few(int64_t tokens, int64_t in, int64_t out) {
-  const int64_t n = in * out;
-  return n <= (tokens <= 2 ? 48 << 20 : tokens <= 8 ? 32 << 20 : tokens <= 16 ? 8 << 20 : tokens <= kFewTokens ? 4 << 20 : 0);
+// A layer of few rows, one launch that reads the weights at the rate of memory (kernels/linear_few.cu).  Rows of any alignment, which the tiles would
+// have copied.
+// us of bf16 from memory, here and by tiles (of which a narrow layer has few, each with all of the reduction): 1 token 1024 x 1024 2.5 and 5.1, 1024 x 4096
+// 6.1 and 5.8, 4096 x 4096 11.4 and 14.2, 2048 x 8192 12 and 9.5, 4096 x 10240 26 and 20; 16 tokens 2048 x 2048 5.5 and 8.4, 8192 x 2048 16 and 25, 4096 x
+// 4096 16.3 and 14.2; rows that begin anywhere, 1723 x 5258, 1 token 16 and 22, 16 tokens 21 and 22, 32 tokens 32 and 23.
+inline bool layer_is_few(int64_t tokens, int64_t out, bool aligned) {
+  return tokens <= 8 ? out <= 4096 || !aligned : tokens <= 16 ? out <= 2560 || !aligned : tokens <= kFewTokens && out <= 2560;
 }
 struct LayerFew {
   int64_t tokens, in, out;

@@ -68,14 +68,14 @@ at::Tensor forward16(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
   const kern::LayerRows r = layer_rows(residual);
   const kern::LayerFinish finish{act, bias.defined() ? bias.const_data_ptr() : nullptr, r.data, r.ld, type == at::kFloat};
   const kern::GatedShape s = shape_of(x, w);
-  if (z == nullptr && wait_limit < 0 && kern::layer_is_few(tokens, w.size(1), out)) {
+  Operands m;
+  const int ox = m.add(x), ow = m.add(w);
+  if (z == nullptr && wait_limit < 0 && kern::layer_is_few(tokens, out, !m.any())) {
     const at::Tensor xs = few_rows(x), ws = few_rows(w);
     const kern::LayerFew few{tokens, w.size(1), out, s.bf16, {xs.const_data_ptr(), row_stride(xs)}, {ws.const_data_ptr(), row_stride(ws)}, finish, y.data_ptr()};
     OPS_CK(kern::launch_layer_few(few, at::cuda::getCurrentCUDAStream()));
     return y;
   }
-  Operands m;
-  const int ox = m.add(x), ow = m.add(w);
   m.copy(x);
   if (kern::layer_tile(tokens, w.size(1), out) > 0) {
     const kern::LayerTiles tiles{tokens, w.size(1), out, s.bf16, m[ox], m[ow], finish, y.data_ptr(), z != nullptr ? z->data_ptr() : nullptr, wait_status(x), wait_limit};
