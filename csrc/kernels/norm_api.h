@@ -16,6 +16,7 @@ struct NormRows {
   int64_t ld;
   Elem type;
 };
+constexpr int64_t kNormMostCols = 0x7FFF0000;
 struct NormShape {
   int64_t rows;
   int cols;

@@ -243,7 +243,7 @@ int64_t norm_partial_bytes(const NormShape& s) { return s.rows <= 0 ? 0 : static
 
 cudaError_t launch_norm_backward(const NormBackward& a, cudaStream_t s) {
   const NormShape& h = a.shape;
-  if (h.cols <= 0 || h.rows < 0 || h.rows > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  if (h.cols <= 0 || h.cols > kNormMostCols || h.rows < 0 || h.rows > 0x7FFFFFFF) return cudaErrorInvalidValue;
   if (h.rows == 0) return cudaSuccess;
   Alignment l(h.cols);
   l.with(a.s.data, a.s.ld, a.s.type);

@@ -177,7 +177,7 @@ cudaError_t forward(const NormForward& a, cudaStream_t s, Types<X, S, Y, W>, std
 
 cudaError_t launch_norm_forward(const NormForward& a, cudaStream_t s) {
   const NormShape& h = a.shape;
-  if (h.cols <= 0 || h.rows < 0 || h.rows > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  if (h.cols <= 0 || h.cols > kNormMostCols || h.rows < 0 || h.rows > 0x7FFFFFFF) return cudaErrorInvalidValue;
   if (h.rows == 0) return cudaSuccess;
   const bool sum = a.residual.data != nullptr;
   Alignment l(h.cols);

@@ -39,7 +39,10 @@ kern::NormShape shape_of(const at::Tensor& rows, const Affine& p, double eps) {
 void check_call(const at::Tensor& x, const Affine& p, double eps, const at::Tensor& residual, at::ScalarType dtype) {
   check_block_tensor(x, kWhat);
   elem_of(x, kWhat);
-  MCCL_CHECK_T(TensorError, x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) <= 0x7FFFFF00, kWhat << ": rows of at least one number expected, got " << x.sizes());
+  MCCL_CHECK_T(TensorError, x.dim() >= 1 && x.size(-1) > 0, kWhat << ": rows of at least one number expected, got " << x.sizes());
+  // (32 bits count a row's numbers, up to a block's step behind the last)
+  MCCL_CHECK_T(TensorError, x.size(-1) <= kern::kNormMostCols && x.numel() / x.size(-1) <= 0x7FFFFFFF,
+               kWhat << ": at most " << kern::kNormMostCols << " numbers a row and 2^31 - 1 rows, got " << x.sizes());
   for (const at::Tensor* t : {&p.weight, &p.bias}) {
     if (!t->defined()) continue;
     check_block_tensor(*t, kWhat);

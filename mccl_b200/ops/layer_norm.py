@@ -1,4 +1,4 @@
-"""Layer norm of rows, with the sum with a residual before it, in one pass (``csrc/kernels/norm.cu``).
+"""Layer norm of rows, with the sum with a residual before it, in one pass (``csrc/kernels/norm_forward.cu``, ``norm_backward.cu``).
 
 ``y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias`` along the last dimension, where ``s`` is ``x`` or, with a residual, ``x +
 residual`` as the residual's type keeps it; then the sum comes back beside ``y``, and its gradient goes into the one backward pass.  All

@@ -320,3 +320,33 @@ def test_places_beyond_32_bits(cuda_device):
     assert torch.equal(y.detach()[ends], want.detach())
     g = torch.autograd.grad(y, x, y.detach())[0]
     assert torch.equal(g[ends], torch.autograd.grad(want, part, want.detach())[0])
+
+
+@pytest.mark.gpu
+def test_rows_whose_numbers_32_bits_cannot_count_are_refused(cuda_device):
+    one = torch.ones(1, device=cuda_device, dtype=torch.bfloat16)
+    for shape in ((1, 2 ** 31 - 256), (2 ** 31, 1), (2, 2 ** 31)):
+        with pytest.raises(RuntimeError, match="layer_norm: at most"):
+            layer_norm(one.expand(shape))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_one_tensor_twice(device):
+    x = torch.randn(5, 24, device=device, generator=torch.Generator(device=device).manual_seed(1))
+    w = torch.randn(24, device=device, generator=torch.Generator(device=device).manual_seed(2))
+    ds, dy = torch.randn_like(x), torch.randn_like(x)
+
+    def run(leaf, of):
+        y, s = of(leaf)
+        torch.autograd.backward((y, s), (dy.to(y.dtype), ds.to(s.dtype)))
+        return y.detach().double(), s.detach().double(), leaf.grad.double()
+
+    def plain(t):
+        s = t + t
+        return torch.nn.functional.layer_norm(s, (24,), w.double(), w.double()), s
+
+    got = run(x.clone().requires_grad_(), lambda t: layer_norm(t, w, w, residual=t))
+    want = run(x.double().requires_grad_(), plain)
+    for a, b in zip(got, want):
+        # a few dozen roundings of terms a few times the result's size
+        assert torch.allclose(a, b, rtol=64 * 2.0 ** -24, atol=64 * 2.0 ** -24 * b.abs().max().item())
