@@ -107,6 +107,10 @@ class AdamWPlan {
     const double bc1 = 1.0 - std::pow(beta1, static_cast<double>(step));
     const double bc2 = 1.0 - std::pow(beta2, static_cast<double>(step));
     if (!extra_.empty()) {
+      // a replay would round with the same dither every time, and moments would drift
+      cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+      MCCL_PLAN_CK(cudaStreamIsCapturing(stream, &capture));
+      MCCL_CHECK_TENSOR(capture == cudaStreamCaptureStatusNone, "FusedAdamW: a step with moments in 8 bits or bfloat16 parameters cannot be captured, its number is the host's");
       kern::AdamWStep h;
       h.beta1 = static_cast<float>(beta1);
       h.one_less_beta1 = static_cast<float>(1.0 - beta1);

@@ -12,7 +12,8 @@ interchangeable with ``torch.optim.AdamW`` (checkpoints load either way).
 tensors with ``exp_avg_scale`` and ``exp_avg_sq_scale`` beside them, 2.03 bytes a parameter instead of 8, and a step streams 16 bytes
 instead of 28.  ``bfloat16`` parameters are the upper half of an fp32 value that the update is made on; the lower half is their
 state ``low`` (int16), so that no update is too small for them.  Checkpoints of either kind, and ``torch.optim.AdamW``'s, load
-into the other; :meth:`FusedAdamW.moments` gives a parameter's moments as fp32 numbers.
+into the other; :meth:`FusedAdamW.moments` gives a parameter's moments as fp32 numbers.  The step's number, which counts for what is
+rounded up, is the host's: a step of either kind is not captured into a graph.
 """
 from __future__ import annotations
 

@@ -393,6 +393,27 @@ def test_refusals(cuda_device):
         plan.step([q.bfloat16()], 1e-3, 0.9, 0.999, 1e-8, 0.0, 1)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bits", KINDS)
+def test_a_captured_step_is_refused_and_does_nothing(cuda_device, dtype, bits):
+    p = torch.nn.Parameter(torch.randn(1000, device=cuda_device).to(dtype))
+    opt = FusedAdamW([p], state_bits=bits)
+    p.grad = torch.randn_like(p)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.synchronize()
+    before = [p.detach().clone(), *opt.moments(p)]
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            opt.step()
+    torch.cuda.synchronize()
+    assert float(opt.state[p]["step"]) == 1 and all(torch.equal(a, b) for a, b in zip(before, [p.detach(), *opt.moments(p)]))
+    opt.step()
+    assert float(opt.state[p]["step"]) == 2 and not torch.equal(before[0], p.detach())
+
+
 def _in_backward(rank, ws):
     import os
     import torch
