@@ -427,3 +427,42 @@ def test_places_beyond_32_bits(cuda_device, activation, residual):
     # (a sum of 32776 terms whose order and parts may differ)
     size = dy[ends].abs().double() @ w.abs().double()
     assert ((g[ends].double() - few.double()).abs() <= few.abs().double() * 2.0 ** -7 + size * (out / 8 + 40) * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_tensor_twice(device, dtype):
+    # x beside itself as the residual, and a matrix times itself
+    t = _inputs(40, 40, 40, dtype, dtype, True, "cpu")
+
+    def run(x, to):
+        y = to(x)
+        y.backward(t["dy"].to(y.device, y.dtype))
+        return y.detach().double().cpu(), x.grad.double().cpu()
+
+    bias = t["bias"].to(device)
+    for of, plain in ((lambda x: fused_linear(x, x, bias, residual=x), lambda x: x @ x.t() + t["bias"].double() + x),
+                      (lambda x: fused_linear(x.t(), x, residual=x), lambda x: x.t() @ x.t() + x)):
+        got = run(t["x"].to(device, copy=True).requires_grad_(), of)
+        want = run(t["x"].double().requires_grad_(), plain)
+        for a, b in zip(got, want):
+            # 3 gradients of one leaf, each rounded, and their two sums: 5 half steps of at most the sum of their sizes, some 4 of the largest entry
+            assert (a - b).abs().max() <= 20 * ROUNDOFF[dtype] * b.abs().max()
+
+
+@pytest.mark.gpu
+def test_two_threads_on_streams_of_their_own(cuda_device):
+    from concurrent.futures import ThreadPoolExecutor
+    cases = [_inputs(tokens, 264, out, torch.bfloat16, torch.float32, True, cuda_device, seed=out) for tokens, out in ((9, 136), (333, 1032), (3000, 1032), (3000, 520))]
+    want = [_call(t, "gelu") for t in cases]
+    torch.cuda.synchronize()
+
+    def many(t):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [_call(t, "gelu") for _ in range(8)]
+            torch.cuda.current_stream().synchronize()
+        return got
+
+    with ThreadPoolExecutor(len(cases)) as pool:
+        for got, one in zip(pool.map(many, cases), want):
+            assert all(torch.equal(a, b) for g in got for a, b in zip(g, one))
