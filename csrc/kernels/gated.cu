@@ -635,7 +635,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           __syncwarp();
           if (!l.residual_vec) put_residual(l, y, j.rows, at.col + c, lane, y_boxes);
         };
-        if (t.part < 0 && first < last) ask(first);
+        if (ok && t.part < 0 && first < last) ask(first);  // (where a wait has run out the last one's may be on its way still)
         float sum[kShare];
 #pragma unroll
         for (int i = 0; i < kShare; ++i) sum[i] = 0.f;
@@ -663,7 +663,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           for (int turn = 0; turn < kShare; turn += kTurn) {
             const int c = first + turn;
             if (c >= last) break;
-            if (turn > 0) ask(c);
+            if (ok && turn > 0) ask(c);
             float* const v = sum + turn;
             if (l.bias != nullptr)
 #pragma unroll
