@@ -307,8 +307,15 @@ def test_captured_replayed_and_on_another_stream(cuda_device):
     _check(t, None, *out)
 
 
+@pytest.fixture
+def emptied():
+    """What a test of several GB leaves in torch's cache is given back behind it: other tests count on what is free."""
+    yield
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.gpu
-def test_places_beyond_32_bits(cuda_device):
+def test_places_beyond_32_bits(emptied, cuda_device):
     rows, cols = 70000, 32768
     x = torch.empty(rows, cols, device=cuda_device, dtype=torch.bfloat16)
     x.normal_(generator=torch.Generator(device=cuda_device).manual_seed(2))
