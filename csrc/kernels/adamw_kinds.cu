@@ -55,23 +55,46 @@ __device__ __forceinline__ uint32_t power_of(uint32_t most, int top) {
   const int power = static_cast<int>((most + 0x1FFFFFu) >> 23) - top;
   return static_cast<uint32_t>(max(power, 127 - 120));
 }
+// Two fp32 numbers side by side, for instructions that take both: each is rounded as by an instruction of its own.
+struct Two {
+  uint64_t bits;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+  __device__ __forceinline__ void apart(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two fma_of(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+// a + b, with a one that the compiler does not know: of a product and a sum of pairs it makes one instruction, which rounds once, whatever is asked for.
+__device__ __forceinline__ Two sum_of(Two a, Two b, Two one) { return fma_of(a, one, b); }
 // Root and quotient, correctly rounded, of numbers far from either end of fp32's range, by Markstein's theorems (Computation of elementary
 // functions on the IBM RISC System/6000 processor, 1990): Newton's iteration to a root or reciprocal within a rounding, then one step on the
 // remainder, which a fused multiplication and addition gives exactly.  No branch stands between one element's and the next one's, as
-// there does in the general functions.
-__device__ __forceinline__ float root_of(float v) {
-  float y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
-  const float s = v * y, half = 0.5f * y, e = fmaf(-s, half, 0.5f);
-  const float s1 = fmaf(s, e, s), half1 = fmaf(half, e, half);
-  return fmaf(fmaf(-s1, s1, v), half1, s1);
+// there does in the general functions.  Signs are turned where that saves turning a factor's: -root(v), and a / -b.
+__device__ __forceinline__ Two negative_root_of(Two v) {
+  float a, b;
+  v.apart(a, b);
+  asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(b));
+  const Two y(a, b), less_v = v * Two(-1.f), s = less_v * y, half = y * Two(0.5f), e = fma_of(s, half, Two(0.5f));
+  const Two s1 = fma_of(s, e, s), half1 = fma_of(half, e, half);
+  return fma_of(fma_of(s1, s1, less_v), half1, s1);
 }
-__device__ __forceinline__ float quotient_of(float a, float b) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(b));
-  y = fmaf(fmaf(-b, y, 1.f), y, y);
-  const float q = a * y;
-  return fmaf(fmaf(-b, q, a), y, q);
+__device__ __forceinline__ Two quotient_of(Two a, Two less_b) {
+  float b0, b1;
+  less_b.apart(b0, b1);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b0) : "f"(-b0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b1) : "f"(-b1));
+  const Two y0(b0, b1), y = fma_of(fma_of(less_b, y0, Two(1.f)), y0, y0), q = a * y;
+  return fma_of(fma_of(less_b, q, a), y, q);
 }
 // Bits of the smallest and the largest number these are used for: 2^-60 and 2^60.
 constexpr uint32_t kLeast = (127u - 60u) << 23, kMost = (127u + 60u) << 23;
@@ -123,8 +146,11 @@ __device__ __forceinline__ void codes_of(const float* x, const Bounds& lane_boun
   uint32_t word[kLane];
   if (__all_sync(0xFFFFFFFFu, __fmul_rn(__uint_as_float(least), inverse) >= small)) {
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      word[i] = (__float_as_uint(__fmul_rn(fabsf(x[i]), inverse)) << (1 + kDigits)) + (kFirst ? dither[i].of_m : dither[i].of_v);
+    for (int i = 0; i < kLane; i += 2) {  // (the shift drops the sign)
+      float y[2];
+      (Two(x[i], x[i + 1]) * Two(inverse)).apart(y[0], y[1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) word[i + e] = (__float_as_uint(y[e]) << (1 + kDigits)) + (kFirst ? dither[i + e].of_m : dither[i + e].of_v);
     }
   } else {
 #pragma unroll
@@ -298,35 +324,43 @@ struct Group {
       values_of<false>(raw.v, v);
     }
     if constexpr (kHalf) join(raw.p, raw.low, p);
+    const Two grad_scale(h.grad_scale), of_one(h.one_less_beta1), of_two(h.one_less_beta2), times_m(by_m), times_v(by_v), one(h.one);
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      float g;
+    for (int i = 0; i < kLane; i += 2) {
+      Two g;
       if constexpr (kHalf) {
-        g = __uint_as_float(i % 2 ? raw.g[i / 2] & 0xFFFF0000u : raw.g[i / 2] << 16);
+        g = Two(__uint_as_float(raw.g[i / 2] << 16), __uint_as_float(raw.g[i / 2] & 0xFFFF0000u));
       } else {
         p[i] = __uint_as_float(raw.p[i]);
-        g = __uint_as_float(raw.g[i]);
+        p[i + 1] = __uint_as_float(raw.p[i + 1]);
+        g = Two(__uint_as_float(raw.g[i]), __uint_as_float(raw.g[i + 1]));
       }
       if constexpr (!kEight) {
-        m[i] = __uint_as_float(raw.m[i]);
-        v[i] = __uint_as_float(raw.v[i]);
+#pragma unroll
+        for (int e = i; e < i + 2; ++e) {
+          m[e] = __uint_as_float(raw.m[e]);
+          v[e] = __uint_as_float(raw.v[e]);
+        }
       }
-      const float d = __fmul_rn(g, h.grad_scale);
-      m[i] = __fadd_rn(__fmul_rn(m[i], by_m), __fmul_rn(d, h.one_less_beta1));
-      v[i] = __fadd_rn(__fmul_rn(v[i], by_v), __fmul_rn(__fmul_rn(d, h.one_less_beta2), d));
+      const Two d = g * grad_scale;
+      sum_of(Two(m[i], m[i + 1]) * times_m, d * of_one, one).apart(m[i], m[i + 1]);
+      sum_of(Two(v[i], v[i + 1]) * times_v, d * of_two * d, one).apart(v[i], v[i + 1]);
     }
     const Bounds of_m(m), of_v(v);
-    auto move = [&](auto root, auto quotient) {
+    if (h.ordinary && __all_sync(0xFFFFFFFFu, of_m.inside() && of_v.inside())) {
+      const Two less_eps(-h.eps), inv_sqrt_bias2(h.inv_sqrt_bias2), decay(h.decay), less_step(-h.step_size);
+#pragma unroll
+      for (int i = 0; i < kLane; i += 2) {
+        const Two less_below = sum_of(negative_root_of(Two(v[i], v[i + 1])) * inv_sqrt_bias2, less_eps, one);
+        sum_of(Two(p[i], p[i + 1]) * decay, quotient_of(Two(m[i], m[i + 1]), less_below) * less_step, one).apart(p[i], p[i + 1]);
+      }
+    } else {
 #pragma unroll
       for (int i = 0; i < kLane; ++i) {
-        const float below = __fadd_rn(__fmul_rn(root(v[i]), h.inv_sqrt_bias2), h.eps);
-        p[i] = __fsub_rn(__fmul_rn(p[i], h.decay), __fmul_rn(quotient(m[i], below), h.step_size));
+        const float below = __fadd_rn(__fmul_rn(__fsqrt_rn(v[i]), h.inv_sqrt_bias2), h.eps);
+        p[i] = __fsub_rn(__fmul_rn(p[i], h.decay), __fmul_rn(__fdiv_rn(m[i], below), h.step_size));
       }
-    };
-    if (h.ordinary && __all_sync(0xFFFFFFFFu, of_m.inside() && of_v.inside()))
-      move([](float x) { return root_of(x); }, [](float x, float y) { return quotient_of(x, y); });
-    else
-      move([](float x) { return __fsqrt_rn(x); }, [](float x, float y) { return __fdiv_rn(x, y); });
+    }
   }
 
   // kN words in the array's runs, from the number `at` on.
@@ -463,12 +497,18 @@ __global__ void __launch_bounds__(kThreads, 10) adamw_kinds_kernel(const AdamWTe
   }
 }
 
-// For tests: what the step takes for a root of b and a quotient a / b.
+// For tests: what the step takes for a root of b and a quotient a / b, in either place beside another number; NaN where the places differ.
 __global__ void root_quotient_kernel(const float* a, const float* b, float* root, float* quotient, int64_t n) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= n) return;
-  root[i] = root_of(b[i]);
-  quotient[i] = quotient_of(a[i], b[i]);
+  const int64_t j = n - 1 - i;
+  float first, second, other;
+  (negative_root_of(Two(b[i], b[j])) * Two(-1.f)).apart(first, other);
+  (negative_root_of(Two(b[j], b[i])) * Two(-1.f)).apart(other, second);
+  root[i] = __float_as_uint(first) == __float_as_uint(second) ? first : NAN;
+  quotient_of(Two(a[i], a[j]), Two(-b[i], -b[j])).apart(first, other);
+  quotient_of(Two(a[j], a[i]), Two(-b[j], -b[i])).apart(other, second);
+  quotient[i] = __float_as_uint(first) == __float_as_uint(second) ? first : NAN;
 }
 
 }  // namespace

@@ -62,6 +62,7 @@ struct AdamWStep {
   float step_size;       // lr / (1 - beta1^t)
   float inv_sqrt_bias2;  // 1 / sqrt(1 - beta2^t)
   float grad_scale;
+  float one;             // 1
   uint32_t ordinary;     // eps and inv_sqrt_bias2 are far from either end of fp32's range
   uint32_t step_word;    // t times the golden ratio's digits, for the dither
 };

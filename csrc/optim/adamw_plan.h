@@ -121,6 +121,7 @@ class AdamWPlan {
       h.step_size = static_cast<float>(lr / bc1);
       h.inv_sqrt_bias2 = static_cast<float>(1.0 / std::sqrt(bc2));
       h.grad_scale = static_cast<float>(grad_scale);
+      h.one = 1.f;
       h.ordinary = h.eps >= 0.f && h.eps <= 0x1p20f && h.inv_sqrt_bias2 <= 0x1p20f;
       h.step_word = static_cast<uint32_t>(step) * 0x9E3779B9u;
       MCCL_PLAN_CK(kern::launch_adamw_kinds(reinterpret_cast<const kern::AdamWTensor*>(d_tensors_.data_ptr<int64_t>()),
