@@ -14,10 +14,12 @@
 // bf16 parameters are the upper 16 bits of an fp32 value, rounded to nearest; `low` is what these leave of its bits, as a whole number.  A program that
 // changes the parameter moves the value with it.  (fp32 copies of the parameters: 2 more bytes of traffic and of memory each, and they go stale.)
 //
-// 16.03 bytes a number (fp32 parameters), 14.03 (bf16), where fp32 moments have 28.  About 70 instructions a number, so the issue slots are two
-// thirds full beside it: 48 M numbers 149 us (5.4 TB/s), bf16 157 (4.5), with fp32 moments 210 (6.2).  A warp has a group, so that what the group
-// shares is two reductions; CTAs of two warps, ten to an SM.  (Without what is asked for ahead, or that in registers, which leaves half as many
-// warps: 219; with the general root and quotient 235; CTAs of four warps 167; 8 and 16 thousand numbers a CTA 147 and 161.)
+// 16.03 bytes a number (fp32 parameters), 14.03 (bf16), where fp32 moments have 28.  57 instructions a number, as pairs of numbers go through
+// the packed fp32 instructions (70, and 78 % of the issue slots, without): 48 M numbers 143 us (5.6 TB/s), bf16 138 (5.1), with fp32 moments
+// 206 (6.4); 96 M 269 (6.0), 271 (5.2) and 396 (6.6).  A warp has a group, so that what the group shares is two reductions; CTAs of two warps, ten to
+// an SM (twelve, whose threads have fewer registers: 148, 139 and 207).  What is left is the start of each CTA, three reads behind each other,
+// which the others have to fill.  (Without what is asked for ahead, or that in registers, which leaves half as many warps: 219; with
+// the general root and quotient 235; CTAs of four warps 167; a third more room for what is asked for: 162.)
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -212,7 +214,7 @@ struct Chunk {
   int size;        // of the chunk
   uint32_t first;  // its first number's
   bool aligned;
-  __device__ __forceinline__ Chunk(const AdamWTensor& t, const void* grad_of, int64_t begin, int number_size, int moment_size) {
+  __device__ __forceinline__ Chunk(const AdamWTensor& t, const void* grad_of, int64_t begin, int chunk, int number_size, int moment_size) {
     param = static_cast<char*>(t.param) + begin * number_size;
     grad = static_cast<const char*>(grad_of) + begin * number_size;
     low = t.low + begin;
@@ -220,7 +222,7 @@ struct Chunk {
     exp_avg_sq = static_cast<char*>(t.exp_avg_sq) + begin * moment_size;
     exp_avg_scale = t.exp_avg_scale + begin / kMomentGroup;
     exp_avg_sq_scale = t.exp_avg_sq_scale + begin / kMomentGroup;
-    size = static_cast<int>(min(static_cast<int64_t>(kAdamWChunk), t.size - begin));
+    size = static_cast<int>(min(static_cast<int64_t>(chunk), t.size - begin));
     first = static_cast<uint32_t>(begin);
     aligned = t.aligned && reinterpret_cast<uintptr_t>(grad_of) % 16 == 0;
   }
@@ -439,7 +441,7 @@ __device__ __forceinline__ void chunk_of(const AdamWTensor& tensor, const void* 
   constexpr int kPlace = R::kWords * 128, kAhead = kShared / kPlace, kStep = kWarps * kMomentGroup;
   static_assert(kAhead >= 1, "one group at least");
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const Chunk t(tensor, grad, begin, kHalf ? 2 : 4, kEight ? 1 : 4);
+  const Chunk t(tensor, grad, begin, h.chunk, kHalf ? 2 : 4, kEight ? 1 : 4);
   // groups from `i` on: alike in a warp
   auto whole = [&](int i) { return t.aligned && i + kMomentGroup <= t.size; };
   auto ask = [&](int i, uint32_t place) {
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 10) adamw_kinds_kernel(const AdamWTe
     const int2 place = chunks[c];
     const AdamWTensor t = tensors[place.x];
     const void* grad = reinterpret_cast<const void*>(grads[place.x]);
-    const int64_t first = static_cast<int64_t>(place.y) * kAdamWChunk;
+    const int64_t first = static_cast<int64_t>(place.y) * h.chunk;
     if (t.eight) {
       if (t.half) chunk_of<true, true>(t, grad, h, first, shared);
       else chunk_of<false, true>(t, grad, h, first, shared);

@@ -42,7 +42,10 @@ cudaError_t launch_adamw_multi(const AdamWTable& tab, const AdamWHyper& h, cudaS
 // ---- tensors of several kinds (kernels/adamw_kinds.cu) ---------------------------------------------
 // Moments that share one scale where they are kept in 8 bits.
 constexpr int kMomentGroup = 256;
-static_assert(kAdamWChunk % kMomentGroup == 0, "a CTA has whole groups");
+// Numbers of a CTA: with few, more CTAs share a small step; with many, each starts less often.  us by 2048 and by 8192: 1 M numbers 16 and 22, 12 M 50
+// and 51, 24 M 85 and 84, 96 M 290 and 269 (bf16 parameters: 16 and 24, 46 and 51, 80 and 81, 269 and 271); fp32 moments, of which fewer are on
+// their way, 16 and 20, 62 and 69, 110 and 119, 396 and 411.
+inline int adamw_kinds_chunk(int64_t numbers, bool eight) { return eight && numbers >= 24ll << 20 ? 8192 : 2048; }
 
 // One tensor, in device memory.
 struct AdamWTensor {
@@ -65,6 +68,7 @@ struct AdamWStep {
   float one;             // 1
   uint32_t ordinary;     // eps and inv_sqrt_bias2 are far from either end of fp32's range
   uint32_t step_word;    // t times the golden ratio's digits, for the dither
+  int chunk;             // numbers of a CTA, whole groups
 };
 cudaError_t launch_adamw_kinds(const AdamWTensor* tensors, const uint64_t* grads, const int2* chunks, int num_chunks, const AdamWStep& h, cudaStream_t s,
                                int max_ctas = 0);

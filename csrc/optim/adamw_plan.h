@@ -41,14 +41,21 @@ class AdamWPlan {
                       "AdamWPlan: list sizes differ");
     std::vector<int64_t> ptr_p, ptr_m, ptr_v, sizes;
     std::vector<int32_t> chunks;
+    int64_t numbers = 0;
+    bool eight = false;
     for (size_t i = 0; i < params_.size(); ++i) {
       check_tensors(i);
+      numbers += params_[i].numel();
+      eight = eight || m_[i].scalar_type() != at::kFloat;
+    }
+    chunk_ = extra_.empty() ? kern::kAdamWChunk : kern::adamw_kinds_chunk(numbers, eight);
+    for (size_t i = 0; i < params_.size(); ++i) {
       ptr_p.push_back(reinterpret_cast<int64_t>(params_[i].data_ptr()));
       ptr_m.push_back(reinterpret_cast<int64_t>(m_[i].data_ptr()));
       ptr_v.push_back(reinterpret_cast<int64_t>(v_[i].data_ptr()));
       const int64_t n = params_[i].numel();
       sizes.push_back(n);
-      for (int64_t c = 0; c * kern::kAdamWChunk < n; ++c) {
+      for (int64_t c = 0; c * chunk_ < n; ++c) {
         chunks.push_back(static_cast<int32_t>(i));
         chunks.push_back(static_cast<int32_t>(c));
       }
@@ -124,6 +131,7 @@ class AdamWPlan {
       h.one = 1.f;
       h.ordinary = h.eps >= 0.f && h.eps <= 0x1p20f && h.inv_sqrt_bias2 <= 0x1p20f;
       h.step_word = static_cast<uint32_t>(step) * 0x9E3779B9u;
+      h.chunk = chunk_;
       MCCL_PLAN_CK(kern::launch_adamw_kinds(reinterpret_cast<const kern::AdamWTensor*>(d_tensors_.data_ptr<int64_t>()),
                                             reinterpret_cast<const uint64_t*>(d_g_.data_ptr<int64_t>()),
                                             reinterpret_cast<const int2*>(d_chunks_.data_ptr<int32_t>()), num_chunks_, h, stream, max_ctas));
@@ -207,7 +215,7 @@ class AdamWPlan {
   std::vector<AdamWExtra> extra_;
   std::vector<int64_t> grad_ptrs_;
   at::Tensor d_p_, d_g_, d_m_, d_v_, d_sizes_, d_chunks_, d_tensors_;
-  int num_chunks_ = 0;
+  int num_chunks_ = 0, chunk_ = 0;
 };
 
 

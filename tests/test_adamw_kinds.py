@@ -414,6 +414,32 @@ def test_a_captured_step_is_refused_and_does_nothing(cuda_device, dtype, bits):
     assert float(opt.state[p]["step"]) == 2 and not torch.equal(before[0], p.detach())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bits", KINDS)
+def test_what_a_block_takes_does_not_show(cuda_device, dtype, bits):
+    # 24 Mi numbers and more in all go by larger parts than fewer do
+    sizes = [1, 255, 8191, 8193, 20000, 100000]
+    sizes.append((24 << 20) - sum(sizes))
+    gen = torch.Generator(device=cuda_device).manual_seed(5)
+    values = [torch.randn(n, device=cuda_device, generator=gen).to(dtype) for n in sizes]
+    grads = [torch.randn(n, device=cuda_device, generator=gen).to(dtype) for n in sizes]
+
+    def steps(which):
+        params = [torch.nn.Parameter(values[i].clone()) for i in which]
+        opt = FusedAdamW(params, lr=1e-2, state_bits=bits)
+        for _ in range(3):
+            for p, i in zip(params, which):
+                p.grad = grads[i]
+            opt.step()
+        return [(p.detach(), opt.state[p]) for p in params]
+
+    together, apart = steps(range(7)), steps(range(6)) + steps([6])
+    for (p, s), (q, t) in zip(together, apart):
+        assert torch.equal(p, q)
+        for k in s:
+            assert torch.equal(s[k].view(torch.uint8) if s[k].element_size() == 1 else s[k], t[k].view(torch.uint8) if t[k].element_size() == 1 else t[k]), k
+
+
 def _in_backward(rank, ws):
     import os
     import torch
