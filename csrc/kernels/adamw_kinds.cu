@@ -28,6 +28,7 @@
 
 #include "kernels/launch_count.h"
 #include "kernels/optim_api.h"
+#include "kernels/two.cuh"
 
 namespace mccl {
 namespace kern {
@@ -56,24 +57,6 @@ struct Dither {
 __device__ __forceinline__ uint32_t power_of(uint32_t most, int top) {
   const int power = static_cast<int>((most + 0x1FFFFFu) >> 23) - top;
   return static_cast<uint32_t>(max(power, 127 - 120));
-}
-// Two fp32 numbers side by side, for instructions that take both: each is rounded as by an instruction of its own.
-struct Two {
-  uint64_t bits;
-  __device__ __forceinline__ Two() {}
-  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
-  __device__ __forceinline__ void apart(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
-};
-__device__ __forceinline__ Two operator*(Two a, Two b) {
-  Two r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
-  return r;
-}
-__device__ __forceinline__ Two fma_of(Two a, Two b, Two c) {
-  Two r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
-  return r;
 }
 // a + b, with a one that the compiler does not know: of a product and a sum of pairs it makes one instruction, which rounds once, whatever is asked for.
 __device__ __forceinline__ Two sum_of(Two a, Two b, Two one) { return fma_of(a, one, b); }

@@ -290,16 +290,12 @@ __device__ __forceinline__ void finish_layer(const Finish& f, float* z, const La
     for (int b = 0; b < kN / 8; ++b) {
       float bias[8];
       halves<kBf16>(now.bias[b], bias);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[8 * b + e] += bias[e];
+      add_to<8>(z + 8 * b, bias);
     }
   if constexpr (kKeep)
 #pragma unroll
     for (int b = 0; b < kN; b += 8) put_z<kBf16>(sink, i0 + b, z + b);
-  with_activation(l.activation, [&](auto act) {
-#pragma unroll
-    for (int e = 0; e < kN; ++e) z[e] = Act16::value<decltype(act)::kValue>(z[e]);
-  });
+  with_activation(l.activation, [&](auto act) { Act16::values<decltype(act)::kValue, kN>(z); });
 #pragma unroll
   for (int b = 0; b < kN; b += 8) more(i0 + b, z + b);
 #pragma unroll
@@ -649,9 +645,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
             if (ok) {
               tmem_load<kN>(from + i, v);
               tmem_wait<kN>(v);
-            }
+            } else {
 #pragma unroll
-            for (int e = 0; e < kN; ++e) sum[i + e] += ok ? v[e] : NAN;  // no number that looks like a result
+              for (int e = 0; e < kN; ++e) v[e] = NAN;  // no number that looks like a result
+            }
+            add_to<kN>(sum + i, v);
           }
           fence_before();
           __syncwarp();
@@ -672,8 +670,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
                 const uint4 raw = run_of<2>(l.bias + 2 * (at.col + c + i), l.cols - at.col - c - i, l.bias_vec);
                 if (w.f.bf16) halves<true>(raw, bias);
                 else halves<false>(raw, bias);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[i + e] += bias[e];
+                add_to<8>(v + i, bias);
               }
             if constexpr (kKeepsZ<kOut>)
 #pragma unroll
@@ -682,20 +679,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
                 else put_z<false>(Staged<false>(boxes, lane), i, v + i);
               }
             if (l.activation != LayerActivation::kNone)
-              with_activation(l.activation, [&](auto act) {
-#pragma unroll
-                for (int e = 0; e < kTurn; ++e) v[e] = Act16::value<decltype(act)::kValue>(v[e]);
-              });
+              with_activation(l.activation, [&](auto act) { Act16::values<decltype(act)::kValue, kTurn>(v); });
             if (l.residual_vec && y < j.rows) {
               ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(came, phase, w.limit));
               phase ^= 1;
             }
+            if (!ok)
+#pragma unroll
+              for (int e = 0; e < kTurn; ++e) v[e] = NAN;
 #pragma unroll
             for (int i = 0; i < kTurn; i += 8) {
               float r[8];
               own.get_f32(kY, i, r);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) r[e] = ok ? v[i + e] + r[e] : NAN;
+              add_to<8>(r, v + i);
               own.put_f32(kY, i, r);
             }
             flush_layer<kKeepsZ<kOut>, kWideY<kOut>>(LayerTarget{&j.out[0], &j.out[1], j.to[0], j.ldo, j.rows, j.wide}, at.col + c, last - c, y, boxes, lane);
@@ -743,8 +739,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
                 if (l.residual == nullptr) return;
                 float r[8];
                 halves<kBf16>(sink.get(kY, i), r);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += r[e];
+                add_to<8>(v, r);
               });
             };
             if (w.f.bf16) run(std::true_type());

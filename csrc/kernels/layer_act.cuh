@@ -3,68 +3,96 @@
 
 #include "kernels/gate.cuh"
 #include "kernels/gated_api.h"
+#include "kernels/two.cuh"
 
 namespace mccl {
 namespace kern {
 
 // For results that are rounded to 16 bits.  Each is within 2^-18 of its size: exponentials and reciprocals by the instructions for them.
+// Of numbers (N: float) or of two side by side (Two), for which half as many instructions do.
 struct Act16 {
-  static __device__ __forceinline__ float exp2_of(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+  template <typename N>
+  static __device__ __forceinline__ N exp2_of(N x) {
+    return each_of(x, [](float x) {
+      float y;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+      return y;
+    });
   }
-  static __device__ __forceinline__ float reciprocal(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+  template <typename N>
+  static __device__ __forceinline__ N reciprocal(N x) {
+    return each_of(x, [](float x) {
+      float y;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+      return y;
+    });
   }
   // The logistic function of z, or of 2 sqrt(2 / pi) (z + 0.044715 z^3): s = 1 / (1 + 2^(z (c0 + c1 z^2))).  (Where the square overflows the
   // exponent does, to the right end.)
   static constexpr float kC0 = -1.4426950408889634f;
-  static __device__ __forceinline__ float logistic(float z) { return reciprocal(1.f + exp2_of(kC0 * z)); }
-  static __device__ __forceinline__ float cubic(float z, float square) { return reciprocal(1.f + exp2_of(z * fmaf(kC0 * kGelu * kCubic, square, kC0 * kGelu))); }
+  template <typename N>
+  static __device__ __forceinline__ N logistic(N z) { return reciprocal(N(1.f) + exp2_of(N(kC0) * z)); }
+  template <typename N>
+  static __device__ __forceinline__ N cubic(N z, N square) {
+    return reciprocal(N(1.f) + exp2_of(z * fma_of(N(kC0 * kGelu * kCubic), square, N(kC0 * kGelu))));
+  }
   // The normal distribution up to z, and its density times z.  The tail is t P(t) exp(-z^2 / 2) / 2 with t = 1 / (1 + |z| / sqrt(8)) and a polynomial
   // fitted to erfc(x) exp(x^2) / t by reweighted least squares, 2^-19.5 of its size off at most between x = 0 and 10.
+  template <typename N>
   struct Normal {
-    float share, slope;
+    N share, slope;
   };
-  static __device__ __forceinline__ Normal normal(float z) {
-    const float a = fabsf(z), e = exp2_of(-0.7213475204444817f * fminf(a * a, 1e30f)), t = reciprocal(fmaf(a, 0.35355339059327373f, 1.f));
-    float p = 0.0882045243f;
-    p = fmaf(p, t, -0.35673875f);
-    p = fmaf(p, t, 0.38922509f);
-    p = fmaf(p, t, 0.0378904397f);
-    p = fmaf(p, t, 0.281503786f);
-    p = fmaf(p, t, 0.277582146f);
-    p = fmaf(p, t, 0.282331411f);
-    const float tail = 0.5f * t * p * e;
-    return {z < 0.f ? tail : 1.f - tail, z * (0.3989422804014327f * e)};
+  static __device__ __forceinline__ float share_of(float z, float tail) { return z < 0.f ? tail : 1.f - tail; }
+  static __device__ __forceinline__ Two share_of(Two z, Two tail) {
+    float a, b, s, t;
+    z.apart(a, b);
+    tail.apart(s, t);
+    return Two(share_of(a, s), share_of(b, t));
   }
-  template <LayerActivation kAct>
-  static __device__ __forceinline__ float value(float z) {
-    if constexpr (kAct == LayerActivation::kRelu) return z > 0.f || z != z ? z : 0.f;
+  template <typename N>
+  static __device__ __forceinline__ Normal<N> normal(N z) {
+    const N a = each_of(z, [](float z) { return fabsf(z); }), e = exp2_of(N(-0.7213475204444817f) * z * z);
+    const N t = reciprocal(fma_of(a, N(0.35355339059327373f), N(1.f)));
+    N p = N(0.0882045243f);
+    p = fma_of(p, t, N(-0.35673875f));
+    p = fma_of(p, t, N(0.38922509f));
+    p = fma_of(p, t, N(0.0378904397f));
+    p = fma_of(p, t, N(0.281503786f));
+    p = fma_of(p, t, N(0.277582146f));
+    p = fma_of(p, t, N(0.282331411f));
+    return {share_of(z, N(0.5f) * t * p * e), z * (N(0.3989422804014327f) * e)};
+  }
+  template <LayerActivation kAct, typename N>
+  static __device__ __forceinline__ N value(N z) {
+    if constexpr (kAct == LayerActivation::kRelu) return each_of(z, [](float z) { return z > 0.f || z != z ? z : 0.f; });
     else if constexpr (kAct == LayerActivation::kSilu) return z * logistic(z);
     else if constexpr (kAct == LayerActivation::kGelu) return z * normal(z).share;
     else if constexpr (kAct == LayerActivation::kGeluTanh) return z * cubic(z, z * z);
     else return z;
   }
-  template <LayerActivation kAct>
-  static __device__ __forceinline__ float slope(float z) {
+  template <LayerActivation kAct, typename N>
+  static __device__ __forceinline__ N slope(N z) {
     if constexpr (kAct == LayerActivation::kRelu) {
-      return z > 0.f ? 1.f : z != z ? z : 0.f;
+      return each_of(z, [](float z) { return z > 0.f ? 1.f : z != z ? z : 0.f; });
     } else if constexpr (kAct == LayerActivation::kSilu) {
-      const float s = logistic(z);
-      return fmaf(z, fmaf(-s, s, s), s);
+      const N s = logistic(z);
+      return fma_of(z, fma_of(N(-1.f) * s, s, s), s);
     } else if constexpr (kAct == LayerActivation::kGelu) {
-      const Normal n = normal(z);
+      const Normal<N> n = normal(z);
       return n.share + n.slope;
     } else if constexpr (kAct == LayerActivation::kGeluTanh) {
-      const float square = fminf(z * z, 1e30f), s = cubic(z, square);
-      return fmaf(z * fmaf(-s, s, s), fmaf(kGelu * 3.f * kCubic, square, kGelu), s);
+      const N square = each_of(z * z, [](float x) { return fminf(x, 1e30f); }), s = cubic(z, square);
+      return fma_of(z * fma_of(N(-1.f) * s, s, s), fma_of(N(kGelu * 3.f * kCubic), square, N(kGelu)), s);
     } else {
-      return 1.f;
+      return N(1.f);
     }
+  }
+  // Of kN numbers, each by its value.
+  template <LayerActivation kAct, int kN>
+  static __device__ __forceinline__ void values(float* z) {
+    if constexpr (kAct != LayerActivation::kNone)
+#pragma unroll
+      for (int i = 0; i < kN; i += 2) value<kAct>(Two(z[i], z[i + 1])).apart(z[i], z[i + 1]);
   }
 };
 // For results in fp32: the functions of the CUDA library.

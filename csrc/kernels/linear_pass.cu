@@ -94,10 +94,18 @@ __global__ void __launch_bounds__(kThreads, 2) layer_derive_kernel(const LayerDe
           if constexpr (kSlope) v[i] = next_z[r][i];
         }
         ask(r, at + kRowsAhead * kWarps);
+        if constexpr (kV > 1 && !std::is_same_v<T, float>) {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          if constexpr (kSlope) d[i] *= Act::template slope<kAct>(v[i]);
-          sum[i] += d[i];
+          for (int i = 0; i < kV; i += 2) {
+            if constexpr (kSlope) (Two(d[i], d[i + 1]) * Act::template slope<kAct>(Two(v[i], v[i + 1]))).apart(d[i], d[i + 1]);
+            add_to<2>(sum + i, d + i);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kV; ++i) {
+            if constexpr (kSlope) d[i] *= Act::template slope<kAct>(v[i]);
+            sum[i] += d[i];
+          }
         }
         if (g.dz != nullptr) store_run<T, kV>(dz + at * g.dz_ld, kV, true, d);
       }

@@ -181,9 +181,11 @@ __global__ void __launch_bounds__(kThreads<kN>, 1) layer_tiles_kernel(const __gr
         if (ok) {
           tmem_load<32>(from + i, part);
           tmem_wait<32>(part);
-        }
+        } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[i + e] += ok ? part[e] : NAN;  // no number that looks like a result
+          for (int e = 0; e < 32; ++e) part[e] = NAN;  // no number that looks like a result
+        }
+        add_to<32>(v + i, part);
       }
       fence_before();
       __syncwarp();
@@ -196,29 +198,27 @@ __global__ void __launch_bounds__(kThreads<kN>, 1) layer_tiles_kernel(const __gr
         for (int i = 0; i < kTurn; i += 8) {
           float bias[8];
           halves<kBf16>(run_of<2>(l.bias + 2 * (col + i), w.cols - col - i, l.bias_vec), bias);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[i + e] += bias[e];
+          add_to<8>(v + i, bias);
         }
       if constexpr (kKeep)
 #pragma unroll
         for (int i = 0; i < kTurn; i += 8) put_z<kBf16>(own, i, v + i);
       if (l.activation != LayerActivation::kNone)
-        with_activation(l.activation, [&](auto act) {
-#pragma unroll
-          for (int e = 0; e < kTurn; ++e) v[e] = Act16::value<decltype(act)::kValue>(v[e]);
-        });
+        with_activation(l.activation, [&](auto act) { Act16::values<decltype(act)::kValue, kTurn>(v); });
       if (more && l.residual_vec) ok = __all_sync(0xFFFFFFFFu, ok && bar_wait(came, 0, w.limit));
+      if (!ok)
+#pragma unroll
+        for (int e = 0; e < kTurn; ++e) v[e] = NAN;
 #pragma unroll
       for (int i = 0; i < kTurn; i += 8) {
-        float r[8];
         if (more) {
+          float r[8];
           if constexpr (kWide) own.get_f32(kY, i, r);
           else halves<kBf16>(own.get(kY, i), r);
+          add_to<8>(v + i, r);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = !ok ? NAN : more ? v[i + e] + r[e] : v[i + e];
-        if constexpr (kWide) own.put_f32(kY, i, r);
-        else own.put(kY, i, r);
+        if constexpr (kWide) own.put_f32(kY, i, v + i);
+        else own.put(kY, i, v + i);
       }
       LayerTarget target = w.target;
       target.y_map = &w.y;
