@@ -478,6 +478,11 @@ __device__ __forceinline__ void finish_turn(const Finish& f, const Spot& at, int
 // Left: 16 warps to take the accumulators out (no faster, 397 for 339 of the wide gate), what was kept asked for two runs ahead through
 // shared memory (72 for 75, but 418 for 379 of the wide one, which has then a stage less) or a tile ahead into the second-level cache
 // (83 and 431).
+//
+// A linear layer, 8192 x 1024 x 4096 bf16, by itself: 48 us (1.43 PFLOP/s), with silu 57, gelu_tanh 60 and gelu 64 (50 without their exponentials
+// and reciprocals, which go through a unit of a quarter of the rate), with z kept 64 to 70, and 61 of that without an activation:
+// the other 67 MB through the second-level cache, as are a 16-bit residual's, 61.  fp32 residual 75.  8192 x 4096 x 1024 53, 56 and 64; 16384 x 2048 x 8192
+// 372 (1.48), 384 and 496.  Waiting for the boxes later, behind the arithmetic, changes nothing.
 template <Out kOut, GatedKeep kKeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   constexpr int kDepths = kStages<kOut>, kOuts = kBoxes<kOut>;

@@ -4,6 +4,10 @@
 // Bound by the way to its first byte and by what each CTA loads, 128 rows of x for each 64 or 128 of W, through the second-level cache; all of it is
 // in flight from the start.  A tile is done when it is: nothing overlaps what follows its product, so that is spread over the device too.
 // Sums are taken out of tensor memory every 512 of the reduction and added in registers, as gated.cu does for results in 32 bits.
+//
+// us, bf16, launches one behind the other (B200): 64 rows of 1024 x 4096 6.5, 128 rows 6.7, 333 of 1024 x 2816 6.7, of 1000 x 2731, whose results begin
+// anywhere, 10.1 (fp32 residual 10.7, gelu 11.3; pairs of CTAs 18 to 20), 1024 of 1024 x 4096, which has the larger tiles with eight warps
+// each to take them out, 12.2.  About 2 of each are the launch, and 16 stages of 24 KB an SM the rest.
 #include <algorithm>
 #include <atomic>
 
