@@ -195,7 +195,10 @@ struct Team {
     }
     return r;
   }
-  __device__ __forceinline__ float sum(float a) { return sum(a, 0.f).x; }
+  __device__ __forceinline__ float sum(float a) {
+    if (warps == 1) return warp_sum(a);
+    return sum(a, 0.f).x;
+  }
 };
 
 // ---- host ---------------------------------------------------------------------------------------------------
@@ -221,6 +224,28 @@ cudaError_t with_run(T types, int run, Call f) {
 
 int block_warps(int warps, int most) { return warps * std::max(1, most / warps); }
 
+// Rows that are read one number at a time have kernels for teams of so many warps and numbers a thread, known where they are compiled: places are then a
+// distance from one address, and a thread asks for no more numbers than a row of its kind has.  (8192 x 1024 and the like, by runs, are faster
+// with the team that just holds them, and the addresses are few.)  Calls `f` with the warps and the numbers of the smallest team.
+template <typename Call>
+cudaError_t with_team(int cols, Call f) {
+  auto is = [&](auto warps, auto numbers) { return f(warps, numbers); };
+#define TEAM(w, n) \
+  if (cols <= 32 * w * n) return is(std::integral_constant<int, w>(), std::integral_constant<int, n>())
+  TEAM(1, 1);
+  TEAM(1, 2);
+  TEAM(1, 4);
+  TEAM(1, 8);
+  TEAM(2, 8);
+  TEAM(4, 8);
+  TEAM(8, 6);
+  TEAM(8, 8);
+  TEAM(16, 8);
+  TEAM(16, 12);
+  TEAM(16, 16);
+#undef TEAM
+  return cudaErrorInvalidValue;
+}
 
 }  // namespace
 }  // namespace kern

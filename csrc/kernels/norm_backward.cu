@@ -5,8 +5,9 @@ namespace mccl {
 namespace kern {
 namespace {
 
-template <int kRun, int kN, typename X, typename S, typename Y, typename W>
-__global__ void __launch_bounds__(kBackwardThreads) norm_backward_kernel(const NormBackward a, int warps) {
+// kWarps: of a team, or 0 where it is told.
+template <int kRun, int kN, int kWarps, typename X, typename S, typename Y, typename W>
+__global__ void __launch_bounds__(kBackwardThreads) norm_backward_kernel(const NormBackward a, int told) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float2 slots[2 * kBackwardThreads / 32];
   extern __shared__ float columns[];  // [2][cols]
@@ -15,7 +16,7 @@ __global__ void __launch_bounds__(kBackwardThreads) norm_backward_kernel(const N
   const S s_type(a.s.type);
   const Y y_type(a.dy.type);
   const W w_type(h.weight_type);
-  const int team = 32 * warps, t = threadIdx.x % team, cols = h.cols, teams = blockDim.x / team, number = threadIdx.x / team;
+  const int warps = kWarps > 0 ? kWarps : told, team = 32 * warps, t = threadIdx.x % team, cols = h.cols, teams = blockDim.x / team, number = threadIdx.x / team;
   Team sums(slots, warps, blockDim.x / 32);
   Row<kRun, kN> w;
   w.fill(1.f);
@@ -34,7 +35,7 @@ __global__ void __launch_bounds__(kBackwardThreads) norm_backward_kernel(const N
   auto ask = [&](int64_t row) {
     if (row >= h.rows) return;
     int at = t;
-    asm volatile("" : "+r"(at));  // addresses are made anew: kept over the loop, one for each run and array, they take all registers
+    if (kWarps == 0) asm volatile("" : "+r"(at));  // addresses are made anew: kept over the loop, one for each run and array, they take all registers
     next_s.load(a.s.data, s_type, row * a.s.ld, at, team, cols);
     next_g.load(a.dy.data, y_type, row * a.dy.ld, at, team, cols);
     if (a.ds.data != nullptr) next_ds.load(a.ds.data, s_type, row * a.ds.ld, at, team, cols);
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(kBackwardThreads) norm_backward_kernel(const N
         if (a.ds.data != nullptr) g.v[n][i] += ds.v[n][i];
       }
     int at = t;
-    asm volatile("" : "+r"(at));
+    if (kWarps == 0) asm volatile("" : "+r"(at));
     if (a.dx != nullptr) g.store(a.dx, x_type, row * cols, at, team, cols);
     if (a.dresidual != nullptr) g.store(a.dresidual, s_type, row * cols, at, team, cols);
   }
@@ -187,22 +188,32 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const float* pa
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
-constexpr int kWarps = 8;  // of a block where a team has fewer
+constexpr int kBlockWarps = 8;  // of a block where a team has fewer
 bool backward_wide(const NormShape& s) { return s.cols > kMany * kBackwardThreads; }
-// Warps of a backward team.
-int backward_warps(const NormShape& s) { return static_cast<int>(ceil_div(s.cols, 32 * (s.cols <= kFew * kBackwardThreads ? kFew : kMany))); }
-// Blocks of the backward kernel, or parts of the rows for the columns' sums.
-int parts_of(const NormShape& s) {
-  if (backward_wide(s)) return static_cast<int>(std::clamp<int64_t>(ceil_div(8 * kSms, ceil_div(s.cols, kColumnThreads)), 1, ceil_div(s.rows, 16)));
-  const int warps = backward_warps(s), teams = block_warps(warps, kWarps) / warps;
-  return static_cast<int>(std::min<int64_t>(ceil_div(s.rows, teams), kBackwardBlocks));
-}
+// Parts of the rows for the columns' sums of long ones.
+int parts_of(const NormShape& s) { return static_cast<int>(std::clamp<int64_t>(ceil_div(8 * kSms, ceil_div(s.cols, kColumnThreads)), 1, ceil_div(s.rows, 16))); }
 
-template <int kRun, typename X, typename S, typename Y, typename W>
-cudaError_t backward(const NormBackward& a, cudaStream_t s, Types<X, S, Y, W>, std::integral_constant<int, kRun>) {
+// Its blocks.
+template <int kRun, int kN, int kWarps, typename X, typename S, typename Y, typename W>
+cudaError_t teams(const NormBackward& a, cudaStream_t s, int warps, Types<X, S, Y, W>, int* blocks) {
   const NormShape& h = a.shape;
-  const int parts = parts_of(h);
+  const int all = block_warps(warps, kBlockWarps), shared = 2 * h.cols * 4;
+  const auto kernel = norm_backward_kernel<kRun, kN, kWarps, X, S, Y, W>;
+  if (shared > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMany * kBackwardThreads * 4);
+    if (e != cudaSuccess) return e;
+  }
+  *blocks = static_cast<int>(std::min<int64_t>(ceil_div(h.rows, all / warps), kBackwardBlocks));
+  note_launch();
+  kernel<<<*blocks, 32 * all, shared, s>>>(a, warps);
+  return cudaGetLastError();
+}
+template <int kRun, typename X, typename S, typename Y, typename W>
+cudaError_t backward(const NormBackward& a, cudaStream_t s, Types<X, S, Y, W> types, std::integral_constant<int, kRun>) {
+  const NormShape& h = a.shape;
+  int parts = 0;
   if (backward_wide(h)) {
+    parts = parts_of(h);
     if (a.dx != nullptr || a.dresidual != nullptr) {
       note_launch();
       norm_backward_wide_kernel<kRun><<<static_cast<unsigned>(std::min<int64_t>(h.rows, 4 * kSms)), kWideThreads, 0, s>>>(a);
@@ -213,14 +224,14 @@ cudaError_t backward(const NormBackward& a, cudaStream_t s, Types<X, S, Y, W>, s
       norm_columns_kernel<<<dim3(static_cast<unsigned>(ceil_div(h.cols, kColumnThreads)), parts), kColumnThreads, 0, s>>>(a, each);
     }
   } else {
-    const int warps = backward_warps(h), all = block_warps(warps, kWarps), shared = 2 * h.cols * 4;
-    const auto kernel = h.cols <= kFew * kBackwardThreads ? norm_backward_kernel<kRun, kFew / kRun, X, S, Y, W> : norm_backward_kernel<kRun, kMany / kRun, X, S, Y, W>;
-    if (shared > 40 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMany * kBackwardThreads * 4);
-      if (e != cudaSuccess) return e;
-    }
-    note_launch();
-    kernel<<<parts, 32 * all, shared, s>>>(a, warps);
+    cudaError_t e;
+    if constexpr (kRun == 1)
+      e = with_team(h.cols, [&](auto warps, auto numbers) { return teams<1, decltype(numbers)::value, decltype(warps)::value>(a, s, warps, types, &parts); });
+    else if (h.cols <= kFew * kBackwardThreads)
+      e = teams<kRun, kFew / kRun, 0>(a, s, static_cast<int>(ceil_div(h.cols, 32 * kFew)), types, &parts);
+    else
+      e = teams<kRun, kMany / kRun, 0>(a, s, static_cast<int>(ceil_div(h.cols, 32 * kMany)), types, &parts);
+    if (e != cudaSuccess) return e;
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || a.partial == nullptr) return e;
@@ -239,7 +250,11 @@ cudaError_t backward(const NormBackward& a, cudaStream_t s, Types<X, S, Y, W>, s
 
 }  // namespace
 
-int64_t norm_partial_bytes(const NormShape& s) { return s.rows <= 0 ? 0 : static_cast<int64_t>(parts_of(s)) * 2 * s.cols * 4; }
+// (of the team's kernel as many as it may have)
+int64_t norm_partial_bytes(const NormShape& s) {
+  if (s.rows <= 0) return 0;
+  return (backward_wide(s) ? parts_of(s) : std::min<int64_t>(s.rows, kBackwardBlocks)) * 2 * s.cols * 4;
+}
 
 cudaError_t launch_norm_backward(const NormBackward& a, cudaStream_t s) {
   const NormShape& h = a.shape;

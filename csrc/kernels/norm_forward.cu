@@ -19,10 +19,11 @@ namespace mccl {
 namespace kern {
 namespace {
 
-template <int kRun, int kN, typename X, typename S, typename Y, typename W>
-__global__ void __launch_bounds__(kForwardThreads) norm_forward_kernel(const NormForward a, int warps) {
+// kWarps: of a team, or 0 where it is told.
+template <int kRun, int kN, int kWarps, typename X, typename S, typename Y, typename W>
+__global__ void __launch_bounds__(kForwardThreads) norm_forward_kernel(const NormForward a, int told) {
   __shared__ float2 slots[2 * kForwardThreads / 32];
-  const int team = 32 * warps, t = threadIdx.x % team, cols = a.shape.cols;
+  const int warps = kWarps > 0 ? kWarps : told, team = 32 * warps, t = threadIdx.x % team, cols = a.shape.cols;
   const NormShape& h = a.shape;
   const X x_type(a.x.type);
   const S s_type(a.residual.type);
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(kForwardThreads) norm_forward_kernel(const Nor
   auto ask = [&](int64_t row) {
     if (row >= h.rows) return;
     int at = t;
-    asm volatile("" : "+r"(at));  // addresses are made anew: kept over the loop, one for each run and array, they take the registers
+    if (kWarps == 0) asm volatile("" : "+r"(at));  // addresses are made anew: kept over the loop, one for each run and array, they take the registers
     x.load(a.x.data, x_type, row * a.x.ld, at, team, cols);
     if (a.residual.data != nullptr) r.load(a.residual.data, s_type, row * a.residual.ld, at, team, cols);
   };
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(kForwardThreads) norm_forward_kernel(const Nor
   for (; row < h.rows; row += step) {
     Row<kRun, kN> s, other;
     int at = t;
-    asm volatile("" : "+r"(at));
+    if (kWarps == 0) asm volatile("" : "+r"(at));
     s.take(x, x_type);
     if (a.residual.data != nullptr) {
       other.take(r, s_type);
@@ -152,23 +153,31 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
   }
 }
 
-constexpr int kWarps = 8;  // of a block where a team has fewer
+constexpr int kBlockWarps = 8;  // of a block where a team has fewer
 
+template <int kRun, int kN, int kWarps, typename X, typename S, typename Y, typename W>
+void teams(const NormForward& a, cudaStream_t s, int warps, Types<X, S, Y, W>) {
+  const int all = block_warps(warps, kBlockWarps);
+  norm_forward_kernel<kRun, kN, kWarps, X, S, Y, W>
+      <<<static_cast<unsigned>(std::min<int64_t>(ceil_div(a.shape.rows, all / warps), kForwardBlocks)), 32 * all, 0, s>>>(a, warps);
+}
 template <int kRun, typename X, typename S, typename Y, typename W>
-cudaError_t forward(const NormForward& a, cudaStream_t s, Types<X, S, Y, W>, std::integral_constant<int, kRun>) {
+cudaError_t forward(const NormForward& a, cudaStream_t s, Types<X, S, Y, W> types, std::integral_constant<int, kRun>) {
   const NormShape& h = a.shape;
   note_launch();
-  int warps = static_cast<int>(ceil_div(h.cols, 32 * kMany));
-  // fewer rows than fill the device have more threads each
-  if (h.rows * warps < 16 * kSms && h.cols <= kFew * kForwardThreads) {
-    warps = static_cast<int>(ceil_div(h.cols, 32 * kFew));
-    const int all = block_warps(warps, kWarps);
-    norm_forward_kernel<kRun, kFew / kRun, X, S, Y, W><<<static_cast<unsigned>(std::min<int64_t>(ceil_div(h.rows, all / warps), kForwardBlocks)), 32 * all, 0, s>>>(a, warps);
-  } else if (h.cols <= kMany * kForwardThreads) {
-    const int all = block_warps(warps, kWarps);
-    norm_forward_kernel<kRun, kMany / kRun, X, S, Y, W><<<static_cast<unsigned>(std::min<int64_t>(ceil_div(h.rows, all / warps), kForwardBlocks)), 32 * all, 0, s>>>(a, warps);
-  } else {
+  if (h.cols > kMany * kForwardThreads) {
     norm_forward_wide_kernel<kRun><<<static_cast<unsigned>(std::min<int64_t>(h.rows, 4 * kSms)), kWideThreads, 0, s>>>(a);
+  } else if constexpr (kRun == 1) {
+    const cudaError_t e = with_team(h.cols, [&](auto warps, auto numbers) {
+      teams<1, decltype(numbers)::value, decltype(warps)::value>(a, s, warps, types);
+      return cudaSuccess;
+    });
+    if (e != cudaSuccess) return e;
+  } else {
+    const int warps = static_cast<int>(ceil_div(h.cols, 32 * kMany));
+    // fewer rows than fill the device have more threads each
+    if (h.rows * warps < 16 * kSms && h.cols <= kFew * kForwardThreads) teams<kRun, kFew / kRun, 0>(a, s, static_cast<int>(ceil_div(h.cols, 32 * kFew)), types);
+    else teams<kRun, kMany / kRun, 0>(a, s, warps, types);
   }
   return cudaGetLastError();
 }
