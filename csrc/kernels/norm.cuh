@@ -65,12 +65,6 @@ cudaError_t with_types(Elem x, Elem s, Elem y, Elem w, Call f) {
 
 // kRun numbers that are aligned to their run's size (16 bytes at most).
 template <int kRun>
-__device__ __forceinline__ void get(const void* p, Elem type, int64_t at, float (&v)[kRun]) {
-  if (type == Elem::kF32) load_run<float, kRun>(static_cast<const float*>(p) + at, kRun, true, v);
-  else if (type == Elem::kBF16) load_run<__nv_bfloat16, kRun>(static_cast<const __nv_bfloat16*>(p) + at, kRun, true, v);
-  else load_run<__half, kRun>(static_cast<const __half*>(p) + at, kRun, true, v);
-}
-template <int kRun>
 __device__ __forceinline__ void put(void* p, Elem type, int64_t at, const float (&v)[kRun]) {
   if (type == Elem::kF32) store_run<float, kRun>(static_cast<float*>(p) + at, kRun, true, v);
   else if (type == Elem::kBF16) store_run<__nv_bfloat16, kRun>(static_cast<__nv_bfloat16*>(p) + at, kRun, true, v);
@@ -154,12 +148,12 @@ struct Row {
   // As the type keeps it.
   template <typename T>
   __device__ __forceinline__ void round(T type) {
-    if (type == Elem::kF32) return;
+    if (type != Elem::kF32)
 #pragma unroll
-    for (int n = 0; n < kN; ++n)
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int i = 0; i < kRun; ++i)
-        v[n][i] = type == Elem::kBF16 ? __bfloat162float(__float2bfloat16_rn(v[n][i])) : __half2float(__float2half_rn(v[n][i]));
+        for (int i = 0; i < kRun; ++i)
+          v[n][i] = type == Elem::kBF16 ? __bfloat162float(__float2bfloat16_rn(v[n][i])) : __half2float(__float2half_rn(v[n][i]));
   }
 };
 

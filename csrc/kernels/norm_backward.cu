@@ -100,71 +100,109 @@ __global__ void __launch_bounds__(kBackwardThreads) norm_backward_kernel(const N
   float* to = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
   for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) to[i] = columns[i];
 }
+// Rows that no team has room for: a run, or kFew numbers, a thread at a time, read again from the second-level cache.
 template <int kRun>
-__global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(const NormBackward a) {
+__global__ void __launch_bounds__(kWideThreads, 2) norm_backward_wide_kernel(const NormBackward a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int kN = kRun == 1 ? kFew : 1, kStep = kWideThreads * kRun * kN;
   __shared__ float2 slots[2 * kWideThreads / 32];
   const NormShape& h = a.shape;
-  const int cols = h.cols, step = kWideThreads * kRun;
+  const int cols = h.cols, t = threadIdx.x;
   Team sums(slots, kWideThreads / 32, kWideThreads / 32);
+  const Told x_type(a.dx_type), s_type(a.s.type), y_type(a.dy.type), w_type(h.weight_type);
   const float per = 1.f / static_cast<float>(cols);
   for (int64_t row = blockIdx.x; row < h.rows; row += gridDim.x) {
     const float mean = a.mean[row], rstd = a.rstd[row];
-    float u[kRun], g[kRun];
+    Row<kRun, kN> u, g;
     auto both_of = [&](int c) {
-      float w[kRun];
-      get<kRun>(a.s.data, a.s.type, row * a.s.ld + c, u);
-      get<kRun>(a.dy.data, a.dy.type, row * a.dy.ld + c, g);
-      if (h.weight != nullptr) get<kRun>(h.weight, h.weight_type, c, w);
+      Raw<kRun, kN> s, dy, w;
+      s.load(a.s.data, s_type, row * a.s.ld + c, t, kWideThreads, cols - c);
+      dy.load(a.dy.data, y_type, row * a.dy.ld + c, t, kWideThreads, cols - c);
+      if (h.weight != nullptr) w.load(h.weight, w_type, c, t, kWideThreads, cols - c);
+      u.take(s, s_type);
+      g.take(dy, y_type);
+      Row<kRun, kN> weight;
+      weight.fill(1.f);
+      if (h.weight != nullptr) weight.take(w, w_type);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        u[i] = (u[i] - mean) * rstd;
-        if (h.weight != nullptr) g[i] *= w[i];
-      }
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          u.v[n][i] = (u.v[n][i] - mean) * rstd;
+          g.v[n][i] *= weight.v[n][i];
+        }
     };
     float first = 0.f, second = 0.f;
-    for (int c = threadIdx.x * kRun; c < cols; c += step) {
+    for (int c = 0; c < cols; c += kStep) {
       both_of(c);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        first += g[i];
-        second = fmaf(g[i], u[i], second);
-      }
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {  // (beyond the row dy is zero, and with it these)
+          first += g.v[n][i];
+          second = fmaf(g.v[n][i], u.v[n][i], second);
+        }
     }
     const float2 both = sums.sum(first, second);
     const float c1 = both.x * per, c2 = both.y * per;
-    for (int c = threadIdx.x * kRun; c < cols; c += step) {
+    for (int c = 0; c < cols; c += kStep) {
+      Raw<kRun, kN> more;
+      if (a.ds.data != nullptr) more.load(a.ds.data, s_type, row * a.ds.ld + c, t, kWideThreads, cols - c);
       both_of(c);
-      float ds[kRun];
-      if (a.ds.data != nullptr) get<kRun>(a.ds.data, a.ds.type, row * a.ds.ld + c, ds);
+      Row<kRun, kN> ds;
+      ds.fill(0.f);
+      if (a.ds.data != nullptr) ds.take(more, s_type);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        g[i] = rstd * (g[i] - c1 - u[i] * c2);
-        if (a.ds.data != nullptr) g[i] += ds[i];
-      }
-      if (a.dx != nullptr) put<kRun>(a.dx, a.dx_type, row * cols + c, g);
-      if (a.dresidual != nullptr) put<kRun>(a.dresidual, a.s.type, row * cols + c, g);
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) g.v[n][i] = rstd * (g.v[n][i] - c1 - u.v[n][i] * c2) + ds.v[n][i];
+      if (a.dx != nullptr) g.store(a.dx, x_type, row * cols + c, t, kWideThreads, cols - c);
+      if (a.dresidual != nullptr) g.store(a.dresidual, s_type, row * cols + c, t, kWideThreads, cols - c);
     }
   }
 }
-// The columns' sums over some of the rows, a column a thread, for rows that are too long for the kernel above.
-constexpr int kColumnThreads = 256;
+// The columns' sums over some of the rows, a run of columns a thread, for rows that are too long for the kernel above.
+constexpr int kColumnThreads = 256, kRowsAhead = 4;
+template <int kRun>
 __global__ void __launch_bounds__(kColumnThreads) norm_columns_kernel(const NormBackward a, int64_t rows_each) {
-  const int c = blockIdx.x * kColumnThreads + threadIdx.x, cols = a.shape.cols;
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * kColumnThreads + threadIdx.x) * kRun;
+  const int cols = a.shape.cols;
   if (c >= cols) return;
+  const Told s_type(a.s.type), y_type(a.dy.type);
   const int64_t begin = blockIdx.y * rows_each, end = min(a.shape.rows, begin + rows_each);
-  float dw = 0.f, db = 0.f;
-#pragma unroll 4
-  for (int64_t row = begin; row < end; ++row) {
-    float s[1], dy[1];
-    get<1>(a.s.data, a.s.type, row * a.s.ld + c, s);
-    get<1>(a.dy.data, a.dy.type, row * a.dy.ld + c, dy);
-    dw = fmaf(dy[0], (s[0] - a.mean[row]) * a.rstd[row], dw);
-    db += dy[0];
+  float dw[kRun], db[kRun];
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) dw[i] = db[i] = 0.f;
+  for (int64_t row = begin; row < end; row += kRowsAhead) {
+    Raw<kRun, 1> s[kRowsAhead], dy[kRowsAhead];
+    float mean[kRowsAhead], rstd[kRowsAhead];
+#pragma unroll
+    for (int r = 0; r < kRowsAhead; ++r) {
+      const int64_t at = min(row + r, end - 1);
+      s[r].load(a.s.data, s_type, at * a.s.ld + c, 0, 1, kRun);
+      dy[r].load(a.dy.data, y_type, at * a.dy.ld + c, 0, 1, kRun);
+      mean[r] = a.mean[at];
+      rstd[r] = a.rstd[at];
+    }
+#pragma unroll
+    for (int r = 0; r < kRowsAhead; ++r) {
+      if (row + r >= end) break;
+      Row<kRun, 1> u, g;
+      u.take(s[r], s_type);
+      g.take(dy[r], y_type);
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        dw[i] = fmaf(g.v[0][i], (u.v[0][i] - mean[r]) * rstd[r], dw[i]);
+        db[i] += g.v[0][i];
+      }
+    }
   }
   float* to = a.partial + static_cast<int64_t>(blockIdx.y) * 2 * cols;
-  to[c] = dw;
-  to[cols + c] = db;
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    to[c + i] = dw[i];
+    to[cols + c + i] = db[i];
+  }
 }
 // Adds up the blocks' sums: 32 columns a block, whose warps share the parts.
 constexpr int kJoinThreads = 1024;
@@ -190,8 +228,8 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(const float* pa
 // ---- host ---------------------------------------------------------------------------------------------------
 constexpr int kBlockWarps = 8;  // of a block where a team has fewer
 bool backward_wide(const NormShape& s) { return s.cols > kMany * kBackwardThreads; }
-// Parts of the rows for the columns' sums of long ones.
-int parts_of(const NormShape& s) { return static_cast<int>(std::clamp<int64_t>(ceil_div(8 * kSms, ceil_div(s.cols, kColumnThreads)), 1, ceil_div(s.rows, 16))); }
+// Parts of the rows for the columns' sums of long ones, by runs of `run`.
+int parts_of(const NormShape& s, int run) { return static_cast<int>(std::clamp<int64_t>(ceil_div(8 * kSms, ceil_div(s.cols, run * kColumnThreads)), 1, ceil_div(s.rows, 16))); }
 
 // Its blocks.
 template <int kRun, int kN, int kWarps, typename X, typename S, typename Y, typename W>
@@ -213,7 +251,7 @@ cudaError_t backward(const NormBackward& a, cudaStream_t s, Types<X, S, Y, W> ty
   const NormShape& h = a.shape;
   int parts = 0;
   if (backward_wide(h)) {
-    parts = parts_of(h);
+    parts = parts_of(h, kRun);
     if (a.dx != nullptr || a.dresidual != nullptr) {
       note_launch();
       norm_backward_wide_kernel<kRun><<<static_cast<unsigned>(std::min<int64_t>(h.rows, 4 * kSms)), kWideThreads, 0, s>>>(a);
@@ -221,7 +259,7 @@ cudaError_t backward(const NormBackward& a, cudaStream_t s, Types<X, S, Y, W> ty
     if (a.partial != nullptr) {
       note_launch();
       const int64_t each = ceil_div(h.rows, parts);
-      norm_columns_kernel<<<dim3(static_cast<unsigned>(ceil_div(h.cols, kColumnThreads)), parts), kColumnThreads, 0, s>>>(a, each);
+      norm_columns_kernel<kRun><<<dim3(static_cast<unsigned>(ceil_div(h.cols, kRun * kColumnThreads)), parts), kColumnThreads, 0, s>>>(a, each);
     }
   } else {
     cudaError_t e;
@@ -250,10 +288,10 @@ cudaError_t backward(const NormBackward& a, cudaStream_t s, Types<X, S, Y, W> ty
 
 }  // namespace
 
-// (of the team's kernel as many as it may have)
+// (as many as there may be, whatever the rows are aligned to)
 int64_t norm_partial_bytes(const NormShape& s) {
   if (s.rows <= 0) return 0;
-  return (backward_wide(s) ? parts_of(s) : std::min<int64_t>(s.rows, kBackwardBlocks)) * 2 * s.cols * 4;
+  return (backward_wide(s) ? parts_of(s, 8) : std::min<int64_t>(s.rows, kBackwardBlocks)) * 2 * s.cols * 4;
 }
 
 cudaError_t launch_norm_backward(const NormBackward& a, cudaStream_t s) {

@@ -12,7 +12,9 @@
 //
 // us, bf16 with an fp32 residual, 8192 x 1024 (B200): forward 17 (96 MB: 5.5 TB/s), backward 25 (128 MB: 5.0) and 3 for the blocks' sums.  A row a
 // block at a time, none asked for ahead, 25 and 38; a warp a row, 32 numbers a thread, 31 and 51; three blocks an SM 23 and 31.
-// fp16, 4099 x 1723, whose rows begin anywhere and are read one by one, 22 and 28.
+// Rows that begin anywhere are read one number at a time: fp16, 4099 x 1723, 16 and 16 (with teams that just hold the row, 22 and 28: they make each
+// address anew); bf16, 65535 x 17, 14 and 13 (61 and 41, of which 15 numbers of 16 a thread were none); 2048 x 8191 29 and 56.  Rows longer than 8192, which
+// no team holds, bf16 with an fp32 residual, 2048 x 16384: 86 (4.7 TB/s), 122 and 39 for the columns.
 #include "kernels/norm.cuh"
 
 namespace mccl {
@@ -98,57 +100,82 @@ __global__ void __launch_bounds__(kForwardThreads) norm_forward_kernel(const Nor
   }
 }
 
-// Rows that no team has room for: a block has one, and reads it again from the second-level cache.
+// Rows that no team has room for: a block has one, kFew numbers a thread at a time, and reads it again from the second-level cache.
 template <int kRun>
-__global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const NormForward a) {
+__global__ void __launch_bounds__(kWideThreads, 2) norm_forward_wide_kernel(const NormForward a) {
+  constexpr int kN = kFew / kRun, kStep = kWideThreads * kFew;
   __shared__ float2 slots[2 * kWideThreads / 32];
-  const int cols = a.shape.cols, step = kWideThreads * kRun;
+  const int cols = a.shape.cols, t = threadIdx.x;
   Team sums(slots, kWideThreads / 32, kWideThreads / 32);
   const NormShape& h = a.shape;
+  const bool with = a.residual.data != nullptr;
+  const Told x_type(a.x.type), s_type(with ? a.residual.type : a.x.type), y_type(a.y_type), w_type(h.weight_type);
+  const void* const from = with ? a.sum : a.x.data;
   for (int64_t row = blockIdx.x; row < h.rows; row += gridDim.x) {
+    const int64_t at = row * (with ? cols : a.x.ld);
     float sum = 0.f;
-    for (int c = threadIdx.x * kRun; c < cols; c += step) {
-      float v[kRun];
-      get<kRun>(a.x.data, a.x.type, row * a.x.ld + c, v);
-      if (a.residual.data != nullptr) {
-        float r[kRun];
-        get<kRun>(a.residual.data, a.residual.type, row * a.residual.ld + c, r);
+    for (int c = 0; c < cols; c += kStep) {
+      Raw<kRun, kN> x, r;
+      Row<kRun, kN> s, other;
+      x.load(a.x.data, x_type, row * a.x.ld + c, t, kWideThreads, cols - c);
+      if (with) r.load(a.residual.data, s_type, row * a.residual.ld + c, t, kWideThreads, cols - c);
+      s.take(x, x_type);
+      if (with) {
+        other.take(r, s_type);
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) v[i] += r[i];
-        put<kRun>(a.sum, a.residual.type, row * cols + c, v);
-        get<kRun>(a.sum, a.residual.type, row * cols + c, v);  // this thread's own: what was kept
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int i = 0; i < kRun; ++i) s.v[n][i] += other.v[n][i];
+        s.round(s_type);
+        s.store(a.sum, s_type, row * cols + c, t, kWideThreads, cols - c);  // read again by this thread alone
       }
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) sum += v[i];
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) sum += s.v[n][i];
     }
-    const void* from = a.residual.data != nullptr ? a.sum : a.x.data;
-    const Elem type = a.residual.data != nullptr ? a.residual.type : a.x.type;
-    const int64_t at = row * (a.residual.data != nullptr ? cols : a.x.ld);
     const float mean = sums.sum(sum) / static_cast<float>(cols);
     float square = 0.f;
-    for (int c = threadIdx.x * kRun; c < cols; c += step) {
-      float v[kRun];
-      get<kRun>(from, type, at + c, v);
+    for (int c = 0; c < cols; c += kStep) {
+      Raw<kRun, kN> x;
+      Row<kRun, kN> s;
+      x.load(from, s_type, at + c, t, kWideThreads, cols - c);
+      s.take(x, s_type);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) square = fmaf(v[i] - mean, v[i] - mean, square);
+      for (int n = 0; n < kN; ++n) {
+        const bool there = (n * kWideThreads + t) * kRun < cols - c;
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          const float d = s.v[n][i] - mean;
+          square = fmaf(d, there ? d : 0.f, square);
+        }
+      }
     }
     const float rstd = 1.f / sqrtf(sums.sum(square) / static_cast<float>(cols) + h.eps);
-    if (a.mean != nullptr && threadIdx.x == 0) {
+    if (a.mean != nullptr && t == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
-    for (int c = threadIdx.x * kRun; c < cols; c += step) {
-      float v[kRun], w[kRun], b[kRun];
-      get<kRun>(from, type, at + c, v);
-      if (h.weight != nullptr) get<kRun>(h.weight, h.weight_type, c, w);
-      if (h.bias != nullptr) get<kRun>(h.bias, h.weight_type, c, b);
+    for (int c = 0; c < cols; c += kStep) {
+      Raw<kRun, kN> x, w, b;
+      Row<kRun, kN> s, other;
+      x.load(from, s_type, at + c, t, kWideThreads, cols - c);
+      if (h.weight != nullptr) w.load(h.weight, w_type, c, t, kWideThreads, cols - c);
+      if (h.bias != nullptr) b.load(h.bias, w_type, c, t, kWideThreads, cols - c);
+      s.take(x, s_type);
+      if (h.weight != nullptr) other.take(w, w_type);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        v[i] = (v[i] - mean) * rstd;
-        if (h.weight != nullptr) v[i] *= w[i];
-        if (h.bias != nullptr) v[i] += b[i];
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) s.v[n][i] = (s.v[n][i] - mean) * (h.weight != nullptr ? rstd * other.v[n][i] : rstd);
+      if (h.bias != nullptr) {
+        other.take(b, w_type);
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int i = 0; i < kRun; ++i) s.v[n][i] += other.v[n][i];
       }
-      put<kRun>(a.y, a.y_type, row * cols + c, v);
+      s.store(a.y, y_type, row * cols + c, t, kWideThreads, cols - c);
     }
   }
 }

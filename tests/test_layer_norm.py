@@ -330,6 +330,25 @@ def test_places_beyond_32_bits(emptied, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [17, 31, 33, 63, 65, 127, 129, 253, 259, 511, 513, 1023, 1025, 1535, 1537, 2047, 2049, 4095, 4099, 6143, 6145, 8191, 8209])
+@pytest.mark.parametrize("dtype,stream", [(torch.float32, None), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+def test_rows_that_begin_anywhere(cuda_device, cols, dtype, stream):
+    # more rows than blocks have at once, where the row is short; a few more than one else
+    t = _inputs(5000 if cols < 300 else 600, cols, dtype, stream, dtype, torch.float32, cuda_device, seed=cols)
+    _check(t, None, *_call(t, None))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [8200, 8196, 12290, 24584, 40961])
+def test_rows_that_are_long(cuda_device, cols):
+    # more rows than blocks, and than the sums' parts take at a time
+    t = _inputs(650, cols, torch.bfloat16, torch.float32, torch.bfloat16, torch.float32, cuda_device, seed=cols)
+    _check(t, None, *_call(t, None))
+    t = _inputs(5, cols, torch.bfloat16, None, torch.float32, None, cuda_device, seed=cols)
+    _check(t, torch.float32, *_call(t, torch.float32))
+
+
+@pytest.mark.gpu
 def test_rows_whose_numbers_32_bits_cannot_count_are_refused(cuda_device):
     one = torch.ones(1, device=cuda_device, dtype=torch.bfloat16)
     for shape in ((1, 2 ** 31 - 256), (2 ** 31, 1), (2, 2 ** 31)):
