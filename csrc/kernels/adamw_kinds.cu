@@ -14,8 +14,8 @@
 // bf16 parameters are the upper 16 bits of an fp32 value, rounded to nearest; `low` is what these leave of its bits, as a whole number.  A program that
 // changes the parameter moves the value with it.  (fp32 copies of the parameters: 2 more bytes of traffic and of memory each, and they go stale.)
 //
-// 16.03 bytes a number (fp32 parameters), 14.03 (bf16), where fp32 moments have 28.  57 instructions a number, as pairs of numbers go through
-// the packed fp32 instructions (70, and 78 % of the issue slots, without): 48 M numbers 143 us (5.6 TB/s), bf16 138 (5.1), with fp32 moments
+// 16.03 bytes a number (fp32 parameters), 14.03 (bf16), where fp32 moments have 28.  57 instructions a number (fp32 parameters), as pairs of numbers go
+// through the packed fp32 instructions, 65 % of the issue slots, bf16 72 (78 without): 48 M numbers 143 us (5.6 TB/s), bf16 138 (5.1), with fp32 moments
 // 206 (6.4); 96 M 269 (6.0), 271 (5.2) and 396 (6.6).  A warp has a group, so that what the group shares is two reductions; CTAs of two warps, ten to
 // an SM (twelve, whose threads have fewer registers: 148, 139 and 207).  What is left is the start of each CTA, three reads behind each other,
 // which the others have to fill.  (Without what is asked for ahead, or that in registers, which leaves half as many warps: 219; with
