@@ -149,6 +149,28 @@ struct LayerTiles {
 };
 cudaError_t launch_layer_tiles(const LayerTiles& g, cudaStream_t s);
 
+// A small layer of fp32, each direction one launch (kernels/linear_small.cu, with both sides measured): short reductions, and so little to multiply that
+// products of the library and passes around them are mostly their launches.
+inline bool layer_is_small(int64_t tokens, int64_t in, int64_t out) { return in <= 256 && tokens <= 8192 && out <= 8192 && tokens * in * out <= 1ll << 26; }
+inline bool layer_is_small_backward(int64_t tokens, int64_t in, int64_t out) {
+  return out <= 512 && tokens <= 1024 && in <= 8192 && tokens * in * out <= 1ll << 26;
+}
+struct LayerSmall {
+  int64_t tokens, in, out;
+  const float *x, *weight, *bias, *residual;  // rows ld.. apart; bias and residual may be null
+  int64_t ldx, ldw, ldr;
+  LayerActivation activation;
+  float *y, *z;  // rows of `out`; z null where it is not kept
+};
+cudaError_t launch_layer_small(const LayerSmall& g, cudaStream_t s);
+struct LayerSmallBackward {
+  int64_t tokens, in, out;
+  const float *dz, *x, *weight;
+  int64_t ldz, ldx, ldw;
+  float *dx, *dw, *dbias;  // one behind the other; null where nobody asks
+};
+cudaError_t launch_layer_small_backward(const LayerSmallBackward& g, cudaStream_t s);
+
 // What stands around the products, in one pass each (kernels/linear_pass.cu).  Rows `ld` numbers apart of one type.
 struct LayerRows {
   const void* data;

@@ -148,9 +148,23 @@ Gradients backward16(const at::Tensor& dy, const at::Tensor& x, const at::Tensor
   return r;
 }
 
-// ---- fp32: the linear layer's products, and a pass behind or before them -------------------------------------------
-at::Tensor forward32(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, LayerActivation act, const at::Tensor& residual, at::Tensor* z_out) {
+// ---- fp32: the linear layer's products, and a pass behind or before them; small ones whole ------------------------------
+// (what the linear layer has on the tensor cores stays there)
+bool rows_ok(const at::Tensor& t) { return t.size(1) == 1 || t.stride(1) == 1; }
+bool goes_small(const at::Tensor& x, const at::Tensor& w, bool small) { return small && x.size(0) > 0 && rows_ok(x) && rows_ok(w) && !linear_native(x, w, c10::nullopt); }
+at::Tensor forward32(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias_in, LayerActivation act, const at::Tensor& residual, at::Tensor* z_out) {
   c10::cuda::CUDAGuard guard(x.device());
+  if (goes_small(x, w, kern::layer_is_small(x.size(0), w.size(1), w.size(0)))) {
+    const at::Tensor bias = bias_in.defined() ? bias_in.contiguous() : bias_in;
+    at::Tensor y = at::empty({x.size(0), w.size(0)}, x.options());
+    if (z_out != nullptr) *z_out = at::empty(y.sizes(), x.options());
+    const kern::LayerRows r = layer_rows(residual);
+    const kern::LayerSmall g{x.size(0), w.size(1), w.size(0), x.const_data_ptr<float>(), w.const_data_ptr<float>(), bias.defined() ? bias.const_data_ptr<float>() : nullptr,
+                             static_cast<const float*>(r.data), row_stride(x), row_stride(w), r.ld, act, y.data_ptr<float>(), z_out != nullptr ? z_out->data_ptr<float>() : nullptr};
+    OPS_CK(kern::launch_layer_small(g, at::cuda::getCurrentCUDAStream()));
+    return y;
+  }
+  const at::Tensor& bias = bias_in;
   const at::Tensor z = mccl::linear(x, w, bias.defined() ? c10::optional<at::Tensor>(bias) : c10::nullopt).contiguous();
   if (z_out != nullptr) *z_out = z;
   if (act == LayerActivation::kNone && !residual.defined()) return z;
@@ -161,6 +175,17 @@ at::Tensor forward32(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
 Gradients backward32(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const at::Tensor& z, LayerActivation act, const Needs& need) {
   c10::cuda::CUDAGuard guard(x.device());
   Gradients r;
+  if (goes_small(x, w, kern::layer_is_small_backward(x.size(0), w.size(1), w.size(0)))) {
+    const at::Tensor dz = derive(dy, z, w.size(0), act, x.options(), {true, true, false}, r);
+    if (need.x) r.x = at::empty(x.sizes(), x.options());
+    if (need.w) r.w = at::empty(w.sizes(), w.options());
+    if (need.bias) r.bias = at::empty({w.size(0)}, w.options());
+    auto to = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+    const kern::LayerSmallBackward g{x.size(0), w.size(1), w.size(0), dz.const_data_ptr<float>(), x.const_data_ptr<float>(), w.const_data_ptr<float>(),
+                                     row_stride(dz), row_stride(x), row_stride(w), to(r.x), to(r.w), to(r.bias)};
+    OPS_CK(kern::launch_layer_small_backward(g, at::cuda::getCurrentCUDAStream()));
+    return r;
+  }
   const at::Tensor dz = derive(dy, z, w.size(0), act, x.options(), need, r);
   if (need.x || need.w) std::tie(r.x, r.w) = linear_gradients(dz, x, w, need.x, need.w);
   return r;

@@ -71,6 +71,7 @@ CUDA_SOURCES = [
     "kernels/linear_few.cu",
     "kernels/linear_pass.cu",
     "kernels/linear_tiles.cu",
+    "kernels/linear_small.cu",
     "kernels/norm_forward.cu",
     "kernels/norm_backward.cu",
     "kernels/noalloc.cu",

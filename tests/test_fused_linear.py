@@ -458,6 +458,33 @@ def test_one_tensor_twice(device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("activation", [None, "gelu"])
+@pytest.mark.parametrize("tokens,width,out", [(1, 1, 1), (31, 33, 65), (1024, 64, 512), (1025, 64, 512), (1000, 128, 513), (8192, 5, 7), (8200, 5, 7), (64, 257, 130), (700, 77, 176),
+                                              (2, 256, 8192), (3, 5000, 100)])
+def test_small_in_full_precision(cuda_device, tokens, width, out, activation):
+    # either side of where products are the library's, and sums in both directions over parts of a stage
+    t = _inputs(tokens, width, out, torch.float32, torch.float32, True, cuda_device)
+    _check(t, activation, _call(t, activation))
+    t = {k: v.detach() for k, v in t.items()}
+    for k in ("x", "weight", "residual", "dy"):  # rows that lie apart
+        t[k] = torch.cat((t[k], torch.full_like(t[k], math.nan)), 1)[:, :t[k].shape[1]]
+    t["bias"] = torch.stack((t["bias"], t["bias"]), 1)[:, 0]
+    _check(t, activation, _call(t, activation))
+
+
+@pytest.mark.gpu
+def test_small_in_full_precision_one_gradient_alone(cuda_device):
+    t = _inputs(50, 40, 60, torch.float32, None, True, cuda_device)
+    whole = _call(t, None)[1:]
+    for i, leaf in enumerate(_leaves(t)):
+        others = {k: v.detach() for k, v in t.items()}
+        name = ("x", "weight", "bias")[i]
+        others[name].requires_grad_()
+        y = fused_linear(others["x"], others["weight"], others["bias"])
+        assert torch.equal(torch.autograd.grad(y, others[name], t["dy"])[0], whole[i])
+
+
+@pytest.mark.gpu
 def test_two_threads_on_streams_of_their_own(cuda_device):
     from concurrent.futures import ThreadPoolExecutor
     cases = [_inputs(tokens, 264, out, torch.bfloat16, torch.float32, True, cuda_device, seed=out) for tokens, out in ((9, 136), (333, 1032), (3000, 1032), (3000, 520))]
