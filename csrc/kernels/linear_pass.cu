@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kThreads, 2) layer_derive_kernel(const LayerDe
     float all = 0.f;
 #pragma unroll
     for (int p = 0; p < kWarps; ++p) all += sums[p][i];
-    to[c] = all;
+    if (gridDim.y == 1) static_cast<T*>(g.bias)[c] = Traits<T>::store(all);  // of few rows the one block's are the whole sums
+    else to[c] = all;
   }
 }
 // Adds up the blocks' sums: 32 columns a block, whose warps share the parts.
@@ -154,7 +155,7 @@ cudaError_t derive(const LayerDerive& g, cudaStream_t s) {
   note_launch();
   with_activation(g.activation, [&](auto act) { layer_derive_kernel<T, D, decltype(act)::kValue, kV><<<grid, kThreads, 0, s>>>(g, ceil_div(g.rows, parts)); });
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || g.bias == nullptr) return e;
+  if (e != cudaSuccess || g.bias == nullptr || parts == 1) return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
