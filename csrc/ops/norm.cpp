@@ -60,16 +60,18 @@ void check_call(const at::Tensor& x, const Affine& p, double eps, const at::Tens
   MCCL_CHECK_T(TensorError, eps > 0 && std::isfinite(eps), kWhat << ": eps must be positive");
 }
 
-// y and, with a residual, the sum, as rows; mean and rstd where they are asked for.
-std::vector<at::Tensor> forward_of(const at::Tensor& x, const Affine& p, double eps, const at::Tensor& residual, at::ScalarType dtype, at::Tensor* stats) {
+// y and, with a residual, the sum, of x's shape; mean and rstd where they are asked for, and the rows that were normed.
+std::vector<at::Tensor> forward_of(const at::Tensor& x_in, const Affine& p, double eps, const at::Tensor& residual_in, at::ScalarType dtype, at::Tensor* stats,
+                                   at::Tensor* normed) {
+  const at::Tensor x = rows_of(x_in), residual = residual_in.defined() ? rows_of(residual_in) : residual_in;
   c10::cuda::CUDAGuard guard(x.device());
   kern::NormForward a{};
   a.shape = shape_of(x, p, eps);
   a.x = norm_rows(x);
-  at::Tensor sum, y = at::empty(x.sizes(), x.options().dtype(dtype));
+  at::Tensor sum, y = at::empty(x_in.sizes(), x.options().dtype(dtype));
   if (residual.defined()) {
     a.residual = norm_rows(residual);
-    sum = at::empty(x.sizes(), residual.options());
+    sum = at::empty(x_in.sizes(), residual.options());
     a.sum = sum.data_ptr();
   }
   a.y = y.data_ptr();
@@ -79,25 +81,28 @@ std::vector<at::Tensor> forward_of(const at::Tensor& x, const Affine& p, double 
     a.mean = stats->data_ptr<float>();
     a.rstd = a.mean + x.size(0);
   }
+  if (normed != nullptr) *normed = sum.defined() ? sum : x;
   OPS_CK(kern::launch_norm_forward(a, at::cuda::getCurrentCUDAStream()));
   if (sum.defined()) return {y, sum};
   return {y};
 }
 
+// Takes and gives tensors of the caller's shape.  As views of them rows would each have a gradient of their own over one memory, and leaves keep
+// as theirs what nothing else seems to hold: x and the residual, whose gradients are the same numbers, would add up the next pass's in one place.
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias,
                                const c10::optional<at::Tensor>& residual, double eps, int64_t dtype) {
     const Affine p{weight.value_or(at::Tensor()), bias.value_or(at::Tensor())};
     const bool with = residual.has_value();
-    at::Tensor stats;
-    auto out = forward_of(x, p, eps, residual.value_or(at::Tensor()), static_cast<at::ScalarType>(dtype), &stats);
-    ctx->save_for_backward({with ? out[1] : x, p.weight, p.bias, stats});
+    at::Tensor stats, normed;
+    auto out = forward_of(x, p, eps, residual.value_or(at::Tensor()), static_cast<at::ScalarType>(dtype), &stats, &normed);
+    ctx->save_for_backward({normed, p.weight, p.bias, stats});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["dtype"] = dtype;
     ctx->saved_data["with"] = with;
     ctx->saved_data["x_type"] = static_cast<int64_t>(x.scalar_type());
-    ctx->saved_data["rows"] = x.size(0);
-    ctx->saved_data["cols"] = x.size(1);
+    ctx->saved_data["sizes"] = x.sizes().vec();
+    ctx->saved_data["normed"] = normed.sizes().vec();
     ctx->saved_data["sum_type"] = static_cast<int64_t>(with ? out[1].scalar_type() : x.scalar_type());
     return out;
   }
@@ -108,11 +113,13 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     at::Tensor dy = grads[0], ds = with ? grads[1] : at::Tensor();
     if (!dy.defined() && !ds.defined()) return variable_list(6);
     const auto saved = ctx->get_saved_variables();
-    const int64_t rows = ctx->saved_data["rows"].toInt(), cols = ctx->saved_data["cols"].toInt();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector(), normed = ctx->saved_data["normed"].toIntVector();
     const auto x_type = static_cast<at::ScalarType>(ctx->saved_data["x_type"].toInt()), sum_type = static_cast<at::ScalarType>(ctx->saved_data["sum_type"].toInt()),
                dtype = static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt());
     const at::Device device = (dy.defined() ? dy : ds).device();
-    check_saved(saved[0], {rows, cols}, sum_type, device, kWhat);
+    check_saved(saved[0], normed, sum_type, device, kWhat);
+    const at::Tensor s = rows_of(saved[0]);
+    const int64_t rows = s.size(0), cols = s.size(1);
     check_saved(saved[3], {2, rows}, at::kFloat, device, kWhat);
     Affine p{saved[1], saved[2]};
     for (at::Tensor* t : {&p.weight, &p.bias}) {
@@ -121,11 +128,11 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
       *t = t->contiguous();
     }
     c10::cuda::CUDAGuard guard(device);
-    const at::Tensor s = rows_of(saved[0]), stats = saved[3].contiguous();
-    if (!dy.defined()) dy = at::zeros({rows, cols}, s.options().dtype(dtype));
+    const at::Tensor stats = saved[3].contiguous();
+    if (!dy.defined()) dy = at::zeros(sizes, s.options().dtype(dtype));
     for (const auto& [g, type] : {std::pair<const at::Tensor&, at::ScalarType>(dy, dtype), std::pair<const at::Tensor&, at::ScalarType>(ds, sum_type)}) {
       if (!g.defined()) continue;
-      check_saved(g, {rows, cols}, type, device, kWhat);
+      check_saved(g, sizes, type, device, kWhat);
     }
     size_t input = 0;  // tensors that there are not are not counted
     auto needed = [&](bool there) { return there && ctx->needs_input_grad(input++); };
@@ -139,8 +146,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     a.mean = stats.const_data_ptr<float>();
     a.rstd = a.mean + rows;
     at::Tensor dx, dresidual, dweight, dbias, partial;
-    if (need_x) dx = at::empty({rows, cols}, s.options().dtype(x_type));
-    if (need_residual) dresidual = need_x && x_type == sum_type ? dx : at::empty({rows, cols}, s.options());
+    if (need_x) dx = at::empty(sizes, s.options().dtype(x_type));
+    if (need_residual) dresidual = need_x && x_type == sum_type ? dx : at::empty(sizes, s.options());
     a.dx = need_x ? dx.data_ptr() : nullptr;
     a.dx_type = x_type == at::kFloat ? kern::Elem::kF32 : x_type == at::kHalf ? kern::Elem::kF16 : kern::Elem::kBF16;
     a.dresidual = need_residual && !dresidual.is_same(dx) ? dresidual.data_ptr() : nullptr;
@@ -168,17 +175,9 @@ std::vector<at::Tensor> layer_norm(const at::Tensor& x, const std::optional<at::
   check_call(x, p, eps, r, y_type);
   bool grad = false;
   for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&x, &p.weight, &p.bias, &r}) grad = grad || (t->defined() && t->requires_grad());
-  const at::Tensor rows = rows_of(x), other = r.defined() ? rows_of(r) : r;
-  std::vector<at::Tensor> out;
-  if (grad && at::GradMode::is_enabled()) {
-    auto given = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
-    out = LayerNormFn::apply(rows, given(p.weight), given(p.bias), given(other), eps, static_cast<int64_t>(y_type));
-  } else {
-    out = forward_of(rows, p, eps, other, y_type, nullptr);
-  }
-  if (x.dim() != 2)
-    for (at::Tensor& t : out) t = t.view(x.sizes());
-  return out;
+  if (!grad || !at::GradMode::is_enabled()) return forward_of(x, p, eps, r, y_type, nullptr, nullptr);
+  auto given = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+  return LayerNormFn::apply(x, given(p.weight), given(p.bias), given(r), eps, static_cast<int64_t>(y_type));
 }
 
 }  // namespace mccl

@@ -376,3 +376,22 @@ def test_one_tensor_twice(device):
     for a, b in zip(got, want):
         # a few dozen roundings of terms a few times the result's size
         assert torch.allclose(a, b, rtol=64 * 2.0 ** -24, atol=64 * 2.0 ** -24 * b.abs().max().item())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,stream", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("shape", [(24,), (6, 24), (2, 3, 24), (2, 3, 4, 24)])
+@pytest.mark.parametrize("only", [None, 0, 1])
+def test_gradients_of_leaves_have_memory_of_their_own(device, dtype, stream, shape, only):
+    gen = torch.Generator().manual_seed(4)
+    x, r = torch.randn(shape, generator=gen).to(device, dtype).requires_grad_(), torch.randn(shape, generator=gen).to(device, stream).requires_grad_()
+    given = [torch.randn(shape, generator=gen).to(device, t) for t in (dtype, stream)]
+    kept = [g.clone() for g in given]
+    for turn in (1, 2):
+        out = layer_norm(x, residual=r)
+        (dx, dr) = torch.autograd.grad([o for i, o in enumerate(out) if only in (None, i)], (x, r), [g for i, g in enumerate(given) if only in (None, i)], retain_graph=True)
+        torch.autograd.backward([o for i, o in enumerate(out) if only in (None, i)], [g for i, g in enumerate(given) if only in (None, i)])
+        # (the same numbers twice are twice these, exactly)
+        assert torch.equal(x.grad, turn * dx) and torch.equal(r.grad, turn * dr) and out[0].shape == out[1].shape == shape
+        assert x.grad.untyped_storage().data_ptr() != r.grad.untyped_storage().data_ptr()
+    assert all(torch.equal(a, b) for a, b in zip(given, kept))
