@@ -54,14 +54,14 @@ kern::GatedShape shape_of(const at::Tensor& x, const at::Tensor& w) {
   return {x.size(0), w.size(0), w.size(1), x.scalar_type() == at::kBFloat16, kern::GatedActivation::kSilu, kern::GatedKeep::kNone};
 }
 
-// y of 16-bit rows; x w^T + bias to `z` where there is one to keep.
-at::Tensor forward16(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias_in, LayerActivation act, const at::Tensor& residual, at::Tensor* z,
-                     int64_t wait_limit = -1) {
+// y of 16-bit rows, of the shape `sizes`; x w^T + bias to `z` where there is one to keep.
+at::Tensor forward16(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias_in, LayerActivation act, const at::Tensor& residual, at::IntArrayRef sizes,
+                     at::Tensor* z, int64_t wait_limit = -1) {
   check_waits(x);
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t tokens = x.size(0), out = w.size(0);
   const auto type = residual.defined() ? residual.scalar_type() : x.scalar_type();
-  at::Tensor y = at::empty({tokens, out}, x.options().dtype(type));
+  at::Tensor y = at::empty(sizes, x.options().dtype(type));
   if (z != nullptr) *z = at::empty({tokens, kern::gated_row(out)}, x.options());
   if (tokens == 0) return y;
   const at::Tensor bias = bias_in.defined() ? bias_in.contiguous() : bias_in;
@@ -152,12 +152,13 @@ Gradients backward16(const at::Tensor& dy, const at::Tensor& x, const at::Tensor
 // (what the linear layer has on the tensor cores stays there)
 bool rows_ok(const at::Tensor& t) { return t.size(1) == 1 || t.stride(1) == 1; }
 bool goes_small(const at::Tensor& x, const at::Tensor& w, bool small) { return small && x.size(0) > 0 && rows_ok(x) && rows_ok(w) && !linear_native(x, w, c10::nullopt); }
-at::Tensor forward32(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias_in, LayerActivation act, const at::Tensor& residual, at::Tensor* z_out) {
+at::Tensor forward32(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias_in, LayerActivation act, const at::Tensor& residual, at::IntArrayRef sizes,
+                     at::Tensor* z_out) {
   c10::cuda::CUDAGuard guard(x.device());
   if (goes_small(x, w, kern::layer_is_small(x.size(0), w.size(1), w.size(0)))) {
     const at::Tensor bias = bias_in.defined() ? bias_in.contiguous() : bias_in;
-    at::Tensor y = at::empty({x.size(0), w.size(0)}, x.options());
-    if (z_out != nullptr) *z_out = at::empty(y.sizes(), x.options());
+    at::Tensor y = at::empty(sizes, x.options());
+    if (z_out != nullptr) *z_out = at::empty({x.size(0), w.size(0)}, x.options());
     const kern::LayerRows r = layer_rows(residual);
     const kern::LayerSmall g{x.size(0), w.size(1), w.size(0), x.const_data_ptr<float>(), w.const_data_ptr<float>(), bias.defined() ? bias.const_data_ptr<float>() : nullptr,
                              static_cast<const float*>(r.data), row_stride(x), row_stride(w), r.ld, act, y.data_ptr<float>(), z_out != nullptr ? z_out->data_ptr<float>() : nullptr};
@@ -167,8 +168,8 @@ at::Tensor forward32(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
   const at::Tensor& bias = bias_in;
   const at::Tensor z = mccl::linear(x, w, bias.defined() ? c10::optional<at::Tensor>(bias) : c10::nullopt).contiguous();
   if (z_out != nullptr) *z_out = z;
-  if (act == LayerActivation::kNone && !residual.defined()) return z;
-  at::Tensor y = at::empty(z.sizes(), z.options());
+  if (act == LayerActivation::kNone && !residual.defined()) return sizes.size() == 2 ? z : at::_unsafe_view(z, sizes);
+  at::Tensor y = at::empty(sizes, z.options());
   OPS_CK(kern::launch_layer_finish(z.const_data_ptr<float>(), layer_rows(residual), y.data_ptr<float>(), z.size(0), z.size(1), act, at::cuda::getCurrentCUDAStream()));
   return y;
 }
@@ -191,15 +192,29 @@ Gradients backward32(const at::Tensor& dy, const at::Tensor& x, const at::Tensor
   return r;
 }
 
+std::vector<int64_t> sizes_of(const at::Tensor& x, const at::Tensor& w) {
+  auto sizes = x.sizes().vec();
+  sizes.back() = w.size(0);
+  return sizes;
+}
+at::Tensor forward_of(const at::Tensor& rows, const at::Tensor& w, const at::Tensor& bias, LayerActivation act, const at::Tensor& residual_in, at::IntArrayRef sizes,
+                      at::Tensor* z) {
+  const at::Tensor residual = residual_in.defined() ? rows_of(residual_in) : residual_in;
+  return rows.scalar_type() == at::kFloat ? forward32(rows, w, bias, act, residual, sizes, z) : forward16(rows, w, bias, act, residual, sizes, z);
+}
+
+// Takes and gives tensors of the caller's shape: the residual's gradient is the result's itself, and as a view of it, which nothing else seems to hold, a
+// leaf would keep the caller's memory as its own.
 struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
-  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x_in, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
                             const c10::optional<at::Tensor>& residual, int64_t act) {
     const auto activation = static_cast<LayerActivation>(act);
+    const at::Tensor x = rows_of(x_in);
     c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
     at::Tensor z;
     at::Tensor* const keep = activation == LayerActivation::kNone ? nullptr : &z;
-    const at::Tensor y = x.scalar_type() == at::kFloat ? forward32(x, w, b, activation, r, keep) : forward16(x, w, b, activation, r, keep);
+    const at::Tensor y = forward_of(x, w, b, activation, r, sizes_of(x_in, w), keep);
     ctx->save_for_backward({x, w, z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b.defined();
@@ -209,6 +224,7 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     ctx->saved_data["rows"] = x.size(0);
     ctx->saved_data["in"] = w.size(1);
     ctx->saved_data["out"] = w.size(0);
+    ctx->saved_data["sizes"] = x_in.sizes().vec();
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -222,8 +238,11 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     const auto act = static_cast<LayerActivation>(ctx->saved_data["act"].toInt());
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), y_type = static_cast<at::ScalarType>(ctx->saved_data["y_type"].toInt());
     const int64_t rows = ctx->saved_data["rows"].toInt(), in = ctx->saved_data["in"].toInt(), out = ctx->saved_data["out"].toInt();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    auto y_sizes = sizes;
+    y_sizes.back() = out;
     const at::Device device = dy_in.device();
-    check_saved(dy_in, {rows, out}, y_type, device, kWhat);
+    check_saved(dy_in, y_sizes, y_type, device, kWhat);
     check_saved(saved[0], {rows, in}, type, device, kWhat);
     check_saved(saved[1], {out, in}, type, device, kWhat);
     if (act != LayerActivation::kNone) check_saved(saved[2], {rows, type == at::kFloat ? out : kern::gated_row(out)}, type, device, kWhat);
@@ -235,7 +254,7 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     const Needs need{need_x, need_w, need_bias};
     const at::Tensor dy = rows_of(dy_in), z = act != LayerActivation::kNone ? rows_of(saved[2]) : at::Tensor();
     const Gradients r = type == at::kFloat ? backward32(dy, saved[0], saved[1], z, act, need) : backward16(dy, saved[0], saved[1], z, act, need);
-    return {r.x, r.w, r.bias, need_residual ? dy_in : at::Tensor(), {}};
+    return {need_x ? r.x.view(sizes) : at::Tensor(), r.w, r.bias, need_residual ? dy_in : at::Tensor(), {}};
   }
 };
 
@@ -246,28 +265,17 @@ at::Tensor fused_linear(const at::Tensor& x, const at::Tensor& w, const std::opt
   const LayerActivation act = activation_of(activation);
   const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
   check_call(x, w, b, r);
-  const at::Tensor rows = rows_of(x), other = r.defined() ? rows_of(r) : r;
   bool grad = false;
   for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&x, &w, &b, &r}) grad = grad || (t->defined() && t->requires_grad());
-  at::Tensor y;
-  if (grad && at::GradMode::is_enabled()) {
-    auto given = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
-    y = FusedLinearFn::apply(rows, w, given(b), given(other), static_cast<int64_t>(act));
-  } else if (x.scalar_type() == at::kFloat) {
-    y = forward32(rows, w, b, act, other, nullptr);
-  } else {
-    y = forward16(rows, w, b, act, other, nullptr);
-  }
-  if (x.dim() == 2) return y;
-  auto sizes = x.sizes().vec();
-  sizes.back() = w.size(0);
-  return y.view(sizes);
+  if (!grad || !at::GradMode::is_enabled()) return forward_of(rows_of(x), w, b, act, r, sizes_of(x, w), nullptr);
+  auto given = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+  return FusedLinearFn::apply(x, w, given(b), given(r), static_cast<int64_t>(act));
 }
 
 at::Tensor fused_linear_with_limit(const at::Tensor& x, const at::Tensor& w, int64_t wait_limit) {
   check_call(x, w, at::Tensor(), at::Tensor());
   MCCL_CHECK_T(TensorError, wait_limit >= 0 && x.dim() == 2 && x.scalar_type() != at::kFloat, "not a call for the 16-bit kernels");
-  return forward16(x, w, at::Tensor(), LayerActivation::kNone, at::Tensor(), nullptr, wait_limit);
+  return forward16(x, w, at::Tensor(), LayerActivation::kNone, at::Tensor(), {x.size(0), w.size(0)}, nullptr, wait_limit);
 }
 
 }  // namespace mccl

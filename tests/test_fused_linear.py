@@ -500,3 +500,23 @@ def test_two_threads_on_streams_of_their_own(cuda_device):
     with ThreadPoolExecutor(len(cases)) as pool:
         for got, one in zip(pool.map(many, cases), want):
             assert all(torch.equal(a, b) for g in got for a, b in zip(g, one))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,activation", [(torch.float32, None), (torch.float32, "gelu"), (torch.bfloat16, None), (torch.bfloat16, "gelu")])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("shape", [(24,), (6, 24), (2, 3, 24), (2, 3, 4, 24)])
+def test_gradients_of_leaves_have_memory_of_their_own(device, dtype, activation, wide, shape):
+    gen = torch.Generator().manual_seed(4)
+    kind = torch.float32 if wide else dtype
+    x, r, w = (torch.randn(s, generator=gen).to(device, t).requires_grad_() for s, t in ((shape, dtype), (shape, kind), ((24, 24), dtype)))
+    given = torch.randn(shape, generator=gen).to(device, kind)
+    kept = given.clone()
+    for turn in (1, 2):
+        y = fused_linear(x, w, activation=activation, residual=r)
+        one = torch.autograd.grad(y, (x, w, r), given, retain_graph=True)
+        y.backward(given)
+        # (the same numbers twice are twice these, exactly)
+        assert y.shape == shape and all(torch.equal(t.grad, turn * g) for t, g in zip((x, w, r), one))
+        assert len({t.untyped_storage().data_ptr() for t in (x.grad, w.grad, r.grad, given)}) == 4
+    assert torch.equal(given, kept)
