@@ -183,7 +183,10 @@ class AdamWPlan {
                         "AdamWPlan: moments in 8 bits are float8_e4m3fn and float8_e5m2, padded to whole groups of " << kern::kMomentGroup
                             << " from multiples of 8 bytes on, with a float32 scale for each");
     } else {
-      MCCL_CHECK_TENSOR(fits(m_[i], at::kFloat, p.numel()) && fits(v_[i], at::kFloat, p.numel()), "AdamWPlan: moments are float32 of the parameter's size");
+      // (scales are what the kernel takes moments of 8 bits by)
+      MCCL_CHECK_TENSOR(fits(m_[i], at::kFloat, p.numel()) && fits(v_[i], at::kFloat, p.numel()) && !extra_[i].exp_avg_scale.defined() &&
+                            !extra_[i].exp_avg_sq_scale.defined(),
+                        "AdamWPlan: moments are float32 of the parameter's size, without scales");
     }
   }
   // Rows of kern::AdamWTensor.

@@ -473,3 +473,17 @@ def _in_backward(rank, ws):
 def test_updated_inside_backward(python_hook, dtype, bits):
     env = {"MCCL_PYTHON_BUCKET_HOOK": python_hook, "TEST_DTYPE": dtype, "TEST_BITS": str(bits)}
     run_workers(_in_backward, 1, device="cuda", timeout=180, env=env)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("which", [("exp_avg_scale",), ("exp_avg_sq_scale",), ("exp_avg_scale", "exp_avg_sq_scale")])
+def test_moments_of_32_bits_beside_scales_are_refused(cuda_device, dtype, which):
+    p = torch.nn.Parameter(torch.ones(300, device=cuda_device, dtype=dtype))
+    opt = FusedAdamW([p])
+    for name in which:
+        opt._state_of(p)[name] = torch.ones(2, device=cuda_device)
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="without scales"):
+        opt.step()
+    assert torch.equal(p, torch.ones_like(p)) and float(opt.state[p]["step"]) == 0
