@@ -101,8 +101,8 @@ template <Out kOut>
 constexpr bool kWideY = kOut == kLayer32 || kOut == kLayer32Keep;
 
 // Sums that leave in 32 bits are taken out of tensor memory every kChunk stages (512 of the reduction) and added in registers, rounded to nearest:
-// the tensor cores cut theirs off, 16 products at a time, each time towards zero.  A result is 5e-7 of its size off so, whatever its terms, and 1e-6
-// for each 1024 of them without; of 16 bits it does not show.  The 128 numbers a thread are what the first four warps hand over of their registers:
+// the tensor cores cut theirs off, each time towards zero.  Sums of terms of one sign are 7e-7 of their size too small so, whatever their number, and
+// 6.4e-9 for each term without, which results of 16 bits have room for up to some number of terms (`deepest`, below).  The 128 numbers a thread are what the first four warps hand over of their registers:
 // at launch a thread has 168 (three warps of a quarter SM's 512 a lane), four warps go down to 56 and eight up to 224, as many in all.
 template <Out kOut>
 constexpr bool kAddsUp = kWideY<kOut>;
@@ -130,7 +130,7 @@ struct Job {
   int tiles_i, tiles_j;     // tiles_i: of all results
   int stages, segment;      // of the reduction; stages of its first part (dg Wg, then du Wu)
   int first;                // item
-  int whole;                // items that are whole tiles; behind them tiles whose reduction `splits` pairs share, with partial sums from `part` on
+  int whole, tail;          // items that are whole tiles; behind them `tail` tiles whose reduction is shared by `splits` items, with partial sums from `part` on
   int splits, per_split, part;
   int join;                 // the first such tile among those of all jobs
 };
@@ -169,12 +169,12 @@ struct Item {
       c1 = j.stages;
       part = -1;
     } else {
-      part = item - j.whole;
-      const int t = part / j.splits;
+      // all tiles' first parts, then all second ones: pairs at work at a time read the same part of the reduction
+      const int at = (item - j.whole) / j.tail, t = item - j.whole - at * j.tail;
       tile_place(j, j.whole + t, ti, tj);
-      c0 = (part - t * j.splits) * j.per_split;
+      c0 = at * j.per_split;
       c1 = min(j.stages, c0 + j.per_split);
-      part += j.part;
+      part = j.part + t * j.splits + at;
     }
   }
 };
@@ -1020,17 +1020,30 @@ void share(Plan& l, int64_t tiles, int64_t most, int64_t rows) {
   l.splits = splits;
   l.per_split = per;
 }
+// Weight gradients add up over the tokens, of which there is no end, in tensor memory, where a sum of terms of one sign comes out 6.4e-9 of its size too
+// small for each of them (measured from 4096 to 262144 terms): a sum of more than this many is shared, so that what is lost stays below half of what rounding
+// the result may take, 2.1e-4 of 2^-11 in fp16 and 1.7e-3 of 2^-8 in bf16, whatever the number of tokens.  (Sums over a layer's width are shorter.)
+// 2048 x 2048 fp16 of 65536 tokens 405 us for 354 of sums that are not shared, of 262144 1.49 ms for 1.38.
+int64_t deepest(const GatedShape& s) { return (s.bf16 ? 1 << 18 : 1 << 15) / kDepth; }
+void bound(GatedProduct p, const GatedShape& s, Plan& l) {
+  if ((p != GatedProduct::kWeightUp && p != GatedProduct::kWeightDown) || l.longest() <= deepest(s)) return;
+  l.tail += l.whole;
+  l.whole = 0;
+  l.per_split = ceil_div(l.stages, ceil_div(l.stages, deepest(s)));
+  l.splits = ceil_div(l.stages, l.per_split);
+}
 // One product: whole tiles as long as they fill the device; the rest, less than one tile a pair, is shared along the reduction where that
 // pays.
 void plan_one(GatedProduct p, const GatedShape& s, Plan& l) {
   l = plan_of(p, s);
   const int64_t tail = l.whole % kPairs;
   if (tail > 0) share(l, tail, kPairs / tail, sizes_of(p, s).rows);
+  bound(p, s, l);
 }
 // Stages that a product by itself takes, with 8 us for sums that are joined and 4 for a launch.
 double stages_alone(const Plan& l) {
   const int64_t rounds = ceil_div(l.whole, kPairs);
-  return static_cast<double>(rounds * l.stages + (l.tail > 0 ? l.per_split : 0)) + (l.tail > 0 ? 12.0 : 4.0) / kStageUs;
+  return static_cast<double>(rounds * l.stages + ceil_div(l.tail * l.splits, kPairs) * l.per_split) + (l.tail > 0 ? 12.0 : 4.0) / kStageUs;
 }
 // Several products side by side: whole tiles, but for a product whose tiles are so few and long that the device would wait for them.
 // Whether that is faster than one after the other, of which each leaves part of the device idle in its last round: 8192 tokens of 1024 x
@@ -1051,6 +1064,7 @@ bool plan_together(const GatedProduct* p, const GatedShape& s, int n, Plan* l, i
   bool joins = false;
   for (int i = 0; i < n; ++i) {
     if (2 * l[i].stages > 3 * fair) share(l[i], l[i].whole, ceil_div(l[i].stages, fair), sizes_of(p[i], s).rows);
+    bound(p[i], s, l[i]);
     joins = joins || l[i].tail > 0;
   }
   std::sort(order, order + n, [&](int a, int b) { return l[a].longest() != l[b].longest() ? l[a].longest() > l[b].longest() : a < b; });
@@ -1245,6 +1259,7 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
     j.segment = static_cast<int>(q.segment);
     j.first = static_cast<int>(items);
     j.whole = static_cast<int>(q.whole);
+    j.tail = static_cast<int>(q.tail);
     j.splits = static_cast<int>(q.splits);
     j.per_split = static_cast<int>(q.per_split);
     j.part = static_cast<int>(parts);

@@ -520,3 +520,38 @@ def test_gradients_of_leaves_have_memory_of_their_own(device, dtype, activation,
         assert y.shape == shape and all(torch.equal(t.grad, turn * g) for t, g in zip((x, w, r), one))
         assert len({t.untyped_storage().data_ptr() for t in (x.grad, w.grad, r.grad, given)}) == 4
     assert torch.equal(given, kept)
+
+
+@pytest.fixture
+def emptied():
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tokens,shared", [(torch.float16, 32768, False), (torch.float16, 32769, True), (torch.float16, 262144, True),
+                                                 (torch.bfloat16, 262144, False), (torch.bfloat16, 262145, True)])
+@pytest.mark.parametrize("both", [False, True])
+def test_weight_gradients_of_many_tokens_of_one_sign(emptied, cuda_device, dtype, tokens, shared, both):
+    from mccl_b200 import require_native
+    gen = torch.Generator(device=cuda_device).manual_seed(tokens)
+    x = torch.rand(tokens, 2048, device=cuda_device, generator=gen, dtype=dtype).requires_grad_(both)
+    w = torch.rand(2048, 2048, device=cuda_device, generator=gen, dtype=dtype).requires_grad_()
+    # 64 terms of the sums are of size one
+    dy = torch.rand(tokens, 2048, device=cuda_device, generator=gen, dtype=dtype) * (64.0 / tokens)
+    y = fused_linear(x, w)
+    before = require_native()._kernel_launches()
+    got = torch.autograd.grad(y, (x, w) if both else w, dy)
+    launches = require_native()._kernel_launches() - before
+    if not both:
+        assert launches == (2 if shared else 1)  # sums that are shared are joined by a second one
+    at = torch.arange(0, 2048, 7, device=cuda_device)
+    want = dy[:, at].double().t() @ x.detach()[:, at].double()
+    # a part has 2^15 (bf16 2^18) terms at most, each 8 of them cut off at 2^-23; parts are added up in fp32, and the result rounded once
+    deepest = 1 << (15 if dtype is torch.float16 else 18)
+    off = ((got[-1][at][:, at].double() - want).abs() / want).max()
+    assert off <= (min(tokens, deepest) / 8 + 4) * 2.0 ** -23 + 16 * U + ROUNDOFF[dtype] * 1.01
+    if both:
+        rows = torch.arange(0, tokens, tokens // 97, device=cuda_device)
+        want = dy[rows].double() @ w.detach().double()
+        assert ((got[0][rows].double() - want).abs() / want).max() <= _sum(dtype, 2048) + ROUNDOFF[dtype] * 1.01
