@@ -72,19 +72,16 @@ struct Act16 {
   }
   template <LayerActivation kAct, typename N>
   static __device__ __forceinline__ N slope(N z) {
-    if constexpr (kAct == LayerActivation::kRelu) {
-      return each_of(z, [](float z) { return z > 0.f ? 1.f : z != z ? z : 0.f; });
-    } else if constexpr (kAct == LayerActivation::kSilu) {
+    static_assert(kAct != LayerActivation::kNone && kAct != LayerActivation::kRelu, "one and a choice");
+    if constexpr (kAct == LayerActivation::kSilu) {
       const N s = logistic(z);
       return fma_of(z, fma_of(N(-1.f) * s, s, s), s);
     } else if constexpr (kAct == LayerActivation::kGelu) {
       const Normal<N> n = normal(z);
       return n.share + n.slope;
-    } else if constexpr (kAct == LayerActivation::kGeluTanh) {
+    } else {
       const N square = each_of(z * z, [](float x) { return fminf(x, 1e30f); }), s = cubic(z, square);
       return fma_of(z * fma_of(N(-1.f) * s, s, s), fma_of(N(kGelu * 3.f * kCubic), square, N(kGelu)), s);
-    } else {
-      return N(1.f);
     }
   }
   // Of kN numbers, each by its value.
@@ -105,19 +102,31 @@ struct Act32 {
   }
   template <LayerActivation kAct>
   static __device__ __forceinline__ float slope(float z) {
+    static_assert(kAct != LayerActivation::kNone && kAct != LayerActivation::kRelu, "one and a choice");
     if constexpr (kAct == LayerActivation::kSilu || kAct == LayerActivation::kGeluTanh) {
       constexpr bool silu = kAct == LayerActivation::kSilu;
       const float s = gate_of(z, silu), t = s * (1.f - s);
       // (where the curve is flat the cubic's slope may be infinite)
       return t > 0.f ? s + z * t * (silu ? 1.f : kGelu * (1.f + 3.f * kCubic * z * z)) : s;
-    } else if constexpr (kAct == LayerActivation::kGelu) {
+    } else {
       const float e = expf(-0.5f * z * z);
       return e > 0.f ? fmaf(z * 0.3989422804014327f, e, normcdff(z)) : normcdff(z);
-    } else {
-      return Act16::slope<kAct>(z);
     }
   }
 };
+// The gradient of z from that of act(z).  relu's is a choice and no product: of what is infinite or NaN where z is not above zero nothing is left.
+__device__ __forceinline__ float choice(float d, float z) { return z <= 0.f ? 0.f : d; }
+__device__ __forceinline__ Two choice(Two d, Two z) {
+  float a, b, x, y;
+  d.apart(a, b);
+  z.apart(x, y);
+  return Two(choice(a, x), choice(b, y));
+}
+template <typename Act, LayerActivation kAct, typename N>
+__device__ __forceinline__ N derived(N d, N z) {
+  if constexpr (kAct == LayerActivation::kRelu) return choice(d, z);
+  else return d * Act::template slope<kAct>(z);
+}
 // Calls `f` with the activation as a type.
 template <LayerActivation kAct>
 struct ActIs {

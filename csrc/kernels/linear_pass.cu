@@ -98,13 +98,13 @@ __global__ void __launch_bounds__(kThreads, 2) layer_derive_kernel(const LayerDe
         if constexpr (kV > 1 && !std::is_same_v<T, float>) {
 #pragma unroll
           for (int i = 0; i < kV; i += 2) {
-            if constexpr (kSlope) (Two(d[i], d[i + 1]) * Act::template slope<kAct>(Two(v[i], v[i + 1]))).apart(d[i], d[i + 1]);
+            if constexpr (kSlope) derived<Act, kAct>(Two(d[i], d[i + 1]), Two(v[i], v[i + 1])).apart(d[i], d[i + 1]);
             add_to<2>(sum + i, d + i);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < kV; ++i) {
-            if constexpr (kSlope) d[i] *= Act::template slope<kAct>(v[i]);
+            if constexpr (kSlope) d[i] = derived<Act, kAct>(d[i], v[i]);
             sum[i] += d[i];
           }
         }

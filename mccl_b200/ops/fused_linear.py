@@ -64,11 +64,9 @@ def _check(x, weight, bias, residual):
 
 
 def _act(name, z):
-    """The activation and its slope."""
-    if name is None:
-        return z, torch.ones_like(z)
-    if name == "relu":
-        return torch.relu(z), (z > 0).to(z.dtype)
+    """The activation and its slope (relu's gradient is no product with one)."""
+    if name is None or name == "relu":
+        return z if name is None else torch.relu(z), None
     if name == "gelu":
         share = 0.5 * torch.erfc(-z * math.sqrt(0.5))
         return z * share, share + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
@@ -96,7 +94,9 @@ class _Plain(torch.autograd.Function):
     @without_autocast
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
-        dz = _wide(dy) if z is None else _wide(dy) * _act(ctx.activation, _wide(z))[1]
+        dz = _wide(dy)
+        if z is not None:
+            dz = dz.masked_fill(z <= 0, 0) if ctx.activation == "relu" else dz * _act(ctx.activation, _wide(z))[1]
         rows = dz.reshape(-1, dz.shape[-1])
         db = rows.sum(0).to(x.dtype) if ctx.bias else None
         rows = _wide(rows.to(x.dtype))  # an operand of the products

@@ -555,3 +555,28 @@ def test_weight_gradients_of_many_tokens_of_one_sign(emptied, cuda_device, dtype
         rows = torch.arange(0, tokens, tokens // 97, device=cuda_device)
         want = dy[rows].double() @ w.detach().double()
         assert ((got[0][rows].double() - want).abs() / want).max() <= _sum(dtype, 2048) + ROUNDOFF[dtype] * 1.01
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,residual", [(torch.float32, None), (torch.float16, None), (torch.bfloat16, None), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("tokens,out", [(3, 24), (40, 45), (700, 64)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_relu_leaves_nothing_of_a_gradient_that_is_not_finite_below_zero(device, dtype, residual, tokens, out, value):
+    t = _inputs(tokens, 16, out, dtype, residual, True, device, seed=6)
+    z = (t["x"].double() @ t["weight"].double().t() + t["bias"].double()).cpu()
+    low, high = (z < -0.1).nonzero()[0].tolist(), (z > 0.1).nonzero()[-1].tolist()
+    clean = t["dy"].clone()
+    clean[low[0], low[1]] = 0
+    t["dy"][low[0], low[1]] = value
+    got = _call(t, "relu")[1:]
+    want = _call({**t, "dy": clean}, "relu")[1:]
+    for a, b in list(zip(got, want))[:3]:  # the residual's gradient is dy itself
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    # above zero it goes on, as where z is a NaN
+    t["dy"] = clean.clone()
+    t["dy"][high[0], high[1]] = value
+    got = _call(t, "relu")[1:]
+    assert not torch.isfinite(got[0][high[0]]).any() and not torch.isfinite(got[1][high[1]]).any() and not torch.isfinite(got[2][high[1]])
+    x = torch.full((2, 16), math.nan, device=device, dtype=dtype).requires_grad_()
+    y = fused_linear(x, t["weight"].detach(), activation="relu")
+    assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], torch.autograd.grad(fused_linear(x, t["weight"].detach()), x, torch.ones_like(y))[0])
