@@ -271,9 +271,10 @@ class FusedAdamW(torch.optim.Optimizer):
         """A parameter's saved state as this optimizer keeps it; the base class has cast every tensor to the parameter's type."""
         if "exp_avg" not in saved or "exp_avg_sq" not in saved:
             return
+        st = self.state[p]
+        st.pop("low", None)  # a bf16 parameter's, for one that may be of another type now
         if self.state_bits == 32 and p.dtype is torch.float32 and "exp_avg_scale" not in saved:
             return  # as it came
-        st = self.state[p]
         for name, kind in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
             moment, scale = saved[name].to(p.device), saved.get(name + "_scale")
             scale = scale if scale is None else scale.to(p.device)
@@ -286,6 +287,5 @@ class FusedAdamW(torch.optim.Optimizer):
             else:
                 st[name] = unpack_moment(moment, scale, p.shape)
                 st.pop(name + "_scale", None)
-        st.pop("low", None)
         if p.dtype is torch.bfloat16 and "low" in saved:
             st["low"] = saved["low"].to(p.device)

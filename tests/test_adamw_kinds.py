@@ -487,3 +487,46 @@ def test_moments_of_32_bits_beside_scales_are_refused(cuda_device, dtype, which)
     with pytest.raises(RuntimeError, match="without scales"):
         opt.step()
     assert torch.equal(p, torch.ones_like(p)) and float(opt.state[p]["step"]) == 0
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype,other", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("into", [8, 32])
+def test_checkpoints_load_into_parameters_of_another_type(device, dtype, other, bits, into):
+    gen = torch.Generator().manual_seed(5)
+    first = [torch.randn(*s, generator=gen).to(device, dtype).requires_grad_() for s in ((30, 20), (5,))]
+    a = FusedAdamW(first, state_bits=bits, **HYPER)
+    for p in first:
+        st = a._state_of(p)
+        st["step"] = torch.tensor(7.0)
+        for name, kind in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
+            x = (torch.rand(p.shape, generator=gen) + 1e-3).to(device)
+            if bits == 8:
+                st[name], st[name + "_scale"] = pack_moment(x, kind)
+            else:
+                st[name] = x
+        if dtype is torch.bfloat16:
+            st["low"] = torch.randint(-32768, 32768, p.shape, generator=gen, dtype=torch.int16).to(device)
+    second = [p.detach().to(other).requires_grad_() for p in first]
+    b = FusedAdamW(second, state_bits=into, **HYPER)
+    b.load_state_dict(copy.deepcopy(a.state_dict()))
+    names = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if into == 8 else set())
+    for p, q in zip(first, second):
+        st = b.state[q]
+        assert set(st) - {"low"} == names and ("low" in st) == (dtype is other is torch.bfloat16) and float(st["step"]) == 7
+        if "low" in st:
+            assert torch.equal(st["low"], a.state[p]["low"])
+        for x, y, step in zip(a.moments(p), b.moments(q), (2.0 ** -4, 2.0 ** -3)):
+            assert torch.equal(x, y) if bits == 8 or into == 32 else ((x - y).abs() <= x * step).all()
+    if device == "cpu":
+        return
+    for q in second:
+        q.grad = torch.ones_like(q)
+    b.step()
+    for p, q in zip(first, second):
+        assert float(b.state[q]["step"]) == 8 and torch.isfinite(q).all() and not torch.equal(q, p.detach().to(other))
+        # m = 0.9 m + 0.1 of what was loaded, itself half a step off where it was packed; a step of 8 bits is an eighth at most
+        want = a.moments(p)[0] * 0.9 + 0.1
+        loaded = 0.0 if bits == 8 or into == 32 else 2.0 ** -4
+        assert ((b.moments(q)[0] - want).abs() <= want * (loaded + (2.0 ** -3 * (1 + loaded) if into == 8 else 0.0) + 2.0 ** -20)).all()
