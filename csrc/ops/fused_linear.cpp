@@ -216,6 +216,7 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     at::Tensor* const keep = activation == LayerActivation::kNone ? nullptr : &z;
     const at::Tensor y = forward_of(x, w, b, activation, r, sizes_of(x_in, w), keep);
     ctx->save_for_backward({x, w, z});
+    ctx->set_materialize_grads(false);
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b.defined();
     ctx->saved_data["residual"] = r.defined();

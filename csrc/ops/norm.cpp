@@ -97,6 +97,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     at::Tensor stats, normed;
     auto out = forward_of(x, p, eps, residual.value_or(at::Tensor()), static_cast<at::ScalarType>(dtype), &stats, &normed);
     ctx->save_for_backward({normed, p.weight, p.bias, stats});
+    ctx->set_materialize_grads(false);
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["dtype"] = dtype;
     ctx->saved_data["with"] = with;
@@ -129,7 +130,6 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     }
     c10::cuda::CUDAGuard guard(device);
     const at::Tensor stats = saved[3].contiguous();
-    if (!dy.defined()) dy = at::zeros(sizes, s.options().dtype(dtype));
     for (const auto& [g, type] : {std::pair<const at::Tensor&, at::ScalarType>(dy, dtype), std::pair<const at::Tensor&, at::ScalarType>(ds, sum_type)}) {
       if (!g.defined()) continue;
       check_saved(g, sizes, type, device, kWhat);
@@ -137,6 +137,9 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     size_t input = 0;  // tensors that there are not are not counted
     auto needed = [&](bool there) { return there && ctx->needs_input_grad(input++); };
     const bool need_x = needed(true), need_weight = needed(p.weight.defined()), need_bias = needed(p.bias.defined()), need_residual = needed(with);
+    if (!dy.defined())  // the sum's alone: it is x's and the residual's
+      return {need_x ? ds.to(x_type) : at::Tensor(), need_weight ? at::zeros_like(p.weight) : at::Tensor(), need_bias ? at::zeros_like(p.bias) : at::Tensor(),
+              need_residual ? ds : at::Tensor(), {}, {}};
     kern::NormBackward a{};
     a.shape = shape_of(s, p, ctx->saved_data["eps"].toDouble());
     a.s = norm_rows(s);

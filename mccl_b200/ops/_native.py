@@ -31,7 +31,7 @@ def without_autocast(backward):
     """A backward pass whose products are of its tensors' types, also where it is called inside of an autocast region."""
     @functools.wraps(backward)
     def run(ctx, grad):
-        device = autocast_of(grad)
+        device = None if grad is None else autocast_of(grad)
         if device is None:
             return backward(ctx, grad)
         torch.set_autocast_enabled(device, False)

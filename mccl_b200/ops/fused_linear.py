@@ -86,6 +86,7 @@ class _Plain(torch.autograd.Function):
         ctx.activation, ctx.bias = activation, bias is not None
         kept = z if z.dtype == x.dtype or activation is None else z.clamp(-65504, 65504).to(x.dtype) if x.dtype == torch.float16 else z.to(x.dtype)
         ctx.save_for_backward(x, weight, None if activation is None else kept)
+        ctx.set_materialize_grads(False)
         y = _act(activation, z)[0]
         return y.to(x.dtype) if residual is None else (y + _wide(residual)).to(residual.dtype)
 
@@ -93,6 +94,8 @@ class _Plain(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     @without_autocast
     def backward(ctx, dy):
+        if dy is None:
+            return (None,) * 5
         x, weight, z = ctx.saved_tensors
         dz = _wide(dy)
         if z is not None:

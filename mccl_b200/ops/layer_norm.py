@@ -58,9 +58,12 @@ class _Plain(torch.autograd.Function):
         if dy is None and ds is None:
             return (None,) * 6
         s, weight, rstd = ctx.saved_tensors
+        if dy is None:  # the sum's alone: it is x's and the residual's
+            none = None if ctx.bias_type is None else torch.zeros(s.shape[-1], dtype=ctx.bias_type, device=s.device)
+            return ds.to(ctx.x_type), None if weight is None else torch.zeros_like(weight), none, ds if ctx.needs_input_grad[3] else None, None, None
         u = s.float()
         u = (u - u.mean(-1, keepdim=True)) * rstd
-        dy = torch.zeros_like(u) if dy is None else dy.float()
+        dy = dy.float()
         g = dy if weight is None else dy * weight.float()
         dx = rstd * (g - g.mean(-1, keepdim=True) - u * (g * u).mean(-1, keepdim=True))
         if ds is not None:

@@ -580,3 +580,21 @@ def test_relu_leaves_nothing_of_a_gradient_that_is_not_finite_below_zero(device,
     x = torch.full((2, 16), math.nan, device=device, dtype=dtype).requires_grad_()
     y = fused_linear(x, t["weight"].detach(), activation="relu")
     assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], torch.autograd.grad(fused_linear(x, t["weight"].detach()), x, torch.ones_like(y))[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_result_that_nobody_has_a_gradient_of(device, dtype):
+    class Stop(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, y):
+            return y.clone()
+
+        @staticmethod
+        def backward(ctx, dy):
+            return None
+
+    t = _inputs(9, 24, 40, dtype, dtype, True, device)
+    leaves = [v.requires_grad_() for v in _leaves(t)]
+    y = fused_linear(t["x"], t["weight"], t["bias"], activation="gelu", residual=t["residual"])
+    assert torch.autograd.grad(Stop.apply(y).sum(), leaves, allow_unused=True) == (None,) * 4

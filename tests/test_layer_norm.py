@@ -395,3 +395,35 @@ def test_gradients_of_leaves_have_memory_of_their_own(device, dtype, stream, sha
         assert torch.equal(x.grad, turn * dx) and torch.equal(r.grad, turn * dr) and out[0].shape == out[1].shape == shape
         assert x.grad.untyped_storage().data_ptr() != r.grad.untyped_storage().data_ptr()
     assert all(torch.equal(a, b) for a, b in zip(given, kept))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,stream", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+def test_one_of_the_results_alone(device, dtype, stream):
+    gen = torch.Generator().manual_seed(9)
+    x, r, w, b = (torch.randn(s, generator=gen).to(device, t).requires_grad_() for s, t in (((3, 5, 40), dtype), ((3, 5, 40), stream), ((40,), torch.float32), ((40,), torch.float32)))
+    dy, ds = torch.randn(3, 5, 40, generator=gen).to(device, dtype), torch.randn(3, 5, 40, generator=gen).to(device, stream)
+    leaves = (x, w, b, r)
+    none_s = torch.autograd.grad(layer_norm(x, w, b, residual=r), leaves, (dy, torch.zeros_like(ds)))
+    got = torch.autograd.grad(layer_norm(x, w, b, residual=r)[0], leaves, dy)
+    assert all(torch.equal(a, c) for a, c in zip(got, none_s))
+    got = torch.autograd.grad(layer_norm(x, w, b, residual=r)[1], leaves, ds)
+    assert torch.equal(got[0], ds.to(dtype)) and torch.equal(got[3], ds) and float(got[1].abs().sum()) == float(got[2].abs().sum()) == 0
+    assert [g.dtype for g in got] == [t.dtype for t in leaves] and [g.shape for g in got] == [t.shape for t in leaves]
+    got = torch.autograd.grad(layer_norm(x, w, b, residual=r.detach())[1], leaves[:3], ds)
+    assert torch.equal(got[0], ds.to(dtype))
+
+
+@pytest.mark.gpu
+def test_gradients_that_there_are_not_take_no_memory(cuda_device):
+    x = torch.randn(2048, 1024, device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
+    r = torch.randn(2048, 1024, device=cuda_device, requires_grad=True)
+    for which, most in ((0, 2048 * 1024 * 6), (1, 2048 * 1024 * 2)):  # dx and the residual's; of the sum alone dx is ds in another type
+        out = layer_norm(x, residual=r)[which]
+        given = torch.randn_like(out)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        grads = torch.autograd.grad(out, (x, r), given)
+        assert torch.cuda.max_memory_allocated() - before <= most
+        del out, grads
