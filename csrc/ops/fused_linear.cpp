@@ -212,12 +212,14 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     const at::Tensor x = rows_of(x_in);
     c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
-    at::Tensor z;
-    at::Tensor* const keep = activation == LayerActivation::kNone ? nullptr : &z;
+    at::Tensor z;  // where one but the residual wants a gradient
+    at::Tensor* const keep =
+        activation == LayerActivation::kNone || !(x_in.requires_grad() || w.requires_grad() || (b.defined() && b.requires_grad())) ? nullptr : &z;
     const at::Tensor y = forward_of(x, w, b, activation, r, sizes_of(x_in, w), keep);
     ctx->save_for_backward({x, w, z});
     ctx->set_materialize_grads(false);
     ctx->saved_data["act"] = act;
+    ctx->saved_data["kept"] = keep != nullptr;
     ctx->saved_data["bias"] = b.defined();
     ctx->saved_data["residual"] = r.defined();
     ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
@@ -246,14 +248,16 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     check_saved(dy_in, y_sizes, y_type, device, kWhat);
     check_saved(saved[0], {rows, in}, type, device, kWhat);
     check_saved(saved[1], {out, in}, type, device, kWhat);
-    if (act != LayerActivation::kNone) check_saved(saved[2], {rows, type == at::kFloat ? out : kern::gated_row(out)}, type, device, kWhat);
+    const bool kept = ctx->saved_data["kept"].toBool();
+    if (kept) check_saved(saved[2], {rows, type == at::kFloat ? out : kern::gated_row(out)}, type, device, kWhat);
     c10::cuda::CUDAGuard guard(device);
     size_t input = 0;  // tensors that there are not are not counted
     auto needed = [&](bool there) { return there && ctx->needs_input_grad(input++); };
     const bool need_x = needed(true), need_w = needed(true), need_bias = needed(ctx->saved_data["bias"].toBool()),
                need_residual = needed(ctx->saved_data["residual"].toBool());
+    if (!need_x && !need_w && !need_bias) return {{}, {}, {}, need_residual ? dy_in : at::Tensor(), {}};
     const Needs need{need_x, need_w, need_bias};
-    const at::Tensor dy = rows_of(dy_in), z = act != LayerActivation::kNone ? rows_of(saved[2]) : at::Tensor();
+    const at::Tensor dy = rows_of(dy_in), z = kept ? rows_of(saved[2]) : at::Tensor();
     const Gradients r = type == at::kFloat ? backward32(dy, saved[0], saved[1], z, act, need) : backward16(dy, saved[0], saved[1], z, act, need);
     return {need_x ? r.x.view(sizes) : at::Tensor(), r.w, r.bias, need_residual ? dy_in : at::Tensor(), {}};
   }

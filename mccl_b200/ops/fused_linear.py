@@ -84,8 +84,9 @@ class _Plain(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, activation):
         z = F.linear(_wide(x), _wide(weight), _wide(bias))
         ctx.activation, ctx.bias = activation, bias is not None
+        keep = activation is not None and any(ctx.needs_input_grad[:3])
         kept = z if z.dtype == x.dtype or activation is None else z.clamp(-65504, 65504).to(x.dtype) if x.dtype == torch.float16 else z.to(x.dtype)
-        ctx.save_for_backward(x, weight, None if activation is None else kept)
+        ctx.save_for_backward(x, weight, kept if keep else None)
         ctx.set_materialize_grads(False)
         y = _act(activation, z)[0]
         return y.to(x.dtype) if residual is None else (y + _wide(residual)).to(residual.dtype)
@@ -96,6 +97,8 @@ class _Plain(torch.autograd.Function):
     def backward(ctx, dy):
         if dy is None:
             return (None,) * 5
+        if not any(ctx.needs_input_grad[:3]):
+            return None, None, None, dy, None
         x, weight, z = ctx.saved_tensors
         dz = _wide(dy)
         if z is not None:

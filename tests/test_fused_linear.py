@@ -598,3 +598,23 @@ def test_a_result_that_nobody_has_a_gradient_of(device, dtype):
     leaves = [v.requires_grad_() for v in _leaves(t)]
     y = fused_linear(t["x"], t["weight"], t["bias"], activation="gelu", residual=t["residual"])
     assert torch.autograd.grad(Stop.apply(y).sum(), leaves, allow_unused=True) == (None,) * 4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("tokens,width,out", [(3, 24, 40), (300, 72, 1000), (256, 1024, 520)])
+def test_nothing_is_kept_for_the_residuals_gradient(device, dtype, tokens, width, out):
+    t = _inputs(tokens, width, out, dtype, torch.float32, True, device, seed=2)
+    t["residual"].requires_grad_()
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: kept.append(s.shape) or s, lambda s: s):
+        y = fused_linear(t["x"], t["weight"], t["bias"], activation="gelu", residual=t["residual"])
+    # the operands, which are the caller's
+    assert all(tuple(s) in ((tokens, width), (out, width)) for s in kept)
+    assert torch.equal(torch.autograd.grad(y, t["residual"], t["dy"])[0], t["dy"])
+    for name in ("x", "weight", "bias"):  # one other is enough
+        u = {k: v.detach().requires_grad_(k in (name, "residual")) for k, v in t.items()}
+        full = {k: v.detach().requires_grad_(k != "dy") for k, v in t.items()}
+        a, b = (fused_linear(v["x"], v["weight"], v["bias"], activation="gelu", residual=v["residual"]) for v in (u, full))
+        # (few tokens of which nothing is kept have a kernel of their own)
+        assert torch.equal(torch.autograd.grad(a, u[name], t["dy"])[0], torch.autograd.grad(b, full[name], t["dy"])[0])
