@@ -49,7 +49,12 @@ def parse():
     ap.add_argument("--lr", type=float, default=1e-4)
     ap.add_argument("--save-stats", default="")
     ap.add_argument("--cpu", action="store_true", help="CPU tensors (host transport)")
-    return ap.parse_args()
+    args = ap.parse_args()
+    if args.fused_blocks and not args.model.startswith("gpt2"):
+        ap.error("--fused-blocks is for the GPT-2 models")
+    if args.moment_bits != 32 and (not args.fused_optim or args.cpu or not torch.cuda.is_available()):
+        ap.error("--moment-bits 8 is for --fused-optim on a GPU")
+    return args
 
 
 def build(args, device):

@@ -36,6 +36,10 @@ def main(argv=None):
     ap.add_argument("--moment-bits", type=int, default=32, choices=[8, 32], help="of AdamW's moments")
     ap.add_argument("--optim-in-backward", action="store_true", help="AdamW per bucket behind its allreduce (native hook)")
     args = ap.parse_args(argv)
+    if args.fused_blocks and not args.model.startswith("gpt2"):
+        ap.error("--fused-blocks is for the GPT-2 models")
+    if args.moment_bits != 32 and (args.impl != "mccl" or args.model == "resnet50"):
+        ap.error("--moment-bits 8 is for the fused AdamW, which --impl nccl and resnet50 do not train with")
 
     rank, ws, local = (int(os.environ.get(k, d)) for k, d in (("RANK", "0"), ("WORLD_SIZE", "1"), ("LOCAL_RANK", "0")))
     os.environ.setdefault("MASTER_ADDR", "127.0.0.1")

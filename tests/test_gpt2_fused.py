@@ -184,3 +184,28 @@ def test_example_on_the_cpu():
 @pytest.mark.gpu
 def test_example_with_moments_in_8_bits():
     _example("--fused-optim", "--moment-bits", "8", "--fp16")
+
+
+@pytest.mark.parametrize("args,what", [
+    (["--cpu", "--model", "gpt2-tiny", "--moment-bits", "8"], "--moment-bits 8 is for"),
+    (["--cpu", "--model", "gpt2-tiny", "--fused-optim", "--moment-bits", "8"], "--moment-bits 8 is for"),
+    (["--cpu", "--model", "gated-tiny", "--fused-blocks"], "--fused-blocks is for"),
+    (["--model", "mlp", "--fused-blocks"], "--fused-blocks is for")])
+def test_example_refuses_flags_without_effect(args, what, monkeypatch, capsys):
+    import runpy
+    monkeypatch.setattr(sys, "argv", ["ddp_dummy_train.py", "--baseline", *args])
+    with pytest.raises(SystemExit) as e:
+        runpy.run_path(str(ROOT / "examples/ddp_dummy_train.py"), run_name="__main__")
+    assert e.value.code == 2 and what in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("args,what", [
+    (["--model", "gpt2-tiny", "--impl", "nccl", "--moment-bits", "8"], "--moment-bits 8 is for"),
+    (["--model", "resnet50", "--moment-bits", "8"], "--moment-bits 8 is for"),
+    (["--model", "resnet50", "--fused-blocks"], "--fused-blocks is for"),
+    (["--model", "mlp", "--fused-blocks"], "--fused-blocks is for")])
+def test_benchmark_refuses_flags_without_effect(args, what, capsys):
+    from mccl_b200.bench.ddp import main
+    with pytest.raises(SystemExit) as e:
+        main(args)
+    assert e.value.code == 2 and what in capsys.readouterr().err
