@@ -618,3 +618,51 @@ def test_nothing_is_kept_for_the_residuals_gradient(device, dtype, tokens, width
         a, b = (fused_linear(v["x"], v["weight"], v["bias"], activation="gelu", residual=v["residual"]) for v in (u, full))
         # (few tokens of which nothing is kept have a kernel of their own)
         assert torch.equal(torch.autograd.grad(a, u[name], t["dy"])[0], torch.autograd.grad(b, full[name], t["dy"])[0])
+
+
+def _launches():
+    from mccl_b200 import require_native
+    return require_native()._kernel_launches()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [1504, 1503])
+@pytest.mark.parametrize("dtype,residual", [(torch.float16, None), (torch.bfloat16, None), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
+                                            (torch.float16, torch.float32), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("activation", [None, "gelu"])
+def test_tiles_whose_reduction_is_shared(cuda_device, out, dtype, residual, activation):
+    # 13 x 6 tiles of 256 x 256 for 74 pairs: the last four are shared, and a second launch adds their parts up
+    t = _inputs(3300, 1024, out, dtype, residual, True, cuda_device, seed=out)
+    before = _launches()
+    y = _call(t, activation, grad=False)
+    assert _launches() == before + 2
+    _check(t, activation, y)
+    _check(t, activation, _call(t, activation))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", [3000, 3001])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("residual", [None, torch.float32])
+@pytest.mark.parametrize("activation", [None, "gelu_tanh"])
+def test_several_tiles_a_pair_of_several_parts_each(cuda_device, out, dtype, residual, activation):
+    # 25 x 12 tiles for 74 pairs, four whole ones each and four that are shared; sums of 1600 leave tensor memory in four parts where y is in 32 bits
+    t = _inputs(6400, 1600, out, dtype, residual, True, cuda_device, seed=out)
+    rows = torch.arange(0, 6400, 37, device=cuda_device)
+    some = {k: v[rows] if k in ("x", "residual", "dy") else v for k, v in t.items()}
+    before = _launches()
+    y = _call(t, activation, grad=False)[0]
+    assert _launches() == before + 2
+    _check(some, activation, [y[rows]])
+    saved = []
+    t["x"].requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: saved.append(s) or s, lambda s: s):
+        kept = fused_linear(t["x"], t["weight"], t["bias"], activation=activation, residual=t.get("residual"))
+    assert torch.equal(kept, y)
+    if activation is None:
+        return
+    (z,) = (s for s in saved if s.shape == (6400, (out + 7) // 8 * 8))
+    x, w, b = (some[k].detach().double() for k in ("x", "weight", "bias"))
+    want = x @ w.T + b
+    ez = x.abs() @ w.abs().T * _sum(dtype, 1600) + U * (want.abs() + b.abs())
+    assert ((z[rows, :out].double() - want).abs() <= ez + (want.abs() + ez) * ROUNDOFF[dtype] + SMALLEST[dtype]).all()
