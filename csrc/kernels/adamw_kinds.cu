@@ -62,7 +62,9 @@ __device__ __forceinline__ uint32_t power_of(uint32_t most, int top) {
 __device__ __forceinline__ Two sum_of(Two a, Two b, Two one) { return fma_of(a, one, b); }
 // Root and quotient, correctly rounded, of numbers far from either end of fp32's range, by Markstein's theorems (Computation of elementary
 // functions on the IBM RISC System/6000 processor, 1990): Newton's iteration to a root or reciprocal within a rounding, then one step on the
-// remainder, which a fused multiplication and addition gives exactly.  No branch stands between one element's and the next one's, as
+// remainder, which a fused multiplication and addition gives exactly.  The theorem on quotients asks for a reciprocal that is correctly rounded itself,
+// which the one step here may miss for a divisor beside a power of two (0x1.fffffe, 0x1.fffffa).  What that moves is some 2^-22 of a unit of the quotient,
+// before it is rounded: it shows where a quotient is that near to the middle of two numbers.  All that are within 2^-20 are tested, and right.  No branch stands between one element's and the next one's, as
 // there does in the general functions.  Signs are turned where that saves turning a factor's: -root(v), and a / -b.
 __device__ __forceinline__ Two negative_root_of(Two v) {
   float a, b;

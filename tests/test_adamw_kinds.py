@@ -532,3 +532,28 @@ def test_checkpoints_load_into_parameters_of_another_type(device, dtype, other, 
         want = a.moments(p)[0] * 0.9 + 0.1
         loaded = 0.0 if bits == 8 or into == 32 else 2.0 ** -4
         assert ((b.moments(q)[0] - want).abs() <= want * (loaded + (2.0 ** -3 * (1 + loaded) if into == 8 else 0.0) + 2.0 ** -20)).all()
+
+
+@pytest.mark.gpu
+def test_quotients_beside_the_middle_of_two_numbers(cuda_device):
+    import mccl_b200
+    native = mccl_b200.require_native()
+    hard = [(float.fromhex(a), float.fromhex(b)) for a, b in (("0x1.aaaaa6p0", "0x1.fffffap0"), ("0x1p0", "0x1.fffffep0"), ("0x1.fffffcp0", "0x1.fffffep0"))]
+    a, b = (torch.tensor(v, device=cuda_device) for v in zip(*hard))
+    assert torch.equal(native._test_root_quotient(a, b)[1], (a.double() / b.double()).float())
+    # a = A and b = 2^j B with B odd, both of 24 digits: a / b is r / (2 B) units beside Q + 1/2 where (2 Q + 1) B = A 2^k + r, which fixes Q by B's
+    # inverse modulo 2^k.  (A quotient of such numbers rounded to 64 bits first is rounded alike.)
+    for j in range(5):
+        odd = torch.arange((1 << (23 - j)) + 1, 1 << (24 - j), 2, device=cuda_device)
+        for k in (24 - j, 25 - j):
+            inverse = odd.clone()
+            for _ in range(5):
+                inverse = (inverse * (2 - odd * inverse)) & ((1 << k) - 1)
+            for r in range(1 - (32 >> j), 32 >> j, 2):  # all within 2^-20
+                for more in range((1 << 25) >> k):
+                    middle = ((inverse * r) & ((1 << k) - 1)) + (more << k)
+                    numerator = (middle * odd - r) >> k
+                    assert bool(((middle * odd - r) == numerator << k).all())
+                    inside = (middle >= 1 << 24) & (numerator >= 1 << 23) & (numerator < 1 << 24)
+                    a, b = numerator[inside].float(), odd[inside].float()
+                    assert torch.equal(native._test_root_quotient(a, b)[1], (a.double() / b.double()).float())
