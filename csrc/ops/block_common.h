@@ -66,6 +66,9 @@ inline at::Tensor rows_of(const at::Tensor& t) {
   if (r.numel() > 0 && (r.stride(1) != 1 && cols != 1)) r = r.contiguous();
   return r;
 }
+// The same of an input of an autograd function, to be kept: a view of another tensor than the input itself, but with its count of changes, so that
+// it is refused as the input would be where that was changed in place.
+inline at::Tensor rows_kept(const at::Tensor& t) { return rows_of(t.dim() == 2 ? t : t.detach()); }
 inline int64_t row_stride(const at::Tensor& r) { return r.size(0) <= 1 ? r.size(1) : r.stride(0); }
 
 }  // namespace mccl

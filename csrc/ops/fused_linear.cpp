@@ -209,7 +209,7 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x_in, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
                             const c10::optional<at::Tensor>& residual, int64_t act) {
     const auto activation = static_cast<LayerActivation>(act);
-    const at::Tensor x = rows_of(x_in);
+    const at::Tensor x = rows_kept(x_in);
     c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor b = bias.value_or(at::Tensor()), r = residual.value_or(at::Tensor());
     at::Tensor z;  // where one but the residual wants a gradient

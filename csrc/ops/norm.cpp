@@ -63,7 +63,7 @@ void check_call(const at::Tensor& x, const Affine& p, double eps, const at::Tens
 // y and, with a residual, the sum, of x's shape; mean and rstd where they are asked for, and the rows that were normed.
 std::vector<at::Tensor> forward_of(const at::Tensor& x_in, const Affine& p, double eps, const at::Tensor& residual_in, at::ScalarType dtype, at::Tensor* stats,
                                    at::Tensor* normed) {
-  const at::Tensor x = rows_of(x_in), residual = residual_in.defined() ? rows_of(residual_in) : residual_in;
+  const at::Tensor x = normed != nullptr ? rows_kept(x_in) : rows_of(x_in), residual = residual_in.defined() ? rows_of(residual_in) : residual_in;
   c10::cuda::CUDAGuard guard(x.device());
   kern::NormForward a{};
   a.shape = shape_of(x, p, eps);

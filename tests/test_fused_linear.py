@@ -666,3 +666,19 @@ def test_several_tiles_a_pair_of_several_parts_each(cuda_device, out, dtype, res
     want = x @ w.T + b
     ez = x.abs() @ w.abs().T * _sum(dtype, 1600) + U * (want.abs() + b.abs())
     assert ((z[rows, :out].double() - want).abs() <= ez + (want.abs() + ez) * ROUNDOFF[dtype] + SMALLEST[dtype]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(16,), (5, 16), (2, 3, 16), (2, 2, 3, 16)])
+def test_tensors_that_are_changed_in_place(device, shape):
+    w = torch.randn(16, 16, device=device, requires_grad=True)
+    for activation in (None, "gelu"):
+        x = torch.randn(shape, device=device, requires_grad=True) * 2
+        y = fused_linear(x, w, activation=activation, residual=x)
+        x.add_(1)  # what backward would read
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        x = torch.randn(shape, device=device, requires_grad=True) * 2
+        y = fused_linear(x, w, activation=activation, residual=x)
+        y.mul_(2)  # what it would not
+        y.sum().backward()

@@ -427,3 +427,18 @@ def test_gradients_that_there_are_not_take_no_memory(cuda_device):
         grads = torch.autograd.grad(out, (x, r), given)
         assert torch.cuda.max_memory_allocated() - before <= most
         del out, grads
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(16,), (5, 16), (2, 3, 16), (2, 2, 3, 16)])
+def test_tensors_that_are_changed_in_place(device, shape):
+    for call, changed in ((lambda x: (layer_norm(x),), lambda x, out: x), (lambda x: layer_norm(x, residual=x), lambda x, out: out[1])):
+        x = torch.randn(shape, device=device, requires_grad=True) * 2
+        out = call(x)
+        changed(x, out).add_(1)  # what backward would read
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out[0].sum().backward()
+        x = torch.randn(shape, device=device, requires_grad=True) * 2
+        out = call(x)[0]
+        out.mul_(2)  # what it would not
+        out.sum().backward()
