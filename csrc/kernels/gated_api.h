@@ -150,7 +150,9 @@ struct LayerTiles {
 cudaError_t launch_layer_tiles(const LayerTiles& g, cudaStream_t s);
 
 // A small layer of fp32, each direction one launch (kernels/linear_small.cu, with both sides measured): short reductions, and so little to multiply that
-// products of the library and passes around them are mostly their launches.
+// products of the library and passes around them are mostly their launches.  What is gained is the host's time, 6 to 10 us a call forward and 33 with gradients:
+// on the device a few shapes are slower by it than by the library (3 x 256 x 192 6.5 us for 2.7, 1024 x 256 x 256 11.4 for 9.8), which shows where calls are
+// replayed from a graph or wait behind longer ones.
 inline bool layer_is_small(int64_t tokens, int64_t in, int64_t out) { return in <= 256 && tokens <= 8192 && out <= 8192 && tokens * in * out <= 1ll << 26; }
 inline bool layer_is_small_backward(int64_t tokens, int64_t in, int64_t out) {
   return out <= 512 && tokens <= 1024 && in <= 8192 && tokens * in * out <= 1ll << 26;

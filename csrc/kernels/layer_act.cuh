@@ -8,7 +8,8 @@
 namespace mccl {
 namespace kern {
 
-// For results that are rounded to 16 bits.  Each is within 2^-18 of its size: exponentials and reciprocals by the instructions for them.
+// For products of 16-bit numbers.  Each is within 2^-18 of its size, a hundredth of the operands' own rounding in fp16, whether the result is rounded to 16
+// bits or, with a residual in 32, is not: exponentials and reciprocals by the instructions for them.
 // Of numbers (N: float) or of two side by side (Two), for which half as many instructions do.
 struct Act16 {
   template <typename N>

@@ -6,7 +6,7 @@
 // groups' sums are added in a fixed order.
 //
 // us on the device, and the library's products and sums in brackets (B200): forward 136 x 128 x 128 5.2 (6.3), 656 x 77 x 176 5.4 (6.2), 3 x 256 x 192 6.5 (2.7), 1024 x
-// 256 x 256 11.4 (9.8), 300 x 512 x 512 18.5 (14), and 2 to 3 more in brackets behind an activation; backward 8.3 (13), 20 (24), 6.6 (8.2), 34 (35), 28 (25).  The host
+// 256 x 256 11.4 (9.8), and 2 to 3 more in brackets behind an activation; backward 8.3 (13), 20 (24), 6.6 (8.2), 34 (35).  The host
 // gets there in 9 us and 57 (autograd's engine included) where the library's calls and the passes around them take 15 to 19 and 90.
 #include "kernels/gated_api.h"
 #include "kernels/launch_count.h"

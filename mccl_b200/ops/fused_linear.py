@@ -1,10 +1,12 @@
-"""Linear layer with its bias, an activation and a residual behind the product, ``act(x weight^T + bias) + residual``, in one kernel.
+"""Linear layer with its bias, an activation and a residual behind the product, ``act(x weight^T + bias) + residual``.
 
-``float16`` and ``bfloat16``: the product is on the tensor cores (``csrc/kernels/gated.cu``, some tens or hundreds of rows
-``linear_tiles.cu``), and what follows it is done on its fp32 sums, rounded once; a few tokens of which nothing is kept have a kernel that
-reads the weights at the rate of memory (``linear_few.cu``).  With a ``float32`` residual, such as the stream of a model under autocast, the
-result is ``float32`` too.  ``float32``: the products of ``mccl_b200.ops.linear`` (torch's where TF32 is allowed), with one pass behind
-them; small layers that these would leave to torch's products are whole kernels, in full precision (``linear_small.cu``).
+``float16`` and ``bfloat16``, one kernel (and a second one that adds up the parts of tiles whose reduction is shared): the product is on
+the tensor cores (``csrc/kernels/gated.cu``, some tens or hundreds of rows ``linear_tiles.cu``), and what follows it is done on its
+fp32 sums, rounded once, the activation within 2^-18 of its size, also where the result is ``float32``; a few tokens of which nothing
+is kept have a kernel that reads the weights at the rate of memory (``linear_few.cu``).  With a ``float32`` residual, such as the stream
+of a model under autocast, the result is ``float32`` too.  ``float32``: the products of ``mccl_b200.ops.linear`` (torch's where it
+leaves them to torch or TF32 is allowed), with one pass behind the first and one or two before those of the gradients; small layers
+that these would leave to torch's products are whole kernels, in full precision (``linear_small.cu``).
 
 Gradients: of all four.  Behind an activation ``x weight^T + bias`` is kept in the operands' type for the backward pass, which makes
 ``dz`` of it and of the result's gradient, rounded to that type as an operand of the two products, and the gradient of the bias of
