@@ -192,8 +192,8 @@ Gradients backward32(const at::Tensor& dy, const at::Tensor& x, const at::Tensor
   return r;
 }
 
-std::vector<int64_t> sizes_of(const at::Tensor& x, const at::Tensor& w) {
-  auto sizes = x.sizes().vec();
+at::DimVector sizes_of(const at::Tensor& x, const at::Tensor& w) {
+  at::DimVector sizes(x.sizes());
   sizes.back() = w.size(0);
   return sizes;
 }
@@ -219,13 +219,10 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     ctx->save_for_backward({x, w, z});
     ctx->set_materialize_grads(false);
     ctx->saved_data["act"] = act;
-    ctx->saved_data["kept"] = keep != nullptr;
     ctx->saved_data["bias"] = b.defined();
     ctx->saved_data["residual"] = r.defined();
     ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
     ctx->saved_data["y_type"] = static_cast<int64_t>(y.scalar_type());
-    ctx->saved_data["rows"] = x.size(0);
-    ctx->saved_data["in"] = w.size(1);
     ctx->saved_data["out"] = w.size(0);
     ctx->saved_data["sizes"] = x_in.sizes().vec();
     return y;
@@ -240,16 +237,15 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
     const auto saved = ctx->get_saved_variables();
     const auto act = static_cast<LayerActivation>(ctx->saved_data["act"].toInt());
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), y_type = static_cast<at::ScalarType>(ctx->saved_data["y_type"].toInt());
-    const int64_t rows = ctx->saved_data["rows"].toInt(), in = ctx->saved_data["in"].toInt(), out = ctx->saved_data["out"].toInt();
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
-    auto y_sizes = sizes;
+    const int64_t in = sizes.back(), out = ctx->saved_data["out"].toInt();
+    at::DimVector y_sizes(sizes.begin(), sizes.end());
     y_sizes.back() = out;
     const at::Device device = dy_in.device();
     check_saved(dy_in, y_sizes, y_type, device, kWhat);
+    const int64_t rows = dy_in.numel() / out;
     check_saved(saved[0], {rows, in}, type, device, kWhat);
     check_saved(saved[1], {out, in}, type, device, kWhat);
-    const bool kept = ctx->saved_data["kept"].toBool();
-    if (kept) check_saved(saved[2], {rows, type == at::kFloat ? out : kern::gated_row(out)}, type, device, kWhat);
     c10::cuda::CUDAGuard guard(device);
     size_t input = 0;  // tensors that there are not are not counted
     auto needed = [&](bool there) { return there && ctx->needs_input_grad(input++); };
@@ -257,9 +253,10 @@ struct FusedLinearFn : torch::autograd::Function<FusedLinearFn> {
                need_residual = needed(ctx->saved_data["residual"].toBool());
     if (!need_x && !need_w && !need_bias) return {{}, {}, {}, need_residual ? dy_in : at::Tensor(), {}};
     const Needs need{need_x, need_w, need_bias};
-    const at::Tensor dy = rows_of(dy_in), z = kept ? rows_of(saved[2]) : at::Tensor();
+    if (act != LayerActivation::kNone) check_saved(saved[2], {rows, type == at::kFloat ? out : kern::gated_row(out)}, type, device, kWhat);
+    const at::Tensor dy = rows_of(dy_in), z = act != LayerActivation::kNone ? rows_of(saved[2]) : at::Tensor();
     const Gradients r = type == at::kFloat ? backward32(dy, saved[0], saved[1], z, act, need) : backward16(dy, saved[0], saved[1], z, act, need);
-    return {need_x ? r.x.view(sizes) : at::Tensor(), r.w, r.bias, need_residual ? dy_in : at::Tensor(), {}};
+    return {need_x && sizes.size() != 2 ? r.x.view(sizes) : r.x, r.w, r.bias, need_residual ? dy_in : at::Tensor(), {}};
   }
 };
 

@@ -2,6 +2,7 @@
 
 #include <torch/csrc/autograd/custom_function.h>
 
+#include <array>
 #include <cmath>
 
 #include "kernels/norm_api.h"
@@ -103,7 +104,6 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     ctx->saved_data["with"] = with;
     ctx->saved_data["x_type"] = static_cast<int64_t>(x.scalar_type());
     ctx->saved_data["sizes"] = x.sizes().vec();
-    ctx->saved_data["normed"] = normed.sizes().vec();
     ctx->saved_data["sum_type"] = static_cast<int64_t>(with ? out[1].scalar_type() : x.scalar_type());
     return out;
   }
@@ -114,13 +114,14 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     at::Tensor dy = grads[0], ds = with ? grads[1] : at::Tensor();
     if (!dy.defined() && !ds.defined()) return variable_list(6);
     const auto saved = ctx->get_saved_variables();
-    const auto sizes = ctx->saved_data["sizes"].toIntVector(), normed = ctx->saved_data["normed"].toIntVector();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const auto x_type = static_cast<at::ScalarType>(ctx->saved_data["x_type"].toInt()), sum_type = static_cast<at::ScalarType>(ctx->saved_data["sum_type"].toInt()),
                dtype = static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt());
     const at::Device device = (dy.defined() ? dy : ds).device();
-    check_saved(saved[0], normed, sum_type, device, kWhat);
+    const int64_t cols = sizes.back(), rows = (dy.defined() ? dy : ds).numel() / cols;
+    const std::array<int64_t, 2> flat{rows, cols};
+    check_saved(saved[0], with ? at::IntArrayRef(sizes) : at::IntArrayRef(flat), sum_type, device, kWhat);
     const at::Tensor s = rows_of(saved[0]);
-    const int64_t rows = s.size(0), cols = s.size(1);
     check_saved(saved[3], {2, rows}, at::kFloat, device, kWhat);
     Affine p{saved[1], saved[2]};
     for (at::Tensor* t : {&p.weight, &p.bias}) {
