@@ -92,7 +92,10 @@ struct Curve {
 };
 
 // What follows the product.  kLayer..: bias, activation and residual of a linear layer, whose result is in 16 or in 32 bits, and z kept or not.
-enum Out { kStore, kActivate, kDerive, kLayer, kLayerKeep, kLayer32, kLayer32Keep };
+// kSums: kStore of long sums.
+enum Out { kStore, kSums, kActivate, kDerive, kLayer, kLayerKeep, kLayer32, kLayer32Keep };
+template <Out kOut>
+constexpr bool kStores = kOut == kStore || kOut == kSums;
 template <Out kOut>
 constexpr bool kIsLayer = kOut >= kLayer;
 template <Out kOut>
@@ -100,12 +103,12 @@ constexpr bool kKeepsZ = kOut == kLayerKeep || kOut == kLayer32Keep;
 template <Out kOut>
 constexpr bool kWideY = kOut == kLayer32 || kOut == kLayer32Keep;
 
-// Sums that leave in 32 bits are taken out of tensor memory every kChunk stages (512 of the reduction) and added in registers, rounded to nearest:
-// the tensor cores cut theirs off, each time towards zero.  Sums of terms of one sign are 7e-7 of their size too small so, whatever their number, and
-// 6.4e-9 for each term without, which results of 16 bits have room for up to some number of terms (`deepest`, below).  The 128 numbers a thread are what the first four warps hand over of their registers:
+// Sums that leave in 32 bits, and long ones, are taken out of tensor memory every kChunk stages (512 of the reduction) and added in registers, rounded to
+// nearest: the tensor cores cut theirs off, each time towards zero.  Sums of terms of one sign are 7e-7 of their size too small so, whatever their number,
+// and 6.4e-9 for each term without (measured from 4096 to 262144).  The 128 numbers a thread are what the first four warps hand over of their registers:
 // at launch a thread has 168 (three warps of a quarter SM's 512 a lane), four warps go down to 56 and eight up to 224, as many in all.
 template <Out kOut>
-constexpr bool kAddsUp = kWideY<kOut>;
+constexpr bool kAddsUp = kWideY<kOut> || kOut == kSums;
 template <Out kOut>
 constexpr int kChunk = kAddsUp<kOut> ? 8 : 1 << 30;
 constexpr int kLaunched = 168, kKept = 56, kTaken = 224;
@@ -130,13 +133,13 @@ struct Job {
   int tiles_i, tiles_j;     // tiles_i: of all results
   int stages, segment;      // of the reduction; stages of its first part (dg Wg, then du Wu)
   int first;                // item
-  int whole, tail;          // items that are whole tiles; behind them `tail` tiles whose reduction is shared by `splits` items, with partial sums from `part` on
+  int whole;                // items that are whole tiles; behind them tiles whose reduction `splits` pairs share, with partial sums from `part` on
   int splits, per_split, part;
   int join;                 // the first such tile among those of all jobs
 };
 constexpr int kMostJobs = 3;
 template <Out kOut>
-constexpr int kJobs = kOut == kStore ? kMostJobs : 1;
+constexpr int kJobs = kStores<kOut> ? kMostJobs : 1;
 template <int kN>
 struct Work {
   Job job[kN];
@@ -169,12 +172,12 @@ struct Item {
       c1 = j.stages;
       part = -1;
     } else {
-      // all tiles' first parts, then all second ones: pairs at work at a time read the same part of the reduction
-      const int at = (item - j.whole) / j.tail, t = item - j.whole - at * j.tail;
+      part = item - j.whole;
+      const int t = part / j.splits;
       tile_place(j, j.whole + t, ti, tj);
-      c0 = at * j.per_split;
+      c0 = (part - t * j.splits) * j.per_split;
       c1 = min(j.stages, c0 + j.per_split);
-      part = j.part + t * j.splits + at;
+      part += j.part;
     }
   }
 };
@@ -427,12 +430,40 @@ using Ahead = std::conditional_t<kOut == kDerive, Kept<kKeep>, std::conditional_
 // A thread's row and columns of a tile: `row` of the result that the tile is of, its columns from `col` on.
 struct Spot {
   int64_t row, col;
-  int which;      // kStore: which of two results
+  int which;      // kStore, kSums: which of two results
 };
 template <Out kOut>
 __device__ __forceinline__ Spot spot_of(const Job& j, int ti, int tj, int row_in_tile) {
-  const int second = kOut == kStore && ti >= j.rows_segment;
+  const int second = kStores<kOut> && ti >= j.rows_segment;
   return {static_cast<int64_t>(second ? ti - j.rows_segment : ti) * kTile + row_in_tile, static_cast<int64_t>(tj) * (kOut == kActivate ? kHalf : kTile), second};
+}
+// The boxes of 64 columns, from the tile's column `c` on and up to `last`, of the warp's rows from `y` on, to the results.
+template <Out kOut>
+__device__ __forceinline__ void flush_store(const Job& j, const Spot& at, int c, int last, int64_t y, uint32_t boxes, int lane) {
+  if (!kStores<kOut> || j.wide) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      if (y < j.rows)
+#pragma unroll
+        for (int b = 0; b < kBoxes<kOut>; ++b)
+          store_box(&j.out[kOut == kDerive ? b : at.which], boxes + b * kBoxBytes, static_cast<int>(at.col) + c, static_cast<int>(y));
+      stores_commit();
+    }
+  } else {  // rows that are not aligned: two numbers a lane, row by row
+    __syncwarp();
+    const int n = static_cast<int>(min(static_cast<int64_t>(32), j.rows - y));
+    uint16_t* to = static_cast<uint16_t*>(j.to[at.which]) + y * j.ldo + at.col + c + 2 * lane;
+    const int here = last - c - 2 * lane;
+#pragma unroll 4
+    for (int r = 0; r < n; ++r, to += j.ldo) {
+      uint32_t v;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(boxes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
+      if (here > 0) to[0] = static_cast<uint16_t>(v);
+      if (here > 1) to[1] = static_cast<uint16_t>(v >> 16);
+    }
+    __syncwarp();
+  }
 }
 // kCols columns from `c` of the tile on, into a sink.
 struct NoMore {
@@ -487,7 +518,7 @@ template <Out kOut, GatedKeep kKeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Work<kJobs<kOut>> w) {
   constexpr int kDepths = kStages<kOut>, kOuts = kBoxes<kOut>;
   extern __shared__ char raw[];
-  __shared__ alignas(8) uint64_t bars[2 * kDepths + 5 + (kAddsUp<kOut> ? kOutWarps : 0)];
+  __shared__ alignas(8) uint64_t bars[2 * kDepths + 5 + (kWideY<kOut> ? kOutWarps : 0)];
   __shared__ uint32_t tmem_base;
   const uint32_t smem0 = (smem_addr(raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -508,7 +539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
       bar_init(acc_free(b), 2 * kOutWarps);
     }
     bar_init(drained, 1);
-    if constexpr (kAddsUp<kOut>)
+    if constexpr (kWideY<kOut>)
       for (int i = 0; i < kOutWarps; ++i) bar_init(drained + 8u * (1 + i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -636,7 +667,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           __syncwarp();
           if (!l.residual_vec) put_residual(l, y, j.rows, at.col + c, lane, y_boxes);
         };
-        if (ok && t.part < 0 && first < last) ask(first);  // (where a wait has run out the last one's may be on its way still)
+        if (kWideY<kOut> && ok && t.part < 0 && first < last) ask(first);  // (where a wait has run out the last one's may be on its way still)
         float sum[kShare];
 #pragma unroll
         for (int i = 0; i < kShare; ++i) sum[i] = 0.f;
@@ -660,7 +691,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           __syncwarp();
           if (lane == 0 && ok) bar_arrive_cluster(in_leader(acc_free(done & 1)));
         }
-        if (t.part < 0) {
+        if (t.part < 0 && !kWideY<kOut>) {
+#pragma unroll
+          for (int turn = 0; turn < kShare; turn += kTurn) {
+            const int c = first + turn;
+            if (c >= last) break;
+            if (lane == 0) stores_left();
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kTurn; i += 8) {
+              if (w.f.bf16) Staged<true>(boxes, lane).put(0, i, sum + turn + i);
+              else Staged<false>(boxes, lane).put(0, i, sum + turn + i);
+            }
+            flush_store<kOut>(j, at, c, last, y, boxes, lane);
+          }
+        } else if (t.part < 0) {
           const Staged<true> own(boxes, lane);
 #pragma unroll
           for (int turn = 0; turn < kShare; turn += kTurn) {
@@ -755,29 +800,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_k
           }
           if constexpr (kIsLayer<kOut>) {
             flush_layer<kKeepsZ<kOut>, kWideY<kOut>>(LayerTarget{&j.out[0], &j.out[1], j.to[0], j.ldo, j.rows, j.wide}, at.col + c, last - c, y, boxes, lane);
-          } else if (kOut != kStore || j.wide) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-              if (y < j.rows)
-#pragma unroll
-                for (int b = 0; b < kOuts; ++b)
-                  store_box(&j.out[kOut == kDerive ? b : at.which], boxes + b * kBoxBytes, static_cast<int>(at.col) + c, static_cast<int>(y));
-              stores_commit();
-            }
-          } else {  // rows that are not aligned: two numbers a lane, row by row
-            __syncwarp();
-            const int n = static_cast<int>(min(static_cast<int64_t>(32), j.rows - y));
-            uint16_t* to = static_cast<uint16_t*>(j.to[at.which]) + y * j.ldo + at.col + c + 2 * lane;
-            const int here = last - c - 2 * lane;
-#pragma unroll 4
-            for (int r = 0; r < n; ++r, to += j.ldo) {
-              uint32_t v;
-              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(boxes + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4));
-              if (here > 0) to[0] = static_cast<uint16_t>(v);
-              if (here > 1) to[1] = static_cast<uint16_t>(v >> 16);
-            }
-            __syncwarp();
+          } else {
+            flush_store<kOut>(j, at, c, last, y, boxes, lane);
           }
         }
       } else {
@@ -1020,30 +1044,21 @@ void share(Plan& l, int64_t tiles, int64_t most, int64_t rows) {
   l.splits = splits;
   l.per_split = per;
 }
-// Weight gradients add up over the tokens, of which there is no end, in tensor memory, where a sum of terms of one sign comes out 6.4e-9 of its size too
-// small for each of them (measured from 4096 to 262144 terms): a sum of more than this many is shared, so that what is lost stays below half of what rounding
-// the result may take, 2.1e-4 of 2^-11 in fp16 and 1.7e-3 of 2^-8 in bf16, whatever the number of tokens.  (Sums over a layer's width are shorter.)
-// 2048 x 2048 fp16 of 65536 tokens 405 us for 354 of sums that are not shared, of 262144 1.49 ms for 1.38.
-int64_t deepest(const GatedShape& s) { return (s.bf16 ? 1 << 18 : 1 << 15) / kDepth; }
-void bound(GatedProduct p, const GatedShape& s, Plan& l) {
-  if ((p != GatedProduct::kWeightUp && p != GatedProduct::kWeightDown) || l.longest() <= deepest(s)) return;
-  l.tail += l.whole;
-  l.whole = 0;
-  l.per_split = ceil_div(l.stages, ceil_div(l.stages, deepest(s)));
-  l.splits = ceil_div(l.stages, l.per_split);
-}
+// Stages of a sum that may stay in tensor memory where the result is of 16 bits: what terms of one sign lose there is below half of what rounding may
+// take, 2.1e-4 of 2^-11 in fp16 and 1.7e-3 of 2^-8 in bf16.  Gradients of weights, sums over the tokens, are longer at times.  us of 2048 x 2048, in registers and
+// not: 65536 tokens 380 and 354, 262144 tokens 1504 and 1380.  (Shared along the tokens, parts of 2^15 each: 405 and 1493, and 16 MB of scratch a part.)
+int64_t longest_sum(const GatedShape& s) { return (s.bf16 ? 1 << 18 : 1 << 15) / kDepth; }
 // One product: whole tiles as long as they fill the device; the rest, less than one tile a pair, is shared along the reduction where that
 // pays.
 void plan_one(GatedProduct p, const GatedShape& s, Plan& l) {
   l = plan_of(p, s);
   const int64_t tail = l.whole % kPairs;
   if (tail > 0) share(l, tail, kPairs / tail, sizes_of(p, s).rows);
-  bound(p, s, l);
 }
 // Stages that a product by itself takes, with 8 us for sums that are joined and 4 for a launch.
 double stages_alone(const Plan& l) {
   const int64_t rounds = ceil_div(l.whole, kPairs);
-  return static_cast<double>(rounds * l.stages + ceil_div(l.tail * l.splits, kPairs) * l.per_split) + (l.tail > 0 ? 12.0 : 4.0) / kStageUs;
+  return static_cast<double>(rounds * l.stages + (l.tail > 0 ? l.per_split : 0)) + (l.tail > 0 ? 12.0 : 4.0) / kStageUs;
 }
 // Several products side by side: whole tiles, but for a product whose tiles are so few and long that the device would wait for them.
 // Whether that is faster than one after the other, of which each leaves part of the device idle in its last round: 8192 tokens of 1024 x
@@ -1064,7 +1079,6 @@ bool plan_together(const GatedProduct* p, const GatedShape& s, int n, Plan* l, i
   bool joins = false;
   for (int i = 0; i < n; ++i) {
     if (2 * l[i].stages > 3 * fair) share(l[i], l[i].whole, ceil_div(l[i].stages, fair), sizes_of(p[i], s).rows);
-    bound(p[i], s, l[i]);
     joins = joins || l[i].tail > 0;
   }
   std::sort(order, order + n, [&](int a, int b) { return l[a].longest() != l[b].longest() ? l[a].longest() > l[b].longest() : a < b; });
@@ -1095,7 +1109,9 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
   w.partial = all.partial;
   w.failed = all.failed;
   w.limit = all.limit;
+  constexpr Out kJoined = kOut == kSums ? kStore : kOut;
   const auto kernel = gated_kernel<kOut, kKeep>;
+  const auto join = gated_join_kernel<kJoined, kKeep>;
   static std::atomic<uint64_t> smem_set{0};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -1104,7 +1120,7 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
   if (!(smem_set.load(std::memory_order_acquire) & bit)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<kOut>);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(gated_join_kernel<kOut, kKeep>, cudaFuncAttributeMaxDynamicSharedMemorySize, kJoinSmem<kOut, kKeep>);
+    e = cudaFuncSetAttribute(join, cudaFuncAttributeMaxDynamicSharedMemorySize, kJoinSmem<kJoined, kKeep>);
     if (e != cudaSuccess) return e;
     if constexpr (kAddsUp<kOut>) {  // the split of registers is one of as many as the launch has
       cudaFuncAttributes at{};
@@ -1127,11 +1143,11 @@ cudaError_t run(const Work<kMostJobs>& all, int64_t tail, bool high, cudaStream_
   note_launch();
   e = cudaLaunchKernelEx(&cfg, kernel, w);
   if (e != cudaSuccess || tail == 0) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(tail), high ? 2 : 1, (kOut == kActivate ? kHalf : kTile) / kTake<kOut, kKeep>);
+  cfg.gridDim = dim3(static_cast<unsigned>(tail), high ? 2 : 1, (kOut == kActivate ? kHalf : kTile) / kTake<kJoined, kKeep>);
   cfg.blockDim = dim3(kJoinThreads);
-  cfg.dynamicSmemBytes = kJoinSmem<kOut, kKeep>;
+  cfg.dynamicSmemBytes = kJoinSmem<kJoined, kKeep>;
   note_launch();
-  return cudaLaunchKernelEx(&cfg, gated_join_kernel<kOut, kKeep>, w);
+  return cudaLaunchKernelEx(&cfg, join, w);
 }
 
 // A product's maps and shape.
@@ -1247,7 +1263,7 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
   }
   Work<kMostJobs> w{};
   int64_t items = 0, parts = 0, joins = 0;
-  bool high = false;
+  bool high = false, sums = false;
   for (int i = 0; i < n; ++i) {
     const Plan& q = l[order[i]];
     Job& j = w.job[i];
@@ -1259,7 +1275,6 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
     j.segment = static_cast<int>(q.segment);
     j.first = static_cast<int>(items);
     j.whole = static_cast<int>(q.whole);
-    j.tail = static_cast<int>(q.tail);
     j.splits = static_cast<int>(q.splits);
     j.per_split = static_cast<int>(q.per_split);
     j.part = static_cast<int>(parts);
@@ -1268,6 +1283,7 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
     parts += q.tail * q.splits;
     joins += q.tail;
     high = high || (q.tail > 0 && j.rows > kHalf);
+    sums = sums || q.longest() > longest_sum(h);
     if (items + kPairs > 0x7FFFFFFF) return cudaErrorInvalidValue;
   }
   w.jobs = n;
@@ -1298,7 +1314,7 @@ cudaError_t launch_gated(const GatedArgs* g, int n, const GatedLaunch& r, cudaSt
     case GatedProduct::kLayer:
       if (r.layer->y_f32) return g[0].out1 != nullptr ? run<kLayer32Keep, GatedKeep::kNone>(w, joins, high, s) : run<kLayer32, GatedKeep::kNone>(w, joins, high, s);
       return g[0].out1 != nullptr ? run<kLayerKeep, GatedKeep::kNone>(w, joins, high, s) : run<kLayer, GatedKeep::kNone>(w, joins, high, s);
-    default: return run<kStore, GatedKeep::kNone>(w, joins, high, s);
+    default: return sums ? run<kSums, GatedKeep::kNone>(w, joins, high, s) : run<kStore, GatedKeep::kNone>(w, joins, high, s);
   }
 }
 

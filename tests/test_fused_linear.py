@@ -529,28 +529,37 @@ def emptied():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,tokens,shared", [(torch.float16, 32768, False), (torch.float16, 32769, True), (torch.float16, 262144, True),
-                                                 (torch.bfloat16, 262144, False), (torch.bfloat16, 262145, True)])
+@pytest.mark.parametrize("width,out", [(64, 64), (61, 300)])
+def test_long_sums_that_are_shared_too(emptied, cuda_device, width, out):
+    # one tile or two, whose reduction 16 pairs share, each with more than 2^15 terms
+    gen = torch.Generator(device=cuda_device).manual_seed(out)
+    x = torch.rand(600_001, width, device=cuda_device, generator=gen, dtype=torch.float16)
+    w = torch.rand(out, width, device=cuda_device, generator=gen, dtype=torch.float16).requires_grad_()
+    dy = torch.rand(600_001, out, device=cuda_device, generator=gen, dtype=torch.float16) * 2.0 ** -10
+    before = _launches()
+    (got,) = torch.autograd.grad(fused_linear(x, w), w, dy)
+    assert _launches() >= before + 3
+    want = dy.double().t() @ x.double()
+    assert ((got.double() - want).abs() / want).max() <= 68 * 2.0 ** -23 + (600_001 / 512 / 16 + 17) * U + ROUNDOFF[torch.float16] * 1.01
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tokens", [(torch.float16, 32768), (torch.float16, 32769), (torch.float16, 262144), (torch.bfloat16, 262144), (torch.bfloat16, 262145)])
 @pytest.mark.parametrize("both", [False, True])
-def test_weight_gradients_of_many_tokens_of_one_sign(emptied, cuda_device, dtype, tokens, shared, both):
-    from mccl_b200 import require_native
+@pytest.mark.parametrize("width", [2048, 2043])
+def test_weight_gradients_of_many_tokens_of_one_sign(emptied, cuda_device, dtype, tokens, both, width):
     gen = torch.Generator(device=cuda_device).manual_seed(tokens)
-    x = torch.rand(tokens, 2048, device=cuda_device, generator=gen, dtype=dtype).requires_grad_(both)
-    w = torch.rand(2048, 2048, device=cuda_device, generator=gen, dtype=dtype).requires_grad_()
+    x = torch.rand(tokens, width, device=cuda_device, generator=gen, dtype=dtype).requires_grad_(both)
+    w = torch.rand(2048, width, device=cuda_device, generator=gen, dtype=dtype).requires_grad_()
     # 64 terms of the sums are of size one
     dy = torch.rand(tokens, 2048, device=cuda_device, generator=gen, dtype=dtype) * (64.0 / tokens)
-    y = fused_linear(x, w)
-    before = require_native()._kernel_launches()
-    got = torch.autograd.grad(y, (x, w) if both else w, dy)
-    launches = require_native()._kernel_launches() - before
-    if not both:
-        assert launches == (2 if shared else 1)  # sums that are shared are joined by a second one
-    at = torch.arange(0, 2048, 7, device=cuda_device)
-    want = dy[:, at].double().t() @ x.detach()[:, at].double()
-    # a part has 2^15 (bf16 2^18) terms at most, each 8 of them cut off at 2^-23; parts are added up in fp32, and the result rounded once
-    deepest = 1 << (15 if dtype is torch.float16 else 18)
-    off = ((got[-1][at][:, at].double() - want).abs() / want).max()
-    assert off <= (min(tokens, deepest) / 8 + 4) * 2.0 ** -23 + 16 * U + ROUNDOFF[dtype] * 1.01
+    got = torch.autograd.grad(fused_linear(x, w), (x, w) if both else w, dy)
+    rows, columns = (torch.arange(0, n, 7, device=cuda_device) for n in (2048, width))
+    want = dy[:, rows].double().t() @ x.detach()[:, columns].double()
+    # Sums of up to 2^15 terms (bf16 2^18): each 8 of them cut off at 2^-23.  Longer ones: 512 terms so, added up in fp32.  The result is rounded once.
+    longest = 1 << (15 if dtype is torch.float16 else 18)
+    off = ((got[-1][rows][:, columns].double() - want).abs() / want).max()
+    assert off <= ((tokens / 8 + 4) * 2.0 ** -23 if tokens <= longest else 68 * 2.0 ** -23 + tokens / 512 * U) + ROUNDOFF[dtype] * 1.01
     if both:
         rows = torch.arange(0, tokens, tokens // 97, device=cuda_device)
         want = dy[rows].double() @ w.detach().double()

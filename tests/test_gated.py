@@ -624,3 +624,13 @@ def test_float32_products_are_torchs_where_tf32_is_allowed():
         torch.backends.cuda.matmul.allow_tf32 = was
     # what stands between the products is two launches; each product has others of its own
     assert counts[0] > 2 and counts[1] == 2
+
+
+@pytest.mark.gpu
+def test_sums_over_many_tokens_of_float16():
+    # gradients of the weights of more than 2^15 terms, which are added up in registers; two results side by side, and rows that are not aligned
+    *args, dy = _inputs(70_000, 712, 2731, torch.float16, seed=2)
+    want = _want(*args, dy, "silu", False, Rounding(torch.float16))
+    _check(_pass([t.requires_grad_() for t in args], dy), want)
+    del args, want
+    torch.cuda.empty_cache()
