@@ -1045,7 +1045,8 @@ void share(Plan& l, int64_t tiles, int64_t most, int64_t rows) {
   l.per_split = per;
 }
 // Stages of a sum that may stay in tensor memory where the result is of 16 bits: what terms of one sign lose there is below half of what rounding may
-// take, 2.1e-4 of 2^-11 in fp16 and 1.7e-3 of 2^-8 in bf16.  Gradients of weights, sums over the tokens, are longer at times.  us of 2048 x 2048, in registers and
+// take, 2.1e-4 of 2^-11 in fp16 and 1.7e-3 of 2^-8 in bf16.  Gradients of weights, sums over the tokens, are longer at times; what is
+// behind a forward product's sums over a layer's width (kUp, kLayer), which are not, has no such form.  us of 2048 x 2048, in registers and
 // not: 65536 tokens 380 and 354, 262144 tokens 1504 and 1380.  (Shared along the tokens, parts of 2^15 each: 405 and 1493, and 16 MB of scratch a part.)
 int64_t longest_sum(const GatedShape& s) { return (s.bf16 ? 1 << 18 : 1 << 15) / kDepth; }
 // One product: whole tiles as long as they fill the device; the rest, less than one tile a pair, is shared along the reduction where that
